@@ -747,6 +747,74 @@ int mi_attention_out_linear_proj(const void* core_attn_out, int64_t x_stride_tok
                                  int64_t workspace_bytes, int32_t T, int32_t hidden_size, int32_t Hq,
                                  int32_t head_dim, int32_t dtype, void* stream);
 
+/*
+ * Speculative decoding: the three calls that a step over drafted tokens has beyond an ordinary one (no counterpart in the
+ * reference, whose dynamic engine decodes one token per request and step).
+ *
+ * A request brings a tree of drafted tokens, its nodes (a chain is a tree): rows cu_seqlens_q[r] .. cu_seqlens_q[r + 1] - 1
+ * of q, of the logits and of the token rows.  Node 0 is the tree's root, the last token accepted before.  The nodes' keys
+ * and values have been appended as the request's last positions in node order (kv_lens counts them): node j lies at
+ * position kv_lens[r] - n_r + j, whatever its depth, which only its rotary position follows.
+ *
+ * mi_paged_tree_attention: every node attends to the request's context (the positions before its nodes) and to the nodes
+ * whose bits are set in its row of `tree_mask`: bit j % 64 of word j / 64 is node j (`mask_words` 1 to 4 words a row,
+ * `mask_stride` apart; its own bit included; nodes past the words are seen by none).  Rows that see nothing, and the rows
+ * of q behind the last request, are zeros.  Caches as for mi_paged_prefill_attention, 16-bit or fp8 (`kv_dtype`; fp8:
+ * head_dim 64 or 128, scales [n_chunks][Hkv]), chunks of any multiple of 16 tokens; lengths beyond the table's columns are
+ * cut to them, and table entries that name no chunk of the cache (`n_chunks`) hold tokens that no row sees.
+ */
+int64_t mi_tree_workspace_bytes(int32_t T, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim);
+int mi_paged_tree_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                            const void* v_cache, int64_t kv_stride_chunk, int64_t kv_stride_tok, int64_t kv_stride_head,
+                            int32_t n_chunks, int32_t kv_dtype, const float* k_scales, const float* v_scales,
+                            const int32_t* block_table, int64_t bt_stride, int32_t table_columns,
+                            const int32_t* cu_seqlens_q, const int32_t* kv_lens, const int64_t* tree_mask,
+                            int64_t mask_stride, int32_t mask_words, void* out, int64_t o_stride_tok,
+                            int64_t o_stride_head, void* workspace, int64_t workspace_bytes, int32_t T, int32_t R,
+                            int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t chunk_tokens, float softmax_scale,
+                            int32_t dtype, void* stream);
+
+/*
+ * mi_verify_drafted_tokens: the accepted path of each tree and the token that follows it.  Row i of `logits` (fp32 0,
+ * bf16 1, fp16 2) is what the target says after node i; tokens[i] is node i's token and parents[i] its parent, an index
+ * within its request (-1 for the root; a parent precedes its children, anything else is never reached; at most the first
+ * 1 024 nodes of a request are looked at).  p at a node is the softmax of logits / temperature (as
+ * mi_sample_from_logits scales them) over the values that are at least cut[i] (the scaled values' cut that
+ * mi_sample_from_logits returns; NULL: all).  From the root on, a node's children are tried in index order:
+ *   greedy != 0       accepted where the token is the first of the largest logits;
+ *   draft_probs NULL  accepted where uniform[i] * (mass left) < p(token); a rejected token leaves the distribution;
+ *   else              row i of draft_probs is the distribution q that the children of node i were drawn from: accepted where
+ *                     uniform[i] * q(token) < p(token), a rejection turns p into (p - q)+, normalised.
+ * The first accepted child is the next node.  The request's last token is drawn from what is left at the last node, by the
+ * inverse CDF in vocabulary order at uniform[root] (where nothing is left: from p); greedy: the largest logit's index.
+ * A path has at most max_path nodes; the children of its last one are then not tried.
+ * Outputs, [R][max_path] and [R]: out_rows the rows of the path's nodes (the root's first), out_tokens the new tokens (those
+ * of the accepted nodes, then the last), out_counts how many of each; -1 behind them; 0 nodes: 0 tokens.
+ */
+int64_t mi_verify_workspace_bytes(int32_t T, int32_t R, int32_t vocab);
+int mi_verify_drafted_tokens(const void* logits, int64_t stride_row, int32_t logits_dtype, int32_t T, int32_t vocab,
+                             const int64_t* tokens, const int32_t* parents, const int32_t* cu_seqlens_q, int32_t R,
+                             int32_t max_path, int32_t greedy, const void* draft_probs, int64_t draft_stride_row,
+                             int32_t draft_dtype, const float* uniform, float temperature, const float* cut,
+                             int64_t* out_tokens, int32_t* out_rows, int32_t* out_counts, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/*
+ * mi_kv_keep_accepted: after the verification, the accepted nodes' rows of the caches move to the positions behind the
+ * context, rows[r][i] (a row of the step, as out_rows; entry 0 is the root) to position kv_lens[r] - n_r + i for
+ * 1 <= i < counts[r], in `layers` layers that lie kv_stride_layer apart; new_kv_lens[r] = kv_lens[r] - n_r + counts[r].
+ * Paths rise.  Elements of 2 bytes are copied; an fp8 cache (1 byte, scales [layers][n_chunks][Hkv], layers
+ * scale_stride_layer apart) is copied inside a chunk and converted to the other scale (rounded to nearest, saturating)
+ * between chunks.  v_cache may be NULL (a cache with one tensor, e.g. MLA latents).  Entries that are no node of their
+ * request, and places outside the block table or the cache, move nothing.
+ */
+int mi_kv_keep_accepted(void* k_cache, void* v_cache, int64_t kv_stride_layer, int64_t kv_stride_chunk,
+                        int64_t kv_stride_tok, int32_t layers, int32_t n_chunks, int32_t chunk_tokens, int32_t Hkv,
+                        int32_t head_dim, int32_t elem_bytes, const float* k_scales, const float* v_scales,
+                        int64_t scale_stride_layer, const int32_t* block_table, int64_t bt_stride, int32_t table_columns,
+                        const int32_t* rows, int64_t rows_stride, int32_t columns, const int32_t* counts,
+                        const int32_t* cu_seqlens_q, const int32_t* kv_lens, int32_t* new_kv_lens, int32_t R, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -128,6 +128,19 @@ SIGNATURES = {
         c_int,
         [_P, _I64, _P, _I64, _P, _I64, _P, _P, _F, _I32, _P, _I64, _I32, _I32, _F,
          _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P]),
+    "mi_tree_workspace_bytes": (_I64, [_I32] * 5),
+    "mi_paged_tree_attention": (
+        c_int,
+        [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P, _P, _P, _I64, _I32, _P, _P, _P, _I64, _I32, _P, _I64,
+         _I64, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _F, _I32, _P]),
+    "mi_verify_workspace_bytes": (_I64, [_I32] * 3),
+    "mi_verify_drafted_tokens": (
+        c_int,
+        [_P, _I64, _I32, _I32, _I32, _P, _P, _P, _I32, _I32, _I32, _P, _I64, _I32, _P, _F, _P, _P, _P, _P, _P, _I64, _P]),
+    "mi_kv_keep_accepted": (
+        c_int,
+        [_P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _I64, _P, _I64, _I32, _P, _I64, _I32, _P,
+         _P, _P, _P, _I32, _P]),
 }
 
 

@@ -16,11 +16,13 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/CachingHostAllocator.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <chrono>
 #include <cmath>
+#include <initializer_list>
 #include <string>
 #include <tuple>
 #include <type_traits>
@@ -1013,6 +1015,154 @@ PyObject* last_token_gather(PyObject* const* a) {
   return a[2] == Py_None ? wrap(made) : same(a[2]);
 }
 
+// ------------------------------------------------------------------------------------------ speculative decoding
+void same_device(const Tensor& ref, std::initializer_list<const Tensor*> others) {
+  for (const Tensor* t : others) REQUIRE(!t || t->device() == ref.device(), "all tensors must be on one device");
+}
+// Rows of nodes: `[R + 1]` int32, R > 0.
+int64_t requests_of(const Tensor& cu) {
+  REQUIRE(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.is_contiguous() && cu.numel() >= 2,
+          "cu_seqlens_q must be a contiguous int32 row of at least two entries");
+  REQUIRE(cu.numel() - 1 < (int64_t)1 << 31, "too many requests");
+  return cu.numel() - 1;
+}
+
+// paged_tree_attention(q, k_cache, v_cache, cu_seqlens_q, kv_lens, block_table, tree_mask, softmax_scale|None, out|None,
+//                      k_scales|None, v_scales|None, override|None)
+PyObject* paged_tree_attention(PyObject* const* a) {
+  const Tensor& q = tensor(a[0], "q");
+  void* stream = stream_of(q);
+  const Tensor &kc = tensor(a[1], "k_cache"), &vc = tensor(a[2], "v_cache"), &cu = tensor(a[3], "cu_seqlens_q");
+  const Tensor &lens = tensor(a[4], "kv_lens"), &table = tensor(a[5], "block_table"), &mask = tensor(a[6], "tree_mask");
+  const Tensor *given = opt_tensor(a[8], "out"), *ks = opt_tensor(a[9], "k_scales"), *vs = opt_tensor(a[10], "v_scales");
+  same_device(q, {&kc, &vc, &cu, &lens, &table, &mask, given, ks, vs});
+  const Rows3 q3 = rows3(q, "q");
+  REQUIRE(kc.dim() == 4 && kc.size(3) == q3.d && same_shape(kc, vc), "cache shape mismatch");
+  const Cache c = cache_of(kc);
+  REQUIRE((ks != nullptr) == (vs != nullptr), "k_scales and v_scales go together");
+  if (ks) {
+    REQUIRE(kc.element_size() == 1 && vc.element_size() == 1, "fp8 caches hold one byte per element");
+    REQUIRE(scales_ok(ks, c.n, c.h) && scales_ok(vs, c.n, c.h), "scales must be contiguous fp32 [N, Hkv]");
+  } else {
+    REQUIRE(kc.scalar_type() == q.scalar_type() && vc.scalar_type() == q.scalar_type(),
+            "the cache must have the queries' 16-bit type, or be bytes with scales");
+  }
+  REQUIRE(same_strides(cache_of(vc), c), "k_cache / v_cache strides differ");
+  const int64_t R = requests_of(cu), T = q3.n;
+  check_table(table, lens, R);
+  REQUIRE(mask.scalar_type() == at::kLong && (mask.dim() == 1 || mask.dim() == 2) && mask.size(0) >= T,
+          "tree_mask must be int64 [T] or [T, words], a row for every row of q");
+  const bool words = mask.dim() == 2;
+  REQUIRE(!words || (mask.size(1) >= 1 && mask.size(1) <= 4 && (mask.stride(1) == 1 || mask.size(1) == 1)),
+          "tree_mask has 1 to 4 contiguous words a row (256 nodes a request)");
+  const float scale = a[7] == Py_None ? default_scale(q3.d) : (float)as_float(a[7]);
+  const c10::DeviceGuard guard(q.device());
+  Tensor made;
+  if (!given) made = at::empty_like(q);
+  const Tensor& out = given ? *given : made;
+  const Rows3 o3 = rows3(out, "out");
+  REQUIRE(o3.n == T && o3.h == q3.h && o3.d == q3.d && out.scalar_type() == q.scalar_type(), "out shape / dtype mismatch");
+  const Scratch ws = scratch(q, stream, mi_tree_workspace_bytes((int)T, (int)R, (int)q3.h, (int)c.h, (int)q3.d), Py_None, a[11]);
+  check(mi_paged_tree_attention(q.data_ptr(), q3.sn, q3.sh, kc.data_ptr(), vc.data_ptr(), c.sc, c.st, c.sh, (int)c.n,
+                                ks ? MI_KV_FP8_E4M3 : MI_KV_16BIT, (const float*)ptr(ks), (const float*)ptr(vs),
+                                (const int32_t*)table.data_ptr(), table.stride(0), (int)table.size(1),
+                                (const int32_t*)cu.data_ptr(), (const int32_t*)lens.data_ptr(), (const int64_t*)mask.data_ptr(),
+                                T > 1 ? mask.stride(0) : 4, words ? (int)mask.size(1) : 1, out.data_ptr(), o3.sn, o3.sh, ws.ptr,
+                                ws.bytes, (int)T, (int)R, (int)q3.h, (int)c.h, (int)q3.d, (int)c.c, scale, dtype_code(q), stream),
+        "mi_paged_tree_attention");
+  return given ? same(a[8]) : wrap(made);
+}
+
+// verify_drafted_tokens(logits, tokens, parents, cu_seqlens_q, max_path, greedy, draft_probs|None, uniform|None,
+//                       temperature, cut|None, override|None) -> (tokens, rows, counts)
+PyObject* verify_drafted_tokens(PyObject* const* a) {
+  const Tensor& logits = tensor(a[0], "logits");
+  void* stream = stream_of(logits);
+  const Tensor &tokens = tensor(a[1], "tokens"), &parents = tensor(a[2], "parents"), &cu = tensor(a[3], "cu_seqlens_q");
+  const Tensor *draft = opt_tensor(a[6], "draft_probs"), *uniform = opt_tensor(a[7], "uniform"), *cut = opt_tensor(a[9], "cut");
+  same_device(logits, {&tokens, &parents, &cu, draft, uniform, cut});
+  REQUIRE(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1), "logits must be [T, V] with contiguous V");
+  const int code = logits_code(logits);
+  const int64_t T = logits.size(0), V = logits.size(1), R = requests_of(cu), path = as_int(a[4]);
+  REQUIRE(path >= 1 && path < (1 << 20), "max_path must be at least 1");
+  const bool greedy = as_bool(a[5]);
+  REQUIRE(tokens.scalar_type() == at::kLong && tokens.is_contiguous() && tokens.numel() >= T, "tokens must be a contiguous int64 row of at least T");
+  REQUIRE(parents.scalar_type() == at::kInt && parents.is_contiguous() && parents.numel() >= T, "parents must be a contiguous int32 row of at least T");
+  int draft_code = 0;
+  if (draft) {
+    REQUIRE(draft->dim() == 2 && draft->size(0) >= T && draft->size(1) == V && (draft->stride(1) == 1 || V == 1),
+            "draft_probs must be [T, V] with contiguous V");
+    REQUIRE(draft->scalar_type() == at::kFloat || is_16bit(*draft), "draft_probs must be fp32, bf16 or fp16");
+    draft_code = logits_code(*draft);
+  }
+  REQUIRE(!greedy || (!draft && !cut), "a greedy call takes neither draft_probs nor cut");
+  if (!greedy) {
+    REQUIRE(uniform, "sampling needs one uniform number per row");
+    REQUIRE(uniform->scalar_type() == at::kFloat && uniform->is_contiguous() && uniform->numel() >= T,
+            "uniform must be a contiguous fp32 row of at least T numbers");
+  }
+  REQUIRE(!cut || (cut->scalar_type() == at::kFloat && cut->is_contiguous() && cut->numel() >= T),
+          "cut must be a contiguous fp32 row of at least T values");
+  const c10::DeviceGuard guard(logits.device());
+  Tensor out = at::empty({R, path}, tokens.options()), rows = at::empty({R, path}, cu.options()), counts = at::empty({R}, cu.options());
+  const int64_t need = mi_verify_workspace_bytes((int)T, (int)R, (int)V);
+  Scratch ws;
+  Tensor own;   // (a use_workspace buffer sized for attention may lack the room)
+  if (a[10] != Py_None && !usable(tensor(a[10], "workspace"), logits, need, 256)) {
+    own = at::empty({need}, logits.options().dtype(at::kByte));
+    ws = {own.data_ptr(), need};
+  } else {
+    ws = scratch(logits, stream, need, Py_None, a[10]);
+  }
+  check(mi_verify_drafted_tokens(logits.data_ptr(), T > 1 ? logits.stride(0) : V, code, (int)T, (int)V, (const int64_t*)tokens.data_ptr(),
+                                 (const int32_t*)parents.data_ptr(), (const int32_t*)cu.data_ptr(), (int)R, (int)path, greedy,
+                                 ptr(draft), draft ? (T > 1 ? draft->stride(0) : V) : 0, draft_code, greedy ? nullptr : (const float*)ptr(uniform),
+                                 (float)as_float(a[8]), (const float*)ptr(cut), (int64_t*)out.data_ptr(), (int32_t*)rows.data_ptr(),
+                                 (int32_t*)counts.data_ptr(), ws.ptr, ws.bytes, stream),
+        "mi_verify_drafted_tokens");
+  return Py_BuildValue("NNN", wrap(out), wrap(rows), wrap(counts));
+}
+
+// kv_keep_accepted(k_cache, v_cache|None, rows, counts, cu_seqlens_q, kv_lens, block_table, k_scales|None, v_scales|None)
+//   -> new kv_lens
+PyObject* kv_keep_accepted(PyObject* const* a) {
+  const Tensor& kc = tensor(a[0], "k_cache");
+  void* stream = stream_of(kc);
+  const Tensor* vc = opt_tensor(a[1], "v_cache");
+  const Tensor &rows = tensor(a[2], "rows"), &counts = tensor(a[3], "counts"), &cu = tensor(a[4], "cu_seqlens_q");
+  const Tensor &lens = tensor(a[5], "kv_lens"), &table = tensor(a[6], "block_table");
+  const Tensor *ks = opt_tensor(a[7], "k_scales"), *vs = opt_tensor(a[8], "v_scales");
+  same_device(kc, {vc, &rows, &counts, &cu, &lens, &table, ks, vs});
+  const int64_t dims = kc.dim();
+  REQUIRE(dims == 4 || dims == 5, "caches must be [N, C, Hkv, d] or [layers, N, C, Hkv, d]");
+  REQUIRE(!vc || (same_shape(kc, *vc) && kc.strides() == vc->strides() && kc.scalar_type() == vc->scalar_type()),
+          "k_cache / v_cache shapes, strides or types differ");
+  const int64_t L = dims == 5 ? kc.size(0) : 1, N = kc.size(dims - 4), C = kc.size(dims - 3), H = kc.size(dims - 2), D = kc.size(dims - 1);
+  REQUIRE(kc.stride(dims - 1) == 1 && (H == 1 || kc.stride(dims - 2) == D), "cache rows must be contiguous [Hkv, d]");
+  REQUIRE(kc.element_size() == 1 || is_16bit(kc), "caches hold 16-bit values, or bytes with scales");
+  REQUIRE((ks != nullptr) == (vs != nullptr) && (ks != nullptr) == (kc.element_size() == 1), "byte caches and k_scales / v_scales go together");
+  for (const Tensor* s : {ks, vs}) {
+    if (!s) continue;
+    REQUIRE(s->scalar_type() == at::kFloat && s->dim() == dims - 2 && s->size(dims - 4) == N && s->size(dims - 3) == H &&
+                (dims == 4 || s->size(0) == L) && s->stride(dims - 3) == 1 && s->stride(dims - 4) == H && s->strides() == ks->strides(),
+            "scales must be contiguous fp32 [(layers,) N, Hkv]");
+  }
+  const int64_t R = requests_of(cu);
+  check_table(table, lens, R);
+  REQUIRE(rows.scalar_type() == at::kInt && rows.dim() == 2 && rows.size(0) >= R && (rows.stride(1) == 1 || rows.size(1) == 1),
+          "rows must be int32 [R, max_path] with contiguous rows");
+  REQUIRE(counts.scalar_type() == at::kInt && counts.is_contiguous() && counts.numel() >= R, "counts must be a contiguous int32 row of at least R");
+  const c10::DeviceGuard guard(kc.device());
+  Tensor out = at::empty({R}, lens.options());
+  check(mi_kv_keep_accepted(kc.data_ptr(), ptr(vc), dims == 5 ? kc.stride(0) : 0, kc.stride(dims - 4), kc.stride(dims - 3), (int)L, (int)N,
+                            (int)C, (int)H, (int)D, (int)kc.element_size(), (const float*)ptr(ks), (const float*)ptr(vs),
+                            ks && dims == 5 ? ks->stride(0) : 0, (const int32_t*)table.data_ptr(), table.stride(0), (int)table.size(1),
+                            (const int32_t*)rows.data_ptr(), rows.stride(0), (int)rows.size(1), (const int32_t*)counts.data_ptr(),
+                            (const int32_t*)cu.data_ptr(), (const int32_t*)lens.data_ptr(), (int32_t*)out.data_ptr(), (int)R, stream),
+        "mi_kv_keep_accepted");
+  return wrap(out);
+}
+
 // ------------------------------------------------------------------------------------------ module
 template <PyObject* (*fn)(PyObject* const*), int count>
 PyObject* op(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -1164,7 +1314,8 @@ PyMethodDef kMethods[] = {
     OP(kv_append, 6), OP(kv_append_fp8, 9), OP(paged_decode_attention, 14), OP(paged_mla_decode_attention, 10),
     OP(paged_prefill_attention, 14), OP(paged_prefill_attention_mla, 11), OP(norm_rope_append, 22), OP(qkv_norm_rope_append, 22), OP(qkv_key_append, 16),
     OP(qkv_prefill_attention, 18), OP(decode_step_attention, 29),
-    OP(linear_decode, 5), OP(attention_layer_decode, 24), OP(sample_from_logits, 12), OP(selected_log_probs, 2), OP(last_token_gather, 3), OP(setup, 3),
+    OP(linear_decode, 5), OP(attention_layer_decode, 24), OP(sample_from_logits, 12), OP(selected_log_probs, 2), OP(last_token_gather, 3),
+    OP(paged_tree_attention, 12), OP(verify_drafted_tokens, 11), OP(kv_keep_accepted, 9), OP(setup, 3),
     OP(set_workspace, 3), OP(layer_views, 3), OP(watch, 4), OP(written_by_kernel, 2), OP(as_defined, 3), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", "Host side of the per-layer calls.", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

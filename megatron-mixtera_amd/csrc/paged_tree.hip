@@ -1,0 +1,731 @@
+// Attention of drafted tokens over the paged cache (gfx950): the step of speculative decoding.
+//
+// Every request brings a tree of drafted tokens ("nodes"; a chain is a tree), whose keys and values are already in the
+// cache as its last positions: node j of request r sits at position kv_lens[r] - n_r + j.  A node attends to the
+// request's whole context (the positions before its nodes) and to the nodes that its row of bits names:
+//   out[i] = sum_k P[i][k] V[k],  P[i] = softmax over the visible k of scale * q[i] . K[k].
+// A row that sees nothing is zero.  The reference has no such call (its attention takes one new token, or a chain:
+// megatron/core/transformer/attention.py:546-600).
+//
+// Work decomposition.  The (node, query head) pairs that share a KV head are its rows, 16 * NQ of them to a wavefront
+// ("part").  The tiles of 16 * NT tokens of all (request, part) pairs are laid end to end and a fixed grid of workgroups
+// takes equal spans of that sequence, whatever the mix of lengths; a workgroup's wavefronts take neighbouring KV heads of
+// the same tokens, so that it reads whole token rows of the cache.  A pair within one span writes its result, any other
+// leaves normalised fp32 partials and a base-2 log-sum-exp for the merge.  A span touches at most one pair that began
+// before it and one that goes on after it, so two slots per workgroup hold all partials.
+//
+// Per tile nothing goes through LDS: S^T = K Q^T lands as lane (row m16, g) slot i = token 4g + i, the B operand of
+// O^T += V^T P^T, whose A operand is built from row loads by byte permutes; a pair of 16-token sub-tiles makes one product
+// of depth 32 (the products only need the same tokens in the same slots on both sides).
+//
+// Only the tiles that reach past the context look at the bits.  A node's value row may hold infinities or NaN that rows
+// which do not see it must not meet, although a product multiplies it by their zeros: such values are taken out of their
+// tile and added to the sums of the rows that see them.
+#include <stdio.h>
+
+#include "mi_capi_internal.h"
+#include "mi_common.h"
+
+namespace mi {
+
+struct TreeParams {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  const uint8_t* kc;
+  const uint8_t* vc;
+  int64_t kv_sc;
+  int32_t kv_st, kv_sh;
+  const int32_t* bt;
+  int64_t bt_stride;
+  const int32_t* cu_q;
+  const int32_t* lens;
+  const uint32_t* mask;  // rows of bits, two words for each of the caller's
+  int64_t mask_st;       // words between rows
+  int32_t mask_words;
+  uint16_t* out;
+  int64_t o_st, o_sh;
+  float* part_o;         // [2 grid][Hkv][ROWS][HD]
+  float* part_lse;       // [2 grid][Hkv][ROWS]
+  int4* pair_info;       // per (request, part): first and last workgroup, request, part
+  int32_t* pairs;        // how many there are
+  const float* k_scale;
+  const float* v_scale;
+  uint64_t chunk_magic;
+  uint32_t g_magic;      // 2^32 / G + 1, 0 for G = 1
+  int32_t T, R, r_base, Hq, Hkv, G, chunk, n_chunks, table_cols, grid;
+  int32_t last_slice;    // the launch that clears the rows behind the last request
+  float scale_log2;
+};
+
+constexpr int kTreeRequestsPerLaunch = 2048;  // (their prefix sums lie in LDS, 24 bytes each)
+
+static __device__ __forceinline__ int tree_div_g(const TreeParams& p, int n) {
+  return p.g_magic ? (int)__umulhi((uint32_t)n, p.g_magic) : n;
+}
+static __device__ __forceinline__ int tree_chunk_of(int tok, uint64_t magic) { return (int)(((uint64_t)(uint32_t)tok * magic) >> 40); }
+
+struct TreeSegment {
+  int r, part;
+  int q_begin, nodes;  // rows of q, nodes of the request
+  int len, ctx;        // cached tokens, those before the first node (may be negative: nodes without a position)
+  int start, end;      // tokens of the segment
+  bool whole;
+  int slot;
+};
+
+// Bits of four tokens, node j0 first, of a row of `words` 32-bit words; what lies before node 0 is context.
+static __device__ __forceinline__ uint32_t tree_bits(const uint32_t* row, int words, int j0) {
+  if (j0 <= -4) return 15u;
+  const int j = max(j0, 0), w = j >> 5;
+  const uint32_t lo = w < words ? row[w] : 0u, hi = w + 1 < words ? row[w + 1] : 0u;
+  const uint32_t bits = (uint32_t)((((uint64_t)hi << 32) | lo) >> (j & 31));
+  return j0 < 0 ? (bits << -j0) | ((1u << -j0) - 1u) : bits;
+}
+
+template <int HD, int NT, int NQ, bool FP8, bool F16>
+static __device__ __forceinline__ void tree_segment(const TreeParams& p, const TreeSegment& s, int h, int lane) {
+  constexpr int KS = HD / 32, DV = HD / 16, ESZ = FP8 ? 1 : 2, TK = 16 * NT, ROWS = 16 * NQ;
+  constexpr int KL = FP8 ? KS / 2 : KS;      // 16-byte loads of a key row and lane
+  constexpr int VD = FP8 ? DV / 4 : DV / 2;  // dwords per token and lane of the value operand
+  const int m16 = lane & 15, g = lane >> 4;
+  const int r = __builtin_amdgcn_readfirstlane(s.r), len = __builtin_amdgcn_readfirstlane(s.len);
+  const int start = __builtin_amdgcn_readfirstlane(s.start), end = __builtin_amdgcn_readfirstlane(s.end);
+  const int ctx = __builtin_amdgcn_readfirstlane(s.ctx);
+  const int last = max(min(end, len) - 1, 0);
+
+  // rows of this lane: row tile nt, row m16
+  int q_row[NQ], q_head[NQ];
+  bool valid[NQ];
+  uint4 qf[NQ][KS];
+#pragma unroll
+  for (int nt = 0; nt < NQ; ++nt) {
+    const int n = s.part * ROWS + 16 * nt + m16, qi = tree_div_g(p, n);
+    valid[nt] = qi < s.nodes;
+    q_row[nt] = s.q_begin + (valid[nt] ? qi : 0);
+    q_head[nt] = h * p.G + (n - qi * p.G);
+    const uint16_t* row = p.q + (int64_t)q_row[nt] * p.q_st + (int64_t)q_head[nt] * p.q_sh;
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+      const int d0 = FP8 ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;  // (16 key bytes to a lane)
+      qf[nt][kk] = valid[nt] ? ld16(row + d0) : make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  const uint8_t* const kbase = p.kc + (int64_t)h * p.kv_sh * ESZ;
+  const uint8_t* const vbase = p.vc + (int64_t)h * p.kv_sh * ESZ;
+  const int64_t chunk_bytes = p.kv_sc * ESZ;
+  const uint32_t tok_bytes = (uint32_t)(p.kv_st * ESZ);
+  const uint32_t k_col = 16u * (uint32_t)g, v_col = (uint32_t)(DV * m16 * ESZ);
+
+  // Block-table cursor: the current chunk's entry and the next one's as scalars, the one after in flight (requested two
+  // chunks before its use).  An entry that names no chunk of the cache becomes -1: its tokens are seen by no row, and
+  // their loads go to chunk 0.
+  const int32_t* const bt_row = p.bt + (int64_t)(p.r_base + r) * p.bt_stride;
+  const int ci_last = tree_chunk_of(last, p.chunk_magic);
+  struct Cursor {
+    int ci, pc, pc_next, pc_after;
+    float sc, sc_next;
+  };
+  auto entry_load = [&](int ci) {
+    const int e = bt_row[min(ci, ci_last)];
+    return (uint32_t)e < (uint32_t)p.n_chunks ? e : -1;
+  };
+  auto scale_load = [&](const float* scales, int pc) { return scales[(int64_t)max(pc, 0) * p.Hkv + h]; };
+  auto uniform_f = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
+  auto follow = [&](Cursor& c, const float* scales, int ci) {
+    if (ci != c.ci) {
+      c.ci = ci;
+      c.pc = c.pc_next;
+      c.pc_next = __builtin_amdgcn_readfirstlane(c.pc_after);
+      c.pc_after = entry_load(ci + 2);
+      if (FP8) {
+        c.sc = uniform_f(c.sc_next);
+        c.sc_next = scale_load(scales, c.pc_next);
+      }
+    }
+  };
+  Cursor kcur, vcur;
+  {
+    const int ci0 = tree_chunk_of(min(start, last), p.chunk_magic);
+    const int e0 = entry_load(ci0), e1 = entry_load(ci0 + 1), e2 = entry_load(ci0 + 2);
+    kcur.ci = ci0;
+    kcur.pc = __builtin_amdgcn_readfirstlane(e0);
+    kcur.pc_next = __builtin_amdgcn_readfirstlane(e1);
+    kcur.pc_after = e2;
+    kcur.sc = kcur.sc_next = 1.f;
+    vcur = kcur;
+    if (FP8) {
+      const float a = scale_load(p.k_scale, kcur.pc), b = scale_load(p.v_scale, kcur.pc);
+      kcur.sc_next = scale_load(p.k_scale, kcur.pc_next);
+      vcur.sc_next = scale_load(p.v_scale, kcur.pc_next);
+      kcur.sc = uniform_f(a);
+      vcur.sc = uniform_f(b);
+    }
+  }
+
+  uint4 kf[NT][KL];
+  uint32_t vf[NT][4][VD];
+  float ksc = 1.f, vsc = 1.f;   // fp8: scales of the staged tiles' chunks
+  bool k_page = true;           // whether the staged keys' chunk exists
+  // Tokens past the segment's last are that one again: their scores are masked, and what lies behind a request in its
+  // last chunk is never read.
+  auto load_k = [&](int T) {
+    const int ci = tree_chunk_of(min(T, last), p.chunk_magic);
+    follow(kcur, p.k_scale, ci);
+    if (FP8) ksc = kcur.sc;
+    k_page = kcur.pc >= 0;
+    const uint8_t* chunk = kbase + (int64_t)max(kcur.pc, 0) * chunk_bytes;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int t0 = min(T + 16 * u, last);
+      const uint8_t* row = chunk + (uint32_t)(t0 - ci * p.chunk + min(last - t0, m16)) * tok_bytes + k_col;
+#pragma unroll
+      for (int kk = 0; kk < KL; ++kk) kf[u][kk] = ld16_stream(row + 64 * kk);
+    }
+  };
+  auto load_v = [&](int T) {
+    const int ci = tree_chunk_of(min(T, last), p.chunk_magic);
+    follow(vcur, p.v_scale, ci);
+    if (FP8) vsc = vcur.sc;
+    const uint8_t* chunk = vbase + (int64_t)max(vcur.pc, 0) * chunk_bytes + v_col;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int t0 = min(T + 16 * u, last);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        ld_dwords_stream(chunk + (uint32_t)(t0 - ci * p.chunk + min(last - t0, 4 * g + j)) * tok_bytes, vf[u][j]);
+    }
+  };
+
+  // The running maximum starts at a finite lowest value: a row that sees nothing keeps it and a sum of zero.
+  float m_run[NQ], l_run[NQ];
+  f32x4_t acc[NQ][DV];
+#pragma unroll
+  for (int nt = 0; nt < NQ; ++nt) {
+    m_run[nt] = -3e38f;
+    l_run[nt] = 0.f;
+#pragma unroll
+    for (int e = 0; e < DV; ++e) acc[nt][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  // fp8: the accumulators are in units of the current value scale (a change of chunk rescales them), so that the
+  // probabilities keep their own range: times a small scale they would be subnormal in fp16.
+  float unit = 1.f;
+  const uint2 ones = make_uint2(ones2<F16>(), ones2<F16>());
+  const f32x4_t zero4 = {0.f, 0.f, 0.f, 0.f};
+
+  if (start < end) {
+    load_k(start);
+    load_v(start);
+  }
+  for (int T = start; T < end; T += TK) {
+    // ---- S^T = K Q^T
+    const float mul = FP8 ? p.scale_log2 * ksc : p.scale_log2;
+    const bool masked = T + TK > min(ctx, end) || !k_page;   // wave-uniform
+    const bool page = k_page;
+    f32x4_t sc[NQ][NT];
+#pragma unroll
+    for (int nt = 0; nt < NQ; ++nt)
+#pragma unroll
+      for (int u = 0; u < NT; ++u) sc[nt][u] = zero4;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+#pragma unroll
+      for (int kk = 0; kk < KL; ++kk) {
+        if constexpr (FP8) {
+          const uint2 a0 = fp8x4_to_16x4<F16>(kf[u][kk].x), a1 = fp8x4_to_16x4<F16>(kf[u][kk].y);
+          const uint2 b0 = fp8x4_to_16x4<F16>(kf[u][kk].z), b1 = fp8x4_to_16x4<F16>(kf[u][kk].w);
+#pragma unroll
+          for (int nt = 0; nt < NQ; ++nt) {
+            sc[nt][u] = mfma_16x16x32<F16>(make_uint4(a0.x, a0.y, a1.x, a1.y), qf[nt][2 * kk], sc[nt][u]);
+            sc[nt][u] = mfma_16x16x32<F16>(make_uint4(b0.x, b0.y, b1.x, b1.y), qf[nt][2 * kk + 1], sc[nt][u]);
+          }
+        } else {
+#pragma unroll
+          for (int nt = 0; nt < NQ; ++nt) sc[nt][u] = mfma_16x16x32<F16>(kf[u][kk], qf[nt][kk], sc[nt][u]);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(T + TK);   // (the key registers are free again)
+    __builtin_amdgcn_sched_barrier(0);
+    if (FP8) {        // a scale may have any sign: the maximum is of the products' own scores
+#pragma unroll
+      for (int nt = 0; nt < NQ; ++nt)
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[nt][u][i] *= mul;
+    }
+    uint32_t seen[NQ];   // four bits per sub-tile: what this lane's row sees of its four tokens (masked tiles only)
+    if (masked) {
+#pragma unroll
+      for (int nt = 0; nt < NQ; ++nt) {
+        const uint32_t* bits = p.mask + (int64_t)q_row[nt] * p.mask_st;
+        seen[nt] = 0;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          const int t0 = T + 16 * u + 4 * g;
+          uint32_t b = page ? tree_bits(bits, p.mask_words, t0 - ctx) & 15u : 0u;
+          const int left = end - t0;
+          b &= left >= 4 ? 15u : left > 0 ? (1u << left) - 1u : 0u;
+          seen[nt] |= b << (4 * u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(b >> i & 1u)) sc[nt][u][i] = -INFINITY;
+        }
+      }
+    }
+    // ---- running maximum and sum (row m16; only the maximum crosses lanes, the sums come from the matrix cores)
+    const float pm = FP8 ? 1.f : mul;
+    uint2 pf[NQ][NT];
+    const float unit_new = FP8 && page ? (vsc == 0.f ? 1e-30f : vsc) : unit;
+#pragma unroll
+    for (int nt = 0; nt < NQ; ++nt) {
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) tmax = fmaxf(fmaxf(tmax, fmaxf(sc[nt][u][0], sc[nt][u][1])), fmaxf(sc[nt][u][2], sc[nt][u][3]));
+      const float m_new = fmaxf(m_run[nt], rowgroup_max(tmax) * pm);
+      const float alpha = fast_exp2(m_run[nt] - m_new);
+      m_run[nt] = m_new;
+      f32x4_t sum = zero4;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const float p0 = fast_exp2(__builtin_fmaf(sc[nt][u][0], pm, -m_new)), p1 = fast_exp2(__builtin_fmaf(sc[nt][u][1], pm, -m_new));
+        const float p2 = fast_exp2(__builtin_fmaf(sc[nt][u][2], pm, -m_new)), p3 = fast_exp2(__builtin_fmaf(sc[nt][u][3], pm, -m_new));
+        pf[nt][u] = make_uint2(pack2<F16>(p0, p1), pack2<F16>(p2, p3));
+        sum = mfma_16x16x16<F16>(ones, pf[nt][u], sum);
+      }
+      l_run[nt] = l_run[nt] * alpha + sum[0];
+      const float scale = FP8 ? alpha * (unit / unit_new) : alpha;
+      if (__builtin_amdgcn_ballot_w64(scale != 1.f)) {
+#pragma unroll
+        for (int e = 0; e < DV; ++e) {
+          acc[nt][e][0] *= scale; acc[nt][e][1] *= scale; acc[nt][e][2] *= scale; acc[nt][e][3] *= scale;
+        }
+      }
+    }
+    unit = unit_new;
+    // ---- O^T += V^T P^T
+    // value operands of sub-tile u: output column e of every four tokens, one half of a depth-32 product
+    auto column = [&](int u, int e) -> uint2 {
+      uint32_t x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (FP8) {
+          const uint2 w = fp8x4_to_16x4<F16>(vf[u][j][e >> 2]);
+          x[j] = (e >> 1) & 1 ? w.y : w.x;
+        } else {
+          x[j] = vf[u][j][e >> 1];
+        }
+      }
+      return (e & 1) ? make_uint2(high_halves(x[1], x[0]), high_halves(x[3], x[2]))
+                     : make_uint2(low_halves(x[1], x[0]), low_halves(x[3], x[2]));
+    };
+    if (masked) {
+      // Infinities and NaN: a product would take them into rows that do not see their token.  Each kind's places as ones
+      // times what the rows see say which sums it belongs to; then they are zeros.
+      auto odd = [](uint32_t x) -> uint32_t {   // the value's sign bit, for every value of a word
+        if constexpr (FP8) return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        else if constexpr (F16) return ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+        else return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+      };
+      uint32_t any = 0;
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int w = 0; w < VD; ++w) any |= odd(vf[u][j][w]);
+      if (__builtin_amdgcn_ballot_w64(any != 0)) {
+        // (an infinity counts 1, a negative one 64, a NaN 4096: exact in either type, and 16 of each fit)
+        constexpr uint32_t kOne = ones2<F16>() & 0xffffu, kInf = F16 ? 0x7c00u : 0x7f80u;
+        constexpr uint32_t k64 = F16 ? 0x5400u : 0x4280u, k4096 = F16 ? 0x6c00u : 0x4580u;
+        auto place = [&](uint32_t x) { return (x & 0x7fffu) > kInf ? k4096 : x == kInf ? kOne : x == (kInf | 0x8000u) ? k64 : 0u; };
+        auto places = [&](uint32_t w) { return place(w & 0xffffu) | place(w >> 16) << 16; };
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+#pragma unroll
+          for (int e = 0; e < DV; ++e) {
+            __builtin_amdgcn_sched_barrier(0);   // (one column at a time: registers)
+            const uint2 c = column(u, e), at = make_uint2(places(c.x), places(c.y));
+#pragma unroll
+            for (int nt = 0; nt < NQ; ++nt) {
+              const uint32_t b = seen[nt] >> (4 * u);
+              const uint2 sees = make_uint2((b & 1u ? kOne : 0u) | (b & 2u ? kOne << 16 : 0u), (b & 4u ? kOne : 0u) | (b & 8u ? kOne << 16 : 0u));
+              const f32x4_t n4 = mfma_16x16x16<F16>(at, sees, zero4);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t n = (uint32_t)n4[i];
+                const float up = n & 63u ? INFINITY : 0.f, down = n >> 6 & 63u ? -INFINITY : 0.f;
+                acc[nt][e][i] += n >> 12 ? __uint_as_float(0x7fc00000u) : up + down;
+              }
+            }
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int w = 0; w < VD; ++w) {
+              const uint32_t o = odd(vf[u][j][w]);
+              vf[u][j][w] &= FP8 ? ~((o >> 7) * 0xffu) : ~((o >> 15) * 0xffffu);
+            }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NT; u += NT >= 2 ? 2 : 1)
+#pragma unroll
+      for (int e = 0; e < DV; ++e) {
+        if constexpr (NT >= 2) {
+          const uint2 a = column(u, e), b = column(u + 1, e);
+#pragma unroll
+          for (int nt = 0; nt < NQ; ++nt)
+            acc[nt][e] = mfma_16x16x32<F16>(make_uint4(a.x, a.y, b.x, b.y),
+                                            make_uint4(pf[nt][u].x, pf[nt][u].y, pf[nt][u + 1].x, pf[nt][u + 1].y), acc[nt][e]);
+        } else {
+          const uint2 a = column(u, e);
+#pragma unroll
+          for (int nt = 0; nt < NQ; ++nt) acc[nt][e] = mfma_16x16x16<F16>(a, pf[nt][u], acc[nt][e]);
+        }
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(T + TK);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // ---- acc[nt][e][i] is element d = DV (4g + i) + e of the row
+#pragma unroll
+  for (int nt = 0; nt < NQ; ++nt) {
+    if (!valid[nt]) continue;
+    const float l = l_run[nt];
+    const float inv = l == 0.f ? 0.f : unit / l;   // (a NaN stays one)
+    if (s.whole) {
+      uint16_t* o = p.out + (int64_t)q_row[nt] * p.o_st + (int64_t)q_head[nt] * p.o_sh + 4 * DV * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[DV / 2];
+#pragma unroll
+        for (int dw = 0; dw < DV / 2; ++dw) w[dw] = pack2<F16>(acc[nt][2 * dw][i] * inv, acc[nt][2 * dw + 1][i] * inv);
+        st_dwords(o + DV * i, w);
+      }
+    } else {
+      const int64_t row = ((int64_t)s.slot * p.Hkv + h) * ROWS + 16 * nt + m16;
+      float* o = p.part_o + row * HD + 4 * DV * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < DV; e += 2)
+          *reinterpret_cast<float2*>(o + DV * i + e) = make_float2(acc[nt][e][i] * inv, acc[nt][e + 1][i] * inv);
+      if (g == 0) p.part_lse[row] = l == 0.f ? -INFINITY : m_run[nt] + fast_log2(l);
+    }
+  }
+}
+
+// What one request brings: rows of q, nodes, cached tokens.  Whatever the arrays hold, rows stay inside q and tokens
+// inside the block table.
+struct TreeRequest {
+  int q_begin, nodes, len;
+};
+static __device__ __forceinline__ TreeRequest tree_request(const TreeParams& p, int i) {
+  TreeRequest t;
+  t.q_begin = min(max(p.cu_q[i], 0), p.T);
+  t.nodes = min(max(p.cu_q[i + 1], t.q_begin), p.T) - t.q_begin;
+  t.len = (int)min((int64_t)max(p.lens[i], 0), (int64_t)p.table_cols * p.chunk);
+  return t;
+}
+
+// Inclusive sum over the lanes of a wavefront.
+static __device__ __forceinline__ int64_t tree_scan(int64_t v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_up(v, d, 64);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+template <int HD, int NT, int NQ, bool FP8, bool F16>
+__global__ __launch_bounds__(512, 2) void paged_tree_kernel(TreeParams p) {
+  constexpr int TK = 16 * NT, ROWS = 16 * NQ;
+  extern __shared__ int64_t tree_lds[];
+  int64_t* const cum = tree_lds;                               // tiles of requests 0 .. i
+  int32_t* const first = reinterpret_cast<int32_t*>(cum + p.R);  // parts of requests 0 .. i
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.y * (blockDim.x >> 6) + wave;
+
+  if (wave == 0) {
+    int64_t tiles = 0;
+    int64_t parts = 0;
+    for (int base = 0; base < p.R; base += 64) {
+      const int i = base + lane;
+      int n_parts = 0, n_tiles = 0;
+      if (i < p.R) {
+        const TreeRequest t = tree_request(p, i);
+        n_parts = (int)(((int64_t)t.nodes * p.G + ROWS - 1) / ROWS);
+        n_tiles = max((t.len + TK - 1) / TK, 1);   // (a request without tokens has a tile in which nothing is seen)
+      }
+      const int64_t ct = tree_scan((int64_t)n_parts * n_tiles, lane) + tiles, cp = tree_scan(n_parts, lane) + parts;
+      if (i < p.R) {
+        cum[i] = ct;
+        first[i] = (int)cp;
+      }
+      tiles = __shfl(ct, 63, 64);
+      parts = __shfl(cp, 63, 64);
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.pairs = first[p.R - 1];
+
+  // rows behind the last request are zeros
+  if (p.last_slice) {
+    const int tq = min(max(p.cu_q[p.R], 0), p.T);
+    const int64_t per_row = (int64_t)p.Hq * HD / 8, all = (int64_t)(p.T - tq) * per_row;
+    const int64_t step = (int64_t)gridDim.x * gridDim.y * blockDim.x;
+    for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < all; i += step) {
+      const int64_t row = i / per_row;
+      const int e = (int)(i - row * per_row) * 8;
+      st16(p.out + (tq + row) * p.o_st + (int64_t)(e / HD) * p.o_sh + e % HD, make_uint4(0, 0, 0, 0));
+    }
+  }
+
+  // The span: equal shares where the tiles fill the grid, otherwise few tiles each -- a span's tiles follow one another,
+  // every further span of a pair is one more partial to merge.
+  const int64_t total = cum[p.R - 1];
+  const int pairs = first[p.R - 1];
+  if (total == 0) return;
+  const int span = max(1, (int)rintf(__builtin_amdgcn_sqrtf(0.035f * (float)total * __builtin_amdgcn_rcpf((float)pairs))));
+  int64_t t0, t1;
+  if (total >= (int64_t)p.grid * span) {
+    const int64_t per = total / p.grid;
+    const int rem = (int)(total - per * p.grid);
+    t0 = blockIdx.x * per + min((int)blockIdx.x, rem);
+    t1 = t0 + per + ((int)blockIdx.x < rem ? 1 : 0);
+  } else {
+    t0 = (int64_t)blockIdx.x * span;
+    t1 = min(t0 + span, total);
+  }
+  if (t0 >= t1) return;
+  int lo = 0, hi = p.R - 1;   // the first request whose tiles reach beyond t0
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cum[mid] > t0) hi = mid; else lo = mid + 1;
+  }
+  for (int r = lo; t0 < t1 && r < p.R; ++r) {
+    const int64_t rb = r ? cum[r - 1] : 0, re = cum[r];
+    if (t0 >= re) continue;
+    const TreeRequest t = tree_request(p, r);
+    const int tiles = max((t.len + TK - 1) / TK, 1);
+    TreeSegment s;
+    s.r = r; s.q_begin = t.q_begin; s.nodes = t.nodes; s.len = t.len; s.ctx = t.len - t.nodes;
+    while (t0 < t1 && t0 < re) {
+      s.part = __builtin_amdgcn_readfirstlane((int)((t0 - rb) / tiles));
+      const int tb = (int)(t0 - rb - (int64_t)s.part * tiles), te = (int)min((int64_t)tiles, tb + (t1 - t0));
+      const bool begins = tb == 0, ends = te == tiles;
+      s.start = tb * TK;
+      s.end = min(te * TK, t.len);
+      s.whole = begins && ends;
+      s.slot = 2 * blockIdx.x + (begins ? 1 : 0);
+      if (wave == 0 && lane == 0 && blockIdx.y == 0) {
+        int4* info = p.pair_info + ((r ? first[r - 1] : 0) + s.part);
+        if (begins) {
+          info->x = blockIdx.x;
+          info->z = r;
+          info->w = s.part;
+        }
+        if (ends) info->y = blockIdx.x;
+      }
+      tree_segment<HD, NT, NQ, FP8, F16>(p, s, h, lane);
+      t0 += te - tb;
+    }
+  }
+}
+
+// One workgroup per (request, part) and KV head: sum of its partials, weighted by 2^(lse - max).  A thread owns four
+// neighbouring values of a row.
+template <bool F16>
+__global__ __launch_bounds__(256) void paged_tree_merge_kernel(TreeParams p, int head_dim, int rows) {
+  const int pair = blockIdx.x, h = blockIdx.y;
+  if (pair >= *p.pairs) return;
+  const int4 info = p.pair_info[pair];
+  if (info.x == info.y) return;   // written by the streaming kernel
+  const TreeRequest t = tree_request(p, info.z);
+  const int cols = head_dim >> 2;
+  for (int i = threadIdx.x; i < rows * cols; i += blockDim.x) {
+    const int row = i / cols, d = 4 * (i - row * cols);
+    const int n = info.w * rows + row, qi = tree_div_g(p, n);
+    if (qi >= t.nodes) return;
+    float mx = -INFINITY, den = 0.f;
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w0 = info.x; w0 <= info.y; w0 += 4) {
+      float lse[4];
+      float4 po[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int w = min(w0 + j, info.y);
+        const int64_t at = ((int64_t)(2 * w + (w == info.x ? 1 : 0)) * p.Hkv + h) * rows + row;
+        lse[j] = p.part_lse[at];
+        po[j] = *reinterpret_cast<const float4*>(p.part_o + at * head_dim + d);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (w0 + j <= info.y && lse[j] != -INFINITY) {   // (a partial that saw nothing)
+          const float m = fmaxf(mx, lse[j]);
+          const float a = fast_exp2(mx - m), b = fast_exp2(lse[j] - m);
+          num.x = num.x * a + b * po[j].x; num.y = num.y * a + b * po[j].y;
+          num.z = num.z * a + b * po[j].z; num.w = num.w * a + b * po[j].w;
+          den = den * a + b;
+          mx = m;
+        }
+      }
+    }
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    uint16_t* o = p.out + (int64_t)(t.q_begin + qi) * p.o_st + (int64_t)(h * p.G + n - qi * p.G) * p.o_sh + d;
+    st8(o, make_uint2(pack2<F16>(num.x * inv, num.y * inv), pack2<F16>(num.z * inv, num.w * inv)));
+  }
+}
+
+// Wavefronts per workgroup (neighbouring KV heads), workgroups along the tiles, rows of a part.
+struct TreeShape {
+  int waves, grid, rows;
+};
+static TreeShape tree_shape(int Hkv, int head_dim) {
+  TreeShape s;
+  s.waves = 1;
+  for (int w = 2; w <= 8; ++w)
+    if (Hkv % w == 0) s.waves = w;
+  s.grid = device_cu_count() * (8 / s.waves) / (Hkv / s.waves);
+  if (s.grid < 1) s.grid = 1;
+  s.rows = head_dim > 128 ? 16 : 32;
+  return s;
+}
+static int64_t tree_align(int64_t n) { return (n + 255) & ~(int64_t)255; }
+static int64_t tree_most_pairs(int T, int R, int G, int rows) {
+  const int64_t n = R < kTreeRequestsPerLaunch ? R : kTreeRequestsPerLaunch;
+  return (int64_t)T * G / rows + n;
+}
+
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" int64_t mi_tree_workspace_bytes(int32_t T, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim) {
+  if (T <= 0 || R <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0) return 0;
+  const TreeShape s = tree_shape(Hkv, head_dim);
+  const int64_t rows = (int64_t)2 * s.grid * Hkv * s.rows;
+  return 256 + tree_align(16 * tree_most_pairs(T, R, Hq / Hkv, s.rows)) + tree_align(rows * 4) + rows * head_dim * 4;
+}
+
+extern "C" int mi_paged_tree_attention(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache, const void* v_cache,
+    int64_t kv_stride_chunk, int64_t kv_stride_tok, int64_t kv_stride_head, int32_t n_chunks, int32_t kv_dtype,
+    const float* k_scales, const float* v_scales, const int32_t* block_table, int64_t bt_stride, int32_t table_columns,
+    const int32_t* cu_seqlens_q, const int32_t* kv_lens, const int64_t* tree_mask, int64_t mask_stride,
+    int32_t mask_words, void* out, int64_t o_stride_tok, int64_t o_stride_head, void* workspace, int64_t workspace_bytes,
+    int32_t T, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t chunk_tokens, float softmax_scale,
+    int32_t dtype, void* stream) {
+  if (T == 0) return MI_OK;
+  if (dtype != MI_DTYPE_BF16 && dtype != MI_DTYPE_FP16)
+    return mi_fail(MI_ERR_UNSUPPORTED, "mi_paged_tree_attention: dtype must be MI_DTYPE_BF16 or MI_DTYPE_FP16");
+  if (!q || !k_cache || !v_cache || !block_table || !cu_seqlens_q || !kv_lens || !tree_mask || !out)
+    return mi_fail(MI_ERR_NULL, "mi_paged_tree_attention: null pointer argument");
+  if (T < 0 || R <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hkv > 65535)
+    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: need T >= 0, R > 0 and Hq a multiple of Hkv");
+  const int G = Hq / Hkv;
+  if (G > 64) return mi_fail(MI_ERR_UNSUPPORTED, "mi_paged_tree_attention: at most 64 query heads per KV head");
+  if ((int64_t)T * G >= (int64_t)1 << 31 || (int64_t)T * G / 16 + R >= (int64_t)1 << 31)
+    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: too many rows");
+  const bool fp8 = kv_dtype == MI_KV_FP8_E4M3;
+  if (!fp8 && kv_dtype != MI_KV_16BIT) return mi_fail(MI_ERR_UNSUPPORTED, "mi_paged_tree_attention: unknown kv_dtype");
+  if (head_dim != 64 && head_dim != 96 && head_dim != 128 && head_dim != 192 && head_dim != 256)
+    return mi_fail(MI_ERR_UNSUPPORTED, "mi_paged_tree_attention: head_dim must be 64, 96, 128, 192 or 256");
+  if (fp8 && head_dim != 64 && head_dim != 128)
+    return mi_fail(MI_ERR_UNSUPPORTED, "mi_paged_tree_attention: an fp8 cache needs head_dim 64 or 128");
+  if (fp8 && (!k_scales || !v_scales)) return mi_fail(MI_ERR_NULL, "mi_paged_tree_attention: an fp8 cache needs both scale arrays");
+  if (chunk_tokens <= 0 || chunk_tokens % 16)
+    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: chunk size must be a positive multiple of 16");
+  if (n_chunks <= 0 || table_columns <= 0 || (int64_t)table_columns * chunk_tokens > 0x7fffff00)
+    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: need a cache, and a block table of fewer than 2^31 tokens a row");
+  if ((int64_t)table_columns * chunk_tokens * chunk_tokens >= (int64_t)1 << 40)   // (the reciprocal that finds a chunk)
+    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: tokens a row times chunk size must stay below 2^40");
+  if (mask_words < 1 || mask_words > 4 || mask_stride < mask_words)
+    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: a row of the mask has 1 to 4 words");
+  const int esz = fp8 ? 1 : 2;
+  if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15)
+    return mi_fail(MI_ERR_ALIGN, "mi_paged_tree_attention: q/k/v/out must be 16-byte aligned");
+  if ((q_stride_tok | q_stride_head | o_stride_tok | o_stride_head) % 8 ||
+      ((kv_stride_chunk | kv_stride_tok | kv_stride_head) * esz) % 16)
+    return mi_fail(MI_ERR_ALIGN, "mi_paged_tree_attention: strides must keep rows 16-byte aligned");
+  if (kv_stride_tok < 0 || kv_stride_head < 0 || kv_stride_head > 0x7fffffff || kv_stride_tok * (int64_t)chunk_tokens * esz >= (int64_t)1 << 31)
+    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: one chunk must span less than 2 GiB");
+  if (!(softmax_scale > 0.f)) return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: softmax_scale must be positive");
+  if (!workspace || workspace_bytes < mi_tree_workspace_bytes(T, R, Hq, Hkv, head_dim))
+    return mi_fail(MI_ERR_WORKSPACE, "mi_paged_tree_attention: workspace too small (see mi_tree_workspace_bytes)");
+  if ((uintptr_t)workspace & 15) return mi_fail(MI_ERR_ALIGN, "mi_paged_tree_attention: workspace must be 16-byte aligned");
+
+  const TreeShape shape = tree_shape(Hkv, head_dim);
+  const bool f16 = dtype == MI_DTYPE_FP16;
+  TreeParams p;
+  p.q = (const uint16_t*)q; p.q_st = q_stride_tok; p.q_sh = q_stride_head;
+  p.kc = (const uint8_t*)k_cache; p.vc = (const uint8_t*)v_cache;
+  p.kv_sc = kv_stride_chunk; p.kv_st = (int32_t)kv_stride_tok; p.kv_sh = (int32_t)kv_stride_head;
+  p.bt = block_table; p.bt_stride = bt_stride;
+  p.mask = (const uint32_t*)tree_mask; p.mask_st = 2 * mask_stride; p.mask_words = 2 * mask_words;
+  p.out = (uint16_t*)out; p.o_st = o_stride_tok; p.o_sh = o_stride_head;
+  uint8_t* ws = (uint8_t*)workspace;
+  const int64_t rows = (int64_t)2 * shape.grid * Hkv * shape.rows;
+  p.pairs = (int32_t*)ws;
+  p.pair_info = (int4*)(ws + 256);
+  ws += 256 + tree_align(16 * tree_most_pairs(T, R, G, shape.rows));
+  p.part_lse = (float*)ws;
+  p.part_o = (float*)(ws + tree_align(rows * 4));
+  p.k_scale = k_scales; p.v_scale = v_scales;
+  p.chunk_magic = (((uint64_t)1 << 40) + chunk_tokens - 1) / chunk_tokens;
+  p.g_magic = G == 1 ? 0u : (uint32_t)(((uint64_t)1 << 32) / G + 1);
+  p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = G; p.chunk = chunk_tokens; p.n_chunks = n_chunks; p.table_cols = table_columns;
+  p.grid = shape.grid; p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid(shape.grid, Hkv / shape.waves), block(64 * shape.waves);
+  const bool wide = head_dim > 128;
+  // tokens of a tile: 32, 16 of wide heads, 64 of an fp8 cache with narrow ones (what the registers hold in flight); a tile
+  // lies in one chunk
+  const int nt = wide || chunk_tokens % 32 ? 1 : fp8 && head_dim == 64 && chunk_tokens % 64 == 0 ? 4 : 2;
+  for (int r0 = 0; r0 < R; r0 += kTreeRequestsPerLaunch) {
+    p.r_base = r0;
+    p.R = R - r0 < kTreeRequestsPerLaunch ? R - r0 : kTreeRequestsPerLaunch;
+    p.cu_q = cu_seqlens_q + r0; p.lens = kv_lens + r0;
+    p.last_slice = r0 + p.R == R;
+    const size_t lds = (size_t)p.R * (sizeof(int64_t) + sizeof(int32_t));
+#define MI_TREE(HD_, NT_, NQ_, FP8_)                                                                                   \
+    do {                                                                                                               \
+      if (f16) hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, true>), grid, block, lds, st, p);            \
+      else hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, false>), grid, block, lds, st, p);               \
+    } while (0)
+#define MI_TREE_16(HD_)                                                                                                \
+    do {                                                                                                               \
+      if (nt == 1) MI_TREE(HD_, 1, 2, false);                                                                          \
+      else MI_TREE(HD_, 2, 2, false);                                                                                  \
+    } while (0)
+#define MI_TREE_8(HD_)                                                                                                 \
+    do {                                                                                                               \
+      if (nt == 1) MI_TREE(HD_, 1, 2, true);                                                                           \
+      else MI_TREE(HD_, 2, 2, true);                                                                                   \
+    } while (0)
+    if (fp8 && nt == 4) MI_TREE(64, 4, 2, true);
+    else if (fp8 && head_dim == 64) MI_TREE_8(64);
+    else if (fp8) MI_TREE_8(128);
+    else if (head_dim == 64) MI_TREE_16(64);
+    else if (head_dim == 96) MI_TREE_16(96);
+    else if (head_dim == 128) MI_TREE_16(128);
+    else if (head_dim == 192) MI_TREE(192, 1, 1, false);
+    else MI_TREE(256, 1, 1, false);
+#undef MI_TREE_8
+#undef MI_TREE_16
+#undef MI_TREE
+    const dim3 mgrid((unsigned)tree_most_pairs(T, p.R, G, shape.rows), Hkv);
+    if (f16) hipLaunchKernelGGL((paged_tree_merge_kernel<true>), mgrid, dim3(256), 0, st, p, head_dim, shape.rows);
+    else hipLaunchKernelGGL((paged_tree_merge_kernel<false>), mgrid, dim3(256), 0, st, p, head_dim, shape.rows);
+  }
+  return mi_check_launch("mi_paged_tree_attention");
+}

@@ -1,0 +1,754 @@
+// Verification of drafted tokens and the move of the accepted nodes' cache rows (gfx950).
+//
+// Every request brings a tree of drafted tokens (see paged_tree.hip for the attention over it): row i of the logits is
+// the target's view of what follows node i, parents[i] the node (inside the request) that token i was drafted after.
+//
+// Verification walks each tree from its root.  With p the target's distribution at a node (softmax of logits /
+// temperature over the values that reach `cut`), the node's children are tried in order:
+//   * draft probabilities q (the distribution that the children were drawn from, one row per node): a child with token t is
+//     accepted where u q(t) < p_j(t), and after a rejection p_{j+1} = (p_j - q)+, normalised.  Written out this is
+//       p_j = (p - c_j q)+ / n_j,   c_0 = 0, n_0 = 1,   c_{j+1} = c_j + n_j,   n_{j+1} = sum (p - c_{j+1} q)+,
+//     so a node needs two numbers besides p and q, however often it was rejected;
+//   * without them (tokens that the draft chose rather than drew): accepted where u < p_j(t), and a rejected token leaves
+//     the distribution;
+//   * greedy: accepted where t is the largest logit's index.
+// The first accepted child is the next node; where there is none the request's last token is drawn from what is left by an
+// inverse CDF in vocabulary order, so that the tokens are distributed as the target's own draws would be.
+//
+// Tokens are whole numbers picked at borders of long sums, so exponentials and sums are 64-bit: one rounding of a 32-bit
+// cumulative sum (6e-8) is as wide as the whole share of many a token of a 128 k vocabulary.  The exponential is a table of
+// 2^(i/128) in LDS and a polynomial of degree 4 (relative error 1e-15).
+#include <type_traits>
+
+#include "mi_capi_internal.h"
+#include "mi_common.h"
+
+namespace mi {
+
+constexpr int kVerifyThreads = 256;
+constexpr int kVerifyNodes = 1024;    // nodes of a request that are looked at: what the walk holds in LDS
+constexpr int kVerifyMostParts = 64;
+constexpr int kVerifyPart = 8192;     // elements of a part, at most (their weights lie in LDS for the draw)
+
+struct VerifyPartial {   // of one part of a row
+  double sum;            // of exp(x - max); greedy: unused
+  float max;
+  int32_t index;         // greedy: the first place of the maximum
+};
+struct VerifyState {     // what the walk hands the draw
+  double c;              // weights are (p - c q)+
+  int32_t row;           // the last node's row, -1: the request is empty
+  int32_t tested;        // whether its children were tried
+};
+
+struct VerifyParams {
+  const uint8_t* logits; int64_t stride;   // bytes between rows
+  const uint8_t* draft; int64_t draft_stride; int32_t draft_dtype;
+  const int64_t* tokens;
+  const int32_t* parents;
+  const int32_t* cu;
+  const float* uniform;
+  const float* cut;
+  int64_t* out_tokens; int32_t* out_rows; int32_t* out_counts;
+  VerifyPartial* partial;    // [T][parts]
+  double* residual;          // [R][parts]
+  VerifyState* state;        // [R]
+  int32_t T, R, V, max_path, parts, part;   // part: elements, a multiple of 8
+  float inv_temperature; int32_t scaled;
+};
+
+constexpr double kLog2e = 1.4426950408889634074;
+
+// The table of 2^(i / 128), filled by the workgroup.
+static __device__ __forceinline__ void fill_exp_table(double* table) {
+  for (int i = threadIdx.x; i < 128; i += blockDim.x) table[i] = exp2(i * (1.0 / 128));
+}
+// 2^t for t <= 0 (far below zero: 0; NaN: 0)
+static __device__ __forceinline__ double table_exp2(const double* table, double t) {
+  constexpr double kMagic = 1.5 * 35184372088832.0;   // 1.5 2^45: an addition rounds to multiples of 1/128
+  t = fmax(t, -2000.0);
+  const double u = t + kMagic;
+  const double r = (t - (u - kMagic)) * 0.69314718055994530942;
+  const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, u);
+  double y = __builtin_fma(r, 1.0 / 24, 1.0 / 6);
+  y = __builtin_fma(r, y, 0.5);
+  y = __builtin_fma(r, y, 1.0);
+  y = __builtin_fma(r, y, 1.0);
+  return __builtin_ldexp(table[k & 127] * y, k >> 7);
+}
+
+static __device__ __forceinline__ float load_element(const uint8_t* row, int dtype, int i) {
+  if (dtype == 0) return reinterpret_cast<const float*>(row)[i];
+  const uint16_t x = reinterpret_cast<const uint16_t*>(row)[i];
+  return dtype == 1 ? bf16_to_f32(x) : to_f32<true>(x);
+}
+
+// Eight elements e0 .. e0 + 7 of a row, `fill` outside [0, V): 16-byte loads where they are aligned and inside.
+template <int DT>
+static __device__ __forceinline__ void load8(const uint8_t* row, int e0, int V, float fill, float (&x)[8]) {
+  constexpr int ES = DT == 0 ? 4 : 2;
+  const uint8_t* at = row + (int64_t)e0 * ES;
+  if (e0 >= 0 && e0 + 8 <= V && !((uintptr_t)at & 15)) {
+    const uint4 a = ld16(at);
+    if constexpr (DT == 0) {
+      const uint4 b = ld16(at + 16);
+      x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
+      x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
+    } else {
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[2 * j] = lo_to_f32<DT == 2>(w[j]);
+        x[2 * j + 1] = hi_to_f32<DT == 2>(w[j]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = e0 + j >= 0 && e0 + j < V ? load_element(row, DT, e0 + j) : fill;
+  }
+}
+static __device__ __forceinline__ void load8_any(const uint8_t* row, int dtype, int e0, int V, float fill, float (&x)[8]) {
+  if (dtype == 0) load8<0>(row, e0, V, fill, x);
+  else if (dtype == 1) load8<1>(row, e0, V, fill, x);
+  else load8<2>(row, e0, V, fill, x);
+}
+
+// A row of logits cut into parts of `part` elements.  Parts are counted from the last 16-byte line at or before the row's
+// first element, so that the groups of eight are aligned whatever the row's own address: element e lies at place e + shift.
+template <int DT>
+struct VerifyRow {
+  const uint8_t* row;
+  int shift;
+  float cut;
+  __device__ __forceinline__ VerifyRow(const VerifyParams& p, int i) {
+    row = p.logits + (int64_t)i * p.stride;
+    shift = (int)((uintptr_t)row & 15) / (DT == 0 ? 4 : 2);
+    cut = p.cut ? p.cut[i] : -INFINITY;
+  }
+  // a logit as the sampler sees it: times the reciprocal of the temperature, rounded to the logits' type; -inf: left out
+  __device__ __forceinline__ float finish(const VerifyParams& p, float x) const {
+    if (p.scaled) {
+      x *= p.inv_temperature;
+      if (DT != 0) x = to_f32<DT == 2>(f32_to_16<DT == 2>(x));
+    }
+    return x < cut ? -INFINITY : x;
+  }
+  __device__ __forceinline__ float at(const VerifyParams& p, int e) const { return finish(p, load_element(row, DT, e)); }
+};
+
+static __device__ __forceinline__ double wave_sum_f64(double x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
+  return x;
+}
+static __device__ __forceinline__ float wave_max_f32(float x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
+  return x;
+}
+
+// Maximum and sum of exponentials (greedy: maximum and its first place) of one part of one row.
+template <int DT, bool GREEDY>
+__global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParams p) {
+  __shared__ double table[128];
+  __shared__ double sums[4];
+  __shared__ float tops[4];
+  __shared__ int places[4];
+  const int part = blockIdx.y, row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (!GREEDY) fill_exp_table(table);
+  __syncthreads();
+  const VerifyRow<DT> rd(p, row);
+  const int begin = part * p.part - rd.shift, end = min(begin + p.part, p.V);
+  float top = -INFINITY;
+  int place = 0x7fffffff;
+  double sum = 0;
+  for (int e0 = begin + 8 * (int)threadIdx.x; e0 < end; e0 += 8 * kVerifyThreads) {
+    float x[8];
+    load8<DT>(rd.row, e0, p.V, -INFINITY, x);
+    if constexpr (GREEDY) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if ((x[j] > top || place == 0x7fffffff) && e0 + j >= 0 && e0 + j < p.V && x[j] == x[j]) {
+          top = x[j];
+          place = e0 + j;
+        }
+    } else {
+      float m = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = rd.finish(p, x[j]);
+        m = fmaxf(m, x[j]);
+      }
+      if (m > top) {
+        sum *= table_exp2(table, ((double)top - m) * kLog2e);
+        top = m;
+      }
+      if (top > -INFINITY) {
+        const double ref = -(double)top * kLog2e;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += table_exp2(table, __builtin_fma((double)x[j], kLog2e, ref));
+      }
+    }
+  }
+  float all = wave_max_f32(top);
+  if constexpr (GREEDY) {
+    int best = top == all ? place : 0x7fffffff;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
+    if (lane == 0) { tops[wave] = all; places[wave] = best; }
+  } else {
+    double s = all > -INFINITY ? sum * table_exp2(table, ((double)top - all) * kLog2e) : 0.0;
+    s = wave_sum_f64(s);
+    if (lane == 0) { tops[wave] = all; sums[wave] = s; }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    VerifyPartial o;
+    o.sum = 0; o.max = -INFINITY; o.index = 0x7fffffff;
+    for (int w = 0; w < 4; ++w) o.max = fmaxf(o.max, tops[w]);
+    for (int w = 0; w < 4; ++w) {
+      if (GREEDY) { if (tops[w] == o.max) o.index = min(o.index, places[w]); }
+      else if (tops[w] > -INFINITY) o.sum += sums[w] * table_exp2(table, ((double)tops[w] - o.max) * kLog2e);
+    }
+    p.partial[(int64_t)row * p.parts + part] = o;
+  }
+}
+
+// Sum over the workgroup, in every thread.
+static __device__ __forceinline__ double block_sum(double x, double* scratch) {
+  x = wave_sum_f64(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;
+  __syncthreads();
+  double s = 0;
+  for (int w = 0; w < (int)(blockDim.x >> 6); ++w) s += scratch[w];
+  return s;
+}
+
+// The walk of one request's tree, one workgroup each.
+constexpr int kWalkThreads = 1024;
+enum { kGreedy = 0, kTarget = 1, kDraft = 2 };
+template <int DT, int MODE>
+__global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams p) {
+  __shared__ double table[128];
+  __shared__ double scratch[kWalkThreads / 64];
+  __shared__ double prob[kVerifyNodes], sum_s[kVerifyNodes];
+  __shared__ float top_s[kVerifyNodes], q_s[kVerifyNodes];
+  __shared__ int32_t parent[kVerifyNodes], token[kVerifyNodes], after[kVerifyNodes];
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const int begin = min(max(p.cu[r], 0), p.T), n = min(min(max(p.cu[r + 1], begin), p.T) - begin, kVerifyNodes);
+  int32_t* const rows = p.out_rows + (int64_t)r * p.max_path;
+  int64_t* const out = p.out_tokens + (int64_t)r * p.max_path;
+  for (int i = tid; i < p.max_path; i += kWalkThreads) {
+    rows[i] = -1;
+    out[i] = -1;
+  }
+  if (n <= 0) {
+    if (tid == 0) {
+      p.out_counts[r] = 0;
+      p.state[r] = VerifyState{0, -1, 0};
+    }
+    return;
+  }
+  fill_exp_table(table);
+  __syncthreads();
+  for (int i = tid; i < n; i += kWalkThreads) {
+    const VerifyPartial* part = p.partial + (int64_t)(begin + i) * p.parts;
+    float top = -INFINITY;
+    for (int k = 0; k < p.parts; ++k) top = fmaxf(top, part[k].max);
+    top_s[i] = top;
+    if (MODE == kGreedy) {
+      int best = 0x7fffffff;
+      for (int k = 0; k < p.parts; ++k)
+        if (part[k].max == top) best = min(best, part[k].index);
+      token[i] = best;   // (of the row, here)
+    } else {
+      double s = 0;
+      for (int k = 0; k < p.parts; ++k)
+        if (part[k].max > -INFINITY) s += part[k].sum * table_exp2(table, ((double)part[k].max - top) * kLog2e);
+      sum_s[i] = s;
+    }
+    after[i] = 0x7fffffff;
+    const int up = p.parents[begin + i];
+    parent[i] = i > 0 && up >= 0 && up < i ? up : -1;
+  }
+  __syncthreads();
+  if (MODE == kGreedy) {
+    for (int i = tid; i < n; i += kWalkThreads)
+      if (parent[i] >= 0 && p.tokens[begin + i] == token[parent[i]]) atomicMin(&after[parent[i]], i);
+  } else {
+    for (int i = tid; i < n; i += kWalkThreads) {
+      const int64_t t = p.tokens[begin + i];
+      const bool inside = t >= 0 && t < p.V;
+      token[i] = inside ? (int)t : -1;
+      prob[i] = 0;
+      q_s[i] = 0;
+      if (parent[i] >= 0 && inside) {
+        const int up = parent[i];
+        const VerifyRow<DT> rd(p, begin + up);
+        const float x = rd.at(p, (int)t);
+        if (sum_s[up] > 0) prob[i] = table_exp2(table, ((double)x - top_s[up]) * kLog2e) / sum_s[up];
+        if (MODE == kDraft) q_s[i] = load_element(p.draft + (int64_t)(begin + up) * p.draft_stride, p.draft_dtype, (int)t);
+      }
+    }
+  }
+  __syncthreads();
+  if (MODE == kTarget) {
+    // a token that an earlier sibling had has left the distribution
+    bool again = false;
+    double before = 0;
+    const int i = tid;   // (kVerifyNodes == kWalkThreads)
+    const int up = i < n ? parent[i] : -1;
+    if (up >= 0)
+      for (int j = up + 1; j < i; ++j) again |= parent[j] == up && token[j] == token[i];
+    __syncthreads();
+    if (again) prob[i] = 0;
+    __syncthreads();
+    if (up >= 0) {
+      for (int j = up + 1; j < i; ++j) before += parent[j] == up ? prob[j] : 0.0;
+      if ((double)p.uniform[begin + i] * (1.0 - before) < prob[i]) atomicMin(&after[up], i);
+    }
+    __syncthreads();
+  }
+  static_assert(kVerifyNodes == kWalkThreads, "a node to a thread");
+  if (MODE != kDraft) {
+    if (tid == 0) {
+      int at = 0, count = 1;
+      rows[0] = begin;
+      while (count < p.max_path && after[at] < n) {
+        at = after[at];
+        out[count - 1] = p.tokens[begin + at];
+        rows[count++] = begin + at;
+      }
+      p.out_counts[r] = count;
+      if (MODE == kGreedy) out[count - 1] = token[at] == 0x7fffffff ? 0 : token[at];
+      else p.state[r] = VerifyState{0, begin + at, count < p.max_path};
+    }
+    return;
+  }
+  // Draft probabilities: the rejections of a node's earlier children decide what a later one is held against.
+  int at = 0, count = 1;
+  double c = 0;
+  if (tid == 0) rows[0] = begin;
+  while (count < p.max_path) {
+    c = 0;
+    double left = 1;
+    int next = -1;
+    int child = -1;
+    for (int i = at + 1; i < n && child < 0; ++i)
+      if (parent[i] == at) child = i;
+    while (child >= 0) {
+      const double q = q_s[child], w = prob[child] - c * q;
+      if ((double)p.uniform[begin + child] * left * q < w) {
+        next = child;
+        break;
+      }
+      c += left;
+      int following = -1;
+      for (int i = child + 1; i < n && following < 0; ++i)
+        if (parent[i] == at) following = i;
+      if (following >= 0) {   // (what is left matters to a sibling; the draw makes its own sum)
+        const VerifyRow<DT> rd(p, begin + at);
+        const uint8_t* qr = p.draft + (int64_t)(begin + at) * p.draft_stride;
+        const double ref = -(double)top_s[at] * kLog2e, inv = 1.0 / sum_s[at];
+        double s = 0;
+        for (int e0 = 8 * tid - rd.shift; e0 < p.V; e0 += 8 * kWalkThreads) {
+          float x[8], y[8];
+          load8<DT>(rd.row, e0, p.V, -INFINITY, x);
+          load8_any(qr, p.draft_dtype, e0, p.V, 0.f, y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            s += fmax(table_exp2(table, __builtin_fma((double)rd.finish(p, x[j]), kLog2e, ref)) * inv - c * (double)y[j], 0.0);
+        }
+        left = block_sum(s, scratch);
+      }
+      child = following;
+    }
+    if (next < 0) break;
+    at = next;
+    if (tid == 0) {
+      out[count - 1] = p.tokens[begin + at];
+      rows[count] = begin + at;
+    }
+    ++count;
+  }
+  if (tid == 0) {
+    p.out_counts[r] = count;
+    p.state[r] = VerifyState{c, begin + at, count < p.max_path};
+  }
+}
+
+// Maximum and sum of a row from its parts, in every thread of the workgroup.
+struct RowTotal {
+  float top;
+  double sum;
+};
+static __device__ __forceinline__ RowTotal row_total(const VerifyParams& p, const double* table, int row) {
+  const VerifyPartial* part = p.partial + (int64_t)row * p.parts;
+  RowTotal t{-INFINITY, 0};
+  for (int k = 0; k < p.parts; ++k) t.top = fmaxf(t.top, part[k].max);
+  for (int k = 0; k < p.parts; ++k)
+    if (part[k].max > -INFINITY) t.sum += part[k].sum * table_exp2(table, ((double)part[k].max - t.top) * kLog2e);
+  return t;
+}
+
+// Draft probabilities: what is left of one part of the last node's distribution, sum (p - c q)+.
+template <int DT>
+__global__ __launch_bounds__(kVerifyThreads) void verify_left_kernel(VerifyParams p) {
+  __shared__ double table[128];
+  __shared__ double scratch[kVerifyThreads / 64];
+  const int part = blockIdx.y, r = blockIdx.x;
+  const VerifyState st = p.state[r];
+  if (st.row < 0) return;
+  fill_exp_table(table);
+  __syncthreads();
+  const RowTotal t = row_total(p, table, st.row);
+  const VerifyRow<DT> rd(p, st.row);
+  const uint8_t* qr = p.draft + (int64_t)st.row * p.draft_stride;
+  const int begin = part * p.part - rd.shift, end = min(begin + p.part, p.V);
+  const double ref = -(double)t.top * kLog2e, inv = 1.0 / t.sum;
+  double s = 0;
+  for (int e0 = begin + 8 * (int)threadIdx.x; e0 < end; e0 += 8 * kVerifyThreads) {
+    float x[8], y[8];
+    load8<DT>(rd.row, e0, p.V, -INFINITY, x);
+    load8_any(qr, p.draft_dtype, e0, p.V, 0.f, y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      s += fmax(table_exp2(table, __builtin_fma((double)rd.finish(p, x[j]), kLog2e, ref)) * inv - st.c * (double)y[j], 0.0);
+  }
+  s = block_sum(s, scratch);
+  if (threadIdx.x == 0) p.residual[(int64_t)r * p.parts + part] = s;
+}
+
+// The draw of a request's last token: the part that holds it, then the place inside the part.
+template <int DT, int MODE>
+__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyParams p) {
+  __shared__ double table[128];
+  __shared__ double scratch[kVerifyThreads / 64];
+  __shared__ double mass[kVerifyMostParts];
+  __shared__ double weight[kVerifyPart];
+  __shared__ double before[kVerifyThreads];
+  __shared__ int found[3];
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const VerifyState st = p.state[r];
+  if (st.row < 0) return;
+  fill_exp_table(table);
+  __syncthreads();
+  const int begin = min(max(p.cu[r], 0), p.T), n = min(min(max(p.cu[r + 1], begin), p.T) - begin, kVerifyNodes);
+  const int node = st.row - begin;
+  const VerifyRow<DT> rd(p, st.row);
+  const RowTotal t = row_total(p, table, st.row);
+  const double ref = -(double)t.top * kLog2e, inv = 1.0 / t.sum;
+  auto chance = [&](float x) { return table_exp2(table, __builtin_fma((double)x, kLog2e, ref)) * inv; };
+  auto whole_mass = [&](int k) {
+    const VerifyPartial q = p.partial[(int64_t)st.row * p.parts + k];
+    return q.max > -INFINITY ? q.sum * table_exp2(table, ((double)q.max - t.top) * kLog2e) * inv : 0.0;
+  };
+  for (int k = tid; k < p.parts; k += kVerifyThreads)
+    mass[k] = MODE == kDraft && st.tested ? p.residual[(int64_t)r * p.parts + k] : whole_mass(k);
+  __syncthreads();
+  // tokens that the rejected children took out: each once
+  auto removed = [&](auto f) {
+    if (MODE != kTarget || !st.tested) return;
+    for (int i = node + 1 + tid; i < n; i += kVerifyThreads) {
+      if (p.parents[begin + i] != node) continue;
+      const int64_t tok = p.tokens[begin + i];
+      bool first = tok >= 0 && tok < p.V;
+      for (int j = node + 1; j < i && first; ++j) first = !(p.parents[begin + j] == node && p.tokens[begin + j] == tok);
+      if (first) f((int)tok);
+    }
+  };
+  removed([&](int tok) { atomicAdd(&mass[(tok + rd.shift) / p.part], -chance(rd.at(p, tok))); });
+  __syncthreads();
+  double total = 0;
+  for (int k = 0; k < p.parts; ++k) total += fmax(mass[k], 0.0);
+  // Rejections that leave nothing (a target equal to the draft's, or smaller everywhere that it is kept, up to rounding):
+  // the last token comes from the target itself.
+  const bool nothing = !(total > 1e-13);
+  __syncthreads();
+  if (nothing) {
+    for (int k = tid; k < p.parts; k += kVerifyThreads) mass[k] = whole_mass(k);
+    __syncthreads();
+    total = 0;
+    for (int k = 0; k < p.parts; ++k) total += mass[k];
+  }
+  const double want = (double)p.uniform[begin] * total;
+  if (tid == 0) {
+    double sum = 0;
+    int k = 0, last = 0;
+    for (; k < p.parts; ++k) {
+      const double m = fmax(mass[k], 0.0);
+      if (m > 0) last = k;
+      if (sum + m > want) break;
+      sum += m;
+    }
+    if (k == p.parts) {   // (the sum's own rounding: the last part that has any)
+      k = last;
+      sum = want;
+    }
+    found[0] = k;
+    found[1] = 0x7fffffff;
+    found[2] = -1;
+    scratch[0] = sum;
+  }
+  __syncthreads();
+  const int part = found[0], first = part * p.part - rd.shift;
+  const double rest = want - scratch[0];
+  const uint8_t* qr = MODE == kDraft ? p.draft + (int64_t)st.row * p.draft_stride : nullptr;
+  for (int i = 8 * tid; i < p.part; i += 8 * kVerifyThreads) {
+    float x[8], y[8];
+    load8<DT>(rd.row, first + i, p.V, -INFINITY, x);
+    if (MODE == kDraft) load8_any(qr, p.draft_dtype, first + i, p.V, 0.f, y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      double w = chance(rd.finish(p, x[j]));
+      if (MODE == kDraft && st.tested && !nothing) w = fmax(w - st.c * (double)y[j], 0.0);
+      weight[i + j] = w;
+    }
+  }
+  __syncthreads();
+  if (!nothing)
+    removed([&](int tok) {
+      const int i = tok - first;
+      if (i >= 0 && i < p.part) weight[i] = 0;
+    });
+  __syncthreads();
+  // every thread a run of neighbours: their sum, the sums before it, then the place
+  const int run = (p.part + kVerifyThreads - 1) / kVerifyThreads, a = min(tid * run, p.part), b = min(a + run, p.part);
+  double mine = 0;
+  for (int i = a; i < b; ++i) mine += weight[i];
+  before[tid] = mine;
+  __syncthreads();
+  double sum = 0;
+  for (int k = 0; k < tid; ++k) sum += before[k];
+  int last = -1;
+  for (int i = a; i < b; ++i) {
+    if (weight[i] > 0) last = i;
+    sum += weight[i];
+    if (sum > rest && weight[i] > 0) {
+      atomicMin(&found[1], i);
+      break;
+    }
+  }
+  atomicMax(&found[2], last);
+  __syncthreads();
+  if (tid == 0) {
+    const int i = found[1] != 0x7fffffff ? found[1] : found[2];
+    p.out_tokens[(int64_t)r * p.max_path + p.out_counts[r] - 1] = min(max(first + i, 0), p.V - 1);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the cache afterwards
+struct KeepParams {
+  uint8_t* kc; uint8_t* vc;
+  int64_t layer_bytes, chunk_bytes; int64_t tok_bytes;
+  const float* k_scale; const float* v_scale; int64_t scale_layer;
+  const int32_t* bt; int64_t bt_stride;
+  const int32_t* rows; int64_t rows_stride;
+  const int32_t* counts; const int32_t* cu; const int32_t* lens;
+  int32_t* new_lens;
+  int32_t columns, chunk, n_chunks, table_cols, units, units_per_head, Hkv;
+};
+
+constexpr int kKeepBatch = 64;   // path entries whose places lie in LDS at a time
+constexpr int kKeepLoads = 8;    // rows in flight per thread
+
+// One workgroup per request, layer and cache: the accepted nodes' rows move to where the path puts them.  A path rises, so
+// node path[i] >= i lies at or behind its place i, and a place never lies on a node that a later entry still needs:
+// a thread reads a few rows of its 16-byte column, then writes them, from the front of the path to its end.
+template <bool FP8>
+__global__ __launch_bounds__(256) void kv_keep_kernel(KeepParams p) {
+  __shared__ int src_chunk[kKeepBatch], dst_chunk[kKeepBatch];   // -1: nothing moves
+  __shared__ int src_pos[kKeepBatch], dst_pos[kKeepBatch];
+  const int r = blockIdx.x, layer = blockIdx.y, tid = threadIdx.x;
+  const bool value = blockIdx.z != 0;
+  const int begin = p.cu[r], n = max(p.cu[r + 1] - begin, 0), len = p.lens[r];
+  const int count = min(max(p.counts[r], 0), p.columns);
+  if (layer == 0 && !value && tid == 0) p.new_lens[r] = len - n + count;
+  uint8_t* const cache = (value ? p.vc : p.kc) + (int64_t)layer * p.layer_bytes;
+  const float* const scale = FP8 ? (value ? p.v_scale : p.k_scale) + (int64_t)layer * p.scale_layer : nullptr;
+  const int64_t first = (int64_t)len - n, most = (int64_t)p.table_cols * p.chunk;
+  for (int base = 1; base < count; base += kKeepBatch) {
+    __syncthreads();
+    const int m = min(kKeepBatch, count - base);
+    int any = 0;
+    if (tid < m) {
+      const int i = base + tid, node = p.rows[(int64_t)r * p.rows_stride + i] - begin;
+      const int64_t from = first + node, to = first + i;
+      int a = -1, b = -1;
+      if (node >= 0 && node < n && node != i && from >= 0 && from < most && to >= 0 && to < most) {
+        a = p.bt[(int64_t)r * p.bt_stride + from / p.chunk];
+        b = p.bt[(int64_t)r * p.bt_stride + to / p.chunk];
+        if ((uint32_t)a >= (uint32_t)p.n_chunks || (uint32_t)b >= (uint32_t)p.n_chunks) a = b = -1;
+      }
+      src_chunk[tid] = a;
+      dst_chunk[tid] = b;
+      src_pos[tid] = (int)(from % p.chunk);
+      dst_pos[tid] = (int)(to % p.chunk);
+      any = a >= 0;
+    }
+    if (!__syncthreads_or(any)) continue;
+    for (int u = tid; u < p.units; u += blockDim.x) {
+      const int head = FP8 ? u / p.units_per_head : 0;
+      for (int i0 = 0; i0 < m; i0 += kKeepLoads) {
+        uint4 x[kKeepLoads];
+#pragma unroll
+        for (int j = 0; j < kKeepLoads; ++j)
+          if (i0 + j < m && src_chunk[i0 + j] >= 0)
+            x[j] = ld16(cache + src_chunk[i0 + j] * p.chunk_bytes + src_pos[i0 + j] * p.tok_bytes + 16 * u);
+#pragma unroll
+        for (int j = 0; j < kKeepLoads; ++j) {
+          if (i0 + j >= m || src_chunk[i0 + j] < 0) continue;
+          const int a = src_chunk[i0 + j], b = dst_chunk[i0 + j];
+          uint4 y = x[j];
+          if (FP8 && a != b) {   // another chunk, another scale: e4m3 of value * scale / scale, saturating
+            const float f = scale[(int64_t)a * p.Hkv + head] / scale[(int64_t)b * p.Hkv + head];
+            uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const f32x2_t lo = fp8x2_lo_to_f32(w[k]), hi = fp8x2_hi_to_f32(w[k]);
+              w[k] = f32_to_e4m3_sat(lo.x * f) | f32_to_e4m3_sat(lo.y * f) << 8 | f32_to_e4m3_sat(hi.x * f) << 16 |
+                     f32_to_e4m3_sat(hi.y * f) << 24;
+            }
+            y = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          st16(cache + b * p.chunk_bytes + dst_pos[i0 + j] * p.tok_bytes + 16 * u, y);
+        }
+      }
+    }
+  }
+}
+
+static int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+// Parts of a row: enough workgroups to fill the chip, no fewer than 2 048 elements each, no more than kVerifyPart.
+static void verify_parts(int T, int V, int* parts, int* part) {
+  const int64_t places = (int64_t)V + 7;   // (with the shift of a row that does not start at a 16-byte line)
+  int64_t n = (places + kVerifyPart - 1) / kVerifyPart;
+  const int64_t wish = 2048 / (T > 0 ? T : 1) + 1;
+  if (n < wish) n = wish;
+  if (n > places / 2048 + 1) n = places / 2048 + 1;
+  if (n > kVerifyMostParts) n = kVerifyMostParts;
+  const int64_t size = ((places + n - 1) / n + 7) & ~(int64_t)7;
+  *part = (int)size;
+  *parts = (int)((places + size - 1) / size);
+}
+
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" int64_t mi_verify_workspace_bytes(int32_t T, int32_t R, int32_t vocab) {
+  if (T < 0 || R <= 0 || vocab <= 0 || vocab > kVerifyMostParts * kVerifyPart - 8) return 0;
+  int parts, part;
+  verify_parts(T, vocab, &parts, &part);
+  return align256((int64_t)T * parts * sizeof(VerifyPartial)) + align256((int64_t)R * parts * sizeof(double)) +
+         align256((int64_t)R * sizeof(VerifyState));
+}
+
+template <int DT>
+static void launch_verify(const VerifyParams& p, int mode, hipStream_t st) {
+  const dim3 grid(p.T, p.parts), block(kVerifyThreads);
+  if (mode == kGreedy) {
+    if (p.T) hipLaunchKernelGGL((verify_rows_kernel<DT, true>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((verify_walk_kernel<DT, kGreedy>), dim3(p.R), dim3(kWalkThreads), 0, st, p);
+    return;
+  }
+  if (p.T) hipLaunchKernelGGL((verify_rows_kernel<DT, false>), grid, block, 0, st, p);
+  if (mode == kTarget) {
+    hipLaunchKernelGGL((verify_walk_kernel<DT, kTarget>), dim3(p.R), dim3(kWalkThreads), 0, st, p);
+    hipLaunchKernelGGL((verify_draw_kernel<DT, kTarget>), dim3(p.R), block, 0, st, p);
+  } else {
+    hipLaunchKernelGGL((verify_walk_kernel<DT, kDraft>), dim3(p.R), dim3(kWalkThreads), 0, st, p);
+    hipLaunchKernelGGL((verify_left_kernel<DT>), dim3(p.R, p.parts), block, 0, st, p);
+    hipLaunchKernelGGL((verify_draw_kernel<DT, kDraft>), dim3(p.R), block, 0, st, p);
+  }
+}
+
+extern "C" int mi_verify_drafted_tokens(const void* logits, int64_t stride_row, int32_t logits_dtype, int32_t T,
+                                        int32_t vocab, const int64_t* tokens, const int32_t* parents,
+                                        const int32_t* cu_seqlens_q, int32_t R, int32_t max_path, int32_t greedy,
+                                        const void* draft_probs, int64_t draft_stride_row, int32_t draft_dtype,
+                                        const float* uniform, float temperature, const float* cut,
+                                        int64_t* out_tokens, int32_t* out_rows, int32_t* out_counts, void* workspace,
+                                        int64_t workspace_bytes, void* stream) {
+  if (R == 0) return MI_OK;
+  if (!cu_seqlens_q || !out_tokens || !out_rows || !out_counts)
+    return mi_fail(MI_ERR_NULL, "mi_verify_drafted_tokens: null pointer argument");
+  if (T > 0 && (!logits || !tokens || !parents)) return mi_fail(MI_ERR_NULL, "mi_verify_drafted_tokens: null pointer argument");
+  if (T < 0 || R < 0 || max_path < 1)
+    return mi_fail(MI_ERR_SHAPE, "mi_verify_drafted_tokens: need T >= 0, R >= 0 and max_path >= 1");
+  if (vocab <= 0 || stride_row < vocab || vocab > kVerifyMostParts * kVerifyPart - 8)
+    return mi_fail(MI_ERR_SHAPE, "mi_verify_drafted_tokens: need 0 < vocab <= 524280 and a row stride of at least vocab");
+  if (logits_dtype < 0 || logits_dtype > 2 || draft_dtype < 0 || draft_dtype > 2)
+    return mi_fail(MI_ERR_UNSUPPORTED, "mi_verify_drafted_tokens: logits and draft_probs must be fp32 (0), bf16 (1) or fp16 (2)");
+  if (greedy && (draft_probs || cut)) return mi_fail(MI_ERR_SHAPE, "mi_verify_drafted_tokens: a greedy call takes neither draft_probs nor cut");
+  if (!greedy && T > 0 && !uniform) return mi_fail(MI_ERR_NULL, "mi_verify_drafted_tokens: sampling needs one uniform number per row");
+  if (!greedy && !(temperature > 0.f)) return mi_fail(MI_ERR_SHAPE, "mi_verify_drafted_tokens: temperature must be positive");
+  if (draft_probs && draft_stride_row < vocab)
+    return mi_fail(MI_ERR_SHAPE, "mi_verify_drafted_tokens: draft_probs need a row stride of at least vocab");
+  const int esz = logits_dtype ? 2 : 4, dsz = draft_dtype ? 2 : 4;
+  if (((uintptr_t)logits & (esz - 1)) || ((uintptr_t)draft_probs & (dsz - 1)))
+    return mi_fail(MI_ERR_ALIGN, "mi_verify_drafted_tokens: rows must be aligned to their elements");
+  if (!workspace || workspace_bytes < mi_verify_workspace_bytes(T, R, vocab))
+    return mi_fail(MI_ERR_WORKSPACE, "mi_verify_drafted_tokens: workspace smaller than mi_verify_workspace_bytes()");
+  if ((uintptr_t)workspace & 15) return mi_fail(MI_ERR_ALIGN, "mi_verify_drafted_tokens: the workspace must be 16-byte aligned");
+  VerifyParams p;
+  p.logits = (const uint8_t*)logits; p.stride = stride_row * esz;
+  p.draft = (const uint8_t*)draft_probs; p.draft_stride = draft_stride_row * dsz; p.draft_dtype = draft_dtype;
+  p.tokens = tokens; p.parents = parents; p.cu = cu_seqlens_q; p.uniform = uniform; p.cut = cut;
+  p.out_tokens = out_tokens; p.out_rows = out_rows; p.out_counts = out_counts;
+  p.T = T; p.R = R; p.V = vocab; p.max_path = max_path;
+  verify_parts(T, vocab, &p.parts, &p.part);
+  uint8_t* ws = (uint8_t*)workspace;
+  p.partial = (VerifyPartial*)ws;
+  ws += align256((int64_t)T * p.parts * sizeof(VerifyPartial));
+  p.residual = (double*)ws;
+  ws += align256((int64_t)R * p.parts * sizeof(double));
+  p.state = (VerifyState*)ws;
+  p.scaled = !greedy && temperature != 1.f;
+  p.inv_temperature = greedy ? 1.f : 1.f / temperature;
+  const int mode = greedy ? kGreedy : draft_probs ? kDraft : kTarget;
+  hipStream_t st = (hipStream_t)stream;
+  if (logits_dtype == 0) launch_verify<0>(p, mode, st);
+  else if (logits_dtype == 1) launch_verify<1>(p, mode, st);
+  else launch_verify<2>(p, mode, st);
+  return mi_check_launch("mi_verify_drafted_tokens");
+}
+
+extern "C" int mi_kv_keep_accepted(void* k_cache, void* v_cache, int64_t kv_stride_layer, int64_t kv_stride_chunk,
+                                   int64_t kv_stride_tok, int32_t layers, int32_t n_chunks, int32_t chunk_tokens,
+                                   int32_t Hkv, int32_t head_dim, int32_t elem_bytes, const float* k_scales,
+                                   const float* v_scales, int64_t scale_stride_layer, const int32_t* block_table,
+                                   int64_t bt_stride, int32_t table_columns, const int32_t* rows, int64_t rows_stride,
+                                   int32_t columns, const int32_t* counts, const int32_t* cu_seqlens_q,
+                                   const int32_t* kv_lens, int32_t* new_kv_lens, int32_t R, void* stream) {
+  if (R == 0) return MI_OK;
+  if (!k_cache || !block_table || !rows || !counts || !cu_seqlens_q || !kv_lens || !new_kv_lens)
+    return mi_fail(MI_ERR_NULL, "mi_kv_keep_accepted: null pointer argument");
+  if (R < 0 || layers <= 0 || layers > 65535 || n_chunks <= 0 || chunk_tokens <= 0 || Hkv <= 0 || head_dim <= 0 || columns < 0 || table_columns <= 0)
+    return mi_fail(MI_ERR_SHAPE, "mi_kv_keep_accepted: bad sizes");
+  if (elem_bytes != 1 && elem_bytes != 2) return mi_fail(MI_ERR_UNSUPPORTED, "mi_kv_keep_accepted: elements of 1 or 2 bytes");
+  const bool fp8 = k_scales || v_scales;
+  if (fp8 && (elem_bytes != 1 || !k_scales || !v_scales || !v_cache))
+    return mi_fail(MI_ERR_SHAPE, "mi_kv_keep_accepted: scales belong to both caches of bytes");
+  if (elem_bytes == 1 && !fp8) return mi_fail(MI_ERR_NULL, "mi_kv_keep_accepted: a cache of bytes needs k_scales and v_scales");
+  const int64_t row = (int64_t)Hkv * head_dim * elem_bytes;
+  if (row % 16 || (fp8 && head_dim % 16))
+    return mi_fail(MI_ERR_ALIGN, "mi_kv_keep_accepted: token rows (of an fp8 cache: heads) must be whole 16-byte pieces");
+  if ((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) || ((kv_stride_layer | kv_stride_chunk | kv_stride_tok) * elem_bytes) % 16)
+    return mi_fail(MI_ERR_ALIGN, "mi_kv_keep_accepted: caches and strides must keep rows 16-byte aligned");
+  KeepParams p;
+  p.kc = (uint8_t*)k_cache; p.vc = (uint8_t*)v_cache;
+  p.layer_bytes = kv_stride_layer * elem_bytes; p.chunk_bytes = kv_stride_chunk * elem_bytes; p.tok_bytes = kv_stride_tok * elem_bytes;
+  p.k_scale = k_scales; p.v_scale = v_scales; p.scale_layer = scale_stride_layer;
+  p.bt = block_table; p.bt_stride = bt_stride; p.rows = rows; p.rows_stride = rows_stride; p.counts = counts;
+  p.cu = cu_seqlens_q; p.lens = kv_lens; p.new_lens = new_kv_lens;
+  p.columns = columns; p.chunk = chunk_tokens; p.n_chunks = n_chunks; p.table_cols = table_columns;
+  p.units = (int)(row / 16); p.units_per_head = head_dim * elem_bytes / 16; p.Hkv = Hkv;
+  const dim3 grid(R, layers, v_cache ? 2 : 1), block(p.units <= 64 ? 64 : p.units <= 128 ? 128 : 256);
+  hipStream_t st = (hipStream_t)stream;
+  if (fp8) hipLaunchKernelGGL((kv_keep_kernel<true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((kv_keep_kernel<false>), grid, block, 0, st, p);
+  return mi_check_launch("mi_kv_keep_accepted");
+}

@@ -607,3 +607,64 @@ def linear_decode(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, out:
     has ``x``'s leading dimensions and ``N`` columns; ``out`` may lie over ``x``.  What ``linear_qkv`` / ``linear_proj``
     of the attention layer compute at tensor-parallel size 1 (``mi_linear_decode`` of the header)."""
     return _native().linear_decode(x, weight, bias, out, _override())
+
+
+# ---------------------------------------------------------------------------------------------
+# speculative decoding: a step over trees of drafted tokens
+# ---------------------------------------------------------------------------------------------
+def paged_tree_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, cu_seqlens_q: Tensor, kv_lens: Tensor,
+                         block_table: Tensor, tree_mask: Tensor, *, softmax_scale: Optional[float] = None,
+                         max_kv_len: Optional[int] = None, out: Optional[Tensor] = None,
+                         k_scales: Optional[Tensor] = None, v_scales: Optional[Tensor] = None) -> Tensor:
+    """Attention of drafted tokens over the paged cache: rows ``cu_seqlens_q[r] : cu_seqlens_q[r + 1]`` of ``q``
+    ``[T, (1,) Hq, d]`` are the nodes of request r's tree, whose keys and values are the last positions that
+    ``kv_lens`` counts.  A node attends to the context before them and to the nodes of its row of ``tree_mask`` (int64
+    ``[T]`` or ``[T, words]``, up to four words: bit j % 64 of word j // 64 is node j of the request, its own bit
+    included; see :func:`tree_masks`).  Rows that see nothing and rows behind the last request are zeros.  Byte caches
+    with ``k_scales`` / ``v_scales`` ``[N, Hkv]`` hold e4m3 values (head_dim 64 or 128)."""
+    return _native().paged_tree_attention(q, k_cache, v_cache, cu_seqlens_q, kv_lens, block_table, tree_mask,
+                                          softmax_scale, out, k_scales, v_scales, _override())
+
+
+def tree_masks(parents, words: Optional[int] = None, device=None) -> Tensor:
+    """``tree_mask`` rows of one tree from its nodes' parents (a sequence of ints; -1 for the root, a parent precedes its
+    children): every node sees its ancestors and itself.  Host work, done once for a tree that a program keeps."""
+    parents = [int(x) for x in parents]
+    need = max(1, -(-len(parents) // 64))
+    words = need if words is None else words
+    _require(need <= words <= 4, "a tree has at most 256 nodes, 64 to a word")
+    bits = []
+    for i, p in enumerate(parents):
+        _require(-1 <= p < i, "a parent precedes its children")
+        bits.append((bits[p] if p >= 0 else 0) | 1 << i)
+    rows = [[(b >> 64 * w) & (1 << 64) - 1 for w in range(words)] for b in bits]
+    signed = [[x - (1 << 64) if x >> 63 else x for x in row] for row in rows]
+    return torch.tensor(signed, dtype=torch.int64, device=device).view(len(parents), words)
+
+
+def verify_drafted_tokens(logits: Tensor, tokens: Tensor, parents: Tensor, cu_seqlens_q: Tensor, max_path: int, *,
+                          greedy: bool = False, draft_probs: Optional[Tensor] = None, uniform: Optional[Tensor] = None,
+                          temperature: float = 1.0, cut: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """The accepted path of every tree and the token that follows it, from given random numbers.
+
+    ``logits`` ``[T, V]`` (fp32, bf16 or fp16): what the target says after each node; ``tokens`` int64 ``[T]`` the nodes'
+    tokens, ``parents`` int32 ``[T]`` their parents inside the request (-1: the root).  ``draft_probs`` ``[T, V]`` (fp32,
+    bf16 or fp16): row i is the distribution that the children of node i were drawn from; without it the drafted tokens
+    count as chosen.  ``uniform`` fp32 ``[T]``: a root's number draws its request's last token, any other node's decides
+    about it.  ``temperature`` and ``cut`` (``[T]``, as ``sample_from_logits(..., return_cut=True)`` returns it) make the
+    target's distribution.  A path has at most ``max_path`` nodes, the root included.
+
+    Returns ``(tokens int64 [R, max_path], rows int32 [R, max_path], counts int32 [R])``: each request's new tokens, the
+    rows of the nodes on its path (root first) and how many there are of each; -1 behind them."""
+    return _native().verify_drafted_tokens(logits, tokens, parents, cu_seqlens_q, max_path, greedy, draft_probs, uniform,
+                                           temperature, cut, _override())
+
+
+def kv_keep_accepted(k_cache: Tensor, v_cache: Optional[Tensor], rows: Tensor, counts: Tensor, cu_seqlens_q: Tensor,
+                     kv_lens: Tensor, block_table: Tensor, *, k_scales: Optional[Tensor] = None,
+                     v_scales: Optional[Tensor] = None) -> Tensor:
+    """Move the accepted nodes' cache rows behind their request's context (``rows`` / ``counts`` of
+    :func:`verify_drafted_tokens`), in one layer ``[N, C, Hkv, d]`` or in all of ``[layers, N, C, Hkv, d]`` (a half of the
+    context's ``memory_buffer``), and return the new ``kv_lens``.  ``v_cache`` may be ``None`` (latents).  Rows of a byte
+    cache that change their chunk are converted to its scale (``k_scales`` / ``v_scales`` ``[(layers,) N, Hkv]``)."""
+    return _native().kv_keep_accepted(k_cache, v_cache, rows, counts, cu_seqlens_q, kv_lens, block_table, k_scales, v_scales)

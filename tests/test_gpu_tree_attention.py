@@ -1,0 +1,279 @@
+"""GPU parity: attention of drafted tokens over the paged cache against the 64-bit oracle.
+
+Tolerance, element by element, with u half a step of the 16-bit type and A = sum p |v|: the probabilities are rounded once
+(each by at most u, in the numerator and in the row sum: 2 u A), the result once (u |o|), scores are 32-bit sums of exact
+products and the exponentials of 32-bit hardware precision: 2^-24 times a score of at most some 30 and a few roundings, 2e-5 A.
+"""
+import math
+import random
+
+import pytest
+import torch
+
+from oracle import speculative as osp
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _trees(nodes, shape, rng):
+    if shape == "chain":
+        return [list(range(-1, n - 1)) for n in nodes]
+    return [([-1] + [rng.randint(max(0, i - 9), i - 1) for i in range(1, n)])[:n] for n in nodes]
+
+
+class Case:
+    def __init__(self, dev, nodes, ctx, *, Hq=8, Hkv=2, d=128, chunk=64, dtype=BF16, fp8=False, shape="tree", seed=0, bits=None,
+                 spare=0, words=None, spread=1.0):
+        rng, gen = random.Random(seed), torch.Generator().manual_seed(seed)
+        self.lens = [n + c for n, c in zip(nodes, ctx)]
+        self.cu = [0]
+        for n in nodes:
+            self.cu.append(self.cu[-1] + n)
+        T = self.cu[-1]
+        self.bits = sum((osp.ancestors(t) for t in _trees(nodes, shape, rng)), []) if bits is None else bits
+        need = [-(-max(n, 0) // chunk) for n in self.lens]
+        self.N = sum(need) + 2
+        ids = torch.randperm(self.N, generator=gen).tolist()
+        self.table = torch.zeros(len(nodes), max(max(need), 1) + 1, dtype=torch.int32)
+        for r, k in enumerate(need):
+            self.table[r, :k] = torch.tensor([ids.pop() for _ in range(k)], dtype=torch.int32)
+        self.q = (torch.randn(T + spare, Hq, d, generator=gen) * spread).to(dtype)
+        shape4 = (self.N, chunk, Hkv, d)
+        self.scales = None
+        if fp8:
+            self.k, self.v = ((torch.randn(shape4, generator=gen) * 100).clamp(-448, 448).to(torch.float8_e4m3fn) for _ in "kv")
+            self.scales = [0.004 + 0.01 * torch.rand(self.N, Hkv, generator=gen) for _ in "kv"]
+        else:
+            self.k, self.v = (torch.randn(shape4, generator=gen).to(dtype) for _ in "kv")
+        self.words = words or max(1, -(-max(max(nodes), 1) // 64))
+        self.mask = osp.mask_rows(self.bits + [0] * spare, self.words)
+        self.dev, self.scale, self.dtype = dev, d ** -0.5, dtype
+
+    def run(self, mi, q=None, out=None, mask=None, **more):
+        dev = self.dev
+        cache = [x.view(torch.uint8) if self.scales else x for x in (self.k, self.v)]
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        scales = dict(k_scales=self.scales[0].to(dev), v_scales=self.scales[1].to(dev)) if self.scales else {}
+        return mi.ops.paged_tree_attention(
+            self.q.to(dev) if q is None else q, cache[0].to(dev), cache[1].to(dev), i32(self.cu), i32(self.lens), self.table.to(dev),
+            self.mask.to(dev) if mask is None else mask, softmax_scale=self.scale, out=out, **scales, **more)
+
+    def reference(self):
+        k, v = (x.float() if self.scales else x for x in (self.k, self.v))
+        return osp.tree_attention(self.q[:self.cu[-1]], k, v, self.cu, self.lens, self.table, self.bits, self.scale,
+                                  *(self.scales or ()))
+
+    def check(self, mi, got=None, **more):
+        got = self.run(mi, **more) if got is None else got
+        torch.cuda.synchronize()
+        got, (ref, size) = got.cpu().double().view(-1, *self.q.shape[1:]), self.reference()
+        u = torch.finfo(self.dtype).eps / 2
+        assert (got[self.cu[-1]:] == 0).all(), "rows behind the last request"
+        got = got[:self.cu[-1]]
+        assert torch.equal(got.isnan(), ref.isnan())
+        fine = torch.isfinite(ref)
+        assert torch.equal(got[~fine & ~ref.isnan()], ref[~fine & ~ref.isnan()])
+        err = (got - ref).abs()[fine]
+        bound = ((2 * u + 2e-5) * size * (1 + u) + u * ref.abs() + 1e-7)[fine]
+        assert (err <= bound).all(), f"max err / bound {(err / bound).max():.3f}"
+        return got
+
+
+@pytest.mark.parametrize("nodes,ctx", [
+    ([1], [0]), ([1], [1]), ([2], [0]), ([5], [777]), ([5, 1, 8], [64, 63, 65]), ([16, 17, 3], [0, 15, 16]), ([13], [47]),
+    ([64], [130]), ([40, 7, 22, 1], [300, 5, 0, 999]),
+])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_sizes(mi, dev, nodes, ctx, dtype):
+    Case(dev, nodes, ctx, dtype=dtype, seed=sum(nodes)).check(mi)
+
+
+@pytest.mark.parametrize("Hq,Hkv,d", [(8, 8, 64), (32, 8, 128), (7, 1, 96), (12, 4, 192), (16, 2, 256), (64, 1, 64), (28, 4, 128),
+                                      (5, 5, 128), (24, 3, 96), (11, 11, 64), (16, 16, 128)])
+def test_head_layouts(mi, dev, Hq, Hkv, d):
+    Case(dev, [9, 21, 1], [100, 33, 250], Hq=Hq, Hkv=Hkv, d=d, seed=d + Hq).check(mi)
+
+
+@pytest.mark.parametrize("chunk", [16, 48, 32, 80, 64, 256])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_chunk_sizes(mi, dev, chunk, d):
+    Case(dev, [11, 30], [chunk - 5, 3 * chunk + 1], d=d, chunk=chunk, seed=chunk).check(mi)
+
+
+@pytest.mark.parametrize("d,chunk,dtype", [(64, 64, BF16), (64, 16, FP16), (64, 32, BF16), (128, 256, FP16), (128, 48, BF16), (128, 32, FP16)])
+def test_fp8_caches(mi, dev, d, chunk, dtype):
+    Case(dev, [12, 1, 33], [270, 64, 511], Hq=16, Hkv=4, d=d, chunk=chunk, dtype=dtype, fp8=True, seed=d + chunk).check(mi)
+
+
+def test_fp8_scales_of_every_size_and_sign(mi, dev):
+    """Small scales (a probability times one is subnormal in fp16), a large one, a negative one and zeros."""
+    for dtype in (BF16, FP16):
+        c = Case(dev, [6, 9], [500, 130], Hq=8, Hkv=2, chunk=64, dtype=dtype, fp8=True, seed=5)
+        for s in c.scales:
+            s[0::4] *= 1e-4
+            s[1::4] *= -1
+            s[2::8] = 0
+        c.check(mi)
+
+
+@pytest.mark.parametrize("nodes", [65, 128, 200, 256])
+def test_masks_of_several_words(mi, dev, nodes):
+    Case(dev, [nodes, 3], [70, 10], Hq=4, Hkv=2, d=64, seed=nodes).check(mi)
+
+
+def test_any_bits(mi, dev):
+    """Masks that are no trees: rows that see everything, themselves only, later nodes, nothing; more words than needed."""
+    rng, nodes = random.Random(9), [20, 33, 4]
+    bits = [rng.choice((0, rng.getrandbits(n), (1 << n) - 1, 1 << rng.randrange(n))) for n in nodes for _ in range(n)]
+    for ctx in ([40, 100, 7], [0, 0, 0]):
+        Case(dev, nodes, ctx, bits=bits, words=2, seed=10).check(mi)
+
+
+def test_rows_that_see_nothing_are_zeros(mi, dev):
+    got = Case(dev, [4], [0], bits=[0, 1, 0, 15], seed=11).check(mi)
+    assert (got[0] == 0).all() and (got[2] == 0).all() and (got[1] != 0).any()
+
+
+@pytest.mark.parametrize("dtype,fp8,d", [(BF16, False, 128), (FP16, False, 64), (FP16, False, 256), (BF16, True, 128), (FP16, True, 64)])
+def test_what_a_row_does_not_see_does_not_reach_it(mi, dev, dtype, fp8, d):
+    """NaN and infinities in nodes' keys and values meet the rows that see them and no others."""
+    parents = [-1, 0, 0, 1, 2, 2, 4]
+    c = Case(dev, [7, 7], [60, 133], d=d, dtype=dtype, fp8=fp8, bits=osp.ancestors(parents) * 2, seed=12)
+    for r in range(2):
+        for node, v in ((3, math.nan), (5, math.inf), (6, -math.inf)):
+            chunk, at = osp.position(c.table[r].tolist(), 64, c.N, c.lens[r] - 7 + node)
+            bad = torch.full((d // 2,), math.nan if fp8 else v).to(c.v.dtype)
+            c.v[chunk, at, 0, ::2] = bad
+            if node == 3:
+                c.k[chunk, at, 1, :] = torch.full((d,), math.nan).to(c.k.dtype)
+    got = c.check(mi)
+    assert torch.isfinite(got[[0, 1, 2, 4, 7, 8, 9, 11]]).all() and not torch.isfinite(got[3]).all()
+
+
+def test_what_lies_behind_a_request_is_not_read(mi, dev):
+    c = Case(dev, [5, 3], [70, 20], seed=13)
+    used = torch.zeros(c.N, 64, dtype=torch.bool)
+    for r in range(2):
+        for k in range(c.lens[r]):
+            used[osp.position(c.table[r].tolist(), 64, c.N, k)] = True
+    c.k[~used] = math.nan
+    c.v[~used] = math.nan
+    assert torch.isfinite(c.check(mi)).all()
+
+
+def test_table_entries_that_name_no_chunk(mi, dev):
+    c = Case(dev, [5, 9], [300, 200], seed=14)
+    c.table[0, 2], c.table[1, 0], c.table[1, 3] = -1, c.N, 1 << 30
+    c.check(mi)
+
+
+def test_lengths_and_rows_outside_their_arrays(mi, dev):
+    """Lengths beyond the table are cut to it, negative ones are none, nodes without a position have no key."""
+    c = Case(dev, [4, 3, 5, 2], [100, 50, 0, 20], seed=15)
+    c.lens = [4096, -7, 2, 22]
+    c.check(mi)
+
+
+def test_empty_requests_and_padding_rows(mi, dev):
+    c = Case(dev, [0, 5, 0, 0, 2, 0], [10, 40, 0, 33, 7, 1], spare=9, seed=16)
+    out = torch.full_like(c.q, 7).to(dev)
+    assert c.run(mi, out=out) is out
+    c.check(mi, got=out)
+
+
+def test_strides(mi, dev):
+    """Queries inside a wider tensor, results into one, caches with gaps between heads, a mask inside a wider one."""
+    c = Case(dev, [6, 11], [90, 45], Hq=8, Hkv=4, d=64, chunk=32, seed=17)
+    T = c.cu[-1]
+    wide = torch.zeros(T, 3, 8, 128, dtype=BF16, device=dev)
+    q = wide[:, 1, :, :64]
+    q.copy_(c.q)
+    out = torch.full((T, 12, 72), 5.0, dtype=BF16, device=dev)
+    masks = torch.full((T, 7), -1, dtype=torch.int64, device=dev)
+    masks[:, 2:3] = c.mask.to(dev)
+    pools = torch.full((c.N, 32, 4, 2, 80), math.nan, dtype=BF16, device=dev)
+    pools[..., 0, :64], pools[..., 1, :64] = c.k.to(dev), c.v.to(dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    table = torch.full((2, 16), -5, dtype=torch.int32, device=dev)
+    table[:, :c.table.size(1)] = c.table.to(dev)
+    got = mi.ops.paged_tree_attention(q, pools[..., 0, :64], pools[..., 1, :64], i32(c.cu), i32(c.lens), table, masks[:, 2:3],
+                                      softmax_scale=c.scale, out=out[:, 4:, :64])
+    c.check(mi, got=got)
+    assert (out[:, :4] == 5).all() and (out[:, 4:, 64:] == 5).all()
+    c.check(mi, mask=masks[:, 2])                                     # one word a row, as a column
+    assert c.run(mi, q=c.q.to(dev).unsqueeze(1)).shape == (T, 1, 8, 64)
+
+
+def test_many_requests(mi, dev):
+    """More than one launch takes (their prefix sums lie in LDS): every one is answered, ragged and empty ones among them."""
+    rng = random.Random(18)
+    nodes = [rng.randint(0, 3) for _ in range(4999)]
+    Case(dev, nodes, [rng.randint(0, 40) for _ in nodes], Hq=2, Hkv=1, d=64, chunk=16, spare=3, seed=18).check(mi)
+
+
+@pytest.mark.parametrize("dtype,fp8", [(BF16, False), (FP16, False), (BF16, True)])
+def test_long_contexts(mi, dev, dtype, fp8):
+    Case(dev, [13, 2], [20011, 4096], Hq=4, Hkv=1, d=64, chunk=256, dtype=dtype, fp8=fp8, seed=19).check(mi)
+
+
+def test_growing_and_large_scores(mi, dev):
+    """Keys whose scores keep growing move the running maximum in every tile; 16-bit queries ten times as large."""
+    c = Case(dev, [9], [800], seed=20, spread=3.0)
+    for k in range(c.lens[0]):
+        chunk, at = osp.position(c.table[0].tolist(), 64, c.N, k)
+        c.k[chunk, at] = (c.k[chunk, at].float() * (0.1 + k / 400)).to(BF16)
+    c.check(mi)
+
+
+def test_a_chain_is_the_causal_call(mi, dev):
+    c = Case(dev, [6, 6, 1], [500, 31, 64], shape="chain", Hq=32, Hkv=8, seed=21)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    other = mi.ops.paged_prefill_attention(c.q.to(dev), c.k.to(dev), c.v.to(dev), i32(c.cu), i32(c.lens), c.table.to(dev))
+    c.check(mi, got=other)
+    c.check(mi)
+
+
+def test_replays_and_streams(mi, dev):
+    """A captured call replayed among eager work, with new values in place, and a call on a stream of its own."""
+    c = Case(dev, [5, 12], [300, 64], seed=22)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    q, k, v = c.q.to(dev), c.k.to(dev), c.v.to(dev)
+    args = (i32(c.cu), i32(c.lens), c.table.to(dev), c.mask.to(dev))
+    eager = mi.ops.paged_tree_attention(q, k, v, *args, softmax_scale=c.scale)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        aside = mi.ops.paged_tree_attention(q, k, v, *args, softmax_scale=c.scale)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(aside, eager)
+    work = torch.empty(mi._lib.load().mi_tree_workspace_bytes(17, 2, 8, 2, 128), dtype=torch.uint8, device=dev)
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(q)
+    with mi.ops.use_workspace(work):
+        with torch.cuda.graph(graph):
+            mi.ops.paged_tree_attention(q, k, v, *args, softmax_scale=c.scale, out=out)
+    for step in range(4):
+        q.mul_(0.9)
+        out.zero_()
+        graph.replay()
+        again = mi.ops.paged_tree_attention(q, k, v, *args, softmax_scale=c.scale)
+        torch.cuda.synchronize()
+        assert torch.equal(out, again), step
+
+
+def test_refusals(mi, dev):
+    c = Case(dev, [5], [20], seed=23)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    q, k, v, table, mask = c.q.to(dev), c.k.to(dev), c.v.to(dev), c.table.to(dev), c.mask.to(dev)
+    call = lambda **x: mi.ops.paged_tree_attention(*{**dict(q=q, k=k, v=v, cu=i32([0, 5]), lens=i32([25]), t=table, m=mask), **x}.values())  # noqa: E731
+    for change, word in ((dict(m=mask.int()), "int64"), (dict(m=mask[:4]), "row for every"), (dict(m=mask.expand(5, 5)), "words"),
+                         (dict(cu=i32([0])), "two entries"), (dict(k=k.half()), "16-bit type"), (dict(k=k[..., :64]), "shape"),
+                         (dict(lens=i32([])), "shorter"), (dict(t=table.long()), "block_table"), (dict(q=q.float()), "bf16 or fp16"),
+                         (dict(m=mask.cpu()), "one device")):
+        with pytest.raises(ValueError, match=word):
+            call(**change)
+    with pytest.raises(mi._lib.KernelError, match="multiple of 16"):
+        call(k=k[:, :24], v=v[:, :24])
+    with pytest.raises(ValueError, match="go together"):
+        mi.ops.paged_tree_attention(q, k, v, i32([0, 5]), i32([25]), table, mask, k_scales=torch.ones(c.N, 2, device=dev))
