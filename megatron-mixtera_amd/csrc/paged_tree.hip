@@ -8,9 +8,9 @@
 // megatron/core/transformer/attention.py:546-600).
 //
 // Work decomposition.  The (node, query head) pairs that share a KV head are its rows, 16 * NQ of them to a wavefront
-// ("part").  The tiles of 16 * NT tokens of all (request, part) pairs are laid end to end and a fixed grid of workgroups
-// takes equal spans of that sequence, whatever the mix of lengths; a workgroup's wavefronts take neighbouring KV heads of
-// the same tokens, so that it reads whole token rows of the cache.  A pair within one span writes its result, any other
+// ("part"), one to eight parts to a "group".  The tiles of 16 * NT tokens of all (request, group) pairs are laid end to end
+// and a fixed grid of workgroups takes equal spans of that sequence, whatever the mix of lengths; a workgroup's wavefronts
+// take the parts of a group and neighbouring KV heads of the same tokens.  A pair within one span writes its result, any other
 // leaves normalised fp32 partials and a base-2 log-sum-exp for the merge.  A span touches at most one pair that began
 // before it and one that goes on after it, so two slots per workgroup hold all partials.
 //
@@ -44,9 +44,9 @@ struct TreeParams {
   int32_t mask_words;
   uint16_t* out;
   int64_t o_st, o_sh;
-  float* part_o;         // [2 grid][Hkv][ROWS][HD]
-  float* part_lse;       // [2 grid][Hkv][ROWS]
-  int4* pair_info;       // per (request, part): first and last workgroup, request, part
+  float* part_o;         // [2 grid][Hkv][rows][HD]
+  float* part_lse;       // [2 grid][Hkv][rows]
+  int4* pair_info;       // per (request, group): first and last workgroup, request, group
   int32_t* pairs;        // how many there are
   const float* k_scale;
   const float* v_scale;
@@ -54,6 +54,7 @@ struct TreeParams {
   uint32_t g_magic;      // 2^32 / G + 1, 0 for G = 1
   int32_t T, R, r_base, Hq, Hkv, G, chunk, n_chunks, table_cols, grid;
   int32_t last_slice;    // the launch that clears the rows behind the last request
+  int32_t share, rows;   // wavefronts that share a KV head, and the rows they take together (a group)
   float scale_log2;
 };
 
@@ -65,12 +66,12 @@ static __device__ __forceinline__ int tree_div_g(const TreeParams& p, int n) {
 static __device__ __forceinline__ int tree_chunk_of(int tok, uint64_t magic) { return (int)(((uint64_t)(uint32_t)tok * magic) >> 40); }
 
 struct TreeSegment {
-  int r, part;
+  int r, part;         // request, and which of its parts (ROWS rows each)
   int q_begin, nodes;  // rows of q, nodes of the request
   int len, ctx;        // cached tokens, those before the first node (may be negative: nodes without a position)
   int start, end;      // tokens of the segment
   bool whole;
-  int slot;
+  int slot, row0;      // partial: its place, and the part's first row in there
 };
 
 // Bits of four tokens, node j0 first, of a row of `words` 32-bit words; what lies before node 0 is context.
@@ -82,7 +83,9 @@ static __device__ __forceinline__ uint32_t tree_bits(const uint32_t* row, int wo
   return j0 < 0 ? (bits << -j0) | ((1u << -j0) - 1u) : bits;
 }
 
-template <int HD, int NT, int NQ, bool FP8, bool F16>
+// SHARE: neighbouring wavefronts take other parts of the same tokens, and a barrier per tile keeps them on one tile, whose
+// lines then come from memory once and from the CU's cache for the others.
+template <int HD, int NT, int NQ, bool FP8, bool F16, bool SHARE>
 static __device__ __forceinline__ void tree_segment(const TreeParams& p, const TreeSegment& s, int h, int lane) {
   constexpr int KS = HD / 32, DV = HD / 16, ESZ = FP8 ? 1 : 2, TK = 16 * NT, ROWS = 16 * NQ;
   constexpr int KL = FP8 ? KS / 2 : KS;      // 16-byte loads of a key row and lane
@@ -92,6 +95,10 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
   const int start = __builtin_amdgcn_readfirstlane(s.start), end = __builtin_amdgcn_readfirstlane(s.end);
   const int ctx = __builtin_amdgcn_readfirstlane(s.ctx);
   const int last = max(min(end, len) - 1, 0);
+  if (SHARE && tree_div_g(p, s.part * ROWS) >= s.nodes) {   // (a part without rows)
+    for (int T = start; T < end; T += TK) __builtin_amdgcn_s_barrier();
+    return;
+  }
 
   // rows of this lane: row tile nt, row m16
   int q_row[NQ], q_head[NQ];
@@ -180,7 +187,7 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
       const int t0 = min(T + 16 * u, last);
       const uint8_t* row = chunk + (uint32_t)(t0 - ci * p.chunk + min(last - t0, m16)) * tok_bytes + k_col;
 #pragma unroll
-      for (int kk = 0; kk < KL; ++kk) kf[u][kk] = ld16_stream(row + 64 * kk);
+      for (int kk = 0; kk < KL; ++kk) kf[u][kk] = SHARE ? ld16(row + 64 * kk) : ld16_stream(row + 64 * kk);
     }
   };
   auto load_v = [&](int T) {
@@ -192,8 +199,11 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
     for (int u = 0; u < NT; ++u) {
       const int t0 = min(T + 16 * u, last);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        ld_dwords_stream(chunk + (uint32_t)(t0 - ci * p.chunk + min(last - t0, 4 * g + j)) * tok_bytes, vf[u][j]);
+      for (int j = 0; j < 4; ++j) {
+        const uint8_t* row = chunk + (uint32_t)(t0 - ci * p.chunk + min(last - t0, 4 * g + j)) * tok_bytes;
+        if constexpr (SHARE) ld_dwords(row, vf[u][j]);
+        else ld_dwords_stream(row, vf[u][j]);
+      }
     }
   };
 
@@ -246,6 +256,7 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
       }
     }
     __builtin_amdgcn_sched_barrier(0);
+    if (SHARE) __builtin_amdgcn_s_barrier();
     load_k(T + TK);   // (the key registers are free again)
     __builtin_amdgcn_sched_barrier(0);
     if (FP8) {        // a scale may have any sign: the maximum is of the products' own scores
@@ -411,7 +422,7 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
         st_dwords(o + DV * i, w);
       }
     } else {
-      const int64_t row = ((int64_t)s.slot * p.Hkv + h) * ROWS + 16 * nt + m16;
+      const int64_t row = ((int64_t)s.slot * p.Hkv + h) * p.rows + s.row0 + 16 * nt + m16;
       float* o = p.part_o + row * HD + 4 * DV * g;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -446,14 +457,15 @@ static __device__ __forceinline__ int64_t tree_scan(int64_t v, int lane) {
   return v;
 }
 
-template <int HD, int NT, int NQ, bool FP8, bool F16>
+template <int HD, int NT, int NQ, bool FP8, bool F16, bool SHARE>
 __global__ __launch_bounds__(512, 2) void paged_tree_kernel(TreeParams p) {
-  constexpr int TK = 16 * NT, ROWS = 16 * NQ;
+  constexpr int TK = 16 * NT;
   extern __shared__ int64_t tree_lds[];
   int64_t* const cum = tree_lds;                               // tiles of requests 0 .. i
-  int32_t* const first = reinterpret_cast<int32_t*>(cum + p.R);  // parts of requests 0 .. i
+  int32_t* const first = reinterpret_cast<int32_t*>(cum + p.R);  // groups of requests 0 .. i
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.y * (blockDim.x >> 6) + wave;
+  const int heads = (blockDim.x >> 6) / (SHARE ? p.share : 1);   // KV heads of the workgroup
+  const int h = blockIdx.y * heads + (SHARE ? wave / p.share : wave), sub = SHARE ? wave % p.share : 0;
 
   if (wave == 0) {
     int64_t tiles = 0;
@@ -463,7 +475,7 @@ __global__ __launch_bounds__(512, 2) void paged_tree_kernel(TreeParams p) {
       int n_parts = 0, n_tiles = 0;
       if (i < p.R) {
         const TreeRequest t = tree_request(p, i);
-        n_parts = (int)(((int64_t)t.nodes * p.G + ROWS - 1) / ROWS);
+        n_parts = (int)(((int64_t)t.nodes * p.G + p.rows - 1) / p.rows);
         n_tiles = max((t.len + TK - 1) / TK, 1);   // (a request without tokens has a tile in which nothing is seen)
       }
       const int64_t ct = tree_scan((int64_t)n_parts * n_tiles, lane) + tiles, cp = tree_scan(n_parts, lane) + parts;
@@ -520,84 +532,105 @@ __global__ __launch_bounds__(512, 2) void paged_tree_kernel(TreeParams p) {
     TreeSegment s;
     s.r = r; s.q_begin = t.q_begin; s.nodes = t.nodes; s.len = t.len; s.ctx = t.len - t.nodes;
     while (t0 < t1 && t0 < re) {
-      s.part = __builtin_amdgcn_readfirstlane((int)((t0 - rb) / tiles));
-      const int tb = (int)(t0 - rb - (int64_t)s.part * tiles), te = (int)min((int64_t)tiles, tb + (t1 - t0));
+      const int group = __builtin_amdgcn_readfirstlane((int)((t0 - rb) / tiles));
+      s.part = group * (SHARE ? p.share : 1) + sub;
+      s.row0 = sub * 16 * NQ;
+      const int tb = (int)(t0 - rb - (int64_t)group * tiles), te = (int)min((int64_t)tiles, tb + (t1 - t0));
       const bool begins = tb == 0, ends = te == tiles;
       s.start = tb * TK;
       s.end = min(te * TK, t.len);
       s.whole = begins && ends;
       s.slot = 2 * blockIdx.x + (begins ? 1 : 0);
       if (wave == 0 && lane == 0 && blockIdx.y == 0) {
-        int4* info = p.pair_info + ((r ? first[r - 1] : 0) + s.part);
+        int4* info = p.pair_info + ((r ? first[r - 1] : 0) + group);
         if (begins) {
           info->x = blockIdx.x;
           info->z = r;
-          info->w = s.part;
+          info->w = group;
         }
         if (ends) info->y = blockIdx.x;
       }
-      tree_segment<HD, NT, NQ, FP8, F16>(p, s, h, lane);
+      tree_segment<HD, NT, NQ, FP8, F16, SHARE>(p, s, h, lane);
       t0 += te - tb;
     }
   }
 }
 
-// One workgroup per (request, part) and KV head: sum of its partials, weighted by 2^(lse - max).  A thread owns four
-// neighbouring values of a row.
+// Sum of a row's partials, weighted by 2^(lse - max): one workgroup per (request, group), KV head and eight rows or so.  A
+// thread owns four neighbouring values of a row; `groups` sets of threads take its partials in turn, eight in flight each.
+constexpr int kTreeMergeThreads = 256;
 template <bool F16>
-__global__ __launch_bounds__(256) void paged_tree_merge_kernel(TreeParams p, int head_dim, int rows) {
+__global__ __launch_bounds__(1024) void paged_tree_merge_kernel(TreeParams p, int head_dim, int groups) {
+  __shared__ float red[6][1024];
   const int pair = blockIdx.x, h = blockIdx.y;
   if (pair >= *p.pairs) return;
   const int4 info = p.pair_info[pair];
   if (info.x == info.y) return;   // written by the streaming kernel
   const TreeRequest t = tree_request(p, info.z);
-  const int cols = head_dim >> 2;
-  for (int i = threadIdx.x; i < rows * cols; i += blockDim.x) {
-    const int row = i / cols, d = 4 * (i - row * cols);
-    const int n = info.w * rows + row, qi = tree_div_g(p, n);
-    if (qi >= t.nodes) return;
-    float mx = -INFINITY, den = 0.f;
-    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w0 = info.x; w0 <= info.y; w0 += 4) {
-      float lse[4];
-      float4 po[4];
+  const int cols = head_dim >> 2, block_rows = kTreeMergeThreads / cols, set = cols * block_rows;
+  const int grp = threadIdx.x / set, in = threadIdx.x - grp * set;
+  const int row = blockIdx.z * block_rows + in / cols, d = 4 * (in % cols);
+  const int n = info.w * p.rows + row, qi = tree_div_g(p, n);
+  if (tree_div_g(p, info.w * p.rows + blockIdx.z * block_rows) >= t.nodes) return;   // (uniform)
+  const bool live = grp < groups && row < p.rows && qi < t.nodes;
+  float mx = -INFINITY, den = 0.f;
+  float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float lse, float weight, float4 v) {   // `weight` partials' worth of `v`, relative to 2^lse
+    if (lse == -INFINITY) return;                       // (saw nothing)
+    const float m = lse > mx || lse != lse ? lse : mx;  // (NaN goes on)
+    const float a = fast_exp2(mx - m), b = fast_exp2(lse - m);
+    num.x = num.x * a + b * v.x; num.y = num.y * a + b * v.y; num.z = num.z * a + b * v.z; num.w = num.w * a + b * v.w;
+    den = den * a + b * weight;
+    mx = m;
+  };
+  if (live)
+    for (int w0 = info.x + 8 * grp; w0 <= info.y; w0 += 8 * groups) {
+      float lse[8];
+      float4 po[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
         const int w = min(w0 + j, info.y);
-        const int64_t at = ((int64_t)(2 * w + (w == info.x ? 1 : 0)) * p.Hkv + h) * rows + row;
+        const int64_t at = ((int64_t)(2 * w + (w == info.x ? 1 : 0)) * p.Hkv + h) * p.rows + row;
         lse[j] = p.part_lse[at];
         po[j] = *reinterpret_cast<const float4*>(p.part_o + at * head_dim + d);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (w0 + j <= info.y && lse[j] != -INFINITY) {   // (a partial that saw nothing)
-          const float m = fmaxf(mx, lse[j]);
-          const float a = fast_exp2(mx - m), b = fast_exp2(lse[j] - m);
-          num.x = num.x * a + b * po[j].x; num.y = num.y * a + b * po[j].y;
-          num.z = num.z * a + b * po[j].z; num.w = num.w * a + b * po[j].w;
-          den = den * a + b;
-          mx = m;
-        }
-      }
+      for (int j = 0; j < 8; ++j)
+        if (w0 + j <= info.y) add(lse[j], 1.f, po[j]);
     }
-    const float inv = den == 0.f ? 0.f : 1.f / den;
-    uint16_t* o = p.out + (int64_t)(t.q_begin + qi) * p.o_st + (int64_t)(h * p.G + n - qi * p.G) * p.o_sh + d;
-    st8(o, make_uint2(pack2<F16>(num.x * inv, num.y * inv), pack2<F16>(num.z * inv, num.w * inv)));
+  if (groups > 1) {
+    const int i = threadIdx.x;
+    red[0][i] = mx; red[1][i] = den; red[2][i] = num.x; red[3][i] = num.y; red[4][i] = num.z; red[5][i] = num.w;
+    __syncthreads();
+    if (grp) return;
+    for (int g = 1; g < groups; ++g) {
+      const int k = g * set + in;
+      add(red[0][k], red[1][k], make_float4(red[2][k], red[3][k], red[4][k], red[5][k]));
+    }
   }
+  if (!live) return;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  uint16_t* o = p.out + (int64_t)(t.q_begin + qi) * p.o_st + (int64_t)(h * p.G + n - qi * p.G) * p.o_sh + d;
+  st8(o, make_uint2(pack2<F16>(num.x * inv, num.y * inv), pack2<F16>(num.z * inv, num.w * inv)));
 }
 
-// Wavefronts per workgroup (neighbouring KV heads), workgroups along the tiles, rows of a part.
+// Wavefronts per workgroup (`share` parts of a group times neighbouring KV heads), workgroups along the tiles, rows of a
+// group.  Parts share where the average request has more rows than one takes.
 struct TreeShape {
-  int waves, grid, rows;
+  int waves, share, grid, heads, rows;
 };
-static TreeShape tree_shape(int Hkv, int head_dim) {
+static TreeShape tree_shape(int T, int R, int Hq, int Hkv, int head_dim) {
   TreeShape s;
-  s.waves = 1;
-  for (int w = 2; w <= 8; ++w)
-    if (Hkv % w == 0) s.waves = w;
-  s.grid = device_cu_count() * (8 / s.waves) / (Hkv / s.waves);
+  const int rows = head_dim > 128 ? 16 : 32;
+  const int64_t mean = (int64_t)T * (Hq / Hkv) / R;
+  s.share = mean <= rows ? 1 : mean <= 2 * rows ? 2 : mean <= 4 * rows ? 4 : 8;
+  s.heads = 1;
+  for (int w = 2; w <= 8 / s.share; ++w)
+    if (Hkv % w == 0) s.heads = w;
+  s.waves = s.heads * s.share;
+  s.grid = device_cu_count() * (8 / s.waves) / (Hkv / s.heads);
   if (s.grid < 1) s.grid = 1;
-  s.rows = head_dim > 128 ? 16 : 32;
+  s.rows = rows * s.share;
   return s;
 }
 static int64_t tree_align(int64_t n) { return (n + 255) & ~(int64_t)255; }
@@ -612,7 +645,7 @@ using namespace mi;
 
 extern "C" int64_t mi_tree_workspace_bytes(int32_t T, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim) {
   if (T <= 0 || R <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0) return 0;
-  const TreeShape s = tree_shape(Hkv, head_dim);
+  const TreeShape s = tree_shape(T, R, Hq, Hkv, head_dim);
   const int64_t rows = (int64_t)2 * s.grid * Hkv * s.rows;
   return 256 + tree_align(16 * tree_most_pairs(T, R, Hq / Hkv, s.rows)) + tree_align(rows * 4) + rows * head_dim * 4;
 }
@@ -664,7 +697,7 @@ extern "C" int mi_paged_tree_attention(
     return mi_fail(MI_ERR_WORKSPACE, "mi_paged_tree_attention: workspace too small (see mi_tree_workspace_bytes)");
   if ((uintptr_t)workspace & 15) return mi_fail(MI_ERR_ALIGN, "mi_paged_tree_attention: workspace must be 16-byte aligned");
 
-  const TreeShape shape = tree_shape(Hkv, head_dim);
+  const TreeShape shape = tree_shape(T, R, Hq, Hkv, head_dim);
   const bool f16 = dtype == MI_DTYPE_FP16;
   TreeParams p;
   p.q = (const uint16_t*)q; p.q_st = q_stride_tok; p.q_sh = q_stride_head;
@@ -684,9 +717,9 @@ extern "C" int mi_paged_tree_attention(
   p.chunk_magic = (((uint64_t)1 << 40) + chunk_tokens - 1) / chunk_tokens;
   p.g_magic = G == 1 ? 0u : (uint32_t)(((uint64_t)1 << 32) / G + 1);
   p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = G; p.chunk = chunk_tokens; p.n_chunks = n_chunks; p.table_cols = table_columns;
-  p.grid = shape.grid; p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.grid = shape.grid; p.share = shape.share; p.rows = shape.rows; p.scale_log2 = softmax_scale * 1.4426950408889634f;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid(shape.grid, Hkv / shape.waves), block(64 * shape.waves);
+  const dim3 grid(shape.grid, Hkv / shape.heads), block(64 * shape.waves);
   const bool wide = head_dim > 128;
   // tokens of a tile: 32, 16 of wide heads, 64 of an fp8 cache with narrow ones (what the registers hold in flight); a tile
   // lies in one chunk
@@ -699,8 +732,10 @@ extern "C" int mi_paged_tree_attention(
     const size_t lds = (size_t)p.R * (sizeof(int64_t) + sizeof(int32_t));
 #define MI_TREE(HD_, NT_, NQ_, FP8_)                                                                                   \
     do {                                                                                                               \
-      if (f16) hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, true>), grid, block, lds, st, p);            \
-      else hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, false>), grid, block, lds, st, p);               \
+      if (f16 && p.share > 1) hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, true, true>), grid, block, lds, st, p);   \
+      else if (f16) hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, true, false>), grid, block, lds, st, p);            \
+      else if (p.share > 1) hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, false, true>), grid, block, lds, st, p);    \
+      else hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, false, false>), grid, block, lds, st, p);                    \
     } while (0)
 #define MI_TREE_16(HD_)                                                                                                \
     do {                                                                                                               \
@@ -723,9 +758,13 @@ extern "C" int mi_paged_tree_attention(
 #undef MI_TREE_8
 #undef MI_TREE_16
 #undef MI_TREE
-    const dim3 mgrid((unsigned)tree_most_pairs(T, p.R, G, shape.rows), Hkv);
-    if (f16) hipLaunchKernelGGL((paged_tree_merge_kernel<true>), mgrid, dim3(256), 0, st, p, head_dim, shape.rows);
-    else hipLaunchKernelGGL((paged_tree_merge_kernel<false>), mgrid, dim3(256), 0, st, p, head_dim, shape.rows);
+    // (thread sets per row: for the partials that a request is expected to be cut into)
+    const int cols = head_dim / 4, block_rows = kTreeMergeThreads / cols;
+    const int64_t pairs = tree_most_pairs(T, p.R, G, shape.rows);
+    const int groups = shape.grid / pairs > 16 ? 4 : shape.grid / pairs > 8 ? 2 : 1;
+    const dim3 mgrid((unsigned)pairs, Hkv, (shape.rows + block_rows - 1) / block_rows), mblock(groups > 1 ? groups * cols * block_rows : kTreeMergeThreads);
+    if (f16) hipLaunchKernelGGL((paged_tree_merge_kernel<true>), mgrid, mblock, 0, st, p, head_dim, groups);
+    else hipLaunchKernelGGL((paged_tree_merge_kernel<false>), mgrid, mblock, 0, st, p, head_dim, groups);
   }
   return mi_check_launch("mi_paged_tree_attention");
 }

@@ -72,7 +72,7 @@ class Case:
         u = torch.finfo(self.dtype).eps / 2
         assert (got[self.cu[-1]:] == 0).all(), "rows behind the last request"
         got = got[:self.cu[-1]]
-        assert torch.equal(got.isnan(), ref.isnan())
+        assert torch.equal(got.isnan(), ref.isnan()), "NaN"
         fine = torch.isfinite(ref)
         assert torch.equal(got[~fine & ~ref.isnan()], ref[~fine & ~ref.isnan()])
         err = (got - ref).abs()[fine]
