@@ -66,7 +66,7 @@ static __device__ __forceinline__ int tree_div_g(const TreeParams& p, int n) {
 static __device__ __forceinline__ int tree_chunk_of(int tok, uint64_t magic) { return (int)(((uint64_t)(uint32_t)tok * magic) >> 40); }
 
 struct TreeSegment {
-  int r, part;         // request, and which of its parts (ROWS rows each)
+  int r, group, part;  // request, which of its groups, and which of its parts (the rows of a wavefront)
   int q_begin, nodes;  // rows of q, nodes of the request
   int len, ctx;        // cached tokens, those before the first node (may be negative: nodes without a position)
   int start, end;      // tokens of the segment
@@ -81,6 +81,35 @@ static __device__ __forceinline__ uint32_t tree_bits(const uint32_t* row, int wo
   const uint32_t lo = w < words ? row[w] : 0u, hi = w + 1 < words ? row[w + 1] : 0u;
   const uint32_t bits = (uint32_t)((((uint64_t)hi << 32) | lo) >> (j & 31));
   return j0 < 0 ? (bits << -j0) | ((1u << -j0) - 1u) : bits;
+}
+
+// Infinities and NaN among the values of a word (the sign bit of each that is one), the word without them, and, as operands
+// of a product with what a row sees of their tokens, their places: an infinity counts 1, a negative one 64, a NaN 4096
+// (exact in either type, and 16 of each fit).  The product says what a row's sum meets.
+template <bool F16>
+static __device__ __forceinline__ uint32_t tree_odd16(uint32_t x) {
+  return F16 ? ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+static __device__ __forceinline__ uint32_t tree_odd8(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+template <bool F16>
+static __device__ __forceinline__ uint32_t tree_even16(uint32_t x) { return x & ~((tree_odd16<F16>(x) >> 15) * 0xffffu); }
+static __device__ __forceinline__ uint32_t tree_even8(uint32_t x) { return x & ~((tree_odd8(x) >> 7) * 0xffu); }
+template <bool F16>
+static __device__ __forceinline__ uint32_t tree_places(uint32_t w) {
+  constexpr uint32_t one = F16 ? 0x3c00u : 0x3f80u, inf = F16 ? 0x7c00u : 0x7f80u, k64 = F16 ? 0x5400u : 0x4280u, k4096 = F16 ? 0x6c00u : 0x4580u;
+  auto place = [](uint32_t x) { return (x & 0x7fffu) > inf ? k4096 : x == inf ? one : x == (inf | 0x8000u) ? k64 : 0u; };
+  return place(w & 0xffffu) | place(w >> 16) << 16;
+}
+// four bits as ones
+template <bool F16>
+static __device__ __forceinline__ uint2 tree_sees(uint32_t b) {
+  constexpr uint32_t one = F16 ? 0x3c00u : 0x3f80u;
+  return make_uint2((b & 1u ? one : 0u) | (b & 2u ? one << 16 : 0u), (b & 4u ? one : 0u) | (b & 8u ? one << 16 : 0u));
+}
+static __device__ __forceinline__ float tree_odd_sum(float count) {
+  const uint32_t n = (uint32_t)count;
+  const float up = n & 63u ? INFINITY : 0.f, down = n >> 6 & 63u ? -INFINITY : 0.f;
+  return n >> 12 ? __uint_as_float(0x7fc00000u) : up + down;
 }
 
 // SHARE: neighbouring wavefronts take other parts of the same tokens, and a barrier per tile keeps them on one tile, whose
@@ -333,13 +362,9 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
                      : make_uint2(low_halves(x[1], x[0]), low_halves(x[3], x[2]));
     };
     if (masked) {
-      // Infinities and NaN: a product would take them into rows that do not see their token.  Each kind's places as ones
-      // times what the rows see say which sums it belongs to; then they are zeros.
-      auto odd = [](uint32_t x) -> uint32_t {   // the value's sign bit, for every value of a word
-        if constexpr (FP8) return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-        else if constexpr (F16) return ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-        else return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-      };
+      // Infinities and NaN: a product would take them into rows that do not see their token.  Their places times what the
+      // rows see say which sums they belong to; then they are zeros.
+      auto odd = [](uint32_t x) { return FP8 ? tree_odd8(x) : tree_odd16<F16>(x); };
       uint32_t any = 0;
 #pragma unroll
       for (int u = 0; u < NT; ++u)
@@ -348,28 +373,17 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
 #pragma unroll
           for (int w = 0; w < VD; ++w) any |= odd(vf[u][j][w]);
       if (__builtin_amdgcn_ballot_w64(any != 0)) {
-        // (an infinity counts 1, a negative one 64, a NaN 4096: exact in either type, and 16 of each fit)
-        constexpr uint32_t kOne = ones2<F16>() & 0xffffu, kInf = F16 ? 0x7c00u : 0x7f80u;
-        constexpr uint32_t k64 = F16 ? 0x5400u : 0x4280u, k4096 = F16 ? 0x6c00u : 0x4580u;
-        auto place = [&](uint32_t x) { return (x & 0x7fffu) > kInf ? k4096 : x == kInf ? kOne : x == (kInf | 0x8000u) ? k64 : 0u; };
-        auto places = [&](uint32_t w) { return place(w & 0xffffu) | place(w >> 16) << 16; };
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
 #pragma unroll
           for (int e = 0; e < DV; ++e) {
             __builtin_amdgcn_sched_barrier(0);   // (one column at a time: registers)
-            const uint2 c = column(u, e), at = make_uint2(places(c.x), places(c.y));
+            const uint2 c = column(u, e), at = make_uint2(tree_places<F16>(c.x), tree_places<F16>(c.y));
 #pragma unroll
             for (int nt = 0; nt < NQ; ++nt) {
-              const uint32_t b = seen[nt] >> (4 * u);
-              const uint2 sees = make_uint2((b & 1u ? kOne : 0u) | (b & 2u ? kOne << 16 : 0u), (b & 4u ? kOne : 0u) | (b & 8u ? kOne << 16 : 0u));
-              const f32x4_t n4 = mfma_16x16x16<F16>(at, sees, zero4);
+              const f32x4_t n = mfma_16x16x16<F16>(at, tree_sees<F16>(seen[nt] >> (4 * u)), zero4);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t n = (uint32_t)n4[i];
-                const float up = n & 63u ? INFINITY : 0.f, down = n >> 6 & 63u ? -INFINITY : 0.f;
-                acc[nt][e][i] += n >> 12 ? __uint_as_float(0x7fc00000u) : up + down;
-              }
+              for (int i = 0; i < 4; ++i) acc[nt][e][i] += tree_odd_sum(n[i]);
             }
           }
         }
@@ -379,10 +393,7 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int w = 0; w < VD; ++w) {
-              const uint32_t o = odd(vf[u][j][w]);
-              vf[u][j][w] &= FP8 ? ~((o >> 7) * 0xffu) : ~((o >> 15) * 0xffffu);
-            }
+            for (int w = 0; w < VD; ++w) vf[u][j][w] = FP8 ? tree_even8(vf[u][j][w]) : tree_even16<F16>(vf[u][j][w]);
       }
     }
 #pragma unroll
@@ -457,15 +468,244 @@ static __device__ __forceinline__ int64_t tree_scan(int64_t v, int lane) {
   return v;
 }
 
-template <int HD, int NT, int NQ, bool FP8, bool F16, bool SHARE>
-__global__ __launch_bounds__(512, 2) void paged_tree_kernel(TreeParams p) {
-  constexpr int TK = 16 * NT;
+// ------------------------------------------------------------------------------------------------ many rows
+// Where a request has many rows per KV head the products are the work, and a CU's cache too slow a feed: a workgroup of
+// WAVES wavefronts takes 32 * WAVES rows of one (request, KV head), and tiles of 32 tokens go straight from memory into LDS
+// (buffer loads with the LDS destination), STAGES - 1 of them ahead, one barrier a tile.  The 16-byte pieces of a row lie
+// in another order in every row (an exclusive or with the row's number, applied where the loads pick their source), which
+// spreads the reads of 16 rows over all banks without padding; the order of a lane's own reads is an exclusive or again.
+// Rows behind the request's last token arrive as zeros (the load's descriptor ends there).
+template <int HD> static __device__ __forceinline__ int tree_swizzle(int row) { return HD == 64 ? (row >> 1) & 7 : row & 15; }
+template <int HD, int WAVES> constexpr int tree_stages() {
+  constexpr int room = WAVES == 8 ? 131072 : 65536;   // LDS of a workgroup: one or two of them on a CU
+  return room / (HD * 128) > 8 ? 8 : room / (HD * 128);
+}
+
+template <int HD, int WAVES, bool F16>
+static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, const TreeSegment& s, int h, int lane, int wave, uint8_t* lds) {
+  constexpr int KS = HD / 32, DV = HD / 16, NQ = 2, TK = 32, ROWB = 2 * HD, STAGES = tree_stages<HD, WAVES>();
+  constexpr int HALF = TK * ROWB, STAGE = 2 * HALF;           // keys, then values
+  constexpr int KLOADS = HALF / 1024, LPW = 2 * KLOADS / WAVES;
+  static_assert(LPW * WAVES == 2 * KLOADS && (KLOADS % LPW == 0 || LPW % KLOADS == 0), "whole loads per wavefront");
+  const int m16 = lane & 15, g = lane >> 4;
+  const int len = __builtin_amdgcn_readfirstlane(s.len), ctx = __builtin_amdgcn_readfirstlane(s.ctx);
+  const int start = __builtin_amdgcn_readfirstlane(s.start), end = __builtin_amdgcn_readfirstlane(s.end);
+
+  int q_row[NQ], q_head[NQ];
+  bool valid[NQ];
+  uint4 qf[NQ][KS];
+#pragma unroll
+  for (int nt = 0; nt < NQ; ++nt) {
+    const int n = s.part * 32 + 16 * nt + m16, qi = tree_div_g(p, n);
+    valid[nt] = qi < s.nodes;
+    q_row[nt] = s.q_begin + (valid[nt] ? qi : 0);
+    q_head[nt] = h * p.G + (n - qi * p.G);
+    const uint16_t* row = p.q + (int64_t)q_row[nt] * p.q_st + (int64_t)q_head[nt] * p.q_sh;
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) qf[nt][kk] = valid[nt] ? ld16(row + 32 * kk + 8 * g) : make_uint4(0, 0, 0, 0);
+  }
+  const bool idle = tree_div_g(p, s.part * 32) >= s.nodes;   // (a part without rows: loads and barriers only)
+
+  auto uniform64 = [](uint64_t x) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+  };
+  const uint64_t kbase = uniform64((uint64_t)(uintptr_t)(p.kc + (int64_t)h * p.kv_sh * 2)) & 0xffffffffffffull;
+  const uint64_t vbase = uniform64((uint64_t)(uintptr_t)(p.vc + (int64_t)h * p.kv_sh * 2)) & 0xffffffffffffull;
+  const int64_t chunk_bytes = p.kv_sc * 2;
+  const int tok_bytes = p.kv_st * 2;
+  // (the block table in the constant address space: scalar loads, which leave the count of the direct loads alone)
+  const auto* const bt_row = (const __attribute__((address_space(4))) int32_t*)uniform64((uint64_t)(uintptr_t)(p.bt + (int64_t)(p.r_base + s.r) * p.bt_stride));
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+
+  // this wavefront's loads of a tile: which piece of which row each lane fetches
+  uint32_t src[LPW];
+#pragma unroll
+  for (int i = 0; i < LPW; ++i) {
+    const int slot = ((wave * LPW + i) % KLOADS) * 64 + lane, row = slot / (HD / 8), piece = slot % (HD / 8);
+    src[i] = (uint32_t)row * (uint32_t)tok_bytes + 16u * (uint32_t)(piece ^ tree_swizzle<HD>(row));
+  }
+  const int tiles_end = (end + TK - 1) / TK;
+  auto entry = [&](int tile) { return bt_row[tree_chunk_of(min(tile, tiles_end - 1) * TK, p.chunk_magic)]; };
+  uint32_t missing = 0;   // bit i: the chunk of the i-th tile in flight does not exist
+  auto issue = [&](int tile, int stage, int pc, int ahead) {
+    const int t0 = min(tile, tiles_end - 1) * TK, ci = tree_chunk_of(t0, p.chunk_magic);
+    const bool there = (uint32_t)pc < (uint32_t)p.n_chunks;
+    const int64_t off = (int64_t)(there ? pc : 0) * chunk_bytes + (int64_t)(t0 - ci * p.chunk) * tok_bytes;
+    const uint32_t nrec = there && tile < tiles_end ? (uint32_t)min(len - t0, TK) * (uint32_t)tok_bytes : 0u;
+    missing |= (there ? 0u : 1u) << ahead;
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      const int k = wave * LPW + i;
+      const bool key = k < KLOADS;
+      const uint64_t a = (key ? kbase : vbase) + (uint64_t)off;
+      u32x4_t rs;
+      rs.x = (uint32_t)a;
+      rs.y = (uint32_t)(a >> 32);
+      rs.z = nrec;
+      rs.w = 0x00020000u;
+      const uint32_t m0 = lds0 + (uint32_t)(stage * STAGE + 1024 * k);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(src[i]), "s"(rs)
+                   : "memory", "m0");
+    }
+  };
+
+  float m_run[NQ], l_run[NQ];
+  f32x4_t acc[NQ][DV];
+#pragma unroll
+  for (int nt = 0; nt < NQ; ++nt) {
+    m_run[nt] = -3e38f;
+    l_run[nt] = 0.f;
+#pragma unroll
+    for (int e = 0; e < DV; ++e) acc[nt][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  const f32x4_t zero4 = {0.f, 0.f, 0.f, 0.f};
+  const uint4 ones = make_uint4(ones2<F16>(), ones2<F16>(), ones2<F16>(), ones2<F16>());
+  // this lane's first key piece and value piece within a stage; step kk: ^ 64 kk, column e: ^ 32 e, sub-tile 1: + 16 rows
+  const uint32_t k_at = (uint32_t)(m16 * ROWB + ((g ^ tree_swizzle<HD>(m16)) << 4));
+  const int v_row = 4 * g + (m16 >> 2);
+  const uint32_t v_at = (uint32_t)(HALF + v_row * ROWB + ((((m16 >> 1) & 1) ^ tree_swizzle<HD>(v_row)) << 4) + 8 * (m16 & 1));
+
+  // (the queries have arrived before any direct load: the compiler waits for them here and not among those)
+#pragma unroll
+  for (int nt = 0; nt < NQ; ++nt)
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) asm volatile("" ::"v"(qf[nt][kk].x), "v"(qf[nt][kk].y), "v"(qf[nt][kk].z), "v"(qf[nt][kk].w));
+  __syncthreads();   // (the stages are free: every wavefront has left the segment before)
+  const int t_first = start / TK;
+  if (start < end) {
+    for (int i = 0; i < STAGES - 1; ++i) issue(t_first + i, i, entry(t_first + i), i);
+    int pc = entry(t_first + STAGES - 1);
+    int stage = 0, fill = STAGES - 1;
+    for (int T = start; T < end; T += TK) {
+      // this wavefront's share of the tile has landed (what it issued after that may be on its way), then everyone's
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * LPW) : "memory");
+      __builtin_amdgcn_s_barrier();
+      const int tile = T / TK;
+      const int next = entry(tile + STAGES);   // (a tile before its use)
+      const bool page = !(missing & 1u);
+      missing >>= 1;
+      issue(tile + STAGES - 1, fill, pc, STAGES - 2);
+      fill = stage;
+      const uint8_t* const at = lds + stage * STAGE;
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      if (!idle) {
+        const bool masked = T + TK > min(ctx, end) || !page;
+        f32x4_t sc[NQ][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int kk = 0; kk < KS; ++kk) {
+            const uint4 k = *reinterpret_cast<const uint4*>(at + (k_at ^ (64u * kk)) + 16 * u * ROWB);
+#pragma unroll
+            for (int nt = 0; nt < NQ; ++nt) sc[nt][u] = mfma_16x16x32<F16>(k, qf[nt][kk], kk ? sc[nt][u] : zero4);
+          }
+        }
+        uint32_t seen[NQ];
+        if (masked) {
+#pragma unroll
+          for (int nt = 0; nt < NQ; ++nt) {
+            const uint32_t* bits = p.mask + (int64_t)q_row[nt] * p.mask_st;
+            seen[nt] = 0;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int t0 = T + 16 * u + 4 * g;
+              uint32_t b = page ? tree_bits(bits, p.mask_words, t0 - ctx) & 15u : 0u;
+              const int left = end - t0;
+              b &= left >= 4 ? 15u : left > 0 ? (1u << left) - 1u : 0u;
+              seen[nt] |= b << (4 * u);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (!(b >> i & 1u)) sc[nt][u][i] = -INFINITY;
+            }
+          }
+        }
+        uint4 pf[NQ];
+#pragma unroll
+        for (int nt = 0; nt < NQ; ++nt) {
+          float tmax = fmaxf(fmaxf(sc[nt][0][0], sc[nt][0][1]), fmaxf(sc[nt][0][2], sc[nt][0][3]));
+          tmax = fmaxf(tmax, fmaxf(fmaxf(sc[nt][1][0], sc[nt][1][1]), fmaxf(sc[nt][1][2], sc[nt][1][3])));
+          const float m_new = fmaxf(m_run[nt], rowgroup_max(tmax) * p.scale_log2);
+          const float alpha = fast_exp2(m_run[nt] - m_new);
+          m_run[nt] = m_new;
+          float e8[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e8[i] = fast_exp2(__builtin_fmaf(sc[nt][i >> 2][i & 3], p.scale_log2, -m_new));
+          pf[nt] = make_uint4(pack2<F16>(e8[0], e8[1]), pack2<F16>(e8[2], e8[3]), pack2<F16>(e8[4], e8[5]), pack2<F16>(e8[6], e8[7]));
+          const f32x4_t sum = mfma_16x16x32<F16>(ones, pf[nt], zero4);
+          l_run[nt] = l_run[nt] * alpha + sum[0];
+          if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+#pragma unroll
+            for (int e = 0; e < DV; ++e) {
+              acc[nt][e][0] *= alpha; acc[nt][e][1] *= alpha; acc[nt][e][2] *= alpha; acc[nt][e][3] *= alpha;
+            }
+          }
+        }
+        auto values = [&](int e) {
+          const uint8_t* v = at + (v_at ^ (32u * e));
+          const uint2 a = lds_ld8_tr(v), b = lds_ld8_tr(v + 16 * ROWB);
+          return make_uint4(a.x, a.y, b.x, b.y);
+        };
+        if (!masked) {
+#pragma unroll
+          for (int e = 0; e < DV; ++e) {
+            const uint4 v = values(e);
+#pragma unroll
+            for (int nt = 0; nt < NQ; ++nt) acc[nt][e] = mfma_16x16x32<F16>(v, pf[nt], acc[nt][e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < DV; ++e) {
+            __builtin_amdgcn_sched_barrier(0);   // (one column at a time: registers)
+            uint4 v = values(e);
+            if (__builtin_amdgcn_ballot_w64((tree_odd16<F16>(v.x) | tree_odd16<F16>(v.y) | tree_odd16<F16>(v.z) | tree_odd16<F16>(v.w)) != 0)) {
+              const uint2 lo = make_uint2(tree_places<F16>(v.x), tree_places<F16>(v.y)), hi = make_uint2(tree_places<F16>(v.z), tree_places<F16>(v.w));
+#pragma unroll
+              for (int nt = 0; nt < NQ; ++nt) {
+                const f32x4_t n = mfma_16x16x16<F16>(hi, tree_sees<F16>(seen[nt] >> 4), mfma_16x16x16<F16>(lo, tree_sees<F16>(seen[nt]), zero4));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[nt][e][i] += tree_odd_sum(n[i]);
+              }
+              v = make_uint4(tree_even16<F16>(v.x), tree_even16<F16>(v.y), tree_even16<F16>(v.z), tree_even16<F16>(v.w));
+            }
+#pragma unroll
+            for (int nt = 0; nt < NQ; ++nt) acc[nt][e] = mfma_16x16x32<F16>(v, pf[nt], acc[nt][e]);
+          }
+        }
+      }
+      pc = next;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load may still be on its way into this workgroup's LDS)
+  }
+
+  // ---- acc[nt][e][i] is element d = 16 e + 4 g + i of the row
+#pragma unroll
+  for (int nt = 0; nt < NQ; ++nt) {
+    if (!valid[nt]) continue;
+    const float l = l_run[nt], inv = l == 0.f ? 0.f : 1.f / l;
+    if (s.whole) {
+      uint16_t* o = p.out + (int64_t)q_row[nt] * p.o_st + (int64_t)q_head[nt] * p.o_sh + 4 * g;
+#pragma unroll
+      for (int e = 0; e < DV; ++e)
+        st8(o + 16 * e, make_uint2(pack2<F16>(acc[nt][e][0] * inv, acc[nt][e][1] * inv), pack2<F16>(acc[nt][e][2] * inv, acc[nt][e][3] * inv)));
+    } else {
+      const int64_t row = ((int64_t)s.slot * p.Hkv + h) * p.rows + s.row0 + 16 * nt + m16;
+      float* o = p.part_o + row * HD + 4 * g;
+#pragma unroll
+      for (int e = 0; e < DV; ++e)
+        *reinterpret_cast<float4*>(o + 16 * e) = make_float4(acc[nt][e][0] * inv, acc[nt][e][1] * inv, acc[nt][e][2] * inv, acc[nt][e][3] * inv);
+      if (g == 0) p.part_lse[row] = l == 0.f ? -INFINITY : m_run[nt] + fast_log2(l);
+    }
+  }
+}
+
+// The span of this workgroup along the tiles of all (request, group) pairs, as segments one after the other: seg(segment) with
+// the segment's group; every wavefront walks the same ones.  Clears the rows behind the last request on the way.
+template <int HD, int TK, typename Seg>
+static __device__ __forceinline__ void tree_walk(const TreeParams& p, Seg seg) {
   extern __shared__ int64_t tree_lds[];
   int64_t* const cum = tree_lds;                               // tiles of requests 0 .. i
   int32_t* const first = reinterpret_cast<int32_t*>(cum + p.R);  // groups of requests 0 .. i
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int heads = (blockDim.x >> 6) / (SHARE ? p.share : 1);   // KV heads of the workgroup
-  const int h = blockIdx.y * heads + (SHARE ? wave / p.share : wave), sub = SHARE ? wave % p.share : 0;
 
   if (wave == 0) {
     int64_t tiles = 0;
@@ -533,8 +773,7 @@ __global__ __launch_bounds__(512, 2) void paged_tree_kernel(TreeParams p) {
     s.r = r; s.q_begin = t.q_begin; s.nodes = t.nodes; s.len = t.len; s.ctx = t.len - t.nodes;
     while (t0 < t1 && t0 < re) {
       const int group = __builtin_amdgcn_readfirstlane((int)((t0 - rb) / tiles));
-      s.part = group * (SHARE ? p.share : 1) + sub;
-      s.row0 = sub * 16 * NQ;
+      s.group = group;
       const int tb = (int)(t0 - rb - (int64_t)group * tiles), te = (int)min((int64_t)tiles, tb + (t1 - t0));
       const bool begins = tb == 0, ends = te == tiles;
       s.start = tb * TK;
@@ -550,10 +789,33 @@ __global__ __launch_bounds__(512, 2) void paged_tree_kernel(TreeParams p) {
         }
         if (ends) info->y = blockIdx.x;
       }
-      tree_segment<HD, NT, NQ, FP8, F16, SHARE>(p, s, h, lane);
+      seg(s);
       t0 += te - tb;
     }
   }
+}
+
+template <int HD, int NT, int NQ, bool FP8, bool F16, bool SHARE>
+__global__ __launch_bounds__(512, 2) void paged_tree_kernel(TreeParams p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = (blockDim.x >> 6) / (SHARE ? p.share : 1);   // KV heads of the workgroup
+  const int h = blockIdx.y * heads + (SHARE ? wave / p.share : wave), sub = SHARE ? wave % p.share : 0;
+  tree_walk<HD, 16 * NT>(p, [&](TreeSegment& s) {
+    s.part = s.group * (SHARE ? p.share : 1) + sub;
+    s.row0 = sub * 16 * NQ;
+    tree_segment<HD, NT, NQ, FP8, F16, SHARE>(p, s, h, lane);
+  });
+}
+
+template <int HD, int WAVES, bool F16>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_tree_rows_kernel(TreeParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t stages[tree_stages<HD, WAVES>() * HD * 128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  tree_walk<HD, 32>(p, [&](TreeSegment& s) {
+    s.part = s.group * WAVES + wave;
+    s.row0 = wave * 32;
+    tree_rows_segment<HD, WAVES, F16>(p, s, blockIdx.y, lane, wave, stages);
+  });
 }
 
 // Sum of a row's partials, weighted by 2^(lse - max): one workgroup per (request, group), KV head and eight rows or so.  A
@@ -615,22 +877,30 @@ __global__ __launch_bounds__(1024) void paged_tree_merge_kernel(TreeParams p, in
 }
 
 // Wavefronts per workgroup (`share` parts of a group times neighbouring KV heads), workgroups along the tiles, rows of a
-// group.  Parts share where the average request has more rows than one takes.
+// group.  Parts share where the average request has more rows than one takes; `many`: paged_tree_rows_kernel.
 struct TreeShape {
   int waves, share, grid, heads, rows;
 };
-static TreeShape tree_shape(int T, int R, int Hq, int Hkv, int head_dim) {
+static int64_t tree_mean_rows(int T, int R, int G) { return (int64_t)T * G / R; }
+static TreeShape tree_shape(int T, int R, int Hq, int Hkv, int head_dim, bool many) {
   TreeShape s;
-  const int rows = head_dim > 128 ? 16 : 32;
-  const int64_t mean = (int64_t)T * (Hq / Hkv) / R;
-  s.share = mean <= rows ? 1 : mean <= 2 * rows ? 2 : mean <= 4 * rows ? 4 : 8;
-  s.heads = 1;
-  for (int w = 2; w <= 8 / s.share; ++w)
-    if (Hkv % w == 0) s.heads = w;
-  s.waves = s.heads * s.share;
-  s.grid = device_cu_count() * (8 / s.waves) / (Hkv / s.heads);
+  const int64_t mean = tree_mean_rows(T, R, Hq / Hkv);
+  if (many) {
+    s.heads = 1;
+    s.waves = s.share = mean <= 128 ? 4 : 8;
+    s.grid = device_cu_count() * (s.waves == 8 ? 1 : 2) / Hkv;
+    s.rows = 32 * s.waves;
+  } else {
+    const int rows = head_dim > 128 ? 16 : 32;
+    s.share = mean <= rows ? 1 : mean <= 2 * rows ? 2 : mean <= 4 * rows ? 4 : 8;
+    s.heads = 1;
+    for (int w = 2; w <= 8 / s.share; ++w)
+      if (Hkv % w == 0) s.heads = w;
+    s.waves = s.heads * s.share;
+    s.grid = device_cu_count() * (8 / s.waves) / (Hkv / s.heads);
+    s.rows = rows * s.share;
+  }
   if (s.grid < 1) s.grid = 1;
-  s.rows = rows * s.share;
   return s;
 }
 static int64_t tree_align(int64_t n) { return (n + 255) & ~(int64_t)255; }
@@ -643,11 +913,18 @@ static int64_t tree_most_pairs(int T, int R, int G, int rows) {
 
 using namespace mi;
 
+static int64_t tree_workspace(const TreeShape& s, int T, int R, int G, int Hkv, int head_dim) {
+  const int64_t rows = (int64_t)2 * s.grid * Hkv * s.rows;
+  return 256 + tree_align(16 * tree_most_pairs(T, R, G, s.rows)) + tree_align(rows * 4) + rows * head_dim * 4;
+}
 extern "C" int64_t mi_tree_workspace_bytes(int32_t T, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim) {
   if (T <= 0 || R <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0) return 0;
-  const TreeShape s = tree_shape(T, R, Hq, Hkv, head_dim);
-  const int64_t rows = (int64_t)2 * s.grid * Hkv * s.rows;
-  return 256 + tree_align(16 * tree_most_pairs(T, R, Hq / Hkv, s.rows)) + tree_align(rows * 4) + rows * head_dim * 4;
+  int64_t most = 0;   // (which kernel a call takes depends on the cache as well)
+  for (int many = 0; many < 2; ++many) {
+    const int64_t n = tree_workspace(tree_shape(T, R, Hq, Hkv, head_dim, many != 0), T, R, Hq / Hkv, Hkv, head_dim);
+    if (n > most) most = n;
+  }
+  return most;
 }
 
 extern "C" int mi_paged_tree_attention(
@@ -697,7 +974,8 @@ extern "C" int mi_paged_tree_attention(
     return mi_fail(MI_ERR_WORKSPACE, "mi_paged_tree_attention: workspace too small (see mi_tree_workspace_bytes)");
   if ((uintptr_t)workspace & 15) return mi_fail(MI_ERR_ALIGN, "mi_paged_tree_attention: workspace must be 16-byte aligned");
 
-  const TreeShape shape = tree_shape(T, R, Hq, Hkv, head_dim);
+  const bool many = !fp8 && (head_dim == 64 || head_dim == 128) && chunk_tokens % 32 == 0 && tree_mean_rows(T, R, G) > 64;
+  const TreeShape shape = tree_shape(T, R, Hq, Hkv, head_dim, many);
   const bool f16 = dtype == MI_DTYPE_FP16;
   TreeParams p;
   p.q = (const uint16_t*)q; p.q_st = q_stride_tok; p.q_sh = q_stride_head;
@@ -747,7 +1025,18 @@ extern "C" int mi_paged_tree_attention(
       if (nt == 1) MI_TREE(HD_, 1, 2, true);                                                                           \
       else MI_TREE(HD_, 2, 2, true);                                                                                   \
     } while (0)
-    if (fp8 && nt == 4) MI_TREE(64, 4, 2, true);
+#define MI_TREE_ROWS(HD_, W_)                                                                                          \
+    do {                                                                                                               \
+      if (f16) hipLaunchKernelGGL((paged_tree_rows_kernel<HD_, W_, true>), grid, block, lds, st, p);                   \
+      else hipLaunchKernelGGL((paged_tree_rows_kernel<HD_, W_, false>), grid, block, lds, st, p);                      \
+    } while (0)
+    if (many && shape.waves == 4) {
+      if (head_dim == 64) MI_TREE_ROWS(64, 4);
+      else MI_TREE_ROWS(128, 4);
+    } else if (many) {
+      if (head_dim == 64) MI_TREE_ROWS(64, 8);
+      else MI_TREE_ROWS(128, 8);
+    } else if (fp8 && nt == 4) MI_TREE(64, 4, 2, true);
     else if (fp8 && head_dim == 64) MI_TREE_8(64);
     else if (fp8) MI_TREE_8(128);
     else if (head_dim == 64) MI_TREE_16(64);
@@ -755,6 +1044,7 @@ extern "C" int mi_paged_tree_attention(
     else if (head_dim == 128) MI_TREE_16(128);
     else if (head_dim == 192) MI_TREE(192, 1, 1, false);
     else MI_TREE(256, 1, 1, false);
+#undef MI_TREE_ROWS
 #undef MI_TREE_8
 #undef MI_TREE_16
 #undef MI_TREE

@@ -152,8 +152,51 @@ def test_what_a_row_does_not_see_does_not_reach_it(mi, dev, dtype, fp8, d):
     assert torch.isfinite(got[[0, 1, 2, 4, 7, 8, 9, 11]]).all() and not torch.isfinite(got[3]).all()
 
 
+@pytest.mark.parametrize("nodes,Hq,d,dtype", [(33, 8, 128, BF16), (70, 8, 128, FP16), (90, 4, 64, BF16), (150, 4, 64, FP16), (40, 8, 96, BF16), (40, 8, 256, FP16)])
+def test_what_a_row_does_not_see_does_not_reach_it_in_large_trees(mi, dev, nodes, Hq, d, dtype):
+    c = Case(dev, [nodes, nodes - 5], [60, 133], Hq=Hq, Hkv=2, d=d, dtype=dtype, shape="tree", seed=nodes)
+    for r in range(2):
+        for node, v in ((3, math.nan), (nodes // 2, math.inf), (nodes // 2 + 1, -math.inf), (nodes - 6, math.nan)):
+            chunk, at = osp.position(c.table[r].tolist(), 64, c.N, c.lens[r] - c.cu[r + 1] + c.cu[r] + node)
+            c.v[chunk, at, 0, ::3] = v
+            c.k[chunk, at, 1, 5] = v
+    got = c.check(mi)
+    assert torch.isfinite(got[0]).all() and not torch.isfinite(got[3]).all()
+
+
+@pytest.mark.parametrize("nodes,Hq,Hkv,d,chunk", [
+    ([64, 64], 16, 2, 128, 256), ([17, 61, 40, 0, 33], 32, 8, 128, 64), ([100, 20], 8, 8, 64, 32), ([256], 16, 2, 64, 64), ([90, 1, 1], 5, 1, 128, 96),
+    ([64, 64], 16, 2, 256, 64), ([64, 30], 16, 2, 96, 64), ([64, 64], 16, 2, 128, 48), ([130], 6, 6, 192, 16),
+])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_many_rows(mi, dev, nodes, Hq, Hkv, d, chunk, dtype):
+    Case(dev, nodes, [700 + 37 * i for i in range(len(nodes))], Hq=Hq, Hkv=Hkv, d=d, chunk=chunk, dtype=dtype, spare=2, seed=d + chunk).check(mi)
+    Case(dev, nodes, [3 * i for i in range(len(nodes))], Hq=Hq, Hkv=Hkv, d=d, chunk=chunk, dtype=dtype, seed=d + chunk).check(mi)
+
+
+def test_many_rows_of_an_fp8_cache(mi, dev):
+    for d, chunk in ((64, 64), (128, 64), (128, 16)):
+        Case(dev, [64, 41], [300, 777], Hq=16, Hkv=2, d=d, chunk=chunk, fp8=True, seed=d).check(mi)
+
+
+def test_many_rows_with_tables_and_lengths_that_do_not_fit(mi, dev):
+    c = Case(dev, [40, 50, 60], [300, 200, 500], seed=24)
+    c.table[0, 2], c.table[1, 0], c.table[1, 3], c.table[2, 8] = -1, c.N, 1 << 30, -7
+    c.check(mi)
+    c.lens = [4096, 30, -1]
+    c.check(mi)
+
+
 def test_what_lies_behind_a_request_is_not_read(mi, dev):
     c = Case(dev, [5, 3], [70, 20], seed=13)
+    used = torch.zeros(c.N, 64, dtype=torch.bool)
+    for r in range(2):
+        for k in range(c.lens[r]):
+            used[osp.position(c.table[r].tolist(), 64, c.N, k)] = True
+    c.k[~used] = math.nan
+    c.v[~used] = math.nan
+    assert torch.isfinite(c.check(mi)).all()
+    c = Case(dev, [45, 33], [70, 20], seed=13)
     used = torch.zeros(c.N, 64, dtype=torch.bool)
     for r in range(2):
         for k in range(c.lens[r]):
@@ -235,9 +278,10 @@ def test_a_chain_is_the_causal_call(mi, dev):
     c.check(mi)
 
 
-def test_replays_and_streams(mi, dev):
+@pytest.mark.parametrize("nodes", [[5, 12], [40, 64]])
+def test_replays_and_streams(mi, dev, nodes):
     """A captured call replayed among eager work, with new values in place, and a call on a stream of its own."""
-    c = Case(dev, [5, 12], [300, 64], seed=22)
+    c = Case(dev, nodes, [300, 64], seed=22)
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
     q, k, v = c.q.to(dev), c.k.to(dev), c.v.to(dev)
     args = (i32(c.cu), i32(c.lens), c.table.to(dev), c.mask.to(dev))
@@ -248,7 +292,7 @@ def test_replays_and_streams(mi, dev):
         aside = mi.ops.paged_tree_attention(q, k, v, *args, softmax_scale=c.scale)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(aside, eager)
-    work = torch.empty(mi._lib.load().mi_tree_workspace_bytes(17, 2, 8, 2, 128), dtype=torch.uint8, device=dev)
+    work = torch.empty(mi._lib.load().mi_tree_workspace_bytes(c.cu[-1], 2, 8, 2, 128), dtype=torch.uint8, device=dev)
     graph, out = torch.cuda.CUDAGraph(), torch.empty_like(q)
     with mi.ops.use_workspace(work):
         with torch.cuda.graph(graph):
