@@ -21,7 +21,7 @@
 // Only the tiles that reach past the context look at the bits.  A node's value row may hold infinities or NaN that rows
 // which do not see it must not meet, although a product multiplies it by their zeros: such values are taken out of their
 // tile and added to the sums of the rows that see them.
-#include <stdio.h>
+#include <type_traits>
 
 #include "mi_capi_internal.h"
 #include "mi_common.h"
@@ -524,37 +524,53 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
     const int slot = ((wave * LPW + i) % KLOADS) * 64 + lane, row = slot / (HD / 8), piece = slot % (HD / 8);
     src[i] = (uint32_t)row * (uint32_t)tok_bytes + 16u * (uint32_t)(piece ^ tree_swizzle<HD>(row));
   }
-  const int tiles_end = (end + TK - 1) / TK;
-  auto entry = [&](int tile) { return bt_row[tree_chunk_of(min(tile, tiles_end - 1) * TK, p.chunk_magic)]; };
-  uint32_t missing = 0;   // bit i: the chunk of the i-th tile in flight does not exist
-  auto issue = [&](int tile, int stage, int pc, int ahead) {
-    const int t0 = min(tile, tiles_end - 1) * TK, ci = tree_chunk_of(t0, p.chunk_magic);
+  // The next tile to load: its chunk's entry, the next chunk's (requested a chunk ahead), its place in the chunk.  Past the
+  // segment's last tile the loads fetch nothing (zeros), and so they do in a chunk that does not exist.
+  const int tiles_end = (end + TK - 1) / TK, chunk_tiles = p.chunk / TK, tile_bytes = TK * tok_bytes;
+  const int ci_last = tree_chunk_of(max(end - 1, 0), p.chunk_magic);
+  int i_tile = start / TK, i_ci = tree_chunk_of(start, p.chunk_magic), i_in = i_tile - i_ci * chunk_tiles, i_stage = 0;
+  int pc = bt_row[min(i_ci, ci_last)], pc_next = bt_row[min(i_ci + 1, ci_last)];
+  uint32_t missing = 0;   // bit of a tile in flight (its number modulo 32): its chunk does not exist
+  auto issue = [&] {
     const bool there = (uint32_t)pc < (uint32_t)p.n_chunks;
-    const int64_t off = (int64_t)(there ? pc : 0) * chunk_bytes + (int64_t)(t0 - ci * p.chunk) * tok_bytes;
-    const uint32_t nrec = there && tile < tiles_end ? (uint32_t)min(len - t0, TK) * (uint32_t)tok_bytes : 0u;
-    missing |= (there ? 0u : 1u) << ahead;
+    const int64_t off = (int64_t)(there ? pc : 0) * chunk_bytes + i_in * tile_bytes;
+    const uint32_t nrec = there && i_tile < tiles_end ? (uint32_t)min(len - i_tile * TK, TK) * (uint32_t)tok_bytes : 0u;
+    const uint32_t bit = 1u << (i_tile & 31);
+    missing = there ? missing & ~bit : missing | bit;
 #pragma unroll
     for (int i = 0; i < LPW; ++i) {
       const int k = wave * LPW + i;
-      const bool key = k < KLOADS;
-      const uint64_t a = (key ? kbase : vbase) + (uint64_t)off;
+      const uint64_t a = (k < KLOADS ? kbase : vbase) + (uint64_t)off;
       u32x4_t rs;
       rs.x = (uint32_t)a;
       rs.y = (uint32_t)(a >> 32);
       rs.z = nrec;
       rs.w = 0x00020000u;
-      const uint32_t m0 = lds0 + (uint32_t)(stage * STAGE + 1024 * k);
+      const uint32_t m0 = lds0 + (uint32_t)(i_stage * STAGE + 1024 * k);
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(src[i]), "s"(rs)
                    : "memory", "m0");
     }
+    i_stage = i_stage + 1 == STAGES ? 0 : i_stage + 1;
+    ++i_tile;
+    if (++i_in == chunk_tiles) {
+      i_in = 0;
+      ++i_ci;
+      pc = pc_next;
+      pc_next = bt_row[min(i_ci + 1, ci_last)];
+    }
   };
 
-  float m_run[NQ], l_run[NQ];
-  f32x4_t acc[NQ][DV];
+  // Softmax: exponentials are taken against a reference per row, which moves only when a probability leaves a window: with
+  // bf16 the row's largest goes to 2^-30 when it moves, with fp16 to 2^-3, and 2 is the limit of both (the exponent's highest
+  // bit, looked at in the packed words: 5 instructions where the maximum of the scores takes 20).  Row sums come from the
+  // matrix cores.
+  constexpr float kHeadroom = F16 ? 3.f : 30.f, kNoReference = 3e38f;   // (none: any score leaves the window, -inf stays 0)
+  float neg[NQ];   // a probability is 2^(score * scale + neg)
+  f32x4_t acc[NQ][DV], sum[NQ];
 #pragma unroll
   for (int nt = 0; nt < NQ; ++nt) {
-    m_run[nt] = -3e38f;
-    l_run[nt] = 0.f;
+    neg[nt] = kNoReference;
+    sum[nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < DV; ++e) acc[nt][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
@@ -565,123 +581,193 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
   const int v_row = 4 * g + (m16 >> 2);
   const uint32_t v_at = (uint32_t)(HALF + v_row * ROWB + ((((m16 >> 1) & 1) ^ tree_swizzle<HD>(v_row)) << 4) + 8 * (m16 & 1));
 
+  // Probabilities of two scores (of a tile's eight per row tile and lane): chunk c is row tile c >> 2, sub-tile c >> 1 & 1.
+  auto chunk = [&](const f32x4_t (&S)[NQ][2], uint4 (&P)[NQ], int c) {
+    const int nt = c >> 2, u = c >> 1 & 1, i = 2 * (c & 1);
+    const uint32_t w = pack2<F16>(fast_exp2(__builtin_fmaf(S[nt][u][i], p.scale_log2, neg[nt])),
+                                  fast_exp2(__builtin_fmaf(S[nt][u][i + 1], p.scale_log2, neg[nt])));
+    const int d = c & 3;
+    if (d == 0) P[nt].x = w; else if (d == 1) P[nt].y = w; else if (d == 2) P[nt].z = w; else P[nt].w = w;
+  };
+  auto leaves_window = [&](const uint4 (&P)[NQ]) {
+    const uint32_t any = (P[0].x | P[0].y | P[0].z | P[0].w) | (P[1].x | P[1].y | P[1].z | P[1].w);
+    return __builtin_amdgcn_ballot_w64((any & 0x40004000u) != 0) != 0;
+  };
+  auto move_reference = [&](const f32x4_t (&S)[NQ][2], uint4 (&P)[NQ]) {
+#pragma unroll
+    for (int nt = 0; nt < NQ; ++nt) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, S[nt][i >> 2][i & 3]);
+      const float to = fminf(neg[nt], __builtin_fmaf(-rowgroup_max(top), p.scale_log2, -kHeadroom));
+      const float alpha = fast_exp2(to - neg[nt]);
+      neg[nt] = to;
+#pragma unroll
+      for (int e = 0; e < DV; ++e) {
+        acc[nt][e][0] *= alpha; acc[nt][e][1] *= alpha; acc[nt][e][2] *= alpha; acc[nt][e][3] *= alpha;
+      }
+      sum[nt][0] *= alpha; sum[nt][1] *= alpha; sum[nt][2] *= alpha; sum[nt][3] *= alpha;
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) chunk(S, P, c);
+  };
+  auto key_piece = [&](const uint8_t* at, int n) {   // sub-tile n & 1, step n >> 1
+    return *reinterpret_cast<const uint4*>(at + (k_at ^ (64u * (n >> 1))) + 16 * (n & 1) * ROWB);
+  };
+  auto value_piece = [&](const uint8_t* at, int e) {
+    const uint8_t* v = at + (v_at ^ (32u * e));
+    const uint2 a = lds_ld8_tr(v), b = lds_ld8_tr(v + 16 * ROWB);
+    return make_uint4(a.x, a.y, b.x, b.y);
+  };
+  // One column of O^T += V^T P^T.  ODD: its values may be infinities or NaN that not every row sees (`seen`).
+  auto column = [&](auto Oc, int e, uint4 v, const uint4 (&P)[NQ], const uint32_t (&seen)[NQ]) {
+    if constexpr (decltype(Oc)::value) {
+      if (__builtin_amdgcn_ballot_w64((tree_odd16<F16>(v.x) | tree_odd16<F16>(v.y) | tree_odd16<F16>(v.z) | tree_odd16<F16>(v.w)) != 0)) {
+        const uint2 lo = make_uint2(tree_places<F16>(v.x), tree_places<F16>(v.y)), hi = make_uint2(tree_places<F16>(v.z), tree_places<F16>(v.w));
+#pragma unroll
+        for (int nt = 0; nt < NQ; ++nt) {
+          const f32x4_t n = mfma_16x16x16<F16>(hi, tree_sees<F16>(seen[nt] >> 4), mfma_16x16x16<F16>(lo, tree_sees<F16>(seen[nt]), zero4));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[nt][e][i] += tree_odd_sum(n[i]);
+        }
+        v = make_uint4(tree_even16<F16>(v.x), tree_even16<F16>(v.y), tree_even16<F16>(v.z), tree_even16<F16>(v.w));
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NQ; ++nt) acc[nt][e] = mfma_16x16x32<F16>(v, P[nt], acc[nt][e]);
+  };
+  // This wavefront's share of the next tile has landed (what it issued after that may be on its way), then everyone's; the
+  // tile two back is read by nobody any more, and its place is filled.
+  auto turn = [&] {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 4) * LPW) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    issue();
+  };
+#define MI_SB() __builtin_amdgcn_sched_barrier(0)
+
   // (the queries have arrived before any direct load: the compiler waits for them here and not among those)
 #pragma unroll
   for (int nt = 0; nt < NQ; ++nt)
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) asm volatile("" ::"v"(qf[nt][kk].x), "v"(qf[nt][kk].y), "v"(qf[nt][kk].z), "v"(qf[nt][kk].w));
   __syncthreads();   // (the stages are free: every wavefront has left the segment before)
-  const int t_first = start / TK;
   if (start < end) {
-    for (int i = 0; i < STAGES - 1; ++i) issue(t_first + i, i, entry(t_first + i), i);
-    int pc = entry(t_first + STAGES - 1);
-    int stage = 0, fill = STAGES - 1;
-    for (int T = start; T < end; T += TK) {
-      // this wavefront's share of the tile has landed (what it issued after that may be on its way), then everyone's
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * LPW) : "memory");
-      __builtin_amdgcn_s_barrier();
-      const int tile = T / TK;
-      const int next = entry(tile + STAGES);   // (a tile before its use)
-      const bool page = !(missing & 1u);
-      missing >>= 1;
-      issue(tile + STAGES - 1, fill, pc, STAGES - 2);
-      fill = stage;
-      const uint8_t* const at = lds + stage * STAGE;
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
-      if (!idle) {
-        const bool masked = T + TK > min(ctx, end) || !page;
-        f32x4_t sc[NQ][2];
+    // (the values "before the first tile" are zeros: their probabilities are, and zero times a stale value must not be NaN)
+    for (int i = lane * 16; i < HALF; i += 1024) *reinterpret_cast<uint4*>(lds + (STAGES - 1) * STAGE + HALF + i) = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < STAGES - 2; ++i) issue();
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 3) * LPW) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+  if (idle) {   // (a part without rows)
+    for (int T = start; T < end; T += TK) turn();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    return;
+  }
+  if (start < end) {
+    // The stream of a tile: its scores, piece by piece, beside the probabilities of the tile before; then the values of that
+    // one.  Pieces come from LDS three ahead of their products, across the barrier and from tile to tile.
+    constexpr int NK = 2 * KS, RING = 4, AHEAD = RING - 1;
+    static_assert((NK + DV) % RING == 0 && 8 % NK == 0, "the next tile's first pieces follow the last column");
+    uint4 fr[RING], P[NQ];
+    uint32_t seen[NQ];
+    f32x4_t S[NQ][2], Sn[NQ][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+    for (int nt = 0; nt < NQ; ++nt) {
+      P[nt] = make_uint4(0, 0, 0, 0);
+      seen[nt] = 255u;
 #pragma unroll
-          for (int kk = 0; kk < KS; ++kk) {
-            const uint4 k = *reinterpret_cast<const uint4*>(at + (k_at ^ (64u * kk)) + 16 * u * ROWB);
+      for (int u = 0; u < 2; ++u) S[nt][u] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    }
+    int T = start, stage = 0, before = STAGES - 1;
 #pragma unroll
-            for (int nt = 0; nt < NQ; ++nt) sc[nt][u] = mfma_16x16x32<F16>(k, qf[nt][kk], kk ? sc[nt][u] : zero4);
-          }
-        }
-        uint32_t seen[NQ];
-        if (masked) {
+    for (int n = 0; n < AHEAD; ++n) fr[n] = key_piece(lds, n);
+    auto step = [&](auto Mc) {
+      constexpr bool MASK = decltype(Mc)::value;
+      const int next = stage + 1 == STAGES ? 0 : stage + 1;
+      const uint8_t* const at_k = lds + stage * STAGE;
+      const uint8_t* const at_v = lds + before * STAGE;
+      const uint8_t* const at_next = lds + next * STAGE;
+      auto request = [&](int n) {
+        fr[n % RING] = n < NK ? key_piece(at_k, n) : n < NK + DV ? value_piece(at_v, n - NK) : key_piece(at_next, n - NK - DV);
+      };
 #pragma unroll
-          for (int nt = 0; nt < NQ; ++nt) {
-            const uint32_t* bits = p.mask + (int64_t)q_row[nt] * p.mask_st;
-            seen[nt] = 0;
+      for (int n = 0; n < NK; ++n) {
+        request(n + AHEAD);
+        MI_SB();
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int t0 = T + 16 * u + 4 * g;
-              uint32_t b = page ? tree_bits(bits, p.mask_words, t0 - ctx) & 15u : 0u;
-              const int left = end - t0;
-              b &= left >= 4 ? 15u : left > 0 ? (1u << left) - 1u : 0u;
-              seen[nt] |= b << (4 * u);
+        for (int nt = 0; nt < NQ; ++nt) Sn[nt][n & 1] = mfma_16x16x32<F16>(fr[n % RING], qf[nt][n >> 1], n >> 1 ? Sn[nt][n & 1] : zero4);
+        MI_SB();
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (!(b >> i & 1u)) sc[nt][u][i] = -INFINITY;
-            }
-          }
-        }
-        uint4 pf[NQ];
+        for (int c = 8 / NK * n; c < 8 / NK * (n + 1); ++c) chunk(S, P, c);
+        MI_SB();
+      }
+      if (leaves_window(P)) move_reference(S, P);
+      turn();
+#pragma unroll
+      for (int e = 0; e < DV; ++e) {
+        request(NK + e + AHEAD);
+        MI_SB();
+        column(Mc, e, fr[(NK + e) % RING], P, seen);
+        MI_SB();
+      }
+#pragma unroll
+      for (int nt = 0; nt < NQ; ++nt) sum[nt] = mfma_16x16x32<F16>(ones, P[nt], sum[nt]);
+      const bool page = !(missing >> ((T / TK) & 31) & 1u);
+#pragma unroll
+      for (int nt = 0; nt < NQ; ++nt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) S[nt][u] = Sn[nt][u];
+      if constexpr (MASK) {
 #pragma unroll
         for (int nt = 0; nt < NQ; ++nt) {
-          float tmax = fmaxf(fmaxf(sc[nt][0][0], sc[nt][0][1]), fmaxf(sc[nt][0][2], sc[nt][0][3]));
-          tmax = fmaxf(tmax, fmaxf(fmaxf(sc[nt][1][0], sc[nt][1][1]), fmaxf(sc[nt][1][2], sc[nt][1][3])));
-          const float m_new = fmaxf(m_run[nt], rowgroup_max(tmax) * p.scale_log2);
-          const float alpha = fast_exp2(m_run[nt] - m_new);
-          m_run[nt] = m_new;
-          float e8[8];
+          const uint32_t* bits = p.mask + (int64_t)q_row[nt] * p.mask_st;
+          seen[nt] = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) e8[i] = fast_exp2(__builtin_fmaf(sc[nt][i >> 2][i & 3], p.scale_log2, -m_new));
-          pf[nt] = make_uint4(pack2<F16>(e8[0], e8[1]), pack2<F16>(e8[2], e8[3]), pack2<F16>(e8[4], e8[5]), pack2<F16>(e8[6], e8[7]));
-          const f32x4_t sum = mfma_16x16x32<F16>(ones, pf[nt], zero4);
-          l_run[nt] = l_run[nt] * alpha + sum[0];
-          if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+          for (int u = 0; u < 2; ++u) {
+            const int t0 = T + 16 * u + 4 * g;
+            uint32_t b = page ? tree_bits(bits, p.mask_words, t0 - ctx) & 15u : 0u;
+            const int left = end - t0;
+            b &= left >= 4 ? 15u : left > 0 ? (1u << left) - 1u : 0u;
+            seen[nt] |= b << (4 * u);
 #pragma unroll
-            for (int e = 0; e < DV; ++e) {
-              acc[nt][e][0] *= alpha; acc[nt][e][1] *= alpha; acc[nt][e][2] *= alpha; acc[nt][e][3] *= alpha;
-            }
+            for (int i = 0; i < 4; ++i)
+              if (!(b >> i & 1u)) S[nt][u][i] = -INFINITY;
           }
         }
-        auto values = [&](int e) {
-          const uint8_t* v = at + (v_at ^ (32u * e));
-          const uint2 a = lds_ld8_tr(v), b = lds_ld8_tr(v + 16 * ROWB);
-          return make_uint4(a.x, a.y, b.x, b.y);
-        };
-        if (!masked) {
+      } else if (!page) {
 #pragma unroll
-          for (int e = 0; e < DV; ++e) {
-            const uint4 v = values(e);
+        for (int nt = 0; nt < NQ; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < NQ; ++nt) acc[nt][e] = mfma_16x16x32<F16>(v, pf[nt], acc[nt][e]);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < DV; ++e) {
-            __builtin_amdgcn_sched_barrier(0);   // (one column at a time: registers)
-            uint4 v = values(e);
-            if (__builtin_amdgcn_ballot_w64((tree_odd16<F16>(v.x) | tree_odd16<F16>(v.y) | tree_odd16<F16>(v.z) | tree_odd16<F16>(v.w)) != 0)) {
-              const uint2 lo = make_uint2(tree_places<F16>(v.x), tree_places<F16>(v.y)), hi = make_uint2(tree_places<F16>(v.z), tree_places<F16>(v.w));
-#pragma unroll
-              for (int nt = 0; nt < NQ; ++nt) {
-                const f32x4_t n = mfma_16x16x16<F16>(hi, tree_sees<F16>(seen[nt] >> 4), mfma_16x16x16<F16>(lo, tree_sees<F16>(seen[nt]), zero4));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[nt][e][i] += tree_odd_sum(n[i]);
-              }
-              v = make_uint4(tree_even16<F16>(v.x), tree_even16<F16>(v.y), tree_even16<F16>(v.z), tree_even16<F16>(v.w));
-            }
-#pragma unroll
-            for (int nt = 0; nt < NQ; ++nt) acc[nt][e] = mfma_16x16x32<F16>(v, pf[nt], acc[nt][e]);
-          }
-        }
+          for (int u = 0; u < 2; ++u) S[nt][u] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       }
-      pc = next;
+      before = stage;
+      stage = next;
+      T += TK;
+    };
+    const int open = min(ctx, end);   // every row sees the tokens before
+    while (T + TK <= open) step(std::false_type{});
+    while (T < end) step(std::true_type{});
+#pragma unroll
+    for (int c = 0; c < 8; ++c) chunk(S, P, c);
+    if (leaves_window(P)) move_reference(S, P);
+#pragma unroll
+    for (int e = 0; e < DV; ++e) {
+      MI_SB();   // (one column at a time: registers)
+      column(std::true_type{}, e, value_piece(lds + before * STAGE, e), P, seen);
     }
+#pragma unroll
+    for (int nt = 0; nt < NQ; ++nt) sum[nt] = mfma_16x16x32<F16>(ones, P[nt], sum[nt]);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load may still be on its way into this workgroup's LDS)
   }
+#undef MI_SB
 
   // ---- acc[nt][e][i] is element d = 16 e + 4 g + i of the row
 #pragma unroll
   for (int nt = 0; nt < NQ; ++nt) {
     if (!valid[nt]) continue;
-    const float l = l_run[nt], inv = l == 0.f ? 0.f : 1.f / l;
+    const float l = sum[nt][0], inv = l == 0.f ? 0.f : 1.f / l;
     if (s.whole) {
       uint16_t* o = p.out + (int64_t)q_row[nt] * p.o_st + (int64_t)q_head[nt] * p.o_sh + 4 * g;
 #pragma unroll
@@ -693,7 +779,7 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
 #pragma unroll
       for (int e = 0; e < DV; ++e)
         *reinterpret_cast<float4*>(o + 16 * e) = make_float4(acc[nt][e][0] * inv, acc[nt][e][1] * inv, acc[nt][e][2] * inv, acc[nt][e][3] * inv);
-      if (g == 0) p.part_lse[row] = l == 0.f ? -INFINITY : m_run[nt] + fast_log2(l);
+      if (g == 0) p.part_lse[row] = l == 0.f ? -INFINITY : fast_log2(l) - neg[nt];
     }
   }
 }
