@@ -589,6 +589,25 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
     const int d = c & 3;
     if (d == 0) P[nt].x = w; else if (d == 1) P[nt].y = w; else if (d == 2) P[nt].z = w; else P[nt].w = w;
   };
+  // The same in three stages -- scale and subtract, exponential, pack -- of three chunks at a time, so that no instruction
+  // waits for the one before it: at position n stage one of chunk n, two of chunk n - 1, three of chunk n - 2.
+  float xs[2][2], ps[2][2];   // of chunks n, n - 1
+  auto stages = [&](const f32x4_t (&S)[NQ][2], uint4 (&P)[NQ], int n) {
+    if (n >= 2 && n < 10) {
+      const int c = n - 2, nt = c >> 2, d = c & 3;
+      const uint32_t w = pack2<F16>(ps[c & 1][0], ps[c & 1][1]);
+      if (d == 0) P[nt].x = w; else if (d == 1) P[nt].y = w; else if (d == 2) P[nt].z = w; else P[nt].w = w;
+    }
+    if (n >= 1 && n < 9) {
+      ps[(n - 1) & 1][0] = fast_exp2(xs[(n - 1) & 1][0]);
+      ps[(n - 1) & 1][1] = fast_exp2(xs[(n - 1) & 1][1]);
+    }
+    if (n < 8) {
+      const int nt = n >> 2, u = n >> 1 & 1, i = 2 * (n & 1);
+      xs[n & 1][0] = __builtin_fmaf(S[nt][u][i], p.scale_log2, neg[nt]);
+      xs[n & 1][1] = __builtin_fmaf(S[nt][u][i + 1], p.scale_log2, neg[nt]);
+    }
+  };
   auto leaves_window = [&](const uint4 (&P)[NQ]) {
     const uint32_t any = (P[0].x | P[0].y | P[0].z | P[0].w) | (P[1].x | P[1].y | P[1].z | P[1].w);
     return __builtin_amdgcn_ballot_w64((any & 0x40004000u) != 0) != 0;
@@ -636,13 +655,16 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
 #pragma unroll
     for (int nt = 0; nt < NQ; ++nt) acc[nt][e] = mfma_16x16x32<F16>(v, P[nt], acc[nt][e]);
   };
-  // This wavefront's share of the next tile has landed (what it issued after that may be on its way), then everyone's; the
-  // tile two back is read by nobody any more, and its place is filled.
+  // This wavefront's share of the next tile (PAIRS: the next two) has landed (what it issued after that may be on its way),
+  // then everyone's; the tiles two (and three) back are read by nobody any more, and their places are filled.
+  constexpr bool PAIRS = STAGES == 8;
+  constexpr int FIRST = PAIRS ? STAGES - 3 : STAGES - 2;   // tiles that set out at the start
   auto turn = [&] {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 4) * LPW) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((PAIRS ? STAGES - 6 : STAGES - 4) * LPW) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     issue();
+    if (PAIRS) issue();
   };
 #define MI_SB() __builtin_amdgcn_sched_barrier(0)
 
@@ -655,13 +677,13 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
   if (start < end) {
     // (the values "before the first tile" are zeros: their probabilities are, and zero times a stale value must not be NaN)
     for (int i = lane * 16; i < HALF; i += 1024) *reinterpret_cast<uint4*>(lds + (STAGES - 1) * STAGE + HALF + i) = make_uint4(0, 0, 0, 0);
-    for (int i = 0; i < STAGES - 2; ++i) issue();
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 3) * LPW) : "memory");
+    for (int i = 0; i < FIRST; ++i) issue();
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((FIRST - 1) * LPW) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   }
   if (idle) {   // (a part without rows)
-    for (int T = start; T < end; T += TK) turn();
+    for (int T = start; T < end; T += PAIRS ? 2 * TK : TK) turn();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     return;
   }
@@ -681,8 +703,12 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
       for (int u = 0; u < 2; ++u) S[nt][u] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     }
     int T = start, stage = 0, before = STAGES - 1;
+    bool odd_tile = false;
+    uint4 Pnone[NQ];   // (stages 0 and 1 pack nothing)
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) fr[n] = key_piece(lds, n);
+    stages(S, Pnone, 0);
+    stages(S, Pnone, 1);
     auto step = [&](auto Mc) {
       constexpr bool MASK = decltype(Mc)::value;
       const int next = stage + 1 == STAGES ? 0 : stage + 1;
@@ -700,48 +726,54 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
         for (int nt = 0; nt < NQ; ++nt) Sn[nt][n & 1] = mfma_16x16x32<F16>(fr[n % RING], qf[nt][n >> 1], n >> 1 ? Sn[nt][n & 1] : zero4);
         MI_SB();
 #pragma unroll
-        for (int c = 8 / NK * n; c < 8 / NK * (n + 1); ++c) chunk(S, P, c);
+        for (int i = 8 / NK * n; i < 8 / NK * (n + 1); ++i) stages(S, P, i + 2);   // (0 and 1 beside the last columns before)
         MI_SB();
       }
       if (leaves_window(P)) move_reference(S, P);
-      turn();
-#pragma unroll
-      for (int e = 0; e < DV; ++e) {
-        request(NK + e + AHEAD);
-        MI_SB();
-        column(Mc, e, fr[(NK + e) % RING], P, seen);
-        MI_SB();
-      }
-#pragma unroll
-      for (int nt = 0; nt < NQ; ++nt) sum[nt] = mfma_16x16x32<F16>(ones, P[nt], sum[nt]);
+      if (!PAIRS || !odd_tile) turn();
+      // what no row of this tile's scores may count
       const bool page = !(missing >> ((T / TK) & 31) & 1u);
-#pragma unroll
-      for (int nt = 0; nt < NQ; ++nt)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) S[nt][u] = Sn[nt][u];
+      uint32_t sees[NQ];
       if constexpr (MASK) {
 #pragma unroll
         for (int nt = 0; nt < NQ; ++nt) {
           const uint32_t* bits = p.mask + (int64_t)q_row[nt] * p.mask_st;
-          seen[nt] = 0;
+          sees[nt] = 0;
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int t0 = T + 16 * u + 4 * g;
             uint32_t b = page ? tree_bits(bits, p.mask_words, t0 - ctx) & 15u : 0u;
             const int left = end - t0;
             b &= left >= 4 ? 15u : left > 0 ? (1u << left) - 1u : 0u;
-            seen[nt] |= b << (4 * u);
+            sees[nt] |= b << (4 * u);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (!(b >> i & 1u)) S[nt][u][i] = -INFINITY;
+              if (!(b >> i & 1u)) Sn[nt][u][i] = -INFINITY;
           }
         }
       } else if (!page) {
 #pragma unroll
         for (int nt = 0; nt < NQ; ++nt)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) S[nt][u] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int u = 0; u < 2; ++u) Sn[nt][u] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       }
+#pragma unroll
+      for (int e = 0; e < DV; ++e) {
+        request(NK + e + AHEAD);
+        MI_SB();
+        column(Mc, e, fr[(NK + e) % RING], P, seen);
+        MI_SB();
+        if (e >= DV - 2) stages(Sn, Pnone, e - (DV - 2));
+        MI_SB();
+      }
+#pragma unroll
+      for (int nt = 0; nt < NQ; ++nt) {
+        sum[nt] = mfma_16x16x32<F16>(ones, P[nt], sum[nt]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) S[nt][u] = Sn[nt][u];
+        if (MASK) seen[nt] = sees[nt];
+      }
+      odd_tile = !odd_tile;
       before = stage;
       stage = next;
       T += TK;
@@ -750,7 +782,7 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
     while (T + TK <= open) step(std::false_type{});
     while (T < end) step(std::true_type{});
 #pragma unroll
-    for (int c = 0; c < 8; ++c) chunk(S, P, c);
+    for (int n = 2; n < 10; ++n) stages(S, P, n);
     if (leaves_window(P)) move_reference(S, P);
 #pragma unroll
     for (int e = 0; e < DV; ++e) {
