@@ -21,6 +21,7 @@
 // Only the tiles that reach past the context look at the bits.  A node's value row may hold infinities or NaN that rows
 // which do not see it must not meet, although a product multiplies it by their zeros: such values are taken out of their
 // tile and added to the sums of the rows that see them.
+#include <atomic>
 #include <type_traits>
 
 #include "mi_capi_internal.h"
@@ -58,12 +59,20 @@ struct TreeParams {
   float scale_log2;
 };
 
-constexpr int kTreeRequestsPerLaunch = 2048;  // (their prefix sums lie in LDS, 24 bytes each)
+constexpr int kTreeRequestsPerLaunch = 2048;  // (their prefix sums lie in LDS)
 
 static __device__ __forceinline__ int tree_div_g(const TreeParams& p, int n) {
   return p.g_magic ? (int)__umulhi((uint32_t)n, p.g_magic) : n;
 }
 static __device__ __forceinline__ int tree_chunk_of(int tok, uint64_t magic) { return (int)(((uint64_t)(uint32_t)tok * magic) >> 40); }
+
+// A wave-uniform pointer to memory that no kernel writes meanwhile: its loads are scalar.
+template <typename T>
+static __device__ __forceinline__ const __attribute__((address_space(4))) T* tree_constant(const T* ptr) {
+  const uint64_t x = (uint64_t)(uintptr_t)ptr;
+  return (const __attribute__((address_space(4))) T*)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) |
+                                                      (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
 
 struct TreeSegment {
   int r, group, part;  // request, which of its groups, and which of its parts (the rows of a wavefront)
@@ -113,9 +122,10 @@ static __device__ __forceinline__ float tree_odd_sum(float count) {
 }
 
 // SHARE: neighbouring wavefronts take other parts of the same tokens, and a barrier per tile keeps them on one tile, whose
-// lines then come from memory once and from the CU's cache for the others.
+// lines then come from memory once and from the CU's cache for the others.  Where a request has fewer parts than there are
+// wavefronts, `ways` of them share a part and take every `ways`-th tile each; what they have is joined in LDS (`join`).
 template <int HD, int NT, int NQ, bool FP8, bool F16, bool SHARE>
-static __device__ __forceinline__ void tree_segment(const TreeParams& p, const TreeSegment& s, int h, int lane) {
+static __device__ __forceinline__ void tree_segment(const TreeParams& p, const TreeSegment& s, int h, int lane, int way, int ways, float* join) {
   constexpr int KS = HD / 32, DV = HD / 16, ESZ = FP8 ? 1 : 2, TK = 16 * NT, ROWS = 16 * NQ;
   constexpr int KL = FP8 ? KS / 2 : KS;      // 16-byte loads of a key row and lane
   constexpr int VD = FP8 ? DV / 4 : DV / 2;  // dwords per token and lane of the value operand
@@ -123,9 +133,15 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
   const int r = __builtin_amdgcn_readfirstlane(s.r), len = __builtin_amdgcn_readfirstlane(s.len);
   const int start = __builtin_amdgcn_readfirstlane(s.start), end = __builtin_amdgcn_readfirstlane(s.end);
   const int ctx = __builtin_amdgcn_readfirstlane(s.ctx);
+  h = __builtin_amdgcn_readfirstlane(h);
   const int last = max(min(end, len) - 1, 0);
+  const int step = SHARE ? TK * ways : TK;
   if (SHARE && tree_div_g(p, s.part * ROWS) >= s.nodes) {   // (a part without rows)
-    for (int T = start; T < end; T += TK) __builtin_amdgcn_s_barrier();
+    for (int T = start; T < end; T += step) __builtin_amdgcn_s_barrier();
+    if (ways > 1) {
+      __syncthreads();
+      __syncthreads();
+    }
     return;
   }
 
@@ -153,49 +169,48 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
   const uint32_t tok_bytes = (uint32_t)(p.kv_st * ESZ);
   const uint32_t k_col = 16u * (uint32_t)g, v_col = (uint32_t)(DV * m16 * ESZ);
 
-  // Block-table cursor: the current chunk's entry and the next one's as scalars, the one after in flight (requested two
-  // chunks before its use).  An entry that names no chunk of the cache becomes -1: its tokens are seen by no row, and
-  // their loads go to chunk 0.
-  const int32_t* const bt_row = p.bt + (int64_t)(p.r_base + r) * p.bt_stride;
+  // Block-table cursor: the current chunk's entry and the next one's, the one after in flight (requested two chunks before
+  // its use), an fp8 cache's scale one chunk ahead.  Table and scales lie in the constant address space: scalar loads, which
+  // wait for no tile.  An entry that names no chunk of the cache becomes -1: its tokens are seen by no row, and their loads
+  // go to chunk 0.
+  const auto* const bt_row = tree_constant(p.bt + (int64_t)(p.r_base + r) * p.bt_stride);
   const int ci_last = tree_chunk_of(last, p.chunk_magic);
   struct Cursor {
     int ci, pc, pc_next, pc_after;
     float sc, sc_next;
   };
-  auto entry_load = [&](int ci) {
-    const int e = bt_row[min(ci, ci_last)];
-    return (uint32_t)e < (uint32_t)p.n_chunks ? e : -1;
-  };
-  auto scale_load = [&](const float* scales, int pc) { return scales[(int64_t)max(pc, 0) * p.Hkv + h]; };
-  auto uniform_f = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
+  auto entry_load = [&](int ci) { return bt_row[min(ci, ci_last)]; };
+  auto entry = [&](int e) { return (uint32_t)e < (uint32_t)p.n_chunks ? e : -1; };
+  auto scale_load = [&](const float* scales, int pc) { return tree_constant(scales)[(int64_t)max(pc, 0) * p.Hkv + h]; };
   auto follow = [&](Cursor& c, const float* scales, int ci) {
     if (ci != c.ci) {
+      const bool far = SHARE && ci != c.ci + 1;   // (a step over several chunks)
       c.ci = ci;
-      c.pc = c.pc_next;
-      c.pc_next = __builtin_amdgcn_readfirstlane(c.pc_after);
+      c.pc = far ? entry(entry_load(ci)) : c.pc_next;
+      c.pc_next = entry(far ? entry_load(ci + 1) : c.pc_after);
       c.pc_after = entry_load(ci + 2);
       if (FP8) {
-        c.sc = uniform_f(c.sc_next);
+        c.sc = far ? scale_load(scales, c.pc) : c.sc_next;
         c.sc_next = scale_load(scales, c.pc_next);
       }
     }
   };
+  const int begin = SHARE ? start + TK * way : start;
   Cursor kcur, vcur;
   {
-    const int ci0 = tree_chunk_of(min(start, last), p.chunk_magic);
+    const int ci0 = tree_chunk_of(min(begin, last), p.chunk_magic);
     const int e0 = entry_load(ci0), e1 = entry_load(ci0 + 1), e2 = entry_load(ci0 + 2);
     kcur.ci = ci0;
-    kcur.pc = __builtin_amdgcn_readfirstlane(e0);
-    kcur.pc_next = __builtin_amdgcn_readfirstlane(e1);
+    kcur.pc = entry(e0);
+    kcur.pc_next = entry(e1);
     kcur.pc_after = e2;
     kcur.sc = kcur.sc_next = 1.f;
     vcur = kcur;
     if (FP8) {
-      const float a = scale_load(p.k_scale, kcur.pc), b = scale_load(p.v_scale, kcur.pc);
+      kcur.sc = scale_load(p.k_scale, kcur.pc);
+      vcur.sc = scale_load(p.v_scale, kcur.pc);
       kcur.sc_next = scale_load(p.k_scale, kcur.pc_next);
       vcur.sc_next = scale_load(p.v_scale, kcur.pc_next);
-      kcur.sc = uniform_f(a);
-      vcur.sc = uniform_f(b);
     }
   }
 
@@ -253,10 +268,11 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
   const f32x4_t zero4 = {0.f, 0.f, 0.f, 0.f};
 
   if (start < end) {
-    load_k(start);
-    load_v(start);
+    load_k(begin);
+    load_v(begin);
   }
-  for (int T = start; T < end; T += TK) {
+  // (SHARE: as many tiles for every wavefront; those past the segment's end are seen by no row)
+  for (int T = begin; T < (SHARE ? end + TK * way : end); T += step) {
     // ---- S^T = K Q^T
     const float mul = FP8 ? p.scale_log2 * ksc : p.scale_log2;
     const bool masked = T + TK > min(ctx, end) || !k_page;   // wave-uniform
@@ -286,7 +302,7 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
     }
     __builtin_amdgcn_sched_barrier(0);
     if (SHARE) __builtin_amdgcn_s_barrier();
-    load_k(T + TK);   // (the key registers are free again)
+    load_k(T + step);   // (the key registers are free again)
     __builtin_amdgcn_sched_barrier(0);
     if (FP8) {        // a scale may have any sign: the maximum is of the products' own scores
 #pragma unroll
@@ -413,10 +429,52 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
         }
       }
     __builtin_amdgcn_sched_barrier(0);
-    load_v(T + TK);
+    load_v(T + step);
     __builtin_amdgcn_sched_barrier(0);
   }
 
+  if (SHARE && ways > 1) {
+    // a register of all lanes after the other: the accumulators, the maximum and the sum of every row tile
+    constexpr int WORDS = NQ * (4 * DV + 2);
+    if (way) {
+      float* at = join + lane;
+#pragma unroll
+      for (int nt = 0; nt < NQ; ++nt) {
+#pragma unroll
+        for (int e = 0; e < DV; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) at[64 * ((nt * DV + e) * 4 + i)] = acc[nt][e][i] * unit;
+        at[64 * (4 * NQ * DV + 2 * nt)] = m_run[nt];
+        at[64 * (4 * NQ * DV + 2 * nt + 1)] = l_run[nt];
+      }
+    }
+    __syncthreads();
+    if (!way) {
+#pragma unroll
+      for (int nt = 0; nt < NQ; ++nt)
+#pragma unroll
+        for (int e = 0; e < DV; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[nt][e][i] *= unit;
+      unit = 1.f;
+      for (int w = 1; w < ways; ++w) {
+        const float* at = join + (size_t)w * 64 * WORDS + lane;
+#pragma unroll
+        for (int nt = 0; nt < NQ; ++nt) {
+          const float m2 = at[64 * (4 * NQ * DV + 2 * nt)], l2 = at[64 * (4 * NQ * DV + 2 * nt + 1)];
+          const float m = fmaxf(m_run[nt], m2), a = fast_exp2(m_run[nt] - m), b = fast_exp2(m2 - m);
+          m_run[nt] = m;
+          l_run[nt] = l_run[nt] * a + l2 * b;
+#pragma unroll
+          for (int e = 0; e < DV; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[nt][e][i] = acc[nt][e][i] * a + at[64 * ((nt * DV + e) * 4 + i)] * b;
+        }
+      }
+    }
+    __syncthreads();   // (the next segment's may come)
+    if (way) return;
+  }
   // ---- acc[nt][e][i] is element d = DV (4g + i) + e of the row
 #pragma unroll
   for (int nt = 0; nt < NQ; ++nt) {
@@ -456,16 +514,6 @@ static __device__ __forceinline__ TreeRequest tree_request(const TreeParams& p, 
   t.nodes = min(max(p.cu_q[i + 1], t.q_begin), p.T) - t.q_begin;
   t.len = (int)min((int64_t)max(p.lens[i], 0), (int64_t)p.table_cols * p.chunk);
   return t;
-}
-
-// Inclusive sum over the lanes of a wavefront.
-static __device__ __forceinline__ int64_t tree_scan(int64_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
-  return v;
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
@@ -513,8 +561,7 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
   const uint64_t vbase = uniform64((uint64_t)(uintptr_t)(p.vc + (int64_t)h * p.kv_sh * 2)) & 0xffffffffffffull;
   const int64_t chunk_bytes = p.kv_sc * 2;
   const int tok_bytes = p.kv_st * 2;
-  // (the block table in the constant address space: scalar loads, which leave the count of the direct loads alone)
-  const auto* const bt_row = (const __attribute__((address_space(4))) int32_t*)uniform64((uint64_t)(uintptr_t)(p.bt + (int64_t)(p.r_base + s.r) * p.bt_stride));
+  const auto* const bt_row = tree_constant(p.bt + (int64_t)(p.r_base + s.r) * p.bt_stride);   // (scalar loads leave the count of the direct loads alone)
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
 
   // this wavefront's loads of a tile: which piece of which row each lane fetches
@@ -816,94 +863,120 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
   }
 }
 
-// The span of this workgroup along the tiles of all (request, group) pairs, as segments one after the other: seg(segment) with
-// the segment's group; every wavefront walks the same ones.  Clears the rows behind the last request on the way.
+// The span of this workgroup along the tiles of all (request, group) pairs, as segments one after the other: seg(segment);
+// every wavefront walks the same ones.  Up to 64 requests lie in the lanes of every wavefront (no LDS, no barrier), more in
+// dynamic LDS: tiles and groups of requests 0 .. i.  (The entry point has made sure that all tiles together are an int.)
+// Clears the rows behind the last request on the way.
 template <int HD, int TK, typename Seg>
 static __device__ __forceinline__ void tree_walk(const TreeParams& p, Seg seg) {
-  extern __shared__ int64_t tree_lds[];
-  int64_t* const cum = tree_lds;                               // tiles of requests 0 .. i
-  int32_t* const first = reinterpret_cast<int32_t*>(cum + p.R);  // groups of requests 0 .. i
+  extern __shared__ int32_t tree_lds[];
+  int32_t* const cum = tree_lds;
+  int32_t* const first = cum + p.R;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool in_lanes = p.R <= 64;
 
-  if (wave == 0) {
-    int64_t tiles = 0;
-    int64_t parts = 0;
-    for (int base = 0; base < p.R; base += 64) {
-      const int i = base + lane;
-      int n_parts = 0, n_tiles = 0;
-      if (i < p.R) {
-        const TreeRequest t = tree_request(p, i);
-        n_parts = (int)(((int64_t)t.nodes * p.G + p.rows - 1) / p.rows);
-        n_tiles = max((t.len + TK - 1) / TK, 1);   // (a request without tokens has a tile in which nothing is seen)
-      }
-      const int64_t ct = tree_scan((int64_t)n_parts * n_tiles, lane) + tiles, cp = tree_scan(n_parts, lane) + parts;
-      if (i < p.R) {
-        cum[i] = ct;
-        first[i] = (int)cp;
-      }
-      tiles = __shfl(ct, 63, 64);
-      parts = __shfl(cp, 63, 64);
+  TreeRequest mine{0, 0, 0};   // of request `lane` (in lanes)
+  int cum_l = 0, first_l = 0;
+  auto scan64 = [&](int base) {
+    const int i = base + lane;
+    int n_groups = 0, n_tiles = 0;
+    if (i < p.R) {
+      mine = tree_request(p, i);
+      n_groups = (int)(((int64_t)mine.nodes * p.G + p.rows - 1) / p.rows);
+      n_tiles = max((mine.len + TK - 1) / TK, 1);   // (a request without tokens has a tile in which nothing is seen)
     }
+    cum_l = wave_scan(n_groups * n_tiles);
+    first_l = wave_scan(n_groups);
+  };
+  if (in_lanes) {
+    scan64(0);
+  } else {
+    if (wave == 0) {
+      int tiles = 0, groups = 0;
+      for (int base = 0; base < p.R; base += 64) {
+        scan64(base);
+        if (base + lane < p.R) {
+          cum[base + lane] = tiles + cum_l;
+          first[base + lane] = groups + first_l;
+        }
+        tiles += __builtin_amdgcn_readlane(cum_l, 63);
+        groups += __builtin_amdgcn_readlane(first_l, 63);
+      }
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.pairs = first[p.R - 1];
+  auto cum_at = [&](int i) { return in_lanes ? __builtin_amdgcn_readlane(cum_l, i) : __builtin_amdgcn_readfirstlane(cum[i]); };
+  auto first_at = [&](int i) { return in_lanes ? __builtin_amdgcn_readlane(first_l, i) : __builtin_amdgcn_readfirstlane(first[i]); };
+  auto request_at = [&](int i) {
+    if (!in_lanes) return tree_request(p, i);
+    return TreeRequest{__builtin_amdgcn_readlane(mine.q_begin, i), __builtin_amdgcn_readlane(mine.nodes, i), __builtin_amdgcn_readlane(mine.len, i)};
+  };
+  const int total = cum_at(p.R - 1), pairs = first_at(p.R - 1);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.pairs = pairs;
 
   // rows behind the last request are zeros
   if (p.last_slice) {
-    const int tq = min(max(p.cu_q[p.R], 0), p.T);
-    const int64_t per_row = (int64_t)p.Hq * HD / 8, all = (int64_t)(p.T - tq) * per_row;
-    const int64_t step = (int64_t)gridDim.x * gridDim.y * blockDim.x;
-    for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < all; i += step) {
-      const int64_t row = i / per_row;
-      const int e = (int)(i - row * per_row) * 8;
-      st16(p.out + (tq + row) * p.o_st + (int64_t)(e / HD) * p.o_sh + e % HD, make_uint4(0, 0, 0, 0));
+    const TreeRequest end = request_at(p.R - 1);
+    const int tq = end.q_begin + end.nodes;
+    if (tq < p.T) {
+      const int64_t per_row = (int64_t)p.Hq * HD / 8, all = (int64_t)(p.T - tq) * per_row;
+      const int64_t step = (int64_t)gridDim.x * gridDim.y * blockDim.x;
+      for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < all; i += step) {
+        const int64_t row = i / per_row;
+        const int e = (int)(i - row * per_row) * 8;
+        st16(p.out + (tq + row) * p.o_st + (int64_t)(e / HD) * p.o_sh + e % HD, make_uint4(0, 0, 0, 0));
+      }
     }
   }
 
   // The span: equal shares where the tiles fill the grid, otherwise few tiles each -- a span's tiles follow one another,
   // every further span of a pair is one more partial to merge.
-  const int64_t total = cum[p.R - 1];
-  const int pairs = first[p.R - 1];
   if (total == 0) return;
   const int span = max(1, (int)rintf(__builtin_amdgcn_sqrtf(0.035f * (float)total * __builtin_amdgcn_rcpf((float)pairs))));
-  int64_t t0, t1;
-  if (total >= (int64_t)p.grid * span) {
-    const int64_t per = total / p.grid;
-    const int rem = (int)(total - per * p.grid);
-    t0 = blockIdx.x * per + min((int)blockIdx.x, rem);
+  int t0, t1;
+  if (total / span >= p.grid) {
+    const int per = total / p.grid, rem = total - per * p.grid;
+    t0 = (int)blockIdx.x * per + min((int)blockIdx.x, rem);
     t1 = t0 + per + ((int)blockIdx.x < rem ? 1 : 0);
   } else {
-    t0 = (int64_t)blockIdx.x * span;
+    t0 = (int)blockIdx.x * span;
     t1 = min(t0 + span, total);
   }
   if (t0 >= t1) return;
-  int lo = 0, hi = p.R - 1;   // the first request whose tiles reach beyond t0
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (cum[mid] > t0) hi = mid; else lo = mid + 1;
+  int r;   // the first request whose tiles reach beyond t0
+  if (in_lanes) {
+    r = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < p.R && cum_l > t0));
+  } else {
+    int lo = 0, hi = p.R - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (cum[mid] > t0) hi = mid; else lo = mid + 1;
+    }
+    r = __builtin_amdgcn_readfirstlane(lo);
   }
-  for (int r = lo; t0 < t1 && r < p.R; ++r) {
-    const int64_t rb = r ? cum[r - 1] : 0, re = cum[r];
+  for (; t0 < t1; ++r) {
+    const int rb = r ? cum_at(r - 1) : 0, re = cum_at(r);
     if (t0 >= re) continue;
-    const TreeRequest t = tree_request(p, r);
+    const TreeRequest t = request_at(r);
     const int tiles = max((t.len + TK - 1) / TK, 1);
     TreeSegment s;
     s.r = r; s.q_begin = t.q_begin; s.nodes = t.nodes; s.len = t.len; s.ctx = t.len - t.nodes;
     while (t0 < t1 && t0 < re) {
-      const int group = __builtin_amdgcn_readfirstlane((int)((t0 - rb) / tiles));
-      s.group = group;
-      const int tb = (int)(t0 - rb - (int64_t)group * tiles), te = (int)min((int64_t)tiles, tb + (t1 - t0));
+      s.group = __builtin_amdgcn_readfirstlane((t0 - rb) / tiles);
+      const int tb = t0 - rb - s.group * tiles, te = min(tiles, tb + (t1 - t0));
       const bool begins = tb == 0, ends = te == tiles;
       s.start = tb * TK;
       s.end = min(te * TK, t.len);
       s.whole = begins && ends;
       s.slot = 2 * blockIdx.x + (begins ? 1 : 0);
+      // (read across the lanes while all of them are on: inside the branch a value that was put aside comes back for lane 0 only)
+      const int pair = (r ? first_at(r - 1) : 0) + s.group;
       if (wave == 0 && lane == 0 && blockIdx.y == 0) {
-        int4* info = p.pair_info + ((r ? first[r - 1] : 0) + group);
+        int4* info = p.pair_info + pair;
         if (begins) {
           info->x = blockIdx.x;
           info->z = r;
-          info->w = group;
+          info->w = s.group;
         }
         if (ends) info->y = blockIdx.x;
       }
@@ -918,11 +991,27 @@ __global__ __launch_bounds__(512, 2) void paged_tree_kernel(TreeParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = (blockDim.x >> 6) / (SHARE ? p.share : 1);   // KV heads of the workgroup
   const int h = blockIdx.y * heads + (SHARE ? wave / p.share : wave), sub = SHARE ? wave % p.share : 0;
-  tree_walk<HD, 16 * NT>(p, [&](TreeSegment& s) {
-    s.part = s.group * (SHARE ? p.share : 1) + sub;
-    s.row0 = sub * 16 * NQ;
-    tree_segment<HD, NT, NQ, FP8, F16, SHARE>(p, s, h, lane);
-  });
+  if constexpr (SHARE) {
+    // (the wavefronts' pieces of LDS: behind the walk's)
+    extern __shared__ int32_t tree_lds[];
+    float* const joins = reinterpret_cast<float*>(tree_lds + (p.R <= 64 ? 0 : 2 * p.R));
+    tree_walk<HD, 16 * NT>(p, [&](TreeSegment& s) {
+      // parts of this group, and how many wavefronts each has
+      const int rows = min(s.nodes * p.G - s.group * p.rows, p.rows);
+      int ways = p.share;
+      while (ways > 1 && (p.share / ways) * 16 * NQ < rows) ways >>= 1;
+      const int part = sub / ways, way = sub - part * ways;
+      s.part = s.group * p.share + part;
+      s.row0 = part * 16 * NQ;
+      tree_segment<HD, NT, NQ, FP8, F16, true>(p, s, h, lane, way, ways, joins + (size_t)wave * 64 * NQ * (HD / 4 + 2));
+    });
+  } else {
+    tree_walk<HD, 16 * NT>(p, [&](TreeSegment& s) {
+      s.part = s.group;
+      s.row0 = 0;
+      tree_segment<HD, NT, NQ, FP8, F16, false>(p, s, h, lane, 0, 1, nullptr);
+    });
+  }
 }
 
 template <int HD, int WAVES, bool F16>
@@ -1010,7 +1099,7 @@ static TreeShape tree_shape(int T, int R, int Hq, int Hkv, int head_dim, bool ma
     s.rows = 32 * s.waves;
   } else {
     const int rows = head_dim > 128 ? 16 : 32;
-    s.share = mean <= rows ? 1 : mean <= 2 * rows ? 2 : mean <= 4 * rows ? 4 : 8;
+    s.share = 4 * mean <= 3 * rows ? 1 : 4 * mean <= 6 * rows ? 2 : 4 * mean <= 12 * rows ? 4 : 8;   // (trees are of all sizes)
     s.heads = 1;
     for (int w = 2; w <= 8 / s.share; ++w)
       if (Hkv % w == 0) s.heads = w;
@@ -1020,6 +1109,17 @@ static TreeShape tree_shape(int T, int R, int Hq, int Hkv, int head_dim, bool ma
   }
   if (s.grid < 1) s.grid = 1;
   return s;
+}
+// More than the default 64 KB of dynamic LDS, once per kernel and device.
+template <void (*K)(TreeParams)>
+static bool tree_raise_lds() {
+  static std::atomic<bool> raised[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return false;
+  if (raised[dev].load(std::memory_order_acquire)) return true;
+  if (hipFuncSetAttribute((const void*)K, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return false;
+  raised[dev].store(true, std::memory_order_release);
+  return true;
 }
 static int64_t tree_align(int64_t n) { return (n + 255) & ~(int64_t)255; }
 static int64_t tree_most_pairs(int T, int R, int G, int rows) {
@@ -1120,18 +1220,29 @@ extern "C" int mi_paged_tree_attention(
   // tokens of a tile: 32, 16 of wide heads, 64 of an fp8 cache with narrow ones (what the registers hold in flight); a tile
   // lies in one chunk
   const int nt = wide || chunk_tokens % 32 ? 1 : fp8 && head_dim == 64 && chunk_tokens % 64 == 0 ? 4 : 2;
+  const int tile = many ? 32 : 16 * nt;
+  if (tree_most_pairs(T, R, G, shape.rows) * ((int64_t)table_columns * chunk_tokens / tile + 1) >= (int64_t)1 << 31)
+    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: rows per KV head times the tokens of a table row must stay below some 2^36");
   for (int r0 = 0; r0 < R; r0 += kTreeRequestsPerLaunch) {
     p.r_base = r0;
     p.R = R - r0 < kTreeRequestsPerLaunch ? R - r0 : kTreeRequestsPerLaunch;
     p.cu_q = cu_seqlens_q + r0; p.lens = kv_lens + r0;
     p.last_slice = r0 + p.R == R;
-    const size_t lds = (size_t)p.R * (sizeof(int64_t) + sizeof(int32_t));
+    // (the walk's arrays; where parts share, what the wavefronts of a part join: 64 lanes' registers each)
+    const size_t walk = p.R <= 64 ? 0 : (size_t)p.R * 2 * sizeof(int32_t);
+    const size_t lds = walk + (!many && shape.share > 1 ? (size_t)shape.waves * 64 * (shape.rows / shape.share / 16) * (head_dim / 4 + 2) * sizeof(float) : 0);
+#define MI_TREE_ONE(HD_, NT_, NQ_, FP8_, F16_, SHARE_)                                                                 \
+    do {                                                                                                               \
+      if (SHARE_ && lds > 65536 && !tree_raise_lds<paged_tree_kernel<HD_, NT_, NQ_, FP8_, F16_, SHARE_>>())            \
+        return mi_fail(MI_ERR_LAUNCH, "mi_paged_tree_attention: cannot raise the dynamic LDS limit");                  \
+      hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, F16_, SHARE_>), grid, block, lds, st, p);             \
+    } while (0)
 #define MI_TREE(HD_, NT_, NQ_, FP8_)                                                                                   \
     do {                                                                                                               \
-      if (f16 && p.share > 1) hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, true, true>), grid, block, lds, st, p);   \
-      else if (f16) hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, true, false>), grid, block, lds, st, p);            \
-      else if (p.share > 1) hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, false, true>), grid, block, lds, st, p);    \
-      else hipLaunchKernelGGL((paged_tree_kernel<HD_, NT_, NQ_, FP8_, false, false>), grid, block, lds, st, p);                    \
+      if (f16 && p.share > 1) MI_TREE_ONE(HD_, NT_, NQ_, FP8_, true, true);                                            \
+      else if (f16) MI_TREE_ONE(HD_, NT_, NQ_, FP8_, true, false);                                                     \
+      else if (p.share > 1) MI_TREE_ONE(HD_, NT_, NQ_, FP8_, false, true);                                             \
+      else MI_TREE_ONE(HD_, NT_, NQ_, FP8_, false, false);                                                             \
     } while (0)
 #define MI_TREE_16(HD_)                                                                                                \
     do {                                                                                                               \
@@ -1166,6 +1277,7 @@ extern "C" int mi_paged_tree_attention(
 #undef MI_TREE_8
 #undef MI_TREE_16
 #undef MI_TREE
+#undef MI_TREE_ONE
     // (thread sets per row: for the partials that a request is expected to be cut into)
     const int cols = head_dim / 4, block_rows = kTreeMergeThreads / cols;
     const int64_t pairs = tree_most_pairs(T, p.R, G, shape.rows);
