@@ -37,8 +37,11 @@ struct VerifyPartial {   // of one part of a row
 };
 struct VerifyState {     // what the walk hands the draw
   double c;              // weights are (p - c q)+
-  int32_t row;           // the last node's row, -1: the request is empty
+  double sum;            // the last node's row: sum of exp(x - top)
+  float top;
+  int32_t row;           // -1: the request is empty
   int32_t tested;        // whether its children were tried
+  int32_t unused;
 };
 
 struct VerifyParams {
@@ -53,6 +56,7 @@ struct VerifyParams {
   VerifyPartial* partial;    // [T][parts]
   double* residual;          // [R][parts]
   VerifyState* state;        // [R]
+  int32_t* removed;          // [T]: the tokens that a request's last node's rejected children took out, -1: none
   int32_t T, R, V, max_path, parts, part;   // part: elements, a multiple of 8
   float inv_temperature; int32_t scaled;
 };
@@ -63,18 +67,31 @@ constexpr double kLog2e = 1.4426950408889634074;
 static __device__ __forceinline__ void fill_exp_table(double* table) {
   for (int i = threadIdx.x; i < 128; i += blockDim.x) table[i] = exp2(i * (1.0 / 128));
 }
-// 2^t for t <= 0 (far below zero: 0; NaN: 0)
-static __device__ __forceinline__ double table_exp2(const double* table, double t) {
-  constexpr double kMagic = 1.5 * 35184372088832.0;   // 1.5 2^45: an addition rounds to multiples of 1/128
-  t = fmax(t, -2000.0);
-  const double u = t + kMagic;
-  const double r = (t - (u - kMagic)) * 0.69314718055994530942;
+constexpr double kExpMagic = 1.5 * 35184372088832.0;   // 1.5 2^45: an addition rounds to multiples of 1/128
+// e^d for d <= 0 (NaN: 0)
+static __device__ __forceinline__ double table_exp(const double* table, double d) {
+  const double t = fmax(d * kLog2e, -2000.0);
+  const double u = t + kExpMagic;
+  const double r = (t - (u - kExpMagic)) * 0.69314718055994530942;
   const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, u);
   double y = __builtin_fma(r, 1.0 / 24, 1.0 / 6);
   y = __builtin_fma(r, y, 0.5);
   y = __builtin_fma(r, y, 1.0);
   y = __builtin_fma(r, y, 1.0);
   return __builtin_ldexp(table[k & 127] * y, k >> 7);
+}
+// The same for long sums, two thirds of the instructions: nothing below e^-690, whose place e^-690 takes.
+static __device__ __forceinline__ void table_exp_parts(const double* table, double d, double& scale, double& y) {
+  constexpr double kLn2 = 0.69314718055994530942;
+  d = fmax(d, -690.0);
+  const double u = __builtin_fma(d, kLog2e, kExpMagic);
+  const double r = __builtin_fma(d, kLog2e, kExpMagic - u);
+  const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, u);
+  y = __builtin_fma(r, kLn2 * kLn2 * kLn2 * kLn2 / 24, kLn2 * kLn2 * kLn2 / 6);
+  y = __builtin_fma(r, y, kLn2 * kLn2 / 2);
+  y = __builtin_fma(r, y, kLn2);
+  y = __builtin_fma(r, y, 1.0);
+  scale = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, table[k & 127]) + ((uint64_t)(uint32_t)(k >> 7) << 52));
 }
 
 static __device__ __forceinline__ float load_element(const uint8_t* row, int dtype, int i) {
@@ -83,29 +100,44 @@ static __device__ __forceinline__ float load_element(const uint8_t* row, int dty
   return dtype == 1 ? bf16_to_f32(x) : to_f32<true>(x);
 }
 
-// Eight elements e0 .. e0 + 7 of a row, `fill` outside [0, V): 16-byte loads where they are aligned and inside.
+// Eight elements e0 .. e0 + 7 of a row: a 16-byte line or two where they are aligned and inside, which `fetch` sends for
+// and `values` waits for; otherwise one by one, `fill` outside [0, V).
+template <int DT>
+struct VerifyLine {
+  uint4 a, b;
+  bool whole;
+  __device__ __forceinline__ void fetch(const uint8_t* row, int e0, int V) {
+    const uint8_t* at = row + (int64_t)e0 * (DT == 0 ? 4 : 2);
+    whole = e0 >= 0 && e0 + 8 <= V && !((uintptr_t)at & 15);
+    if (whole) {
+      a = ld16(at);
+      if constexpr (DT == 0) b = ld16(at + 16);
+    }
+  }
+  __device__ __forceinline__ void values(const uint8_t* row, int e0, int V, float fill, float (&x)[8]) const {
+    if (whole) {
+      if constexpr (DT == 0) {
+        x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
+        x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
+      } else {
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[2 * j] = lo_to_f32<DT == 2>(w[j]);
+          x[2 * j + 1] = hi_to_f32<DT == 2>(w[j]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = e0 + j >= 0 && e0 + j < V ? load_element(row, DT, e0 + j) : fill;
+    }
+  }
+};
 template <int DT>
 static __device__ __forceinline__ void load8(const uint8_t* row, int e0, int V, float fill, float (&x)[8]) {
-  constexpr int ES = DT == 0 ? 4 : 2;
-  const uint8_t* at = row + (int64_t)e0 * ES;
-  if (e0 >= 0 && e0 + 8 <= V && !((uintptr_t)at & 15)) {
-    const uint4 a = ld16(at);
-    if constexpr (DT == 0) {
-      const uint4 b = ld16(at + 16);
-      x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
-      x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
-    } else {
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[2 * j] = lo_to_f32<DT == 2>(w[j]);
-        x[2 * j + 1] = hi_to_f32<DT == 2>(w[j]);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = e0 + j >= 0 && e0 + j < V ? load_element(row, DT, e0 + j) : fill;
-  }
+  VerifyLine<DT> l;
+  l.fetch(row, e0, V);
+  l.values(row, e0, V, fill, x);
 }
 static __device__ __forceinline__ void load8_any(const uint8_t* row, int dtype, int e0, int V, float fill, float (&x)[8]) {
   if (dtype == 0) load8<0>(row, e0, V, fill, x);
@@ -147,7 +179,9 @@ static __device__ __forceinline__ float wave_max_f32(float x) {
   return x;
 }
 
-// Maximum and sum of exponentials (greedy: maximum and its first place) of one part of one row.
+// Maximum and sum of exponentials (greedy: maximum and its first place) of one part of one row, which the threads hold in
+// registers: all loads are on their way before the first value is used.
+constexpr int kVerifyLines = kVerifyPart / (8 * kVerifyThreads);
 template <int DT, bool GREEDY>
 __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParams p) {
   __shared__ double table[128];
@@ -155,50 +189,67 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
   __shared__ float tops[4];
   __shared__ int places[4];
   const int part = blockIdx.y, row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (!GREEDY) fill_exp_table(table);
-  __syncthreads();
   const VerifyRow<DT> rd(p, row);
-  const int begin = part * p.part - rd.shift, end = min(begin + p.part, p.V);
+  const int begin = part * p.part - rd.shift, end = min(begin + p.part, p.V), mine = begin + 8 * (int)threadIdx.x;
+  VerifyLine<DT> lines[kVerifyLines];
+#pragma unroll
+  for (int i = 0; i < kVerifyLines; ++i)
+    if (mine + 8 * kVerifyThreads * i < end) lines[i].fetch(rd.row, mine + 8 * kVerifyThreads * i, p.V);
+  if (!GREEDY) {
+    fill_exp_table(table);
+    __syncthreads();
+  }
   float top = -INFINITY;
   int place = 0x7fffffff;
-  double sum = 0;
-  for (int e0 = begin + 8 * (int)threadIdx.x; e0 < end; e0 += 8 * kVerifyThreads) {
-    float x[8];
-    load8<DT>(rd.row, e0, p.V, -INFINITY, x);
-    if constexpr (GREEDY) {
+  float x[GREEDY ? 1 : kVerifyLines][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if ((x[j] > top || place == 0x7fffffff) && e0 + j >= 0 && e0 + j < p.V && x[j] == x[j]) {
-          top = x[j];
-          place = e0 + j;
+  for (int i = 0; i < kVerifyLines; ++i) {
+    const int e0 = mine + 8 * kVerifyThreads * i;
+    float(&v)[8] = x[GREEDY ? 0 : i];
+    if (e0 < end) {
+      lines[i].values(rd.row, e0, p.V, -INFINITY, v);
+      if constexpr (GREEDY) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if ((v[j] > top || place == 0x7fffffff) && e0 + j >= 0 && e0 + j < p.V && v[j] == v[j]) {
+            top = v[j];
+            place = e0 + j;
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[j] = rd.finish(p, v[j]);
+          top = fmaxf(top, v[j]);
         }
+      }
     } else {
-      float m = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = rd.finish(p, x[j]);
-        m = fmaxf(m, x[j]);
-      }
-      if (m > top) {
-        sum *= table_exp2(table, ((double)top - m) * kLog2e);
-        top = m;
-      }
-      if (top > -INFINITY) {
-        const double ref = -(double)top * kLog2e;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum += table_exp2(table, __builtin_fma((double)x[j], kLog2e, ref));
-      }
+      for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
     }
   }
-  float all = wave_max_f32(top);
+  const float all = wave_max_f32(top);
   if constexpr (GREEDY) {
     int best = top == all ? place : 0x7fffffff;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
     if (lane == 0) { tops[wave] = all; places[wave] = best; }
   } else {
-    double s = all > -INFINITY ? sum * table_exp2(table, ((double)top - all) * kLog2e) : 0.0;
-    s = wave_sum_f64(s);
+    double s0 = 0, s1 = 0;
+#pragma unroll
+    for (int i = 0; i < kVerifyLines; ++i) {
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) any |= x[i][j] > -INFINITY;
+      if (!__builtin_amdgcn_ballot_w64(any)) continue;   // (a cut leaves few)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        double scale, y;
+        table_exp_parts(table, (double)x[i][j] - (double)all, scale, y);
+        double& s = j & 1 ? s1 : s0;
+        s = __builtin_fma(scale, y, s);
+      }
+    }
+    const double s = wave_sum_f64(s0 + s1);
     if (lane == 0) { tops[wave] = all; sums[wave] = s; }
   }
   __syncthreads();
@@ -208,7 +259,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
     for (int w = 0; w < 4; ++w) o.max = fmaxf(o.max, tops[w]);
     for (int w = 0; w < 4; ++w) {
       if (GREEDY) { if (tops[w] == o.max) o.index = min(o.index, places[w]); }
-      else if (tops[w] > -INFINITY) o.sum += sums[w] * table_exp2(table, ((double)tops[w] - o.max) * kLog2e);
+      else if (tops[w] > -INFINITY) o.sum += sums[w] * table_exp(table, (double)tops[w] - (double)o.max);
     }
     p.partial[(int64_t)row * p.parts + part] = o;
   }
@@ -225,6 +276,30 @@ static __device__ __forceinline__ double block_sum(double x, double* scratch) {
   return s;
 }
 
+// This thread's share of the sum of (p - c q)+ over the places [0, places) from `first` on of a row.
+template <int DT>
+static __device__ __forceinline__ double left_over(const VerifyParams& p, const VerifyRow<DT>& rd, const double* table, int row,
+                                                   int first, int places, int threads, float top, double sum, double c) {
+  const uint8_t* qr = p.draft + (int64_t)row * p.draft_stride;
+  const double inv = 1.0 / sum;
+  const int begin = first - rd.shift, end = min(begin + places, p.V);
+  double s = 0;
+  for (int e0 = begin + 8 * (int)threadIdx.x; e0 < end; e0 += 8 * threads) {
+    float x[8], y[8];
+    load8_any(qr, p.draft_dtype, e0, p.V, 0.f, y);
+    load8<DT>(rd.row, e0, p.V, -INFINITY, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = rd.finish(p, x[j]);
+      double scale, z;
+      table_exp_parts(table, (double)v - (double)top, scale, z);
+      const double w = v > -INFINITY ? scale * inv : 0.0;
+      s += fmax(__builtin_fma(w, z, -c * (double)y[j]), 0.0);
+    }
+  }
+  return s;
+}
+
 // The walk of one request's tree, one workgroup each.
 constexpr int kWalkThreads = 1024;
 enum { kGreedy = 0, kTarget = 1, kDraft = 2 };
@@ -234,8 +309,9 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   __shared__ double scratch[kWalkThreads / 64];
   __shared__ double prob[kVerifyNodes], sum_s[kVerifyNodes];
   __shared__ float top_s[kVerifyNodes], q_s[kVerifyNodes];
-  __shared__ int32_t parent[kVerifyNodes], token[kVerifyNodes], after[kVerifyNodes];
-  const int r = blockIdx.x, tid = threadIdx.x;
+  __shared__ int32_t parent[kVerifyNodes], token[kVerifyNodes], after[kVerifyNodes];   // after: the next node; draft: the first child
+  __shared__ int32_t sibling[MODE == kDraft ? kVerifyNodes : 1];
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int begin = min(max(p.cu[r], 0), p.T), n = min(min(max(p.cu[r + 1], begin), p.T) - begin, kVerifyNodes);
   int32_t* const rows = p.out_rows + (int64_t)r * p.max_path;
   int64_t* const out = p.out_tokens + (int64_t)r * p.max_path;
@@ -246,31 +322,36 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   if (n <= 0) {
     if (tid == 0) {
       p.out_counts[r] = 0;
-      p.state[r] = VerifyState{0, -1, 0};
+      p.state[r] = VerifyState{0, 0, 0.f, -1, 0, 0};
     }
     return;
   }
   fill_exp_table(table);
   __syncthreads();
-  for (int i = tid; i < n; i += kWalkThreads) {
-    const VerifyPartial* part = p.partial + (int64_t)(begin + i) * p.parts;
-    float top = -INFINITY;
-    for (int k = 0; k < p.parts; ++k) top = fmaxf(top, part[k].max);
-    top_s[i] = top;
+  // maximum and sum of a row: a wavefront each, a part to a lane
+  static_assert(kVerifyMostParts == 64, "a part to a lane");
+  for (int i = tid >> 6; i < n; i += kWalkThreads / 64) {
+    VerifyPartial part{0, -INFINITY, 0x7fffffff};
+    if (lane < p.parts) part = p.partial[(int64_t)(begin + i) * p.parts + lane];
+    const float top = wave_max_f32(part.max);
     if (MODE == kGreedy) {
-      int best = 0x7fffffff;
-      for (int k = 0; k < p.parts; ++k)
-        if (part[k].max == top) best = min(best, part[k].index);
-      token[i] = best;   // (of the row, here)
+      int best = part.max == top ? part.index : 0x7fffffff;
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
+      if (lane == 0) token[i] = best;   // (of the row, here)
     } else {
-      double s = 0;
-      for (int k = 0; k < p.parts; ++k)
-        if (part[k].max > -INFINITY) s += part[k].sum * table_exp2(table, ((double)part[k].max - top) * kLog2e);
-      sum_s[i] = s;
+      const double s = wave_sum_f64(part.max > -INFINITY ? part.sum * table_exp(table, (double)part.max - (double)top) : 0.0);
+      if (lane == 0) {
+        top_s[i] = top;
+        sum_s[i] = s;
+      }
     }
-    after[i] = 0x7fffffff;
-    const int up = p.parents[begin + i];
-    parent[i] = i > 0 && up >= 0 && up < i ? up : -1;
+  }
+  static_assert(kVerifyNodes == kWalkThreads, "a node to a thread");
+  if (tid < n) {
+    const int up = p.parents[begin + tid];
+    after[tid] = 0x7fffffff;
+    parent[tid] = tid > 0 && up >= 0 && up < tid ? up : -1;
   }
   __syncthreads();
   if (MODE == kGreedy) {
@@ -287,7 +368,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
         const int up = parent[i];
         const VerifyRow<DT> rd(p, begin + up);
         const float x = rd.at(p, (int)t);
-        if (sum_s[up] > 0) prob[i] = table_exp2(table, ((double)x - top_s[up]) * kLog2e) / sum_s[up];
+        if (sum_s[up] > 0) prob[i] = table_exp(table, (double)x - (double)top_s[up]) / sum_s[up];
         if (MODE == kDraft) q_s[i] = load_element(p.draft + (int64_t)(begin + up) * p.draft_stride, p.draft_dtype, (int)t);
       }
     }
@@ -297,20 +378,20 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     // a token that an earlier sibling had has left the distribution
     bool again = false;
     double before = 0;
-    const int i = tid;   // (kVerifyNodes == kWalkThreads)
+    const int i = tid;
     const int up = i < n ? parent[i] : -1;
     if (up >= 0)
       for (int j = up + 1; j < i; ++j) again |= parent[j] == up && token[j] == token[i];
     __syncthreads();
     if (again) prob[i] = 0;
     __syncthreads();
+    if (i < n) p.removed[begin + i] = again ? -1 : token[i];
     if (up >= 0) {
       for (int j = up + 1; j < i; ++j) before += parent[j] == up ? prob[j] : 0.0;
       if ((double)p.uniform[begin + i] * (1.0 - before) < prob[i]) atomicMin(&after[up], i);
     }
     __syncthreads();
   }
-  static_assert(kVerifyNodes == kWalkThreads, "a node to a thread");
   if (MODE != kDraft) {
     if (tid == 0) {
       int at = 0, count = 1;
@@ -322,50 +403,40 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
       }
       p.out_counts[r] = count;
       if (MODE == kGreedy) out[count - 1] = token[at] == 0x7fffffff ? 0 : token[at];
-      else p.state[r] = VerifyState{0, begin + at, count < p.max_path};
+      else p.state[r] = VerifyState{0, sum_s[at], top_s[at], begin + at, count < p.max_path, 0};
     }
     return;
   }
   // Draft probabilities: the rejections of a node's earlier children decide what a later one is held against.
+  if (tid < n) {
+    int next = -1;
+    if (parent[tid] >= 0) {
+      atomicMin(&after[parent[tid]], tid);
+      for (int j = tid + 1; j < n && next < 0; ++j)
+        if (parent[j] == parent[tid]) next = j;
+    }
+    sibling[tid] = next;
+  }
+  __syncthreads();
   int at = 0, count = 1;
   double c = 0;
   if (tid == 0) rows[0] = begin;
   while (count < p.max_path) {
     c = 0;
     double left = 1;
-    int next = -1;
-    int child = -1;
-    for (int i = at + 1; i < n && child < 0; ++i)
-      if (parent[i] == at) child = i;
+    int child = after[at] < n ? after[at] : -1;
     while (child >= 0) {
       const double q = q_s[child], w = prob[child] - c * q;
-      if ((double)p.uniform[begin + child] * left * q < w) {
-        next = child;
-        break;
-      }
+      if ((double)p.uniform[begin + child] * left * q < w) break;
       c += left;
-      int following = -1;
-      for (int i = child + 1; i < n && following < 0; ++i)
-        if (parent[i] == at) following = i;
-      if (following >= 0) {   // (what is left matters to a sibling; the draw makes its own sum)
+      child = sibling[child];
+      if (child >= 0) {   // (what is left matters to a sibling; the draw makes its own sum)
         const VerifyRow<DT> rd(p, begin + at);
-        const uint8_t* qr = p.draft + (int64_t)(begin + at) * p.draft_stride;
-        const double ref = -(double)top_s[at] * kLog2e, inv = 1.0 / sum_s[at];
-        double s = 0;
-        for (int e0 = 8 * tid - rd.shift; e0 < p.V; e0 += 8 * kWalkThreads) {
-          float x[8], y[8];
-          load8<DT>(rd.row, e0, p.V, -INFINITY, x);
-          load8_any(qr, p.draft_dtype, e0, p.V, 0.f, y);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            s += fmax(table_exp2(table, __builtin_fma((double)rd.finish(p, x[j]), kLog2e, ref)) * inv - c * (double)y[j], 0.0);
-        }
-        left = block_sum(s, scratch);
+        left = block_sum(left_over(p, rd, table, begin + at, 0, p.V + rd.shift, kWalkThreads, top_s[at], sum_s[at], c), scratch);
       }
-      child = following;
     }
-    if (next < 0) break;
-    at = next;
+    if (child < 0) break;
+    at = child;
     if (tid == 0) {
       out[count - 1] = p.tokens[begin + at];
       rows[count] = begin + at;
@@ -374,22 +445,8 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   }
   if (tid == 0) {
     p.out_counts[r] = count;
-    p.state[r] = VerifyState{c, begin + at, count < p.max_path};
+    p.state[r] = VerifyState{c, sum_s[at], top_s[at], begin + at, count < p.max_path, 0};
   }
-}
-
-// Maximum and sum of a row from its parts, in every thread of the workgroup.
-struct RowTotal {
-  float top;
-  double sum;
-};
-static __device__ __forceinline__ RowTotal row_total(const VerifyParams& p, const double* table, int row) {
-  const VerifyPartial* part = p.partial + (int64_t)row * p.parts;
-  RowTotal t{-INFINITY, 0};
-  for (int k = 0; k < p.parts; ++k) t.top = fmaxf(t.top, part[k].max);
-  for (int k = 0; k < p.parts; ++k)
-    if (part[k].max > -INFINITY) t.sum += part[k].sum * table_exp2(table, ((double)part[k].max - t.top) * kLog2e);
-  return t;
 }
 
 // Draft probabilities: what is left of one part of the last node's distribution, sum (p - c q)+.
@@ -399,141 +456,150 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_left_kernel(VerifyParam
   __shared__ double scratch[kVerifyThreads / 64];
   const int part = blockIdx.y, r = blockIdx.x;
   const VerifyState st = p.state[r];
-  if (st.row < 0) return;
+  if (st.row < 0 || !st.tested) return;
   fill_exp_table(table);
   __syncthreads();
-  const RowTotal t = row_total(p, table, st.row);
   const VerifyRow<DT> rd(p, st.row);
-  const uint8_t* qr = p.draft + (int64_t)st.row * p.draft_stride;
-  const int begin = part * p.part - rd.shift, end = min(begin + p.part, p.V);
-  const double ref = -(double)t.top * kLog2e, inv = 1.0 / t.sum;
-  double s = 0;
-  for (int e0 = begin + 8 * (int)threadIdx.x; e0 < end; e0 += 8 * kVerifyThreads) {
-    float x[8], y[8];
-    load8<DT>(rd.row, e0, p.V, -INFINITY, x);
-    load8_any(qr, p.draft_dtype, e0, p.V, 0.f, y);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      s += fmax(table_exp2(table, __builtin_fma((double)rd.finish(p, x[j]), kLog2e, ref)) * inv - st.c * (double)y[j], 0.0);
-  }
-  s = block_sum(s, scratch);
+  const double s = block_sum(left_over(p, rd, table, st.row, part * p.part, p.part, kVerifyThreads, st.top, st.sum, st.c), scratch);
   if (threadIdx.x == 0) p.residual[(int64_t)r * p.parts + part] = s;
 }
 
-// The draw of a request's last token: the part that holds it, then the place inside the part.
+// Inclusive sums over the lanes.
+static __device__ __forceinline__ double wave_scan_f64(double x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+// The draw of a request's last token: the part that holds it (every wavefront, a part to a lane), then the place inside the
+// part, whose weights the threads hold.
 template <int DT, int MODE>
 __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyParams p) {
+  constexpr int kWaves = kVerifyThreads / 64;
   __shared__ double table[128];
-  __shared__ double scratch[kVerifyThreads / 64];
-  __shared__ double mass[kVerifyMostParts];
-  __shared__ double weight[kVerifyPart];
-  __shared__ double before[kVerifyThreads];
-  __shared__ int found[3];
-  const int r = blockIdx.x, tid = threadIdx.x;
+  __shared__ double mass_s[kVerifyMostParts];
+  __shared__ double run[kVerifyLines][kWaves];
+  __shared__ uint32_t gone[MODE == kTarget ? kVerifyPart / 32 : 1];
+  __shared__ int found[2];
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const VerifyState st = p.state[r];
   if (st.row < 0) return;
   fill_exp_table(table);
+  if (MODE == kTarget)
+    for (int i = tid; i < kVerifyPart / 32; i += kVerifyThreads) gone[i] = 0;
+  if (tid == 0) {
+    found[0] = 0x7fffffff;
+    found[1] = -1;
+  }
   __syncthreads();
   const int begin = min(max(p.cu[r], 0), p.T), n = min(min(max(p.cu[r + 1], begin), p.T) - begin, kVerifyNodes);
   const int node = st.row - begin;
   const VerifyRow<DT> rd(p, st.row);
-  const RowTotal t = row_total(p, table, st.row);
-  const double ref = -(double)t.top * kLog2e, inv = 1.0 / t.sum;
-  auto chance = [&](float x) { return table_exp2(table, __builtin_fma((double)x, kLog2e, ref)) * inv; };
-  auto whole_mass = [&](int k) {
-    const VerifyPartial q = p.partial[(int64_t)st.row * p.parts + k];
-    return q.max > -INFINITY ? q.sum * table_exp2(table, ((double)q.max - t.top) * kLog2e) * inv : 0.0;
-  };
-  for (int k = tid; k < p.parts; k += kVerifyThreads)
-    mass[k] = MODE == kDraft && st.tested ? p.residual[(int64_t)r * p.parts + k] : whole_mass(k);
-  __syncthreads();
+  const double inv = 1.0 / st.sum;
+  auto chance = [&](float x) { return table_exp(table, (double)x - (double)st.top) * inv; };
+  double whole = 0;
+  if (lane < p.parts) {
+    const VerifyPartial q = p.partial[(int64_t)st.row * p.parts + lane];
+    if (q.max > -INFINITY) whole = q.sum * chance(q.max);
+  }
+  double mass = whole;
+  if (MODE == kDraft && st.tested) mass = lane < p.parts ? p.residual[(int64_t)r * p.parts + lane] : 0.0;
   // tokens that the rejected children took out: each once
   auto removed = [&](auto f) {
     if (MODE != kTarget || !st.tested) return;
-    for (int i = node + 1 + tid; i < n; i += kVerifyThreads) {
-      if (p.parents[begin + i] != node) continue;
-      const int64_t tok = p.tokens[begin + i];
-      bool first = tok >= 0 && tok < p.V;
-      for (int j = node + 1; j < i && first; ++j) first = !(p.parents[begin + j] == node && p.tokens[begin + j] == tok);
-      if (first) f((int)tok);
-    }
+    for (int i = node + 1 + tid; i < n; i += kVerifyThreads)
+      if (p.parents[begin + i] == node && p.removed[begin + i] >= 0) f(p.removed[begin + i]);
   };
-  removed([&](int tok) { atomicAdd(&mass[(tok + rd.shift) / p.part], -chance(rd.at(p, tok))); });
-  __syncthreads();
-  double total = 0;
-  for (int k = 0; k < p.parts; ++k) total += fmax(mass[k], 0.0);
+  if (MODE == kTarget && st.tested) {
+    if (tid < kVerifyMostParts) mass_s[tid] = whole;
+    __syncthreads();
+    removed([&](int tok) { atomicAdd(&mass_s[(tok + rd.shift) / p.part], -chance(rd.at(p, tok))); });
+    __syncthreads();
+    mass = mass_s[lane];
+  }
+  mass = fmax(mass, 0.0);
+  double sums = wave_scan_f64(mass, lane), total = __shfl(sums, 63, 64);
   // Rejections that leave nothing (a target equal to the draft's, or smaller everywhere that it is kept, up to rounding):
   // the last token comes from the target itself.
   const bool nothing = !(total > 1e-13);
-  __syncthreads();
   if (nothing) {
-    for (int k = tid; k < p.parts; k += kVerifyThreads) mass[k] = whole_mass(k);
-    __syncthreads();
-    total = 0;
-    for (int k = 0; k < p.parts; ++k) total += mass[k];
+    mass = whole;
+    sums = wave_scan_f64(mass, lane);
+    total = __shfl(sums, 63, 64);
   }
   const double want = (double)p.uniform[begin] * total;
-  if (tid == 0) {
-    double sum = 0;
-    int k = 0, last = 0;
-    for (; k < p.parts; ++k) {
-      const double m = fmax(mass[k], 0.0);
-      if (m > 0) last = k;
-      if (sum + m > want) break;
-      sum += m;
-    }
-    if (k == p.parts) {   // (the sum's own rounding: the last part that has any)
-      k = last;
-      sum = want;
-    }
-    found[0] = k;
-    found[1] = 0x7fffffff;
-    found[2] = -1;
-    scratch[0] = sum;
-  }
-  __syncthreads();
-  const int part = found[0], first = part * p.part - rd.shift;
-  const double rest = want - scratch[0];
+  const uint64_t beyond = __builtin_amdgcn_ballot_w64(sums > want && mass > 0.0);
+  const uint64_t some = __builtin_amdgcn_ballot_w64(mass > total * 1e-18);   // (the sum's own rounding: the last part that has any)
+  const int part = beyond ? __builtin_ctzll(beyond) : some ? 63 - __builtin_clzll(some) : 0;
+  const double rest = beyond ? want - __shfl(sums - mass, part, 64) : want;
+  const int first = part * p.part - rd.shift;
   const uint8_t* qr = MODE == kDraft ? p.draft + (int64_t)st.row * p.draft_stride : nullptr;
-  for (int i = 8 * tid; i < p.part; i += 8 * kVerifyThreads) {
-    float x[8], y[8];
-    load8<DT>(rd.row, first + i, p.V, -INFINITY, x);
-    if (MODE == kDraft) load8_any(qr, p.draft_dtype, first + i, p.V, 0.f, y);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      double w = chance(rd.finish(p, x[j]));
-      if (MODE == kDraft && st.tested && !nothing) w = fmax(w - st.c * (double)y[j], 0.0);
-      weight[i + j] = w;
-    }
-  }
-  __syncthreads();
-  if (!nothing)
+  const bool minus = MODE == kDraft && st.tested && !nothing;
+  if (!nothing && MODE == kTarget) {
     removed([&](int tok) {
       const int i = tok - first;
-      if (i >= 0 && i < p.part) weight[i] = 0;
+      if (i >= 0 && i < p.part) atomicOr(&gone[i >> 5], 1u << (i & 31));
     });
-  __syncthreads();
-  // every thread a run of neighbours: their sum, the sums before it, then the place
-  const int run = (p.part + kVerifyThreads - 1) / kVerifyThreads, a = min(tid * run, p.part), b = min(a + run, p.part);
-  double mine = 0;
-  for (int i = a; i < b; ++i) mine += weight[i];
-  before[tid] = mine;
-  __syncthreads();
-  double sum = 0;
-  for (int k = 0; k < tid; ++k) sum += before[k];
-  int last = -1;
-  for (int i = a; i < b; ++i) {
-    if (weight[i] > 0) last = i;
-    sum += weight[i];
-    if (sum > rest && weight[i] > 0) {
-      atomicMin(&found[1], i);
-      break;
+    __syncthreads();
+  }
+  double weight[kVerifyLines][8], mine[kVerifyLines];
+#pragma unroll
+  for (int l = 0; l < kVerifyLines; ++l) {
+    const int i = 8 * (tid + l * kVerifyThreads);
+    mine[l] = 0;
+    if (i < p.part) {
+      float x[8], y[8];
+      load8<DT>(rd.row, first + i, p.V, -INFINITY, x);
+      if (minus) load8_any(qr, p.draft_dtype, first + i, p.V, 0.f, y);
+      const uint32_t out = MODE == kTarget ? gone[i >> 5] >> (i & 31) : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        double w = chance(rd.finish(p, x[j]));
+        if (minus) w = fmax(w - st.c * (double)y[j], 0.0);
+        if (MODE == kTarget && (out >> j & 1)) w = 0;
+        weight[l][j] = w;
+        mine[l] += w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) weight[l][j] = 0;
     }
   }
-  atomicMax(&found[2], last);
+  double upto[kVerifyLines];
+#pragma unroll
+  for (int l = 0; l < kVerifyLines; ++l) {
+    upto[l] = wave_scan_f64(mine[l], lane);
+    if (lane == 63) run[l][wave] = upto[l];
+  }
+  __syncthreads();
+  double before = 0;
+  int last = -1, place = 0x7fffffff;
+#pragma unroll
+  for (int l = 0; l < kVerifyLines; ++l) {
+    double sum = before;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) sum += run[l][w];
+      before += run[l][w];
+    }
+    sum += upto[l] - mine[l];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      sum += weight[l][j];
+      if (weight[l][j] > 0) {
+        const int i = 8 * (tid + l * kVerifyThreads) + j;
+        last = i;
+        if (sum > rest && place == 0x7fffffff) place = i;
+      }
+    }
+  }
+  if (place != 0x7fffffff) atomicMin(&found[0], place);
+  if (last >= 0) atomicMax(&found[1], last);
   __syncthreads();
   if (tid == 0) {
-    const int i = found[1] != 0x7fffffff ? found[1] : found[2];
+    const int i = found[0] != 0x7fffffff ? found[0] : found[1];
     p.out_tokens[(int64_t)r * p.max_path + p.out_counts[r] - 1] = min(max(first + i, 0), p.V - 1);
   }
 }
@@ -643,7 +709,7 @@ extern "C" int64_t mi_verify_workspace_bytes(int32_t T, int32_t R, int32_t vocab
   int parts, part;
   verify_parts(T, vocab, &parts, &part);
   return align256((int64_t)T * parts * sizeof(VerifyPartial)) + align256((int64_t)R * parts * sizeof(double)) +
-         align256((int64_t)R * sizeof(VerifyState));
+         align256((int64_t)R * sizeof(VerifyState)) + align256((int64_t)T * sizeof(int32_t));
 }
 
 template <int DT>
@@ -706,6 +772,8 @@ extern "C" int mi_verify_drafted_tokens(const void* logits, int64_t stride_row, 
   p.residual = (double*)ws;
   ws += align256((int64_t)R * p.parts * sizeof(double));
   p.state = (VerifyState*)ws;
+  ws += align256((int64_t)R * sizeof(VerifyState));
+  p.removed = (int32_t*)ws;
   p.scaled = !greedy && temperature != 1.f;
   p.inv_temperature = greedy ? 1.f : 1.f / temperature;
   const int mode = greedy ? kGreedy : draft_probs ? kDraft : kTarget;
