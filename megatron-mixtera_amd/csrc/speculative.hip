@@ -133,17 +133,32 @@ struct VerifyLine {
     }
   }
 };
-template <int DT>
-static __device__ __forceinline__ void load8(const uint8_t* row, int e0, int V, float fill, float (&x)[8]) {
-  VerifyLine<DT> l;
-  l.fetch(row, e0, V);
-  l.values(row, e0, V, fill, x);
-}
-static __device__ __forceinline__ void load8_any(const uint8_t* row, int dtype, int e0, int V, float fill, float (&x)[8]) {
-  if (dtype == 0) load8<0>(row, e0, V, fill, x);
-  else if (dtype == 1) load8<1>(row, e0, V, fill, x);
-  else load8<2>(row, e0, V, fill, x);
-}
+// The same of a type that is known at run time.
+struct VerifyAnyLine {
+  VerifyLine<0> line;
+  __device__ __forceinline__ void fetch(const uint8_t* row, int dtype, int e0, int V) {
+    if (dtype == 0) {
+      line.fetch(row, e0, V);
+    } else {
+      VerifyLine<1> l;
+      l.whole = false;
+      l.fetch(row, e0, V);
+      line.a = l.a;
+      line.whole = l.whole;
+    }
+  }
+  __device__ __forceinline__ void values(const uint8_t* row, int dtype, int e0, int V, float fill, float (&x)[8]) const {
+    if (dtype == 0) {
+      line.values(row, e0, V, fill, x);
+    } else if (dtype == 1) {
+      const VerifyLine<1> l{line.a, line.b, line.whole};
+      l.values(row, e0, V, fill, x);
+    } else {
+      const VerifyLine<2> l{line.a, line.b, line.whole};
+      l.values(row, e0, V, fill, x);
+    }
+  }
+};
 
 // A row of logits cut into parts of `part` elements.  Parts are counted from the last 16-byte line at or before the row's
 // first element, so that the groups of eight are aligned whatever the row's own address: element e lies at place e + shift.
@@ -168,19 +183,64 @@ struct VerifyRow {
   __device__ __forceinline__ float at(const VerifyParams& p, int e) const { return finish(p, load_element(row, DT, e)); }
 };
 
-static __device__ __forceinline__ double wave_sum_f64(double x) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
+// One step of a sum over the lanes: the value of the lane that DPP control CTRL names, 0 where there is none or MASK leaves
+// the lane's row of 16 out.
+template <int CTRL, int MASK>
+static __device__ __forceinline__ double dpp_f64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, MASK, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, MASK, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Inclusive sums over the lanes: inside the rows of 16, then the last of a row to the next one, of two rows to the next two.
+static __device__ __forceinline__ double wave_scan_f64(double x) {
+  x += dpp_f64<0x111, 0xf>(x);
+  x += dpp_f64<0x112, 0xf>(x);
+  x += dpp_f64<0x114, 0xf>(x);
+  x += dpp_f64<0x118, 0xf>(x);
+  x += dpp_f64<0x142, 0xa>(x);
+  x += dpp_f64<0x143, 0xc>(x);
   return x;
 }
+static __device__ __forceinline__ double read_lane_f64(double x, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+static __device__ __forceinline__ double wave_sum_f64(double x) { return read_lane_f64(wave_scan_f64(x), 63); }
 static __device__ __forceinline__ float wave_max_f32(float x) {
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
   return x;
 }
 
+// Sum of e^(x - top) over eight logits, `top` among the row's wavefront, |top| < kNarrow: the exponent's whole 128ths and what
+// is left of them come from 32-bit products (a whole number below 2^23 beside its fraction), 2^(whole/128) from the table, the
+// fraction's own e^. as 1 + a 32-bit polynomial of at most 0.0027: 6e-10 of a weight at most, a hundredth of half a step of the
+// uniform numbers that it meets, in two thirds of the 64-bit form's time.
+constexpr float kNarrow = 16384.f;
+static __device__ __forceinline__ void add_exps(const double* table, const float (&x)[8], float low, int whole, double& sum, double& rest) {
+  constexpr double kStep = kLog2e * 128, kLn = 0.69314718055994530942 / 128;
+  constexpr float kHigh = (float)kStep, kLow = (float)(kStep - (double)kHigh), kMagic = 12582912.f;   // 1.5 2^23
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float v = fmaxf(x[j], low);
+    const float u = __builtin_fmaf(v, kHigh, kMagic);
+    float r = __builtin_fmaf(v, kHigh, -(u - kMagic));
+    r = __builtin_fmaf(v, kLow, r);
+    const int k = (int)__float_as_uint(u) - whole;
+    const float y = r * __builtin_fmaf(r, __builtin_fmaf(r, (float)(kLn * kLn * kLn / 6), (float)(kLn * kLn / 2)), (float)kLn);
+    const uint64_t t = __builtin_bit_cast(uint64_t, table[k & 127]);
+    const uint32_t hi = (uint32_t)(t >> 32) + ((uint32_t)(k & ~127) << 13);
+    const double w = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)t);
+    sum += w;
+    rest = __builtin_fma(w, (double)y, rest);
+  }
+}
+
 // Maximum and sum of exponentials (greedy: maximum and its first place) of one part of one row, which the threads hold in
-// registers: all loads are on their way before the first value is used.
+// registers: all loads are on their way before the first value is used.  Scaling and cut keep the order of logits, so that the
+// largest of eight says whether any of them counts.
 constexpr int kVerifyLines = kVerifyPart / (8 * kVerifyThreads);
 template <int DT, bool GREEDY>
 __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParams p) {
@@ -199,32 +259,26 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
     fill_exp_table(table);
     __syncthreads();
   }
-  float top = -INFINITY;
+  float top = -INFINITY, line_top[kVerifyLines];
   int place = 0x7fffffff;
-  float x[GREEDY ? 1 : kVerifyLines][8];
 #pragma unroll
   for (int i = 0; i < kVerifyLines; ++i) {
     const int e0 = mine + 8 * kVerifyThreads * i;
-    float(&v)[8] = x[GREEDY ? 0 : i];
-    if (e0 < end) {
-      lines[i].values(rd.row, e0, p.V, -INFINITY, v);
-      if constexpr (GREEDY) {
+    line_top[i] = -INFINITY;
+    if (e0 >= end) continue;
+    float v[8];
+    lines[i].values(rd.row, e0, p.V, -INFINITY, v);
+    if constexpr (GREEDY) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if ((v[j] > top || place == 0x7fffffff) && e0 + j >= 0 && e0 + j < p.V && v[j] == v[j]) {
-            top = v[j];
-            place = e0 + j;
-          }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[j] = rd.finish(p, v[j]);
-          top = fmaxf(top, v[j]);
+      for (int j = 0; j < 8; ++j)
+        if ((v[j] > top || place == 0x7fffffff) && e0 + j >= 0 && e0 + j < p.V && v[j] == v[j]) {
+          top = v[j];
+          place = e0 + j;
         }
-      }
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
+      const float m = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+      line_top[i] = rd.finish(p, m);
+      top = fmaxf(top, line_top[i]);
     }
   }
   const float all = wave_max_f32(top);
@@ -235,21 +289,36 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
     if (lane == 0) { tops[wave] = all; places[wave] = best; }
   } else {
     double s0 = 0, s1 = 0;
+    const bool narrow = __builtin_amdgcn_readfirstlane(fabsf(all) < kNarrow), plain = !p.scaled && !p.cut;
+    const float power = narrow ? rintf(all * (float)kLog2e) : 0.f;   // the narrow form's sums are relative to 2^power
+    const int whole = 0x4b400000 + 128 * (int)power;
 #pragma unroll
     for (int i = 0; i < kVerifyLines; ++i) {
-      bool any = false;
+      if (!__builtin_amdgcn_ballot_w64(line_top[i] > -INFINITY)) continue;   // (a cut leaves few)
+      const int e0 = mine + 8 * kVerifyThreads * i;
+      float v[8];
+      if (e0 < end) {
+        lines[i].values(rd.row, e0, p.V, -INFINITY, v);
+        if (!plain)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) any |= x[i][j] > -INFINITY;
-      if (!__builtin_amdgcn_ballot_w64(any)) continue;   // (a cut leaves few)
+          for (int j = 0; j < 8; ++j) v[j] = rd.finish(p, v[j]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        double scale, y;
-        table_exp_parts(table, (double)x[i][j] - (double)all, scale, y);
-        double& s = j & 1 ? s1 : s0;
-        s = __builtin_fma(scale, y, s);
+        for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
+      }
+      if (narrow) {
+        add_exps(table, v, all - 690.f, whole, s0, s1);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          double scale, y;
+          table_exp_parts(table, (double)v[j] - (double)all, scale, y);
+          s0 = __builtin_fma(scale, y, s0);
+        }
       }
     }
-    const double s = wave_sum_f64(s0 + s1);
+    double s = wave_sum_f64(s0 + s1);
+    if (narrow) s *= table_exp(table, (double)power * 0.69314718055994530942 - (double)all);
     if (lane == 0) { tops[wave] = all; sums[wave] = s; }
   }
   __syncthreads();
@@ -276,25 +345,40 @@ static __device__ __forceinline__ double block_sum(double x, double* scratch) {
   return s;
 }
 
-// This thread's share of the sum of (p - c q)+ over the places [0, places) from `first` on of a row.
-template <int DT>
+// This thread's share of the sum of (p - c q)+ over the places [0, places) from `first` on of a row, kAhead lines in flight.
+template <int kAhead, int DT>
 static __device__ __forceinline__ double left_over(const VerifyParams& p, const VerifyRow<DT>& rd, const double* table, int row,
                                                    int first, int places, int threads, float top, double sum, double c) {
   const uint8_t* qr = p.draft + (int64_t)row * p.draft_stride;
   const double inv = 1.0 / sum;
   const int begin = first - rd.shift, end = min(begin + places, p.V);
   double s = 0;
-  for (int e0 = begin + 8 * (int)threadIdx.x; e0 < end; e0 += 8 * threads) {
-    float x[8], y[8];
-    load8_any(qr, p.draft_dtype, e0, p.V, 0.f, y);
-    load8<DT>(rd.row, e0, p.V, -INFINITY, x);
+  for (int e0 = begin + 8 * (int)threadIdx.x; e0 < end; e0 += kAhead * 8 * threads) {
+    VerifyLine<DT> px[kAhead];
+    VerifyAnyLine qx[kAhead];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v = rd.finish(p, x[j]);
-      double scale, z;
-      table_exp_parts(table, (double)v - (double)top, scale, z);
-      const double w = v > -INFINITY ? scale * inv : 0.0;
-      s += fmax(__builtin_fma(w, z, -c * (double)y[j]), 0.0);
+    for (int i = 0; i < kAhead; ++i) {
+      const int e = e0 + i * 8 * threads;
+      if (e < end) {
+        px[i].fetch(rd.row, e, p.V);
+        qx[i].fetch(qr, p.draft_dtype, e, p.V);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int e = e0 + i * 8 * threads;
+      if (e >= end) break;
+      float x[8], y[8];
+      px[i].values(rd.row, e, p.V, -INFINITY, x);
+      qx[i].values(qr, p.draft_dtype, e, p.V, 0.f, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = rd.finish(p, x[j]);
+        double scale, z;
+        table_exp_parts(table, (double)v - (double)top, scale, z);
+        const double w = v > -INFINITY ? scale * inv : 0.0;
+        s += fmax(__builtin_fma(w, z, -c * (double)y[j]), 0.0);
+      }
     }
   }
   return s;
@@ -380,14 +464,16 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     double before = 0;
     const int i = tid;
     const int up = i < n ? parent[i] : -1;
-    if (up >= 0)
-      for (int j = up + 1; j < i; ++j) again |= parent[j] == up && token[j] == token[i];
+    const int tok = i < n ? token[i] : -1, most = min(n, (tid | 63) + 1);   // (one count of turns for the wavefront)
+#pragma unroll 8
+    for (int j = 1; j < most; ++j) again |= (parent[j] == up) & (token[j] == tok) & (j < i);
     __syncthreads();
-    if (again) prob[i] = 0;
+    if (again && up >= 0) prob[i] = 0;
     __syncthreads();
-    if (i < n) p.removed[begin + i] = again ? -1 : token[i];
+    if (i < n) p.removed[begin + i] = again ? -1 : tok;
+#pragma unroll 8
+    for (int j = 1; j < most; ++j) before += (parent[j] == up) & (j < i) ? prob[j] : 0.0;
     if (up >= 0) {
-      for (int j = up + 1; j < i; ++j) before += parent[j] == up ? prob[j] : 0.0;
       if ((double)p.uniform[begin + i] * (1.0 - before) < prob[i]) atomicMin(&after[up], i);
     }
     __syncthreads();
@@ -409,13 +495,12 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   }
   // Draft probabilities: the rejections of a node's earlier children decide what a later one is held against.
   if (tid < n) {
-    int next = -1;
-    if (parent[tid] >= 0) {
-      atomicMin(&after[parent[tid]], tid);
-      for (int j = tid + 1; j < n && next < 0; ++j)
-        if (parent[j] == parent[tid]) next = j;
-    }
-    sibling[tid] = next;
+    const int up = parent[tid];
+    int next = 0x7fffffff;
+    if (up >= 0) atomicMin(&after[up], tid);
+#pragma unroll 8
+    for (int j = (tid & ~63) + 1; j < n; ++j) next = min(next, (parent[j] == up) & (j > tid) ? j : 0x7fffffff);
+    sibling[tid] = up >= 0 && next < n ? next : -1;
   }
   __syncthreads();
   int at = 0, count = 1;
@@ -432,7 +517,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
       child = sibling[child];
       if (child >= 0) {   // (what is left matters to a sibling; the draw makes its own sum)
         const VerifyRow<DT> rd(p, begin + at);
-        left = block_sum(left_over(p, rd, table, begin + at, 0, p.V + rd.shift, kWalkThreads, top_s[at], sum_s[at], c), scratch);
+        left = block_sum(left_over<1>(p, rd, table, begin + at, 0, p.V + rd.shift, kWalkThreads, top_s[at], sum_s[at], c), scratch);
       }
     }
     if (child < 0) break;
@@ -460,28 +545,20 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_left_kernel(VerifyParam
   fill_exp_table(table);
   __syncthreads();
   const VerifyRow<DT> rd(p, st.row);
-  const double s = block_sum(left_over(p, rd, table, st.row, part * p.part, p.part, kVerifyThreads, st.top, st.sum, st.c), scratch);
+  const double s = block_sum(left_over<2>(p, rd, table, st.row, part * p.part, p.part, kVerifyThreads, st.top, st.sum, st.c), scratch);
   if (threadIdx.x == 0) p.residual[(int64_t)r * p.parts + part] = s;
-}
-
-// Inclusive sums over the lanes.
-static __device__ __forceinline__ double wave_scan_f64(double x, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  return x;
 }
 
 // The draw of a request's last token: the part that holds it (every wavefront, a part to a lane), then the place inside the
 // part, whose weights the threads hold.
+constexpr int kDrawThreads = 1024;
+static_assert(kVerifyPart == 8 * kDrawThreads, "eight places to a thread");
 template <int DT, int MODE>
-__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyParams p) {
-  constexpr int kWaves = kVerifyThreads / 64;
+__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams p) {
+  constexpr int kWaves = kDrawThreads / 64;
   __shared__ double table[128];
   __shared__ double mass_s[kVerifyMostParts];
-  __shared__ double run[kVerifyLines][kWaves];
+  __shared__ double run[kWaves];
   __shared__ uint32_t gone[MODE == kTarget ? kVerifyPart / 32 : 1];
   __shared__ int found[2];
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -489,7 +566,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyParam
   if (st.row < 0) return;
   fill_exp_table(table);
   if (MODE == kTarget)
-    for (int i = tid; i < kVerifyPart / 32; i += kVerifyThreads) gone[i] = 0;
+    for (int i = tid; i < kVerifyPart / 32; i += kDrawThreads) gone[i] = 0;
   if (tid == 0) {
     found[0] = 0x7fffffff;
     found[1] = -1;
@@ -510,7 +587,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyParam
   // tokens that the rejected children took out: each once
   auto removed = [&](auto f) {
     if (MODE != kTarget || !st.tested) return;
-    for (int i = node + 1 + tid; i < n; i += kVerifyThreads)
+    for (int i = node + 1 + tid; i < n; i += kDrawThreads)
       if (p.parents[begin + i] == node && p.removed[begin + i] >= 0) f(p.removed[begin + i]);
   };
   if (MODE == kTarget && st.tested) {
@@ -521,20 +598,20 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyParam
     mass = mass_s[lane];
   }
   mass = fmax(mass, 0.0);
-  double sums = wave_scan_f64(mass, lane), total = __shfl(sums, 63, 64);
+  double sums = wave_scan_f64(mass), total = read_lane_f64(sums, 63);
   // Rejections that leave nothing (a target equal to the draft's, or smaller everywhere that it is kept, up to rounding):
   // the last token comes from the target itself.
   const bool nothing = !(total > 1e-13);
   if (nothing) {
     mass = whole;
-    sums = wave_scan_f64(mass, lane);
-    total = __shfl(sums, 63, 64);
+    sums = wave_scan_f64(mass);
+    total = read_lane_f64(sums, 63);
   }
   const double want = (double)p.uniform[begin] * total;
   const uint64_t beyond = __builtin_amdgcn_ballot_w64(sums > want && mass > 0.0);
   const uint64_t some = __builtin_amdgcn_ballot_w64(mass > total * 1e-18);   // (the sum's own rounding: the last part that has any)
   const int part = beyond ? __builtin_ctzll(beyond) : some ? 63 - __builtin_clzll(some) : 0;
-  const double rest = beyond ? want - __shfl(sums - mass, part, 64) : want;
+  const double rest = beyond ? want - read_lane_f64(sums - mass, part) : want;
   const int first = part * p.part - rd.shift;
   const uint8_t* qr = MODE == kDraft ? p.draft + (int64_t)st.row * p.draft_stride : nullptr;
   const bool minus = MODE == kDraft && st.tested && !nothing;
@@ -545,54 +622,41 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyParam
     });
     __syncthreads();
   }
-  double weight[kVerifyLines][8], mine[kVerifyLines];
+  double weight[8], mine = 0;
+  const int at = 8 * tid;
 #pragma unroll
-  for (int l = 0; l < kVerifyLines; ++l) {
-    const int i = 8 * (tid + l * kVerifyThreads);
-    mine[l] = 0;
-    if (i < p.part) {
-      float x[8], y[8];
-      load8<DT>(rd.row, first + i, p.V, -INFINITY, x);
-      if (minus) load8_any(qr, p.draft_dtype, first + i, p.V, 0.f, y);
-      const uint32_t out = MODE == kTarget ? gone[i >> 5] >> (i & 31) : 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        double w = chance(rd.finish(p, x[j]));
-        if (minus) w = fmax(w - st.c * (double)y[j], 0.0);
-        if (MODE == kTarget && (out >> j & 1)) w = 0;
-        weight[l][j] = w;
-        mine[l] += w;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) weight[l][j] = 0;
-    }
-  }
-  double upto[kVerifyLines];
-#pragma unroll
-  for (int l = 0; l < kVerifyLines; ++l) {
-    upto[l] = wave_scan_f64(mine[l], lane);
-    if (lane == 63) run[l][wave] = upto[l];
-  }
-  __syncthreads();
-  double before = 0;
-  int last = -1, place = 0x7fffffff;
-#pragma unroll
-  for (int l = 0; l < kVerifyLines; ++l) {
-    double sum = before;
-    for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) sum += run[l][w];
-      before += run[l][w];
-    }
-    sum += upto[l] - mine[l];
+  for (int j = 0; j < 8; ++j) weight[j] = 0;
+  if (at < p.part) {
+    VerifyLine<DT> px;
+    VerifyAnyLine qx;
+    px.fetch(rd.row, first + at, p.V);
+    if (minus) qx.fetch(qr, p.draft_dtype, first + at, p.V);
+    float x[8], y[8];
+    px.values(rd.row, first + at, p.V, -INFINITY, x);
+    if (minus) qx.values(qr, p.draft_dtype, first + at, p.V, 0.f, y);
+    const uint32_t out = MODE == kTarget ? gone[at >> 5] >> (at & 31) : 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      sum += weight[l][j];
-      if (weight[l][j] > 0) {
-        const int i = 8 * (tid + l * kVerifyThreads) + j;
-        last = i;
-        if (sum > rest && place == 0x7fffffff) place = i;
-      }
+      double w = chance(rd.finish(p, x[j]));
+      if (minus) w = fmax(w - st.c * (double)y[j], 0.0);
+      if (MODE == kTarget && (out >> j & 1)) w = 0;
+      weight[j] = w;
+      mine += w;
+    }
+  }
+  const double upto = wave_scan_f64(mine);
+  if (lane == 63) run[wave] = upto;
+  __syncthreads();
+  double sum = upto - mine;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) sum += w < wave ? run[w] : 0.0;
+  int last = -1, place = 0x7fffffff;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    sum += weight[j];
+    if (weight[j] > 0) {
+      last = at + j;
+      if (sum > rest && place == 0x7fffffff) place = at + j;
     }
   }
   if (place != 0x7fffffff) atomicMin(&found[0], place);
@@ -723,11 +787,11 @@ static void launch_verify(const VerifyParams& p, int mode, hipStream_t st) {
   if (p.T) hipLaunchKernelGGL((verify_rows_kernel<DT, false>), grid, block, 0, st, p);
   if (mode == kTarget) {
     hipLaunchKernelGGL((verify_walk_kernel<DT, kTarget>), dim3(p.R), dim3(kWalkThreads), 0, st, p);
-    hipLaunchKernelGGL((verify_draw_kernel<DT, kTarget>), dim3(p.R), block, 0, st, p);
+    hipLaunchKernelGGL((verify_draw_kernel<DT, kTarget>), dim3(p.R), dim3(kDrawThreads), 0, st, p);
   } else {
     hipLaunchKernelGGL((verify_walk_kernel<DT, kDraft>), dim3(p.R), dim3(kWalkThreads), 0, st, p);
     hipLaunchKernelGGL((verify_left_kernel<DT>), dim3(p.R, p.parts), block, 0, st, p);
-    hipLaunchKernelGGL((verify_draw_kernel<DT, kDraft>), dim3(p.R), block, 0, st, p);
+    hipLaunchKernelGGL((verify_draw_kernel<DT, kDraft>), dim3(p.R), dim3(kDrawThreads), 0, st, p);
   }
 }
 
