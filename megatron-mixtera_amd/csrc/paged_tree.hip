@@ -121,8 +121,8 @@ static __device__ __forceinline__ float tree_odd_sum(float count) {
   return n >> 12 ? __uint_as_float(0x7fc00000u) : up + down;
 }
 
-// SHARE: neighbouring wavefronts take other parts of the same tokens, and a barrier per tile keeps them on one tile, whose
-// lines then come from memory once and from the CU's cache for the others.  Where a request has fewer parts than there are
+// SHARE: neighbouring wavefronts take other parts of the same tokens, whose lines then come from memory once and from the
+// CU's cache for the others.  Where a request has fewer parts than there are
 // wavefronts, `ways` of them share a part and take every `ways`-th tile each; what they have is joined in LDS (`join`).
 template <int HD, int NT, int NQ, bool FP8, bool F16, bool SHARE>
 static __device__ __forceinline__ void tree_segment(const TreeParams& p, const TreeSegment& s, int h, int lane, int way, int ways, float* join) {
@@ -137,7 +137,6 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
   const int last = max(min(end, len) - 1, 0);
   const int step = SHARE ? TK * ways : TK;
   if (SHARE && tree_div_g(p, s.part * ROWS) >= s.nodes) {   // (a part without rows)
-    for (int T = start; T < end; T += step) __builtin_amdgcn_s_barrier();
     if (ways > 1) {
       __syncthreads();
       __syncthreads();
@@ -271,8 +270,7 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
     load_k(begin);
     load_v(begin);
   }
-  // (SHARE: as many tiles for every wavefront; those past the segment's end are seen by no row)
-  for (int T = begin; T < (SHARE ? end + TK * way : end); T += step) {
+  for (int T = begin; T < end; T += step) {
     // ---- S^T = K Q^T
     const float mul = FP8 ? p.scale_log2 * ksc : p.scale_log2;
     const bool masked = T + TK > min(ctx, end) || !k_page;   // wave-uniform
@@ -301,7 +299,6 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (SHARE) __builtin_amdgcn_s_barrier();
     load_k(T + step);   // (the key registers are free again)
     __builtin_amdgcn_sched_barrier(0);
     if (FP8) {        // a scale may have any sign: the maximum is of the products' own scores
@@ -1099,7 +1096,7 @@ static TreeShape tree_shape(int T, int R, int Hq, int Hkv, int head_dim, bool ma
     s.rows = 32 * s.waves;
   } else {
     const int rows = head_dim > 128 ? 16 : 32;
-    s.share = 4 * mean <= 3 * rows ? 1 : 4 * mean <= 6 * rows ? 2 : 4 * mean <= 12 * rows ? 4 : 8;   // (trees are of all sizes)
+    s.share = mean <= rows ? 1 : mean <= 2 * rows ? 2 : mean <= 4 * rows ? 4 : 8;
     s.heads = 1;
     for (int w = 2; w <= 8 / s.share; ++w)
       if (Hkv % w == 0) s.heads = w;

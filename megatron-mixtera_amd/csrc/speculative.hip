@@ -410,6 +410,21 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     }
     return;
   }
+  // a node to a thread: its parent, its token, what the parent's row says about it -- on their way during the sums below
+  static_assert(kVerifyNodes == kWalkThreads, "a node to a thread");
+  int up = -1;
+  int64_t drafted = -1;
+  if (tid < n) {
+    up = p.parents[begin + tid];
+    drafted = p.tokens[begin + tid];
+    if (tid == 0 || up < 0 || up >= tid) up = -1;
+  }
+  const bool inside = drafted >= 0 && drafted < p.V;
+  float said = -INFINITY, q = 0.f;
+  if (MODE != kGreedy && up >= 0 && inside) {
+    said = VerifyRow<DT>(p, begin + up).at(p, (int)drafted);
+    if (MODE == kDraft) q = load_element(p.draft + (int64_t)(begin + up) * p.draft_stride, p.draft_dtype, (int)drafted);
+  }
   fill_exp_table(table);
   __syncthreads();
   // maximum and sum of a row: a wavefront each, a part to a lane
@@ -431,40 +446,24 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
       }
     }
   }
-  static_assert(kVerifyNodes == kWalkThreads, "a node to a thread");
   if (tid < n) {
-    const int up = p.parents[begin + tid];
     after[tid] = 0x7fffffff;
-    parent[tid] = tid > 0 && up >= 0 && up < tid ? up : -1;
+    parent[tid] = up;
   }
   __syncthreads();
   if (MODE == kGreedy) {
-    for (int i = tid; i < n; i += kWalkThreads)
-      if (parent[i] >= 0 && p.tokens[begin + i] == token[parent[i]]) atomicMin(&after[parent[i]], i);
-  } else {
-    for (int i = tid; i < n; i += kWalkThreads) {
-      const int64_t t = p.tokens[begin + i];
-      const bool inside = t >= 0 && t < p.V;
-      token[i] = inside ? (int)t : -1;
-      prob[i] = 0;
-      q_s[i] = 0;
-      if (parent[i] >= 0 && inside) {
-        const int up = parent[i];
-        const VerifyRow<DT> rd(p, begin + up);
-        const float x = rd.at(p, (int)t);
-        if (sum_s[up] > 0) prob[i] = table_exp(table, (double)x - (double)top_s[up]) / sum_s[up];
-        if (MODE == kDraft) q_s[i] = load_element(p.draft + (int64_t)(begin + up) * p.draft_stride, p.draft_dtype, (int)t);
-      }
-    }
+    if (up >= 0 && drafted == token[up]) atomicMin(&after[up], tid);
+  } else if (tid < n) {
+    token[tid] = inside ? (int)drafted : -1;
+    prob[tid] = up >= 0 && inside && sum_s[up] > 0 ? table_exp(table, (double)said - (double)top_s[up]) / sum_s[up] : 0.0;
+    q_s[tid] = q;
   }
   __syncthreads();
   if (MODE == kTarget) {
     // a token that an earlier sibling had has left the distribution
     bool again = false;
     double before = 0;
-    const int i = tid;
-    const int up = i < n ? parent[i] : -1;
-    const int tok = i < n ? token[i] : -1, most = min(n, (tid | 63) + 1);   // (one count of turns for the wavefront)
+    const int i = tid, tok = inside ? (int)drafted : -1, most = min(n, (tid | 63) + 1);   // (one count of turns for the wavefront)
 #pragma unroll 8
     for (int j = 1; j < most; ++j) again |= (parent[j] == up) & (token[j] == tok) & (j < i);
     __syncthreads();
@@ -495,7 +494,6 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   }
   // Draft probabilities: the rejections of a node's earlier children decide what a later one is held against.
   if (tid < n) {
-    const int up = parent[tid];
     int next = 0x7fffffff;
     if (up >= 0) atomicMin(&after[up], tid);
 #pragma unroll 8
@@ -511,8 +509,8 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     double left = 1;
     int child = after[at] < n ? after[at] : -1;
     while (child >= 0) {
-      const double q = q_s[child], w = prob[child] - c * q;
-      if ((double)p.uniform[begin + child] * left * q < w) break;
+      const double of = q_s[child], w = prob[child] - c * of;
+      if ((double)p.uniform[begin + child] * left * of < w) break;
       c += left;
       child = sibling[child];
       if (child >= 0) {   // (what is left matters to a sibling; the draw makes its own sum)
@@ -573,7 +571,8 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
   }
   __syncthreads();
   const int begin = min(max(p.cu[r], 0), p.T), n = min(min(max(p.cu[r + 1], begin), p.T) - begin, kVerifyNodes);
-  const int node = st.row - begin;
+  const int node = st.row - begin, count = p.out_counts[r];
+  const float uniform = p.uniform[begin];
   const VerifyRow<DT> rd(p, st.row);
   const double inv = 1.0 / st.sum;
   auto chance = [&](float x) { return table_exp(table, (double)x - (double)st.top) * inv; };
@@ -607,7 +606,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
     sums = wave_scan_f64(mass);
     total = read_lane_f64(sums, 63);
   }
-  const double want = (double)p.uniform[begin] * total;
+  const double want = (double)uniform * total;
   const uint64_t beyond = __builtin_amdgcn_ballot_w64(sums > want && mass > 0.0);
   const uint64_t some = __builtin_amdgcn_ballot_w64(mass > total * 1e-18);   // (the sum's own rounding: the last part that has any)
   const int part = beyond ? __builtin_ctzll(beyond) : some ? 63 - __builtin_clzll(some) : 0;
@@ -664,7 +663,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
   __syncthreads();
   if (tid == 0) {
     const int i = found[0] != 0x7fffffff ? found[0] : found[1];
-    p.out_tokens[(int64_t)r * p.max_path + p.out_counts[r] - 1] = min(max(first + i, 0), p.V - 1);
+    p.out_tokens[(int64_t)r * p.max_path + count - 1] = min(max(first + i, 0), p.V - 1);
   }
 }
 
