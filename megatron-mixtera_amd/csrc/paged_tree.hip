@@ -217,37 +217,55 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
   uint32_t vf[NT][4][VD];
   float ksc = 1.f, vsc = 1.f;   // fp8: scales of the staged tiles' chunks
   bool k_page = true;           // whether the staged keys' chunk exists
-  // Tokens past the segment's last are that one again: their scores are masked, and what lies behind a request in its
-  // last chunk is never read.
+  // Tiles are read through buffer descriptors that end behind the request's last token: what lies behind arrives as zeros,
+  // and so does all of a chunk that the table does not name (its tokens are seen by no row).
+  constexpr int kPolicy = SHARE ? 0 : 2;   // (read once they stream past the caches)
+  const int k_lane = m16 * tok_bytes + 16 * g;
+  int v_lane[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v_lane[j] = (4 * g + j) * tok_bytes + DV * m16 * ESZ;
+  auto tile_of = [&](Cursor& c, const float* scales, const uint8_t* base, int T) {
+    const int t0 = min(T, last), ci = tree_chunk_of(t0, p.chunk_magic);
+    follow(c, scales, ci);
+    const uint32_t left = c.pc < 0 || T > last ? 0u : (uint32_t)min(len - T, TK);
+    const uint8_t* at = base + (int64_t)max(c.pc, 0) * chunk_bytes + (int64_t)(t0 - ci * p.chunk) * tok_bytes;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at), 0, (int)(left * (uint32_t)tok_bytes), 0x00020000);
+  };
   auto load_k = [&](int T) {
-    const int ci = tree_chunk_of(min(T, last), p.chunk_magic);
-    follow(kcur, p.k_scale, ci);
+    const auto rs = tile_of(kcur, p.k_scale, kbase, T);
     if (FP8) ksc = kcur.sc;
     k_page = kcur.pc >= 0;
-    const uint8_t* chunk = kbase + (int64_t)max(kcur.pc, 0) * chunk_bytes;
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int t0 = min(T + 16 * u, last);
-      const uint8_t* row = chunk + (uint32_t)(t0 - ci * p.chunk + min(last - t0, m16)) * tok_bytes + k_col;
+    for (int u = 0; u < NT; ++u)
 #pragma unroll
-      for (int kk = 0; kk < KL; ++kk) kf[u][kk] = SHARE ? ld16(row + 64 * kk) : ld16_stream(row + 64 * kk);
-    }
+      for (int kk = 0; kk < KL; ++kk)
+        kf[u][kk] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, k_lane + 64 * kk, 16 * u * tok_bytes, kPolicy));
   };
   auto load_v = [&](int T) {
-    const int ci = tree_chunk_of(min(T, last), p.chunk_magic);
-    follow(vcur, p.v_scale, ci);
+    const auto rs = tile_of(vcur, p.v_scale, vbase, T);
     if (FP8) vsc = vcur.sc;
-    const uint8_t* chunk = vbase + (int64_t)max(vcur.pc, 0) * chunk_bytes + v_col;
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int t0 = min(T + 16 * u, last);
+    for (int u = 0; u < NT; ++u)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint8_t* row = chunk + (uint32_t)(t0 - ci * p.chunk + min(last - t0, 4 * g + j)) * tok_bytes;
-        if constexpr (SHARE) ld_dwords(row, vf[u][j]);
-        else ld_dwords_stream(row, vf[u][j]);
+        const int soff = 16 * u * tok_bytes;
+        if constexpr (VD == 1) {
+          vf[u][j][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, v_lane[j], soff, kPolicy);
+        } else if constexpr (VD == 3) {
+          const auto x = __builtin_amdgcn_raw_buffer_load_b96(rs, v_lane[j], soff, kPolicy);
+          vf[u][j][0] = x[0]; vf[u][j][1] = x[1]; vf[u][j][2] = x[2];
+        } else {
+#pragma unroll
+          for (int w = 0; w + 4 <= VD; w += 4) {
+            const auto x = __builtin_amdgcn_raw_buffer_load_b128(rs, v_lane[j] + 4 * w, soff, kPolicy);
+            vf[u][j][w] = x[0]; vf[u][j][w + 1] = x[1]; vf[u][j][w + 2] = x[2]; vf[u][j][w + 3] = x[3];
+          }
+          if constexpr (VD % 4 == 2) {
+            const auto x = __builtin_amdgcn_raw_buffer_load_b64(rs, v_lane[j] + 4 * (VD - 2), soff, kPolicy);
+            vf[u][j][VD - 2] = x[0]; vf[u][j][VD - 1] = x[1];
+          }
+        }
       }
-    }
   };
 
   // The running maximum starts at a finite lowest value: a row that sees nothing keeps it and a sum of zero.
