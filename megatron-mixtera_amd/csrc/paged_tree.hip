@@ -317,6 +317,7 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
       }
     }
     __builtin_amdgcn_sched_barrier(0);
+    if (!SHARE && !((T - begin) & (8 * TK - 1))) __builtin_amdgcn_s_barrier();
     load_k(T + step);   // (the key registers are free again)
     __builtin_amdgcn_sched_barrier(0);
     if (FP8) {        // a scale may have any sign: the maximum is of the products' own scores
@@ -882,6 +883,7 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
 // every wavefront walks the same ones.  Up to 64 requests lie in the lanes of every wavefront (no LDS, no barrier), more in
 // dynamic LDS: tiles and groups of requests 0 .. i.  (The entry point has made sure that all tiles together are an int.)
 // Clears the rows behind the last request on the way.
+constexpr int kTreeStart = 1;   // what a pair's start counts, in tiles
 template <int HD, int TK, typename Seg>
 static __device__ __forceinline__ void tree_walk(const TreeParams& p, Seg seg) {
   extern __shared__ int32_t tree_lds[];
@@ -944,13 +946,15 @@ static __device__ __forceinline__ void tree_walk(const TreeParams& p, Seg seg) {
     }
   }
 
-  // The span: equal shares where the tiles fill the grid, otherwise few tiles each -- a span's tiles follow one another,
-  // every further span of a pair is one more partial to merge.
+  // The span: equal shares where the tiles fill the grid (a pair's start counts as one more: its queries, table entries and
+  // first tile arrive one trip after the other), otherwise few tiles each -- a span's tiles follow one another, every further
+  // span of a pair is one more partial to merge.
   if (total == 0) return;
   const int span = max(1, (int)rintf(__builtin_amdgcn_sqrtf(0.035f * (float)total * __builtin_amdgcn_rcpf((float)pairs))));
+  const int extra = total / span >= p.grid ? kTreeStart : 0;
   int t0, t1;
-  if (total / span >= p.grid) {
-    const int per = total / p.grid, rem = total - per * p.grid;
+  if (extra) {
+    const int all = total + extra * pairs, per = all / p.grid, rem = all - per * p.grid;
     t0 = (int)blockIdx.x * per + min((int)blockIdx.x, rem);
     t1 = t0 + per + ((int)blockIdx.x < rem ? 1 : 0);
   } else {
@@ -960,28 +964,32 @@ static __device__ __forceinline__ void tree_walk(const TreeParams& p, Seg seg) {
   if (t0 >= t1) return;
   int r;   // the first request whose tiles reach beyond t0
   if (in_lanes) {
-    r = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < p.R && cum_l > t0));
+    r = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < p.R && cum_l + extra * first_l > t0));
   } else {
     int lo = 0, hi = p.R - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (cum[mid] > t0) hi = mid; else lo = mid + 1;
+      if (cum[mid] + extra * first[mid] > t0) hi = mid; else lo = mid + 1;
     }
     r = __builtin_amdgcn_readfirstlane(lo);
   }
   for (; t0 < t1; ++r) {
-    const int rb = r ? cum_at(r - 1) : 0, re = cum_at(r);
+    const int rb = r ? cum_at(r - 1) + extra * first_at(r - 1) : 0, re = cum_at(r) + extra * first_at(r);
     if (t0 >= re) continue;
     const TreeRequest t = request_at(r);
-    const int tiles = max((t.len + TK - 1) / TK, 1);
+    const int tiles = max((t.len + TK - 1) / TK, 1) + extra;
     TreeSegment s;
     s.r = r; s.q_begin = t.q_begin; s.nodes = t.nodes; s.len = t.len; s.ctx = t.len - t.nodes;
     while (t0 < t1 && t0 < re) {
       s.group = __builtin_amdgcn_readfirstlane((t0 - rb) / tiles);
       const int tb = t0 - rb - s.group * tiles, te = min(tiles, tb + (t1 - t0));
-      const bool begins = tb == 0, ends = te == tiles;
-      s.start = tb * TK;
-      s.end = min(te * TK, t.len);
+      if (te <= extra) {
+        t0 += te - tb;
+        continue;
+      }
+      const bool begins = tb <= extra, ends = te == tiles;
+      s.start = max(tb - extra, 0) * TK;
+      s.end = min((te - extra) * TK, t.len);
       s.whole = begins && ends;
       s.slot = 2 * blockIdx.x + (begins ? 1 : 0);
       // (read across the lanes while all of them are on: inside the branch a value that was put aside comes back for lane 0 only)
@@ -1236,7 +1244,7 @@ extern "C" int mi_paged_tree_attention(
   // lies in one chunk
   const int nt = wide || chunk_tokens % 32 ? 1 : fp8 && head_dim == 64 && chunk_tokens % 64 == 0 ? 4 : 2;
   const int tile = many ? 32 : 16 * nt;
-  if (tree_most_pairs(T, R, G, shape.rows) * ((int64_t)table_columns * chunk_tokens / tile + 1) >= (int64_t)1 << 31)
+  if (tree_most_pairs(T, R, G, shape.rows) * ((int64_t)table_columns * chunk_tokens / tile + 2) >= (int64_t)1 << 31)
     return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: rows per KV head times the tokens of a table row must stay below some 2^36");
   for (int r0 = 0; r0 < R; r0 += kTreeRequestsPerLaunch) {
     p.r_base = r0;
