@@ -621,7 +621,8 @@ def paged_tree_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, cu_seqlens
     ``kv_lens`` counts.  A node attends to the context before them and to the nodes of its row of ``tree_mask`` (int64
     ``[T]`` or ``[T, words]``, up to four words: bit j % 64 of word j // 64 is node j of the request, its own bit
     included; see :func:`tree_masks`).  Rows that see nothing and rows behind the last request are zeros.  Byte caches
-    with ``k_scales`` / ``v_scales`` ``[N, Hkv]`` hold e4m3 values (head_dim 64 or 128)."""
+    with ``k_scales`` / ``v_scales`` ``[N, Hkv]`` hold e4m3 values (head_dim 64 or 128).  ``max_kv_len`` is taken as the other
+    attention operators take it and decides nothing: the work is split by the lengths, on the GPU."""
     return _native().paged_tree_attention(q, k_cache, v_cache, cu_seqlens_q, kv_lens, block_table, tree_mask,
                                           softmax_scale, out, k_scales, v_scales, _override())
 
