@@ -229,7 +229,7 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
     follow(c, scales, ci);
     const uint32_t left = c.pc < 0 || T > last ? 0u : (uint32_t)min(len - T, TK);
     const uint8_t* at = base + (int64_t)max(c.pc, 0) * chunk_bytes + (int64_t)(t0 - ci * p.chunk) * tok_bytes;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at), 0, (int)(left * (uint32_t)tok_bytes), 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at), 0, (int)(left ? (left - 1) * (uint32_t)tok_bytes + HD * ESZ : 0u), 0x00020000);
   };
   auto load_k = [&](int T) {
     const auto rs = tile_of(kcur, p.k_scale, kbase, T);
@@ -597,7 +597,7 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
   auto issue = [&] {
     const bool there = (uint32_t)pc < (uint32_t)p.n_chunks;
     const int64_t off = (int64_t)(there ? pc : 0) * chunk_bytes + i_in * tile_bytes;
-    const uint32_t nrec = there && i_tile < tiles_end ? (uint32_t)min(len - i_tile * TK, TK) * (uint32_t)tok_bytes : 0u;
+    const uint32_t nrec = there && i_tile < tiles_end ? (uint32_t)(min(len - i_tile * TK, TK) - 1) * (uint32_t)tok_bytes + HD * 2 : 0u;
     const uint32_t bit = 1u << (i_tile & 31);
     missing = there ? missing & ~bit : missing | bit;
 #pragma unroll

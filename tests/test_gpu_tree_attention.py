@@ -249,6 +249,32 @@ def test_strides(mi, dev):
     assert c.run(mi, q=c.q.to(dev).unsqueeze(1)).shape == (T, 1, 8, 64)
 
 
+@pytest.mark.parametrize("layout", ["heads first", "one token for all", "padded rows"])
+@pytest.mark.parametrize("nodes,Hq,fp8", [([5, 9], 8, False), ([12, 3], 16, True), ([40, 61], 16, False), ([30, 50], 16, True)])
+def test_cache_layouts(mi, dev, layout, nodes, Hq, fp8):
+    """Token rows nearer together than a row is long, at the same place, and further apart; the last chunk of the pool is used."""
+    case = Case(dev, nodes, [100, 37], Hq=Hq, Hkv=4, d=64, chunk=32, fp8=fp8, seed=Hq)
+    case.table[0, 0] = case.N - 1
+    if layout == "one token for all":
+        case.k, case.v = (x[:, :1].expand_as(x).contiguous() for x in (case.k, case.v))
+    gpu = []
+    for x in (case.k, case.v):
+        x = (x.view(torch.uint8) if fp8 else x).to(dev)
+        if layout == "heads first":
+            x = x.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+        elif layout == "one token for all":
+            x = x[:, :1].contiguous().expand_as(x)
+        else:
+            wide = torch.empty(*x.shape[:2], 5, x.size(3), dtype=x.dtype, device=dev)
+            wide[:, :, :4] = x
+            x = wide[:, :, :4]
+        gpu.append(x)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    scales = dict(k_scales=case.scales[0].to(dev), v_scales=case.scales[1].to(dev)) if fp8 else {}
+    case.check(mi, mi.ops.paged_tree_attention(case.q.to(dev), *gpu, i32(case.cu), i32(case.lens), case.table.to(dev), case.mask.to(dev),
+                                               softmax_scale=case.scale, max_kv_len=max(case.lens), **scales))
+
+
 def test_many_requests(mi, dev):
     """More than one launch takes (their prefix sums lie in LDS): every one is answered, ragged and empty ones among them."""
     rng = random.Random(18)
