@@ -345,40 +345,30 @@ static __device__ __forceinline__ double block_sum(double x, double* scratch) {
   return s;
 }
 
-// This thread's share of the sum of (p - c q)+ over the places [0, places) from `first` on of a row, kAhead lines in flight.
-template <int kAhead, int DT>
+// This thread's share of the sum of (p - c q)+ over the places [0, places) from `first` on of a row.  (Two or four lines ahead
+// of their use took more registers and as much time.)
+template <int DT>
 static __device__ __forceinline__ double left_over(const VerifyParams& p, const VerifyRow<DT>& rd, const double* table, int row,
                                                    int first, int places, int threads, float top, double sum, double c) {
   const uint8_t* qr = p.draft + (int64_t)row * p.draft_stride;
   const double inv = 1.0 / sum;
   const int begin = first - rd.shift, end = min(begin + places, p.V);
   double s = 0;
-  for (int e0 = begin + 8 * (int)threadIdx.x; e0 < end; e0 += kAhead * 8 * threads) {
-    VerifyLine<DT> px[kAhead];
-    VerifyAnyLine qx[kAhead];
+  for (int e0 = begin + 8 * (int)threadIdx.x; e0 < end; e0 += 8 * threads) {
+    VerifyLine<DT> px;
+    VerifyAnyLine qx;
+    px.fetch(rd.row, e0, p.V);
+    qx.fetch(qr, p.draft_dtype, e0, p.V);
+    float x[8], y[8];
+    px.values(rd.row, e0, p.V, -INFINITY, x);
+    qx.values(qr, p.draft_dtype, e0, p.V, 0.f, y);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int e = e0 + i * 8 * threads;
-      if (e < end) {
-        px[i].fetch(rd.row, e, p.V);
-        qx[i].fetch(qr, p.draft_dtype, e, p.V);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int e = e0 + i * 8 * threads;
-      if (e >= end) break;
-      float x[8], y[8];
-      px[i].values(rd.row, e, p.V, -INFINITY, x);
-      qx[i].values(qr, p.draft_dtype, e, p.V, 0.f, y);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = rd.finish(p, x[j]);
-        double scale, z;
-        table_exp_parts(table, (double)v - (double)top, scale, z);
-        const double w = v > -INFINITY ? scale * inv : 0.0;
-        s += fmax(__builtin_fma(w, z, -c * (double)y[j]), 0.0);
-      }
+    for (int j = 0; j < 8; ++j) {
+      const float v = rd.finish(p, x[j]);
+      double scale, z;
+      table_exp_parts(table, (double)v - (double)top, scale, z);
+      const double w = v > -INFINITY ? scale * inv : 0.0;
+      s += fmax(__builtin_fma(w, z, -c * (double)y[j]), 0.0);
     }
   }
   return s;
@@ -515,7 +505,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
       child = sibling[child];
       if (child >= 0) {   // (what is left matters to a sibling; the draw makes its own sum)
         const VerifyRow<DT> rd(p, begin + at);
-        left = block_sum(left_over<1>(p, rd, table, begin + at, 0, p.V + rd.shift, kWalkThreads, top_s[at], sum_s[at], c), scratch);
+        left = block_sum(left_over(p, rd, table, begin + at, 0, p.V + rd.shift, kWalkThreads, top_s[at], sum_s[at], c), scratch);
       }
     }
     if (child < 0) break;
@@ -539,11 +529,11 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_left_kernel(VerifyParam
   __shared__ double scratch[kVerifyThreads / 64];
   const int part = blockIdx.y, r = blockIdx.x;
   const VerifyState st = p.state[r];
-  if (st.row < 0 || !st.tested) return;
-  fill_exp_table(table);
+  fill_exp_table(table);   // (the state is on its way)
   __syncthreads();
+  if (st.row < 0 || !st.tested) return;
   const VerifyRow<DT> rd(p, st.row);
-  const double s = block_sum(left_over<2>(p, rd, table, st.row, part * p.part, p.part, kVerifyThreads, st.top, st.sum, st.c), scratch);
+  const double s = block_sum(left_over(p, rd, table, st.row, part * p.part, p.part, kVerifyThreads, st.top, st.sum, st.c), scratch);
   if (threadIdx.x == 0) p.residual[(int64_t)r * p.parts + part] = s;
 }
 
@@ -561,8 +551,8 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
   __shared__ int found[2];
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const VerifyState st = p.state[r];
-  if (st.row < 0) return;
-  fill_exp_table(table);
+  const int begin = min(max(p.cu[r], 0), p.T), n = min(min(max(p.cu[r + 1], begin), p.T) - begin, kVerifyNodes);
+  fill_exp_table(table);   // (the state is on its way)
   if (MODE == kTarget)
     for (int i = tid; i < kVerifyPart / 32; i += kDrawThreads) gone[i] = 0;
   if (tid == 0) {
@@ -570,7 +560,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
     found[1] = -1;
   }
   __syncthreads();
-  const int begin = min(max(p.cu[r], 0), p.T), n = min(min(max(p.cu[r + 1], begin), p.T) - begin, kVerifyNodes);
+  if (st.row < 0) return;
   const int node = st.row - begin, count = p.out_counts[r];
   const float uniform = p.uniform[begin];
   const VerifyRow<DT> rd(p, st.row);

@@ -653,7 +653,8 @@ def verify_drafted_tokens(logits: Tensor, tokens: Tensor, parents: Tensor, cu_se
     bf16 or fp16): row i is the distribution that the children of node i were drawn from; without it the drafted tokens
     count as chosen.  ``uniform`` fp32 ``[T]``: a root's number draws its request's last token, any other node's decides
     about it.  ``temperature`` and ``cut`` (``[T]``, as ``sample_from_logits(..., return_cut=True)`` returns it) make the
-    target's distribution.  A path has at most ``max_path`` nodes, the root included.
+    target's distribution.  A path has at most ``max_path`` nodes, the root included; of a request's nodes the first 1 024
+    are looked at.
 
     Returns ``(tokens int64 [R, max_path], rows int32 [R, max_path], counts int32 [R])``: each request's new tokens, the
     rows of the nodes on its path (root first) and how many there are of each; -1 behind them."""
