@@ -410,6 +410,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     if (tid == 0 || up < 0 || up >= tid) up = -1;
   }
   const bool inside = drafted >= 0 && drafted < p.V;
+  const float chance = MODE == kTarget && tid < n ? p.uniform[begin + tid] : 0.f;
   float said = -INFINITY, q = 0.f;
   if (MODE != kGreedy && up >= 0 && inside) {
     said = VerifyRow<DT>(p, begin + up).at(p, (int)drafted);
@@ -419,20 +420,32 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   __syncthreads();
   // maximum and sum of a row: a wavefront each, a part to a lane
   static_assert(kVerifyMostParts == 64, "a part to a lane");
-  for (int i = tid >> 6; i < n; i += kWalkThreads / 64) {
-    VerifyPartial part{0, -INFINITY, 0x7fffffff};
-    if (lane < p.parts) part = p.partial[(int64_t)(begin + i) * p.parts + lane];
-    const float top = wave_max_f32(part.max);
-    if (MODE == kGreedy) {
-      int best = part.max == top ? part.index : 0x7fffffff;
+  constexpr int kWaves = kWalkThreads / 64, kAhead = 4;
+  for (int i0 = tid >> 6; i0 < n; i0 += kAhead * kWaves) {
+    VerifyPartial parts[kAhead];
 #pragma unroll
-      for (int d = 32; d > 0; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
-      if (lane == 0) token[i] = best;   // (of the row, here)
-    } else {
-      const double s = wave_sum_f64(part.max > -INFINITY ? part.sum * table_exp(table, (double)part.max - (double)top) : 0.0);
-      if (lane == 0) {
-        top_s[i] = top;
-        sum_s[i] = s;
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kWaves;
+      parts[k] = VerifyPartial{0, -INFINITY, 0x7fffffff};
+      if (i < n && lane < p.parts) parts[k] = p.partial[(int64_t)(begin + i) * p.parts + lane];
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kWaves;
+      if (i >= n) break;
+      const VerifyPartial& part = parts[k];
+      const float top = wave_max_f32(part.max);
+      if (MODE == kGreedy) {
+        int best = part.max == top ? part.index : 0x7fffffff;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
+        if (lane == 0) token[i] = best;   // (of the row, here)
+      } else {
+        const double s = wave_sum_f64(part.max > -INFINITY ? part.sum * table_exp(table, (double)part.max - (double)top) : 0.0);
+        if (lane == 0) {
+          top_s[i] = top;
+          sum_s[i] = s;
+        }
       }
     }
   }
@@ -453,7 +466,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     // a token that an earlier sibling had has left the distribution
     bool again = false;
     double before = 0;
-    const int i = tid, tok = inside ? (int)drafted : -1, most = min(n, (tid | 63) + 1);   // (one count of turns for the wavefront)
+    const int i = tid, tok = inside ? (int)drafted : -1, most = (tid & ~63) < n ? min(n, (tid | 63) + 1) : 0;   // (one count of turns for the wavefront)
 #pragma unroll 8
     for (int j = 1; j < most; ++j) again |= (parent[j] == up) & (token[j] == tok) & (j < i);
     __syncthreads();
@@ -461,9 +474,9 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     __syncthreads();
     if (i < n) p.removed[begin + i] = again ? -1 : tok;
 #pragma unroll 8
-    for (int j = 1; j < most; ++j) before += (parent[j] == up) & (j < i) ? prob[j] : 0.0;
+    for (int j = 1; j < most; ++j) before = __builtin_fma(prob[j], (parent[j] == up) & (j < i) ? 1.0 : 0.0, before);   // (a load a turn, no branch)
     if (up >= 0) {
-      if ((double)p.uniform[begin + i] * (1.0 - before) < prob[i]) atomicMin(&after[up], i);
+      if ((double)chance * (1.0 - before) < prob[i]) atomicMin(&after[up], i);
     }
     __syncthreads();
   }
@@ -472,8 +485,9 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
       int at = 0, count = 1;
       rows[0] = begin;
       while (count < p.max_path && after[at] < n) {
-        at = after[at];
-        out[count - 1] = p.tokens[begin + at];
+        const int next = after[at];
+        out[count - 1] = token[MODE == kGreedy ? at : next];   // (an accepted token is its parent's largest logit)
+        at = next;
         rows[count++] = begin + at;
       }
       p.out_counts[r] = count;
@@ -511,7 +525,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     if (child < 0) break;
     at = child;
     if (tid == 0) {
-      out[count - 1] = p.tokens[begin + at];
+      out[count - 1] = token[at];
       rows[count] = begin + at;
     }
     ++count;
