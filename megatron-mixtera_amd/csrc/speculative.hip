@@ -208,10 +208,18 @@ static __device__ __forceinline__ double read_lane_f64(double x, int lane) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 static __device__ __forceinline__ double wave_sum_f64(double x) { return read_lane_f64(wave_scan_f64(x), 63); }
+template <int CTRL, int MASK>
+static __device__ __forceinline__ float dpp_max_f32(float x) {   // (-inf where there is no lane)
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp((int)0xff800000u, __float_as_int(x), CTRL, MASK, 0xf, false)));
+}
 static __device__ __forceinline__ float wave_max_f32(float x) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
-  return x;
+  x = dpp_max_f32<0x111, 0xf>(x);
+  x = dpp_max_f32<0x112, 0xf>(x);
+  x = dpp_max_f32<0x114, 0xf>(x);
+  x = dpp_max_f32<0x118, 0xf>(x);
+  x = dpp_max_f32<0x142, 0xa>(x);
+  x = dpp_max_f32<0x143, 0xc>(x);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
 // Sum of e^(x - top) over eight logits, `top` among the row's wavefront, |top| < kNarrow: the exponent's whole 128ths and what
@@ -219,11 +227,12 @@ static __device__ __forceinline__ float wave_max_f32(float x) {
 // fraction's own e^. as 1 + a 32-bit polynomial of at most 0.0027: 6e-10 of a weight at most, a hundredth of half a step of the
 // uniform numbers that it meets, in two thirds of the 64-bit form's time.
 constexpr float kNarrow = 16384.f;
-static __device__ __forceinline__ void add_exps(const double* table, const float (&x)[8], float low, int whole, double& sum, double& rest) {
+static __device__ __forceinline__ void add_exps(const double* table, const float (&x)[8], float low, int whole, bool few, double& sum, double& rest) {
   constexpr double kStep = kLog2e * 128, kLn = 0.69314718055994530942 / 128;
   constexpr float kHigh = (float)kStep, kLow = (float)(kStep - (double)kHigh), kMagic = 12582912.f;   // 1.5 2^23
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
+    if (few && !__builtin_amdgcn_ballot_w64(x[j] > -INFINITY)) continue;
     const float v = fmaxf(x[j], low);
     const float u = __builtin_fmaf(v, kHigh, kMagic);
     float r = __builtin_fmaf(v, kHigh, -(u - kMagic));
@@ -255,10 +264,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
 #pragma unroll
   for (int i = 0; i < kVerifyLines; ++i)
     if (mine + 8 * kVerifyThreads * i < end) lines[i].fetch(rd.row, mine + 8 * kVerifyThreads * i, p.V);
-  if (!GREEDY) {
-    fill_exp_table(table);
-    __syncthreads();
-  }
+  if (!GREEDY) fill_exp_table(table);
   float top = -INFINITY, line_top[kVerifyLines];
   int place = 0x7fffffff;
 #pragma unroll
@@ -281,12 +287,15 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
       top = fmaxf(top, line_top[i]);
     }
   }
-  const float all = wave_max_f32(top);
+  const float wave_top = wave_max_f32(top);
+  if (lane == 0) tops[wave] = wave_top;
+  __syncthreads();   // (the table, too)
+  const float all = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   if constexpr (GREEDY) {
     int best = top == all ? place : 0x7fffffff;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
-    if (lane == 0) { tops[wave] = all; places[wave] = best; }
+    if (lane == 0) places[wave] = best;
   } else {
     double s0 = 0, s1 = 0;
     const bool narrow = __builtin_amdgcn_readfirstlane(fabsf(all) < kNarrow), plain = !p.scaled && !p.cut;
@@ -307,7 +316,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
         for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
       }
       if (narrow) {
-        add_exps(table, v, all - 690.f, whole, s0, s1);
+        add_exps(table, v, all - 690.f, whole, p.cut != nullptr, s0, s1);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -317,18 +326,17 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
         }
       }
     }
-    double s = wave_sum_f64(s0 + s1);
-    if (narrow) s *= table_exp(table, (double)power * 0.69314718055994530942 - (double)all);
-    if (lane == 0) { tops[wave] = all; sums[wave] = s; }
+    const double s = wave_sum_f64(s0 + s1);
+    if (lane == 0) sums[wave] = s;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    VerifyPartial o;
-    o.sum = 0; o.max = -INFINITY; o.index = 0x7fffffff;
-    for (int w = 0; w < 4; ++w) o.max = fmaxf(o.max, tops[w]);
-    for (int w = 0; w < 4; ++w) {
-      if (GREEDY) { if (tops[w] == o.max) o.index = min(o.index, places[w]); }
-      else if (tops[w] > -INFINITY) o.sum += sums[w] * table_exp(table, (double)tops[w] - (double)o.max);
+    VerifyPartial o{0, all, 0x7fffffff};
+    if constexpr (GREEDY) {
+      o.index = min(min(places[0], places[1]), min(places[2], places[3]));
+    } else {
+      o.sum = sums[0] + sums[1] + sums[2] + sums[3];
+      if (fabsf(all) < kNarrow) o.sum *= table_exp(table, (double)rintf(all * (float)kLog2e) * 0.69314718055994530942 - (double)all);
     }
     p.partial[(int64_t)row * p.parts + part] = o;
   }
