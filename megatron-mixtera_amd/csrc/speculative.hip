@@ -227,18 +227,20 @@ static __device__ __forceinline__ float wave_max_f32(float x) {
 // fraction's own e^. as 1 + a 32-bit polynomial of at most 0.0027: 6e-10 of a weight at most, a hundredth of half a step of the
 // uniform numbers that it meets, in two thirds of the 64-bit form's time.
 constexpr float kNarrow = 16384.f;
-static __device__ __forceinline__ void add_exps(const double* table, const float (&x)[8], float low, int whole, bool few, double& sum, double& rest) {
+static __device__ __forceinline__ void add_exps(const double* table, const float (&x)[8], float low, float top, int whole, bool few, double& sum, double& rest) {
   constexpr double kStep = kLog2e * 128, kLn = 0.69314718055994530942 / 128;
-  constexpr float kHigh = (float)kStep, kLow = (float)(kStep - (double)kHigh), kMagic = 12582912.f;   // 1.5 2^23
+  constexpr float kHigh = (float)kStep, kLow = (float)(kStep - (double)kHigh);
+  float magic = 12582912.f, second = (float)(kLn * kLn / 2);   // (1.5 2^23; both stay in registers)
+  asm("" : "+v"(magic), "+v"(second));
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if (few && !__builtin_amdgcn_ballot_w64(x[j] > -INFINITY)) continue;
-    const float v = fmaxf(x[j], low);
-    const float u = __builtin_fmaf(v, kHigh, kMagic);
-    float r = __builtin_fmaf(v, kHigh, -(u - kMagic));
+    const float v = __builtin_amdgcn_fmed3f(x[j], low, top);   // (NaN: low)
+    const float u = __builtin_fmaf(v, kHigh, magic);
+    float r = __builtin_fmaf(v, kHigh, -(u - magic));
     r = __builtin_fmaf(v, kLow, r);
     const int k = (int)__float_as_uint(u) - whole;
-    const float y = r * __builtin_fmaf(r, __builtin_fmaf(r, (float)(kLn * kLn * kLn / 6), (float)(kLn * kLn / 2)), (float)kLn);
+    const float y = r * __builtin_fmaf(r, __builtin_fmaf(r, (float)(kLn * kLn * kLn / 6), second), (float)kLn);
     const uint64_t t = __builtin_bit_cast(uint64_t, table[k & 127]);
     const uint32_t hi = (uint32_t)(t >> 32) + ((uint32_t)(k & ~127) << 13);
     const double w = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)t);
@@ -316,7 +318,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
         for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
       }
       if (narrow) {
-        add_exps(table, v, all - 690.f, whole, p.cut != nullptr, s0, s1);
+        add_exps(table, v, all - 690.f, all, whole, p.cut != nullptr, s0, s1);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
