@@ -532,8 +532,9 @@ static __device__ __forceinline__ TreeRequest tree_request(const TreeParams& p, 
   return t;
 }
 
-// ------------------------------------------------------------------------------------------------ many rows
-// Where a request has many rows per KV head the products are the work, and a CU's cache too slow a feed: a workgroup of
+// ------------------------------------------------------------------------------------------------ tiles through LDS
+// For 16-bit caches of widths 64 and 128.  Where a request has many rows per KV head the products are the work, and a CU's cache too
+// slow a feed; where it has few, tiles that wait in LDS keep more bytes on their way than registers do.  A workgroup of
 // WAVES wavefronts takes 32 * WAVES rows of one (request, KV head), and tiles of 32 tokens go straight from memory into LDS
 // (buffer loads with the LDS destination), STAGES - 1 of them ahead, one barrier a tile.  The 16-byte pieces of a row lie
 // in another order in every row (an exclusive or with the row's number, applied where the loads pick their source), which
@@ -1107,7 +1108,10 @@ __global__ __launch_bounds__(1024) void paged_tree_merge_kernel(TreeParams p, in
 }
 
 // Wavefronts per workgroup (`share` parts of a group times neighbouring KV heads), workgroups along the tiles, rows of a
-// group.  Parts share where the average request has more rows than one takes; `many`: paged_tree_rows_kernel.
+// group.  Parts share where the average request has more rows than one takes: on average 32 rows of an fp8 cache (4 to 12
+// nodes of 4 heads) took 455 us in parts of their own and 523 in shared ones, which read once and convert twice; 36 rows of a 16-bit
+// cache in chunks of 48 69 us shared.  `many`: paged_tree_rows_kernel, four wavefronts (two workgroups on a CU) up to the 128 rows they
+// take (16 requests of 4 096 tokens: 128 rows 75.5 us), eight beyond (132 rows 91.3, 256 rows 110.6).
 struct TreeShape {
   int waves, share, grid, heads, rows;
 };
@@ -1215,7 +1219,10 @@ extern "C" int mi_paged_tree_attention(
     return mi_fail(MI_ERR_WORKSPACE, "mi_paged_tree_attention: workspace too small (see mi_tree_workspace_bytes)");
   if ((uintptr_t)workspace & 15) return mi_fail(MI_ERR_ALIGN, "mi_paged_tree_attention: workspace must be 16-byte aligned");
 
-  const bool many = !fp8 && (head_dim == 64 || head_dim == 128) && chunk_tokens % 32 == 0 && tree_mean_rows(T, R, G) > 64;
+  // Through LDS wherever that kernel has the cache's form (16 requests of 4 096 tokens, 8 KV heads of 128, us: 8 rows 68.7 -> 51.0,
+  // 32 rows 86.8 -> 55.1, 64 rows 90.9 -> 60.4; one of 800, 20 rows: 19.5 -> 14.3; 64 requests of 4 300, 24 rows: 200 and 204), but for a few
+  // rows of width 64, where its steps cost more than the loads (64 requests of 4 300: 6 rows 100 and 125; of 2 000: 12 rows 52.9 and 49.8).
+  const bool many = !fp8 && chunk_tokens % 32 == 0 && (head_dim == 128 || (head_dim == 64 && tree_mean_rows(T, R, G) >= 12));
   const TreeShape shape = tree_shape(T, R, Hq, Hkv, head_dim, many);
   const bool f16 = dtype == MI_DTYPE_FP16;
   TreeParams p;
@@ -1293,7 +1300,7 @@ extern "C" int mi_paged_tree_attention(
     else if (fp8) MI_TREE_8(128);
     else if (head_dim == 64) MI_TREE_16(64);
     else if (head_dim == 96) MI_TREE_16(96);
-    else if (head_dim == 128) MI_TREE_16(128);
+    else if (head_dim == 128) MI_TREE(128, 1, 2, false);
     else if (head_dim == 192) MI_TREE(192, 1, 1, false);
     else MI_TREE(256, 1, 1, false);
 #undef MI_TREE_ROWS
