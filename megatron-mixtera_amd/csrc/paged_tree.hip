@@ -14,13 +14,18 @@
 // leaves normalised fp32 partials and a base-2 log-sum-exp for the merge.  A span touches at most one pair that began
 // before it and one that goes on after it, so two slots per workgroup hold all partials.
 //
-// Per tile nothing goes through LDS: S^T = K Q^T lands as lane (row m16, g) slot i = token 4g + i, the B operand of
-// O^T += V^T P^T, whose A operand is built from row loads by byte permutes; a pair of 16-token sub-tiles makes one product
-// of depth 32 (the products only need the same tokens in the same slots on both sides).
+// S^T = K Q^T lands as lane (row m16, g) slot i = token 4g + i, the B operand of O^T += V^T P^T; a pair of 16-token sub-tiles
+// makes one product of depth 32 (the products only need the same tokens in the same slots on both sides).  Two kernels: one
+// keeps its tiles in registers (any cache; V's operand is built from row loads by byte permutes), one in LDS (below).
 //
 // Only the tiles that reach past the context look at the bits.  A node's value row may hold infinities or NaN that rows
 // which do not see it must not meet, although a product multiplies it by their zeros: such values are taken out of their
 // tile and added to the sums of the rows that see them.
+//
+// The register kernel is bound by memory: 64 requests of 6 nodes over 512-8 192 tokens (24 rows, 8 KV heads of 128, 1.12 GB) took
+// it 205 us, 5.4 TB/s.  Loads through buffer descriptors, whose offsets stay in registers: 226 -> 222 us; wavefronts that meet every
+// eighth tile, so that none is left to read alone at the end: 222 -> 208 (every tile: 210, and an fp8 cache 455 -> 495 where every
+// eighth takes 444); a pair's start counted as a tile: 208 -> 205.
 #include <atomic>
 #include <type_traits>
 
@@ -122,8 +127,8 @@ static __device__ __forceinline__ float tree_odd_sum(float count) {
 }
 
 // SHARE: neighbouring wavefronts take other parts of the same tokens, whose lines then come from memory once and from the
-// CU's cache for the others.  Where a request has fewer parts than there are
-// wavefronts, `ways` of them share a part and take every `ways`-th tile each; what they have is joined in LDS (`join`).
+// CU's cache for the others.  Where a request has fewer parts than there are wavefronts, `ways` of them share a part and take every
+// `ways`-th tile each; what they have is joined in LDS (`join`).
 template <int HD, int NT, int NQ, bool FP8, bool F16, bool SHARE>
 static __device__ __forceinline__ void tree_segment(const TreeParams& p, const TreeSegment& s, int h, int lane, int way, int ways, float* join) {
   constexpr int KS = HD / 32, DV = HD / 16, ESZ = FP8 ? 1 : 2, TK = 16 * NT, ROWS = 16 * NQ;
@@ -536,10 +541,14 @@ static __device__ __forceinline__ TreeRequest tree_request(const TreeParams& p, 
 // For 16-bit caches of widths 64 and 128.  Where a request has many rows per KV head the products are the work, and a CU's cache too
 // slow a feed; where it has few, tiles that wait in LDS keep more bytes on their way than registers do.  A workgroup of
 // WAVES wavefronts takes 32 * WAVES rows of one (request, KV head), and tiles of 32 tokens go straight from memory into LDS
-// (buffer loads with the LDS destination), STAGES - 1 of them ahead, one barrier a tile.  The 16-byte pieces of a row lie
+// (buffer loads with the LDS destination), STAGES - 1 of them ahead, a barrier for one tile or two.  The 16-byte pieces of a row lie
 // in another order in every row (an exclusive or with the row's number, applied where the loads pick their source), which
 // spreads the reads of 16 rows over all banks without padding; the order of a lane's own reads is an exclusive or again.
-// Rows behind the request's last token arrive as zeros (the load's descriptor ends there).
+// Rows behind the request's last token arrive as zeros (the load's descriptor ends there).  With many rows it is bound by the matrix
+// cores and LDS reads, which take about as long: 3 trees of 64 nodes and 64 heads of 128 over 40 000-60 000 tokens 358 us, 887 TFLOP/s;
+// 16 trees of 25-61 nodes, 32 heads, 111 us (a third of the 256 rows is empty); with few by memory: 64 chains of 6 nodes over 512-8 192
+// tokens 207 us, 5.4 TB/s, and 8.7 us for one of 777 tokens.  A tile's scores beside the exponentials of the tile before it, a barrier per
+// two tiles and references that move seldom are what the former gained most by.
 template <int HD> static __device__ __forceinline__ int tree_swizzle(int row) { return HD == 64 ? (row >> 1) & 7 : row & 15; }
 template <int HD, int WAVES> constexpr int tree_stages() {
   constexpr int room = WAVES == 8 ? 131072 : 65536;   // LDS of a workgroup: one or two of them on a CU
