@@ -1229,9 +1229,10 @@ extern "C" int mi_paged_tree_attention(
   if ((uintptr_t)workspace & 15) return mi_fail(MI_ERR_ALIGN, "mi_paged_tree_attention: workspace must be 16-byte aligned");
 
   // Through LDS wherever that kernel has the cache's form (16 requests of 4 096 tokens, 8 KV heads of 128, us: 8 rows 68.7 -> 51.0,
-  // 32 rows 86.8 -> 55.1, 64 rows 90.9 -> 60.4; one of 800, 20 rows: 19.5 -> 14.3; 64 requests of 4 300, 24 rows: 200 and 204), but for a few
-  // rows of width 64, where its steps cost more than the loads (64 requests of 4 300: 6 rows 100 and 125; of 2 000: 12 rows 52.9 and 49.8).
-  const bool many = !fp8 && chunk_tokens % 32 == 0 && (head_dim == 128 || (head_dim == 64 && tree_mean_rows(T, R, G) >= 12));
+  // 32 rows 86.8 -> 55.1, 64 rows 90.9 -> 60.4; one of 800, 20 rows: 19.5 -> 14.3; 64 requests of 4 300, 24 rows: 200 and 204; of 2 000,
+  // 3 rows, 8 KV heads 105.8 -> 101.2, 32 of them 334 and 367), but for few rows of width 64, where its steps cost more than the loads
+  // (16 of 3 000 tokens, 12 rows, 32 KV heads: 73.9 and 95.9; 16 of 4 096, 16 rows, 8 heads: 36.4 and 36.2; 64 of 2 000, 21 rows: 24.8 and 17.4).
+  const bool many = !fp8 && chunk_tokens % 32 == 0 && (head_dim == 128 || (head_dim == 64 && tree_mean_rows(T, R, G) >= 16));
   const TreeShape shape = tree_shape(T, R, Hq, Hkv, head_dim, many);
   const bool f16 = dtype == MI_DTYPE_FP16;
   TreeParams p;
