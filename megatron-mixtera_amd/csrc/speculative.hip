@@ -17,7 +17,9 @@
 //
 // Tokens are whole numbers picked at borders of long sums, so exponentials and sums are 64-bit: one rounding of a 32-bit
 // cumulative sum (6e-8) is as wide as the whole share of many a token of a 128 k vocabulary.  The exponential is a table of
-// 2^(i/128) in LDS and a polynomial of degree 4 (relative error 1e-15); over whole rows a form of 6e-10 (add_exps).
+// 2^(i/128) in LDS and a polynomial of degree 4 (relative error 1e-15).  Where the rows' sums only scale what is compared (draft
+// probabilities: what a rejection leaves is a sum of its own) they take a form of 6e-10 (add_exps); where the rejected tokens are
+// taken off them a difference has to be as exact as its terms, and they take the 64-bit form.
 //
 // One launch for all rows (issue-bound), one workgroup per request for the walk, one launch for what a rejection leaves of the last
 // node's row, one workgroup per request for the draw: the last three are chains of dependent loads.  us, vocabulary 128 256, bf16:
@@ -259,7 +261,8 @@ static __device__ __forceinline__ void add_exps(const double* table, const float
 // largest of eight says whether any of them counts.  Bound by the rate at which vector instructions issue (some 27 a logit, 11 of
 // them for its exponential): 384 rows of 128 256 bf16 logits 35.5 us, 2.8 TB/s; 671 rows of which a cut leaves 50 logits each 33.2 us,
 // 5.2 TB/s.  With 64-bit exponentials the former took 47.5 us, and 52 with a running maximum per thread; without the looks at eights and
-// at single elements under a cut the latter took 45.6.
+// at single elements under a cut the latter took 45.6.  The 64-bit form is what a call without draft probabilities needs (64 chains of
+// 6, the whole call: 51.3 -> 62.2 us; under a cut, which leaves few exponentials, 30.7 and 30.4).
 constexpr int kVerifyLines = kVerifyPart / (8 * kVerifyThreads);
 template <int DT, bool GREEDY>
 __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParams p) {
@@ -301,6 +304,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
   if (lane == 0) tops[wave] = wave_top;
   __syncthreads();   // (the table, too)
   const float all = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const bool narrow = !GREEDY && __builtin_amdgcn_readfirstlane(p.draft && fabsf(all) < kNarrow);
   if constexpr (GREEDY) {
     int best = top == all ? place : 0x7fffffff;
 #pragma unroll
@@ -308,7 +312,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
     if (lane == 0) places[wave] = best;
   } else {
     double s0 = 0, s1 = 0;
-    const bool narrow = __builtin_amdgcn_readfirstlane(fabsf(all) < kNarrow), plain = !p.scaled && !p.cut;
+    const bool plain = !p.scaled && !p.cut, few = p.cut != nullptr;
     const float power = narrow ? rintf(all * (float)kLog2e) : 0.f;   // the narrow form's sums are relative to 2^power
     const int whole = 0x4b400000 + 128 * (int)power;
 #pragma unroll
@@ -326,13 +330,14 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
         for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
       }
       if (narrow) {
-        add_exps(table, v, all - 690.f, all, whole, p.cut != nullptr, s0, s1);
+        add_exps(table, v, all - 690.f, all, whole, few, s0, s1);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+          if (few && !__builtin_amdgcn_ballot_w64(v[j] > -INFINITY)) continue;
           double scale, y;
           table_exp_parts(table, (double)v[j] - (double)all, scale, y);
-          s0 = __builtin_fma(scale, y, s0);
+          s0 = v[j] > -INFINITY ? __builtin_fma(scale, y, s0) : s0;
         }
       }
     }
@@ -346,7 +351,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rows_kernel(VerifyParam
       o.index = min(min(places[0], places[1]), min(places[2], places[3]));
     } else {
       o.sum = sums[0] + sums[1] + sums[2] + sums[3];
-      if (fabsf(all) < kNarrow) o.sum *= table_exp(table, (double)rintf(all * (float)kLog2e) * 0.69314718055994530942 - (double)all);
+      if (narrow) o.sum *= table_exp(table, (double)rintf(all * (float)kLog2e) * 0.69314718055994530942 - (double)all);
     }
     p.partial[(int64_t)row * p.parts + part] = o;
   }
@@ -494,9 +499,8 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     if (i < n) p.removed[begin + i] = again ? -1 : tok;
 #pragma unroll 8
     for (int j = 1; j < most; ++j) before = __builtin_fma(prob[j], (parent[j] == up) & (j < i) ? 1.0 : 0.0, before);   // (a load a turn, no branch)
-    if (up >= 0) {
-      if ((double)chance * (1.0 - before) < prob[i]) atomicMin(&after[up], i);
-    }
+    // (what rounding takes below zero is nothing: no token is accepted on it)
+    if (up >= 0 && (double)chance * fmax(1.0 - before, 0.0) < prob[i]) atomicMin(&after[up], i);
     __syncthreads();
   }
   if (MODE != kDraft) {
@@ -579,7 +583,7 @@ template <int DT, int MODE>
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams p) {
   constexpr int kWaves = kDrawThreads / 64;
   __shared__ double table[128];
-  __shared__ double mass_s[kVerifyMostParts];
+  __shared__ unsigned long long gone_s[kVerifyMostParts];
   __shared__ double run[kWaves];
   __shared__ uint32_t gone[MODE == kTarget ? kVerifyPart / 32 : 1];
   __shared__ int found[2];
@@ -589,6 +593,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
   fill_exp_table(table);   // (the state is on its way)
   if (MODE == kTarget)
     for (int i = tid; i < kVerifyPart / 32; i += kDrawThreads) gone[i] = 0;
+  if (tid < kVerifyMostParts) gone_s[tid] = 0;
   if (tid == 0) {
     found[0] = 0x7fffffff;
     found[1] = -1;
@@ -614,17 +619,18 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
       if (p.parents[begin + i] == node && p.removed[begin + i] >= 0) f(p.removed[begin + i]);
   };
   if (MODE == kTarget && st.tested) {
-    if (tid < kVerifyMostParts) mass_s[tid] = whole;
+    // (in multiples of 2^-60, so that their order does not matter; below 1e-13 of a part's mass its own sum and theirs are
+    // rounding, and a part that lost everything must keep nothing)
+    removed([&](int tok) { atomicAdd(&gone_s[(tok + rd.shift) / p.part], (unsigned long long)(chance(rd.at(p, tok)) * 0x1p60 + 0.5)); });
     __syncthreads();
-    removed([&](int tok) { atomicAdd(&mass_s[(tok + rd.shift) / p.part], -chance(rd.at(p, tok))); });
-    __syncthreads();
-    mass = mass_s[lane];
+    const double kept = whole - (double)gone_s[lane] * 0x1p-60;
+    mass = gone_s[lane] && !(kept > whole * 1e-13) ? 0.0 : kept;
   }
   mass = fmax(mass, 0.0);
   double sums = wave_scan_f64(mass), total = read_lane_f64(sums, 63);
   // Rejections that leave nothing (a target equal to the draft's, or smaller everywhere that it is kept, up to rounding):
   // the last token comes from the target itself.
-  const bool nothing = !(total > 1e-13);
+  bool nothing = !(total > 1e-13);
   if (nothing) {
     mass = whole;
     sums = wave_scan_f64(mass);
@@ -633,62 +639,83 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
   const double want = (double)uniform * total;
   const uint64_t beyond = __builtin_amdgcn_ballot_w64(sums > want && mass > 0.0);
   const uint64_t some = __builtin_amdgcn_ballot_w64(mass > total * 1e-18);   // (the sum's own rounding: the last part that has any)
-  const int part = beyond ? __builtin_ctzll(beyond) : some ? 63 - __builtin_clzll(some) : 0;
-  const double rest = beyond ? want - read_lane_f64(sums - mass, part) : want;
-  const int first = part * p.part - rd.shift;
+  uint64_t alive = __builtin_amdgcn_ballot_w64(mass > 0.0);                  // parts that have not been looked through in vain
+  int part = beyond ? __builtin_ctzll(beyond) : some ? 63 - __builtin_clzll(some) : 0, token = 0;
+  double rest = beyond ? want - read_lane_f64(sums - mass, part) : want;
   const uint8_t* qr = MODE == kDraft ? p.draft + (int64_t)st.row * p.draft_stride : nullptr;
-  const bool minus = MODE == kDraft && st.tested && !nothing;
-  if (!nothing && MODE == kTarget) {
-    removed([&](int tok) {
-      const int i = tok - first;
-      if (i >= 0 && i < p.part) atomicOr(&gone[i >> 5], 1u << (i & 31));
-    });
-    __syncthreads();
-  }
-  double weight[8], mine = 0;
-  const int at = 8 * tid;
+  // Once, but for a part whose mass was rounding after all: then the next part's first token, or the last one before.  (All
+  // wavefronts hold the same masses and go the same way.)
+  for (;;) {
+    const int first = part * p.part - rd.shift;
+    const bool minus = MODE == kDraft && st.tested && !nothing;
+    if (MODE == kTarget && !nothing) {
+      removed([&](int tok) {
+        const int i = tok - first;
+        if (i >= 0 && i < p.part) atomicOr(&gone[i >> 5], 1u << (i & 31));
+      });
+      __syncthreads();
+    }
+    double weight[8], mine = 0;
+    const int at = 8 * tid;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) weight[j] = 0;
-  if (at < p.part) {
-    VerifyLine<DT> px;
-    VerifyAnyLine qx;
-    px.fetch(rd.row, first + at, p.V);
-    if (minus) qx.fetch(qr, p.draft_dtype, first + at, p.V);
-    float x[8], y[8];
-    px.values(rd.row, first + at, p.V, -INFINITY, x);
-    if (minus) qx.values(qr, p.draft_dtype, first + at, p.V, 0.f, y);
-    const uint32_t out = MODE == kTarget ? gone[at >> 5] >> (at & 31) : 0;
+    for (int j = 0; j < 8; ++j) weight[j] = 0;
+    if (at < p.part) {
+      VerifyLine<DT> px;
+      VerifyAnyLine qx;
+      px.fetch(rd.row, first + at, p.V);
+      if (minus) qx.fetch(qr, p.draft_dtype, first + at, p.V);
+      float x[8], y[8];
+      px.values(rd.row, first + at, p.V, -INFINITY, x);
+      if (minus) qx.values(qr, p.draft_dtype, first + at, p.V, 0.f, y);
+      const uint32_t out = MODE == kTarget ? gone[at >> 5] >> (at & 31) : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        double w = chance(rd.finish(p, x[j]));
+        if (minus) w = fmax(w - st.c * (double)y[j], 0.0);
+        if (MODE == kTarget && (out >> j & 1)) w = 0;
+        weight[j] = w;
+        mine += w;
+      }
+    }
+    const double upto = wave_scan_f64(mine);
+    if (lane == 63) run[wave] = upto;
+    __syncthreads();
+    double sum = upto - mine;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) sum += w < wave ? run[w] : 0.0;
+    int last = -1, place = 0x7fffffff;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      double w = chance(rd.finish(p, x[j]));
-      if (minus) w = fmax(w - st.c * (double)y[j], 0.0);
-      if (MODE == kTarget && (out >> j & 1)) w = 0;
-      weight[j] = w;
-      mine += w;
+      sum += weight[j];
+      if (weight[j] > 0) {
+        last = at + j;
+        if (sum > rest && place == 0x7fffffff) place = at + j;
+      }
+    }
+    if (place != 0x7fffffff) atomicMin(&found[0], place);
+    if (last >= 0) atomicMax(&found[1], last);
+    __syncthreads();
+    if (found[1] >= 0) {
+      token = first + (found[0] != 0x7fffffff ? found[0] : found[1]);
+      break;
+    }
+    alive &= ~((uint64_t)1 << part);
+    if (!alive && !nothing) {
+      nothing = true;
+      alive = __builtin_amdgcn_ballot_w64(whole > 0.0);
+      part = -1;
+    }
+    if (!alive) break;   // (no logit reaches the cut: token 0)
+    const uint64_t above = part < 0 ? alive : part < 63 ? alive >> (part + 1) << (part + 1) : 0;
+    rest = above ? -1.0 : INFINITY;
+    part = above ? __builtin_ctzll(above) : 63 - __builtin_clzll(alive);
+    // (nothing was found, by nobody: `found` is as it was)
+    if (MODE == kTarget) {
+      for (int i = tid; i < kVerifyPart / 32; i += kDrawThreads) gone[i] = 0;
+      __syncthreads();
     }
   }
-  const double upto = wave_scan_f64(mine);
-  if (lane == 63) run[wave] = upto;
-  __syncthreads();
-  double sum = upto - mine;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) sum += w < wave ? run[w] : 0.0;
-  int last = -1, place = 0x7fffffff;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    sum += weight[j];
-    if (weight[j] > 0) {
-      last = at + j;
-      if (sum > rest && place == 0x7fffffff) place = at + j;
-    }
-  }
-  if (place != 0x7fffffff) atomicMin(&found[0], place);
-  if (last >= 0) atomicMax(&found[1], last);
-  __syncthreads();
-  if (tid == 0) {
-    const int i = found[0] != 0x7fffffff ? found[0] : found[1];
-    p.out_tokens[(int64_t)r * p.max_path + count - 1] = min(max(first + i, 0), p.V - 1);
-  }
+  if (tid == 0) p.out_tokens[(int64_t)r * p.max_path + count - 1] = token;
 }
 
 // ------------------------------------------------------------------------------------------------ the cache afterwards

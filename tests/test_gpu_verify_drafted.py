@@ -252,3 +252,80 @@ def test_refusals(mi, dev):
             c.run(mi, **change)
     with pytest.raises(mi._lib.KernelError, match="temperature"):
         c.run(mi, temperature=0.0)
+
+
+JUST_UNDER_ONE = 1 - 2.0 ** -24
+
+
+def _kept_tokens(dev, V, kept, drafted, dtype, mode, mask, uniform, root):
+    """Requests of a root and children, ``kept[r]`` a request's {token: logit}, everything else left out of its rows by a cut (or
+    logits of -inf), ``drafted[r]`` its children's tokens."""
+    most = max(len(d) for d in drafted)
+    c = Case(dev, [1 + most] * len(kept), V, mode, dtype=dtype, shape="flat", seed=len(kept))
+    low = -math.inf if mask == "-inf" else -3.0
+    c.logits = torch.full(c.logits.shape, low, dtype=dtype)
+    c.tokens, c.cut = [], None if mask == "-inf" else torch.full((c.cu[-1],), -2.0)
+    for r, (tokens, children) in enumerate(zip(kept, drafted)):
+        for t, x in tokens.items():
+            c.logits[c.cu[r]:c.cu[r + 1], t] = x
+        c.tokens += [0] + children + [-1] * (most - len(children))
+    c.uniform = torch.full((c.cu[-1],), uniform)
+    c.uniform[c.cu[:-1]] = root
+    if mode == "draft":   # drawn by a draft that knows one of the tokens only
+        c.draft = torch.zeros(c.cu[-1], V)
+        for r, children in enumerate(drafted):
+            c.draft[c.cu[r]:c.cu[r + 1], children[0]] = 1.0
+    return c
+
+
+@pytest.mark.parametrize("mask", ["cut", "-inf"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_the_last_token_of_a_cut_is_accepted(mi, dev, dtype, mask):
+    """Two tokens are left, both drafted: the second has all that the first left, and every uniform number accepts it."""
+    rng = random.Random(1)
+    kept = [{700: 17.625, 9000: 10.375}] + [dict(zip(rng.sample(range(20000), 2), (10 + rng.uniform(0, 9), 10 + rng.uniform(0, 1)))) for _ in range(199)]
+    drafted = [sorted(k, key=k.get, reverse=True) for k in kept]
+    c = _kept_tokens(dev, 20000, kept, drafted, dtype, "target", mask, JUST_UNDER_ONE, JUST_UNDER_ONE)
+    tokens, rows, counts = c.check(mi)
+    assert (counts == 2).all()
+
+
+@pytest.mark.parametrize("mode", ["target", "draft"])
+@pytest.mark.parametrize("mask", ["cut", "-inf"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_a_part_without_a_token_is_not_drawn_from(mi, dev, dtype, mask, mode):
+    """A rejected token takes its part's whole mass with it, wherever the part lies: what rounding leaves of it is nothing, also
+    where the draw looks for the first token of all (a uniform number of zero), for the last one, or where little is left."""
+    rng = random.Random(2)
+    for root in (0.0, 2.0 ** -24, 1e-30, JUST_UNDER_ONE):
+        kept, drafted = [], []
+        for r in range(120):
+            a, b, c = rng.choice(((100, 17000, 19999), (19000, 10, 11), (9000, 3, 19500), (12000, 12001, 12002)))
+            kept.append({a: 15 + rng.uniform(0, 5), b: 10 + rng.uniform(0, 2), **({c: 10 + rng.uniform(0, 2)} if r % 2 else {})})
+            drafted.append([a])
+        c = _kept_tokens(dev, 20000, kept, drafted, dtype, mode, mask, JUST_UNDER_ONE, root)
+        tokens, rows, counts = c.check(mi)
+        assert all(int(t) in k for t, k in zip(tokens[:, 0], kept))
+
+
+@pytest.mark.parametrize("mode", ["target", "draft"])
+def test_rows_without_any_token(mi, dev, mode):
+    """A cut above every logit leaves nothing to accept and nothing to draw: token 0, whatever the uniform numbers."""
+    for root in (0.0, 0.5, JUST_UNDER_ONE):
+        c = _kept_tokens(dev, 20000, [{5: 3.0, 17000: 2.0}] * 3, [[5, 17000]] * 3, torch.bfloat16, mode, "cut", 0.3, root)
+        c.cut = torch.full((c.cu[-1],), 4.0)
+        tokens, rows, counts = c.run(mi)
+        assert counts.tolist() == [1, 1, 1] and tokens[:, 0].tolist() == [0, 0, 0]
+
+
+def test_nothing_left_twice_over(mi, dev):
+    """Tokens of probability zero after siblings that took everything: never accepted, and the draw stays among the kept ones."""
+    rng = random.Random(3)
+    kept = [dict(zip(rng.sample(range(500), 3), (10 + rng.uniform(0, 8) for _ in "abc"))) for _ in range(200)]
+    drafted = [sorted(k, key=k.get, reverse=True) + [next(t for t in range(500) if t not in k), -1, sorted(k)[0]] for k in kept]
+    for dtype in (torch.float32, torch.bfloat16):
+        c = _kept_tokens(dev, 500, kept, drafted, dtype, "target", "cut", JUST_UNDER_ONE, 0.5)
+        tokens, rows, counts = c.run(mi)
+        for r, k in enumerate(kept):
+            for i in range(int(counts[r])):
+                assert int(tokens[r, i]) in k, (r, tokens[r], k)
