@@ -64,6 +64,10 @@ struct TreeParams {
   float scale_log2;
 };
 
+// Probabilities of fp16 are multiplied by 2^10 (a row's largest one; the sums are divided by the sum of all, which has the factor too):
+// their normal numbers then reach down to e^-16 of the largest, where one of 1 at most would lose bits from 2^-14 on and be gone at 2^-25
+// -- what a long context far below one token adds up to.  bf16 has the exponents anyway.
+template <bool F16> constexpr float kTreeLift = F16 ? 10.f : 0.f;
 constexpr int kTreeRequestsPerLaunch = 2048;  // (their prefix sums lie in LDS)
 
 static __device__ __forceinline__ int tree_div_g(const TreeParams& p, int n) {
@@ -364,11 +368,12 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
       const float m_new = fmaxf(m_run[nt], rowgroup_max(tmax) * pm);
       const float alpha = fast_exp2(m_run[nt] - m_new);
       m_run[nt] = m_new;
+      const float neg = kTreeLift<F16> - m_new;
       f32x4_t sum = zero4;
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
-        const float p0 = fast_exp2(__builtin_fmaf(sc[nt][u][0], pm, -m_new)), p1 = fast_exp2(__builtin_fmaf(sc[nt][u][1], pm, -m_new));
-        const float p2 = fast_exp2(__builtin_fmaf(sc[nt][u][2], pm, -m_new)), p3 = fast_exp2(__builtin_fmaf(sc[nt][u][3], pm, -m_new));
+        const float p0 = fast_exp2(__builtin_fmaf(sc[nt][u][0], pm, neg)), p1 = fast_exp2(__builtin_fmaf(sc[nt][u][1], pm, neg));
+        const float p2 = fast_exp2(__builtin_fmaf(sc[nt][u][2], pm, neg)), p3 = fast_exp2(__builtin_fmaf(sc[nt][u][3], pm, neg));
         pf[nt][u] = make_uint2(pack2<F16>(p0, p1), pack2<F16>(p2, p3));
         sum = mfma_16x16x16<F16>(ones, pf[nt][u], sum);
       }
@@ -519,7 +524,7 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
 #pragma unroll
         for (int e = 0; e < DV; e += 2)
           *reinterpret_cast<float2*>(o + DV * i + e) = make_float2(acc[nt][e][i] * inv, acc[nt][e + 1][i] * inv);
-      if (g == 0) p.part_lse[row] = l == 0.f ? -INFINITY : m_run[nt] + fast_log2(l);
+      if (g == 0) p.part_lse[row] = l == 0.f ? -INFINITY : m_run[nt] - kTreeLift<F16> + fast_log2(l);
     }
   }
 }
@@ -634,10 +639,10 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
   };
 
   // Softmax: exponentials are taken against a reference per row, which moves only when a probability leaves a window: with
-  // bf16 the row's largest goes to 2^-30 when it moves, with fp16 to 2^-3, and 2 is the limit of both (the exponent's highest
-  // bit, looked at in the packed words: 5 instructions where the maximum of the scores takes 20).  Row sums come from the
-  // matrix cores.
-  constexpr float kHeadroom = F16 ? 3.f : 30.f, kNoReference = 3e38f;   // (none: any score leaves the window, -inf stays 0)
+  // bf16 the row's largest goes to 2^-30 when it moves, and 2 is the limit (the exponent's highest bit, looked at in the packed
+  // words: 5 instructions where the maximum of the scores takes 20); with fp16 to 2^10 (kTreeLift), and 2^15 is the limit (the
+  // largest of the packed words).  Row sums come from the matrix cores.
+  constexpr float kHeadroom = F16 ? -kTreeLift<F16> : 30.f, kNoReference = 3e38f;   // (none: any score leaves the window, -inf stays 0)
   float neg[NQ];   // a probability is 2^(score * scale + neg)
   f32x4_t acc[NQ][DV], sum[NQ];
 #pragma unroll
@@ -682,8 +687,18 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
     }
   };
   auto leaves_window = [&](const uint4 (&P)[NQ]) {
-    const uint32_t any = (P[0].x | P[0].y | P[0].z | P[0].w) | (P[1].x | P[1].y | P[1].z | P[1].w);
-    return __builtin_amdgcn_ballot_w64((any & 0x40004000u) != 0) != 0;
+    if constexpr (F16) {
+      uint32_t t;
+      asm("v_pk_maximum3_f16 %0, %1, %2, %3" : "=v"(t) : "v"(P[0].x), "v"(P[0].y), "v"(P[0].z));
+      asm("v_pk_maximum3_f16 %0, %0, %1, %2" : "+v"(t) : "v"(P[0].w), "v"(P[1].x));
+      asm("v_pk_maximum3_f16 %0, %0, %1, %2" : "+v"(t) : "v"(P[1].y), "v"(P[1].z));
+      asm("v_pk_maximum3_f16 %0, %0, %1, %1" : "+v"(t) : "v"(P[1].w));
+      asm("v_pk_add_u16 %0, %0, %1" : "+v"(t) : "v"(0x08000800u));   // (0x7800, 2^15, becomes the sign; infinity and NaN too)
+      return __builtin_amdgcn_ballot_w64((t & 0x80008000u) != 0) != 0;
+    } else {
+      const uint32_t any = (P[0].x | P[0].y | P[0].z | P[0].w) | (P[1].x | P[1].y | P[1].z | P[1].w);
+      return __builtin_amdgcn_ballot_w64((any & 0x40004000u) != 0) != 0;
+    }
   };
   auto move_reference = [&](const f32x4_t (&S)[NQ][2], uint4 (&P)[NQ]) {
 #pragma unroll

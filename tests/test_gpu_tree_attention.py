@@ -347,3 +347,45 @@ def test_refusals(mi, dev):
         call(k=k[:, :24], v=v[:, :24])
     with pytest.raises(ValueError, match="go together"):
         mi.ops.paged_tree_attention(q, k, v, i32([0, 5]), i32([25]), table, mask, k_scales=torch.ones(c.N, 2, device=dev))
+
+
+def _sink(c, gap, seed):
+    """One key of every request ``gap`` above all others, which score alike; its values are zero, the others' near one."""
+    gen = torch.Generator().manual_seed(seed)
+    c.q.zero_()
+    c.q[..., 0] = 1
+    c.k, c.v = torch.zeros_like(c.k), (0.5 + torch.rand(c.v.shape, generator=gen)).to(c.v.dtype)
+    for r, length in enumerate(c.lens):
+        chunk, at = osp.position(c.table[r].tolist(), c.k.size(1), c.N, 3 if r % 2 else length // 2)
+        c.k[chunk, at, :, 0] = gap / c.scale
+        c.v[chunk, at] = 0
+    return c
+
+
+@pytest.mark.parametrize("gap", [6.0, 12.0, 13.5, 15.0, 16.0])
+@pytest.mark.parametrize("d,chunk,nodes", [(128, 64, [2, 1]), (128, 48, [2, 1]), (64, 64, [9, 7]), (64, 16, [2, 1]), (96, 64, [2, 1]), (256, 64, [2, 1]),
+                                           (128, 64, [40, 3])])
+def test_a_token_far_above_a_long_context(mi, dev, gap, d, chunk, nodes):
+    """fp16 probabilities of a long context far below one token keep their eleven bits: the row's largest one is at 2^10 at
+    least, so that e^-16 of it (2^-23.1) is above the type's smallest normal number, 2^-14.  The bound is the others'."""
+    _sink(Case(dev, nodes, [30011, 9000], Hq=4, Hkv=2, d=d, chunk=chunk, dtype=FP16, seed=25), gap, 25).check(mi)
+
+
+@pytest.mark.parametrize("d,chunk", [(64, 16), (128, 64)])
+def test_a_token_far_above_others_of_its_span(mi, dev, d, chunk):
+    """The same where one wavefront takes a request's whole context (many KV heads), so that no partial leaves the token out."""
+    _sink(Case(dev, [1, 1, 1, 1], [1500, 1000, 700, 1400], Hq=256, Hkv=256, d=d, chunk=chunk, dtype=FP16, seed=27), 16.0, 27).check(mi)
+
+
+def test_scores_that_grow_by_every_amount(mi, dev):
+    """fp16: a row's largest score grows tile by tile, by less and by more than the window of its probabilities."""
+    for growth in (0.4, 3.0, 7.5, 11.0, 30.0):
+        for chunk, nodes in ((64, [4, 2]), (48, [4, 2]), (64, [40, 9])):
+            c = Case(dev, nodes, [700, 333], Hq=8, Hkv=2, dtype=FP16, chunk=chunk, seed=26)
+            c.q.zero_()
+            c.q[..., 0] = 1
+            for r in range(2):
+                for k in range(c.lens[r]):
+                    at = osp.position(c.table[r].tolist(), chunk, c.N, k)
+                    c.k[at[0], at[1], :, 0] = growth * (k // 32) / c.scale if k % 5 else 0
+            c.check(mi)
