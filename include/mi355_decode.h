@@ -804,8 +804,8 @@ int mi_verify_drafted_tokens(const void* logits, int64_t stride_row, int32_t log
  * context, rows[r][i] (a row of the step, as out_rows; entry 0 is the root) to position kv_lens[r] - n_r + i for
  * 1 <= i < counts[r], in `layers` layers that lie kv_stride_layer apart; new_kv_lens[r] = kv_lens[r] - n_r + counts[r].
  * Paths rise.  Elements of 2 bytes are copied; an fp8 cache (1 byte, scales [layers][n_chunks][Hkv], layers
- * scale_stride_layer apart) is copied inside a chunk and converted to the other scale (rounded to nearest, saturating)
- * between chunks.  v_cache may be NULL (a cache with one tensor, e.g. MLA latents).  Entries that are no node of their
+ * scale_stride_layer apart) is copied inside a chunk and converted to the other scale (rounded to nearest, saturating;
+ * what is no number stays none) between chunks.  v_cache may be NULL (a cache with one tensor, e.g. MLA latents).  Entries that are no node of their
  * request, and places outside the block table or the cache, move nothing.
  */
 int mi_kv_keep_accepted(void* k_cache, void* v_cache, int64_t kv_stride_layer, int64_t kv_stride_chunk,

@@ -782,14 +782,17 @@ __global__ __launch_bounds__(256) void kv_keep_kernel(KeepParams p) {
           if (i0 + j >= m || src_chunk[i0 + j] < 0) continue;
           const int a = src_chunk[i0 + j], b = dst_chunk[i0 + j];
           uint4 y = x[j];
-          if (FP8 && a != b) {   // another chunk, another scale: e4m3 of value * scale / scale, saturating
+          if (FP8 && a != b) {   // another chunk, another scale: e4m3 of value * scale / scale, saturating; NaN stays NaN
             const float f = scale[(int64_t)a * p.Hkv + head] / scale[(int64_t)b * p.Hkv + head];
+            auto moved = [&](float x, uint32_t code) {
+              const float v = x * f;
+              return v == v ? f32_to_e4m3_sat(v) : (code & 0x80u) | 0x7fu;
+            };
             uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const f32x2_t lo = fp8x2_lo_to_f32(w[k]), hi = fp8x2_hi_to_f32(w[k]);
-              w[k] = f32_to_e4m3_sat(lo.x * f) | f32_to_e4m3_sat(lo.y * f) << 8 | f32_to_e4m3_sat(hi.x * f) << 16 |
-                     f32_to_e4m3_sat(hi.y * f) << 24;
+              w[k] = moved(lo.x, w[k]) | moved(lo.y, w[k] >> 8) << 8 | moved(hi.x, w[k] >> 16) << 16 | moved(hi.y, w[k] >> 24) << 24;
             }
             y = make_uint4(w[0], w[1], w[2], w[3]);
           }

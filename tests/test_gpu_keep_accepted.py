@@ -137,3 +137,37 @@ def test_refusals(mi, dev):
                          (dict(k=k[0, 0], v=v[0, 0]), "caches must be"), (dict(k=k[..., :32], v=v[..., :32]), "contiguous")):
         with pytest.raises(ValueError, match=word):
             call(**change)
+
+
+@pytest.mark.parametrize("code", [0x7f, 0xff])
+def test_nan_stays_nan(mi, dev, code):
+    """A NaN of an fp8 cache is one wherever its row goes; the values beside it are converted as ever."""
+    c = Case(dev, [9, 1, 30, 0, 5], [20, 0, 100, 7, 31], H=2, d=64, chunk=16, fp8=True, seed=40)
+    for x in (c.k, c.v):
+        x.view(torch.uint8)[:, :, :, 0, ::5] = code
+        x.view(torch.uint8)[:, :, ::3, 1, 7] = code
+    k, v = c.k.view(torch.uint8).to(dev), c.v.view(torch.uint8).to(dev)
+    mi.ops.kv_keep_accepted(k, v, *c.rest(), k_scales=c.scales[0].to(dev), v_scales=c.scales[1].to(dev))
+    torch.cuda.synchronize()
+    for got, cache, s in ((k, c.k, 0), (v, c.v, 1)):
+        want = osp.keep_accepted(cache.float(), c.rows, c.counts, c.cu, c.lens, c.table, c.scales[s])
+        got = got.cpu().view(torch.float8_e4m3fn).float()
+        assert want.isnan().any() and torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(0), want.nan_to_num(0))
+
+
+def test_scales_that_make_no_number(mi, dev):
+    """Scales of zero, infinity and NaN on either side: the quotient's rules, value by value (0 * inf and NaN are NaN)."""
+    c = Case(dev, [9, 1, 30, 0, 5], [20, 0, 100, 7, 31], H=2, d=64, chunk=16, fp8=True, seed=41)
+    for x in (c.k, c.v):
+        x.view(torch.uint8)[..., ::9] = 0
+    for s in c.scales:
+        s[:, 0::5], s[:, 1::7], s[:, 2::9] = 0, float("inf"), float("nan")
+    k, v = c.k.view(torch.uint8).to(dev), c.v.view(torch.uint8).to(dev)
+    mi.ops.kv_keep_accepted(k, v, *c.rest(), k_scales=c.scales[0].to(dev), v_scales=c.scales[1].to(dev))
+    torch.cuda.synchronize()
+    for got, cache, s in ((k, c.k, 0), (v, c.v, 1)):
+        want = osp.keep_accepted(cache.float(), c.rows, c.counts, c.cu, c.lens, c.table, c.scales[s])
+        got = got.cpu().view(torch.float8_e4m3fn).float()
+        assert want.isnan().any() and torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(0), want.nan_to_num(0))
