@@ -52,7 +52,7 @@ struct TreeParams {
   int64_t o_st, o_sh;
   float* part_o;         // [2 grid][Hkv][rows][HD]
   float* part_lse;       // [2 grid][Hkv][rows]
-  int4* pair_info;       // per (request, group): first and last workgroup, request, group
+  int4* pair_info;       // per (request, group), two of them: first and last workgroup, group, first row of q; nodes
   int32_t* pairs;        // how many there are
   const float* k_scale;
   const float* v_scale;
@@ -529,17 +529,25 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
   }
 }
 
-// What one request brings: rows of q, nodes, cached tokens.  Whatever the arrays hold, rows stay inside q and tokens
+// What one request brings: rows of q, nodes, cached tokens.  Whatever the arrays hold, rows stay inside q, no row belongs to two
+// requests of a launch (cu_seqlens_q counts as its own running maximum: the number of groups has a place for each) and tokens stay
 // inside the block table.
 struct TreeRequest {
   int q_begin, nodes, len;
 };
-static __device__ __forceinline__ TreeRequest tree_request(const TreeParams& p, int i) {
-  TreeRequest t;
-  t.q_begin = min(max(p.cu_q[i], 0), p.T);
-  t.nodes = min(max(p.cu_q[i + 1], t.q_begin), p.T) - t.q_begin;
-  t.len = (int)min((int64_t)max(p.lens[i], 0), (int64_t)p.table_cols * p.chunk);
-  return t;
+static __device__ __forceinline__ int tree_row(const TreeParams& p, int i) { return min(max(p.cu_q[i], 0), p.T); }
+static __device__ __forceinline__ int tree_len(const TreeParams& p, int i) {
+  return (int)min((int64_t)max(p.lens[i], 0), (int64_t)p.table_cols * p.chunk);
+}
+// Maximum of this lane's number and those of the lanes before it (none is negative).
+static __device__ __forceinline__ int tree_scan_max(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+  return v;
 }
 
 // ------------------------------------------------------------------------------------------------ tiles through LDS
@@ -906,7 +914,7 @@ static __device__ __forceinline__ void tree_rows_segment(const TreeParams& p, co
 
 // The span of this workgroup along the tiles of all (request, group) pairs, as segments one after the other: seg(segment);
 // every wavefront walks the same ones.  Up to 64 requests lie in the lanes of every wavefront (no LDS, no barrier), more in
-// dynamic LDS: tiles and groups of requests 0 .. i.  (The entry point has made sure that all tiles together are an int.)
+// dynamic LDS: tiles and groups of requests 0 .. i, and where the rows of request i end.  (The entry point has made sure that all tiles together are an int.)
 // Clears the rows behind the last request on the way.
 constexpr int kTreeStart = 1;   // what a pair's start counts, in tiles
 template <int HD, int TK, typename Seg>
@@ -914,16 +922,23 @@ static __device__ __forceinline__ void tree_walk(const TreeParams& p, Seg seg) {
   extern __shared__ int32_t tree_lds[];
   int32_t* const cum = tree_lds;
   int32_t* const first = cum + p.R;
+  int32_t* const row_end = first + p.R;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool in_lanes = p.R <= 64;
 
   TreeRequest mine{0, 0, 0};   // of request `lane` (in lanes)
   int cum_l = 0, first_l = 0;
-  auto scan64 = [&](int base) {
+  auto scan64 = [&](int base, int before) {   // `before`: where the rows of the requests before `base` end
     const int i = base + lane;
-    int n_groups = 0, n_tiles = 0;
+    int n_groups = 0, n_tiles = 0, from = 0, to = 0;
     if (i < p.R) {
-      mine = tree_request(p, i);
+      from = tree_row(p, i);
+      to = tree_row(p, i + 1);
+      mine.len = tree_len(p, i);
+    }
+    mine.q_begin = max(before, tree_scan_max(from));
+    mine.nodes = max(mine.q_begin, tree_scan_max(to)) - mine.q_begin;
+    if (i < p.R) {
       n_groups = (int)(((int64_t)mine.nodes * p.G + p.rows - 1) / p.rows);
       n_tiles = max((mine.len + TK - 1) / TK, 1);   // (a request without tokens has a tile in which nothing is seen)
     }
@@ -931,16 +946,18 @@ static __device__ __forceinline__ void tree_walk(const TreeParams& p, Seg seg) {
     first_l = wave_scan(n_groups);
   };
   if (in_lanes) {
-    scan64(0);
+    scan64(0, 0);
   } else {
     if (wave == 0) {
-      int tiles = 0, groups = 0;
+      int tiles = 0, groups = 0, rows = 0;
       for (int base = 0; base < p.R; base += 64) {
-        scan64(base);
+        scan64(base, rows);
         if (base + lane < p.R) {
           cum[base + lane] = tiles + cum_l;
           first[base + lane] = groups + first_l;
+          row_end[base + lane] = mine.q_begin + mine.nodes;
         }
+        rows = __builtin_amdgcn_readlane(mine.q_begin + mine.nodes, 63);
         tiles += __builtin_amdgcn_readlane(cum_l, 63);
         groups += __builtin_amdgcn_readlane(first_l, 63);
       }
@@ -950,7 +967,10 @@ static __device__ __forceinline__ void tree_walk(const TreeParams& p, Seg seg) {
   auto cum_at = [&](int i) { return in_lanes ? __builtin_amdgcn_readlane(cum_l, i) : __builtin_amdgcn_readfirstlane(cum[i]); };
   auto first_at = [&](int i) { return in_lanes ? __builtin_amdgcn_readlane(first_l, i) : __builtin_amdgcn_readfirstlane(first[i]); };
   auto request_at = [&](int i) {
-    if (!in_lanes) return tree_request(p, i);
+    if (!in_lanes) {
+      const int begin = __builtin_amdgcn_readfirstlane(i ? row_end[i - 1] : tree_row(p, 0));
+      return TreeRequest{begin, __builtin_amdgcn_readfirstlane(row_end[i]) - begin, tree_len(p, i)};
+    }
     return TreeRequest{__builtin_amdgcn_readlane(mine.q_begin, i), __builtin_amdgcn_readlane(mine.nodes, i), __builtin_amdgcn_readlane(mine.len, i)};
   };
   const int total = cum_at(p.R - 1), pairs = first_at(p.R - 1);
@@ -1020,11 +1040,12 @@ static __device__ __forceinline__ void tree_walk(const TreeParams& p, Seg seg) {
       // (read across the lanes while all of them are on: inside the branch a value that was put aside comes back for lane 0 only)
       const int pair = (r ? first_at(r - 1) : 0) + s.group;
       if (wave == 0 && lane == 0 && blockIdx.y == 0) {
-        int4* info = p.pair_info + pair;
+        int4* info = p.pair_info + 2 * (int64_t)pair;
         if (begins) {
           info->x = blockIdx.x;
-          info->z = r;
-          info->w = s.group;
+          info->z = s.group;
+          info->w = s.q_begin;
+          info[1].x = s.nodes;
         }
         if (ends) info->y = blockIdx.x;
       }
@@ -1042,7 +1063,7 @@ __global__ __launch_bounds__(512, 2) void paged_tree_kernel(TreeParams p) {
   if constexpr (SHARE) {
     // (the wavefronts' pieces of LDS: behind the walk's)
     extern __shared__ int32_t tree_lds[];
-    float* const joins = reinterpret_cast<float*>(tree_lds + (p.R <= 64 ? 0 : 2 * p.R));
+    float* const joins = reinterpret_cast<float*>(tree_lds + (p.R <= 64 ? 0 : 3 * p.R));
     tree_walk<HD, 16 * NT>(p, [&](TreeSegment& s) {
       // parts of this group, and how many wavefronts each has
       const int rows = min(s.nodes * p.G - s.group * p.rows, p.rows);
@@ -1081,15 +1102,15 @@ __global__ __launch_bounds__(1024) void paged_tree_merge_kernel(TreeParams p, in
   __shared__ float red[6][1024];
   const int pair = blockIdx.x, h = blockIdx.y;
   if (pair >= *p.pairs) return;
-  const int4 info = p.pair_info[pair];
+  const int4 info = p.pair_info[2 * pair];
+  const int nodes = p.pair_info[2 * pair + 1].x;
   if (info.x == info.y) return;   // written by the streaming kernel
-  const TreeRequest t = tree_request(p, info.z);
   const int cols = head_dim >> 2, block_rows = kTreeMergeThreads / cols, set = cols * block_rows;
   const int grp = threadIdx.x / set, in = threadIdx.x - grp * set;
   const int row = blockIdx.z * block_rows + in / cols, d = 4 * (in % cols);
-  const int n = info.w * p.rows + row, qi = tree_div_g(p, n);
-  if (tree_div_g(p, info.w * p.rows + blockIdx.z * block_rows) >= t.nodes) return;   // (uniform)
-  const bool live = grp < groups && row < p.rows && qi < t.nodes;
+  const int n = info.z * p.rows + row, qi = tree_div_g(p, n);
+  if (tree_div_g(p, info.z * p.rows + blockIdx.z * block_rows) >= nodes) return;   // (uniform)
+  const bool live = grp < groups && row < p.rows && qi < nodes;
   float mx = -INFINITY, den = 0.f;
   float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float lse, float weight, float4 v) {   // `weight` partials' worth of `v`, relative to 2^lse
@@ -1127,7 +1148,7 @@ __global__ __launch_bounds__(1024) void paged_tree_merge_kernel(TreeParams p, in
   }
   if (!live) return;
   const float inv = den == 0.f ? 0.f : 1.f / den;
-  uint16_t* o = p.out + (int64_t)(t.q_begin + qi) * p.o_st + (int64_t)(h * p.G + n - qi * p.G) * p.o_sh + d;
+  uint16_t* o = p.out + (int64_t)(info.w + qi) * p.o_st + (int64_t)(h * p.G + n - qi * p.G) * p.o_sh + d;
   st8(o, make_uint2(pack2<F16>(num.x * inv, num.y * inv), pack2<F16>(num.z * inv, num.w * inv)));
 }
 
@@ -1184,7 +1205,7 @@ using namespace mi;
 
 static int64_t tree_workspace(const TreeShape& s, int T, int R, int G, int Hkv, int head_dim) {
   const int64_t rows = (int64_t)2 * s.grid * Hkv * s.rows;
-  return 256 + tree_align(16 * tree_most_pairs(T, R, G, s.rows)) + tree_align(rows * 4) + rows * head_dim * 4;
+  return 256 + tree_align(32 * tree_most_pairs(T, R, G, s.rows)) + tree_align(rows * 4) + rows * head_dim * 4;
 }
 extern "C" int64_t mi_tree_workspace_bytes(int32_t T, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim) {
   if (T <= 0 || R <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0) return 0;
@@ -1261,7 +1282,7 @@ extern "C" int mi_paged_tree_attention(
   const int64_t rows = (int64_t)2 * shape.grid * Hkv * shape.rows;
   p.pairs = (int32_t*)ws;
   p.pair_info = (int4*)(ws + 256);
-  ws += 256 + tree_align(16 * tree_most_pairs(T, R, G, shape.rows));
+  ws += 256 + tree_align(32 * tree_most_pairs(T, R, G, shape.rows));
   p.part_lse = (float*)ws;
   p.part_o = (float*)(ws + tree_align(rows * 4));
   p.k_scale = k_scales; p.v_scale = v_scales;
@@ -1284,7 +1305,7 @@ extern "C" int mi_paged_tree_attention(
     p.cu_q = cu_seqlens_q + r0; p.lens = kv_lens + r0;
     p.last_slice = r0 + p.R == R;
     // (the walk's arrays; where parts share, what the wavefronts of a part join: 64 lanes' registers each)
-    const size_t walk = p.R <= 64 ? 0 : (size_t)p.R * 2 * sizeof(int32_t);
+    const size_t walk = p.R <= 64 ? 0 : (size_t)p.R * 3 * sizeof(int32_t);
     const size_t lds = walk + (!many && shape.share > 1 ? (size_t)shape.waves * 64 * (shape.rows / shape.share / 16) * (head_dim / 4 + 2) * sizeof(float) : 0);
 #define MI_TREE_ONE(HD_, NT_, NQ_, FP8_, F16_, SHARE_)                                                                 \
     do {                                                                                                               \

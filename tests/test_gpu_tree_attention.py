@@ -389,3 +389,21 @@ def test_scores_that_grow_by_every_amount(mi, dev):
                     at = osp.position(c.table[r].tolist(), chunk, c.N, k)
                     c.k[at[0], at[1], :, 0] = growth * (k // 32) / c.scale if k % 5 else 0
             c.check(mi)
+
+
+@pytest.mark.parametrize("requests", [9, 100])
+@pytest.mark.parametrize("Hq,Hkv,d,chunk", [(8, 2, 128, 64), (64, 1, 128, 64), (4, 2, 64, 16), (16, 2, 96, 48)])
+def test_rows_that_fall(mi, dev, requests, Hq, Hkv, d, chunk):
+    """Where cu_seqlens_q falls its running maximum counts: no row belongs to two requests, and the workspace, which has a place for
+    every group of rows, is written inside its own bytes."""
+    c = Case(dev, [7, 120, 0, 1] + [0] * (requests - 4), [40, 200, 3, 5] + [60] * (requests - 4), Hq=Hq, Hkv=Hkv, d=d, chunk=chunk, seed=28)
+    legit, rows = c.cu, c.cu[-1]
+    falling = [0, 7, 127, -5, 128] + [(0, rows, 3, rows + 9, -1)[i % 5] for i in range(5, requests + 1)]
+    need = mi._lib.load().mi_tree_workspace_bytes(rows, requests, Hq, Hkv, d)
+    work = torch.full((need + 8192,), 0x5a, dtype=torch.uint8, device=dev)
+    c.cu = falling
+    with mi.ops.use_workspace(work[:need]):
+        got = c.run(mi)
+    c.cu = legit
+    c.check(mi, got=got)
+    assert (work[need:] == 0x5a).all()
