@@ -407,3 +407,37 @@ def test_rows_that_fall(mi, dev, requests, Hq, Hkv, d, chunk):
     c.cu = legit
     c.check(mi, got=got)
     assert (work[need:] == 0x5a).all()
+
+
+@pytest.mark.parametrize("requests", [65, 300, 2100])
+@pytest.mark.parametrize("Hq,Hkv,d,chunk,fp8", [
+    (8, 2, 128, 64, False), (64, 1, 128, 64, False),      # tiles through LDS: four wavefronts, eight
+    (8, 1, 64, 64, False), (64, 1, 64, 32, False),        # the same of width 64
+    (64, 1, 128, 48, False), (24, 1, 128, 48, False),     # through registers, eight and two or four parts sharing tokens
+    (32, 4, 256, 64, False), (64, 1, 64, 64, True), (16, 8, 128, 64, True),
+])
+def test_more_requests_than_lanes(mi, dev, requests, Hq, Hkv, d, chunk, fp8):
+    """Ragged batches, empty requests among them, whose sums lie in LDS beside the tiles or what wavefronts join: every row against
+    the causal call (two bounds apart at values of at most five), some requests against the oracle."""
+    rng = random.Random(requests)
+    nodes = [rng.choice((0, 1, 2, 3, 4, 5)) for _ in range(requests)]
+    nodes[rng.randrange(requests)], nodes[-1] = 40, 3
+    c = Case(dev, nodes, [rng.randint(0, 70) for _ in nodes], Hq=Hq, Hkv=Hkv, d=d, chunk=chunk, fp8=fp8, shape="chain", spare=3, seed=requests)
+    got = c.run(mi)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    scales = dict(k_scales=c.scales[0].to(dev), v_scales=c.scales[1].to(dev)) if fp8 else {}
+    k, v = ((x.view(torch.uint8) if fp8 else x).to(dev) for x in (c.k, c.v))
+    if not fp8 or chunk % 64 == 0:
+        other = mi.ops.paged_prefill_attention(c.q.to(dev), k, v, i32(c.cu), i32(c.lens), c.table.to(dev), **scales)
+        assert (got.float() - other.float()).abs().max() < 2 * 3 * 2.0 ** -8 * 5.5
+    torch.cuda.synchronize()
+    assert (got[c.cu[-1]:] == 0).all()
+    picks = sorted({0, 1, 63, 64, requests - 1, requests // 2, min(2047, requests - 1), min(2048, requests - 1), nodes.index(40)})
+    some = Case.__new__(Case)
+    some.__dict__.update(c.__dict__)
+    some.cu, rows = [0], []
+    for r in picks:
+        rows += range(c.cu[r], c.cu[r + 1])
+        some.cu.append(len(rows))
+    some.q, some.bits, some.lens, some.table = c.q[rows], [c.bits[i] for i in rows], [c.lens[r] for r in picks], c.table[picks]
+    some.check(mi, got=got[rows])
