@@ -1247,7 +1247,9 @@ extern "C" int mi_paged_tree_attention(
     return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: chunk size must be a positive multiple of 16");
   if (n_chunks <= 0 || table_columns <= 0 || (int64_t)table_columns * chunk_tokens > 0x7fffff00)
     return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: need a cache, and a block table of fewer than 2^31 tokens a row");
-  if ((int64_t)table_columns * chunk_tokens * chunk_tokens >= (int64_t)1 << 40)   // (the reciprocal that finds a chunk)
+  if (table_columns >= 1 << 24)   // (the 64-bit product with the reciprocal that finds a chunk)
+    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: a block table has fewer than 2^24 columns");
+  if ((int64_t)table_columns * chunk_tokens * chunk_tokens >= (int64_t)1 << 40)   // (the reciprocal's own rounding)
     return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: tokens a row times chunk size must stay below 2^40");
   if (mask_words < 1 || mask_words > 4 || mask_stride < mask_words)
     return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: a row of the mask has 1 to 4 words");

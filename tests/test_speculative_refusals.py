@@ -103,3 +103,12 @@ def test_trees_that_are_none(mi):
         mi.ops.tree_masks(range(-1, 256))
     assert mi.ops.tree_masks([]).shape == (0, 1)
     assert isinstance(ctypes.c_int64(int(mi.ops.tree_masks(range(-1, 255))[255, 3])).value, int)
+
+
+@pytest.mark.parametrize("cols,chunk", [(1 << 25, 16), ((1 << 24) + 1, 64), ((1 << 24) + 5, 32)])
+def test_tables_of_too_many_columns(mi, cols, chunk):
+    """A token's chunk is its number times 2^40 / chunk in 64 bits, which hold fewer than 2^24 chunks: from there on it would be
+    another one, and reads would go astray."""
+    assert cols * chunk <= 0x7fffff00 and cols * chunk * chunk < 1 << 40
+    assert (cols * chunk - 1) * -(-(1 << 40) // chunk) >= 1 << 64
+    _error(mi, _tree(mi, cols=cols, chunk=chunk), "2^24")
