@@ -760,9 +760,9 @@ int mi_attention_out_linear_proj(const void* core_attn_out, int64_t x_stride_tok
  * whose bits are set in its row of `tree_mask`: bit j % 64 of word j / 64 is node j (`mask_words` 1 to 4 words a row,
  * `mask_stride` apart; its own bit included; nodes past the words are seen by none).  Rows that see nothing, and the rows
  * of q behind the last request, are zeros.  Caches as for mi_paged_prefill_attention, 16-bit or fp8 (`kv_dtype`; fp8:
- * head_dim 64 or 128, scales [n_chunks][Hkv]), chunks of any multiple of 16 tokens, fewer than 2^24 columns; lengths
- * beyond the table's columns are cut to them, and table entries that name no chunk of the cache (`n_chunks`) hold tokens
- * that no row sees.  Where cu_seqlens_q falls its running maximum counts: a request has the rows that none before it has.
+ * head_dim 64 or 128, scales [n_chunks][Hkv]), chunks of any multiple of 16 tokens, fewer than 2^24 columns of at most
+ * 2^31 - 4096 tokens together; lengths beyond the table's columns are cut to them, and table entries that name no chunk of
+ * the cache (`n_chunks`) hold tokens that no row sees.  Where cu_seqlens_q falls its running maximum counts: a request has the rows that none before it has.
  */
 int64_t mi_tree_workspace_bytes(int32_t T, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim);
 int mi_paged_tree_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,

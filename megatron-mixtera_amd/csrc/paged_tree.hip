@@ -1245,8 +1245,9 @@ extern "C" int mi_paged_tree_attention(
   if (fp8 && (!k_scales || !v_scales)) return mi_fail(MI_ERR_NULL, "mi_paged_tree_attention: an fp8 cache needs both scale arrays");
   if (chunk_tokens <= 0 || chunk_tokens % 16)
     return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: chunk size must be a positive multiple of 16");
-  if (n_chunks <= 0 || table_columns <= 0 || (int64_t)table_columns * chunk_tokens > 0x7fffff00)
-    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: need a cache, and a block table of fewer than 2^31 tokens a row");
+  // (a tile's number has 32 bits, also that of the one a wavefront asks for behind the last: up to 512 tokens on)
+  if (n_chunks <= 0 || table_columns <= 0 || (int64_t)table_columns * chunk_tokens > 0x7ffff000)
+    return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: need a cache, and a block table of at most 2^31 - 4096 tokens a row");
   if (table_columns >= 1 << 24)   // (the 64-bit product with the reciprocal that finds a chunk)
     return mi_fail(MI_ERR_SHAPE, "mi_paged_tree_attention: a block table has fewer than 2^24 columns");
   if ((int64_t)table_columns * chunk_tokens * chunk_tokens >= (int64_t)1 << 40)   // (the reciprocal's own rounding)

@@ -112,3 +112,10 @@ def test_tables_of_too_many_columns(mi, cols, chunk):
     assert cols * chunk <= 0x7fffff00 and cols * chunk * chunk < 1 << 40
     assert (cols * chunk - 1) * -(-(1 << 40) // chunk) >= 1 << 64
     _error(mi, _tree(mi, cols=cols, chunk=chunk), "2^24")
+
+
+@pytest.mark.parametrize("cols,chunk", [((1 << 23) - 1, 256), (8947847, 240)])
+def test_tables_of_almost_two_to_the_31_tokens(mi, cols, chunk):
+    """A wavefront's next tile lies up to 512 tokens on (every eighth of 64), and its number has 32 bits behind the last token too."""
+    assert cols < 1 << 24 and cols * chunk < 1 << 31 <= cols * chunk + 512
+    _error(mi, _tree(mi, cols=cols, chunk=chunk), "2^31")
