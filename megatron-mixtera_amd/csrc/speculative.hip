@@ -479,7 +479,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   }
   __syncthreads();
   if (MODE == kGreedy) {
-    if (up >= 0 && drafted == token[up]) atomicMin(&after[up], tid);
+    if (up >= 0 && inside && drafted == token[up]) atomicMin(&after[up], tid);   // (a row of NaN has no place: 2^31 - 1)
   } else if (tid < n) {
     token[tid] = inside ? (int)drafted : -1;
     prob[tid] = up >= 0 && inside && sum_s[up] > 0 ? table_exp(table, (double)said - (double)top_s[up]) / sum_s[up] : 0.0;

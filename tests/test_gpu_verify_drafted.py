@@ -329,3 +329,13 @@ def test_nothing_left_twice_over(mi, dev):
         for r, k in enumerate(kept):
             for i in range(int(counts[r])):
                 assert int(tokens[r, i]) in k, (r, tokens[r], k)
+
+
+def test_greedy_rows_of_nan(mi, dev):
+    """A row without a number has no largest logit: no token is accepted after it, whichever is drafted, and token 0 follows."""
+    c = Case(dev, [4, 3], 300, "greedy", shape="flat", seed=14)
+    c.logits[:4] = math.nan
+    c.tokens[1:4] = [0, (1 << 31) - 1, 299]
+    tokens, rows, counts = c.run(mi)
+    assert counts[0] == 1 and tokens[0].tolist() == [0, -1] and rows[0].tolist() == [0, -1]
+    assert tokens[1, 0] == c.logits[4].argmax()
