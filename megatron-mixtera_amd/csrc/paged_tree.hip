@@ -359,7 +359,9 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
     // ---- running maximum and sum (row m16; only the maximum crosses lanes, the sums come from the matrix cores)
     const float pm = FP8 ? 1.f : mul;
     uint2 pf[NQ][NT];
-    const float unit_new = FP8 && page ? (vsc == 0.f ? 1e-30f : vsc) : unit;
+    // (values of a chunk whose scale is zero weigh nothing; the unit stays, since no sum fits one that small)
+    const bool weigh = !FP8 || !(fabsf(vsc) < 1e-30f);
+    const float unit_new = FP8 && page && weigh ? vsc : unit;
 #pragma unroll
     for (int nt = 0; nt < NQ; ++nt) {
       float tmax = -INFINITY;
@@ -376,6 +378,7 @@ static __device__ __forceinline__ void tree_segment(const TreeParams& p, const T
         const float p2 = fast_exp2(__builtin_fmaf(sc[nt][u][2], pm, neg)), p3 = fast_exp2(__builtin_fmaf(sc[nt][u][3], pm, neg));
         pf[nt][u] = make_uint2(pack2<F16>(p0, p1), pack2<F16>(p2, p3));
         sum = mfma_16x16x16<F16>(ones, pf[nt][u], sum);
+        if (FP8 && !weigh) pf[nt][u] = make_uint2(0, 0);
       }
       l_run[nt] = l_run[nt] * alpha + sum[0];
       const float scale = FP8 ? alpha * (unit / unit_new) : alpha;

@@ -441,3 +441,27 @@ def test_more_requests_than_lanes(mi, dev, requests, Hq, Hkv, d, chunk, fp8):
         some.cu.append(len(rows))
     some.q, some.bits, some.lens, some.table = c.q[rows], [c.bits[i] for i in rows], [c.lens[r] for r in picks], c.table[picks]
     some.check(mi, got=got[rows])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_a_value_scale_of_zero_behind_large_sums(mi, dev, dtype):
+    """Every token the same score, values at e4m3's end with scales of one, then chunks with a scale of zero (and one with a scale after
+    them): the sums of a whole context in one wavefront change to that unit and back without leaving fp32."""
+    c = Case(dev, [1, 1], [5000, 3333], Hq=256, Hkv=256, d=64, chunk=64, dtype=dtype, fp8=True, seed=29)
+    c.k = torch.zeros(c.k.shape).to(torch.float8_e4m3fn)
+    c.v = torch.full(c.v.shape, 448.0).to(torch.float8_e4m3fn)
+    for s in c.scales:
+        s.fill_(1.0)
+    for r in range(2):
+        n = c.lens[r] // 64
+        c.scales[1][c.table[r, n - 3:n - 1].long()] = 0
+    c.check(mi)
+
+
+def test_value_scales_that_are_no_number(mi, dev):
+    """A NaN among the scales reaches the rows that see its chunk, and no others; a key scale's the same."""
+    for which in (0, 1):
+        c = Case(dev, [6, 5], [200, 150], chunk=64, fp8=True, dtype=FP16, seed=30)
+        c.scales[which][c.table[0, 1].long(), 1] = math.nan
+        got = c.check(mi)
+        assert got[:6, 4:].isnan().all() and torch.isfinite(got[:6, :4]).all() and torch.isfinite(got[6:]).all()
