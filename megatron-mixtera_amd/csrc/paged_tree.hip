@@ -1271,10 +1271,17 @@ extern "C" int mi_paged_tree_attention(
   if ((uintptr_t)workspace & 15) return mi_fail(MI_ERR_ALIGN, "mi_paged_tree_attention: workspace must be 16-byte aligned");
 
   // Through LDS wherever that kernel has the cache's form (16 requests of 4 096 tokens, 8 KV heads of 128, us: 8 rows 68.7 -> 51.0,
-  // 32 rows 86.8 -> 55.1, 64 rows 90.9 -> 60.4; one of 800, 20 rows: 19.5 -> 14.3; 64 requests of 4 300, 24 rows: 200 and 204; of 2 000,
-  // 3 rows, 8 KV heads 105.8 -> 101.2, 32 of them 334 and 367), but for few rows of width 64, where its steps cost more than the loads
-  // (16 of 3 000 tokens, 12 rows, 32 KV heads: 73.9 and 95.9; 16 of 4 096, 16 rows, 8 heads: 36.4 and 36.2; 64 of 2 000, 21 rows: 24.8 and 17.4).
-  const bool many = !fp8 && chunk_tokens % 32 == 0 && (head_dim == 128 || (head_dim == 64 && tree_mean_rows(T, R, G) >= 16));
+  // 32 rows 86.8 -> 55.1, 64 rows 90.9 -> 60.4; one of 800, 20 rows: 19.5 -> 14.3), but for
+  // - few rows of width 64, where its steps cost more than the loads (16 of 3 000 tokens, 12 rows, 32 KV heads: 73.9 and 95.9;
+  //   16 of 4 096, 16 rows, 8 heads: 36.4 and 36.2; 64 of 2 000, 21 rows: 24.8 and 17.4);
+  // - few rows of width 128 in a call that fills the memory, as far as the host knows (not the lengths): eight heads of a token then
+  //   lie beside one another in a workgroup of the register kernel.  Registers and LDS, us: 64 requests of 2 000 tokens, 32 heads, 3 rows
+  //   313 and 364, 12 rows 314 and 371; 128 of 1 000, 8 heads, 12 rows 97 and 106; 16 of 4 096, 16 heads, 3 rows 92 and 106; in short
+  //   contexts the other way about (128 of 300, 8 heads, 12 rows 43.6 and 41.6).  With more rows to fewer heads LDS: 64 of 2 000,
+  //   8 heads, 12 rows 103.0 and 100.5, 24 rows 119 and 101; 4 heads, 3 rows 52.3 and 49.1.
+  const int64_t mean = tree_mean_rows(T, R, G);
+  const bool flood = head_dim == 128 && Hkv % 8 == 0 && 80 * mean <= (int64_t)R * Hkv;
+  const bool many = !fp8 && chunk_tokens % 32 == 0 && ((head_dim == 128 && !flood) || (head_dim == 64 && mean >= 16));
   const TreeShape shape = tree_shape(T, R, Hq, Hkv, head_dim, many);
   const bool f16 = dtype == MI_DTYPE_FP16;
   TreeParams p;
