@@ -43,11 +43,11 @@ struct VerifyPartial {   // of one part of a row
   int32_t index;         // greedy: the first place of the maximum
 };
 struct VerifyState {     // what the walk hands the draw
-  double c;              // weights are (p - c q)+
+  double c;              // weights are (p - c q)+; 0: no child of the last node was rejected, q is not read
   double sum;            // the last node's row: sum of exp(x - top)
   float top;
   int32_t row;           // -1: the request is empty
-  int32_t tested;        // whether its children were tried
+  int32_t tested;        // whether its children were tried (a path of max_path nodes: no)
   int32_t pad;
 };
 
@@ -532,7 +532,6 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   double c = 0;
   if (tid == 0) rows[0] = begin;
   while (count < p.max_path) {
-    c = 0;
     double left = 1;
     int child = after[at] < n ? after[at] : -1;
     while (child >= 0) {
@@ -547,6 +546,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     }
     if (child < 0) break;
     at = child;
+    c = 0;
     if (tid == 0) {
       out[count - 1] = token[at];
       rows[count] = begin + at;
@@ -555,7 +555,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   }
   if (tid == 0) {
     p.out_counts[r] = count;
-    p.state[r] = VerifyState{c, sum_s[at], top_s[at], begin + at, count < p.max_path, 0};
+    p.state[r] = VerifyState{c, sum_s[at], top_s[at], begin + at, count < p.max_path, 0};   // (c is 0 where max_path ended it)
   }
 }
 
@@ -568,7 +568,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_left_kernel(VerifyParam
   const VerifyState st = p.state[r];
   fill_exp_table(table);   // (the state is on its way)
   __syncthreads();
-  if (st.row < 0 || !st.tested) return;
+  if (st.row < 0 || st.c == 0) return;   // (nothing was rejected: the row of a node without children may hold anything)
   const VerifyRow<DT> rd(p, st.row);
   const double s = block_sum(left_over(p, rd, table, st.row, part * p.part, p.part, kVerifyThreads, st.top, st.sum, st.c), scratch);
   if (threadIdx.x == 0) p.residual[(int64_t)r * p.parts + part] = s;
@@ -611,7 +611,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
     if (q.max > -INFINITY) whole = q.sum * chance(q.max);
   }
   double mass = whole;
-  if (MODE == kDraft && st.tested) mass = lane < p.parts ? p.residual[(int64_t)r * p.parts + lane] : 0.0;
+  if (MODE == kDraft && st.c != 0) mass = lane < p.parts ? p.residual[(int64_t)r * p.parts + lane] : 0.0;
   // tokens that the rejected children took out: each once
   auto removed = [&](auto f) {
     if (MODE != kTarget || !st.tested) return;
@@ -647,7 +647,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
   // wavefronts hold the same masses and go the same way.)
   for (;;) {
     const int first = part * p.part - rd.shift;
-    const bool minus = MODE == kDraft && st.tested && !nothing;
+    const bool minus = MODE == kDraft && st.c != 0 && !nothing;
     if (MODE == kTarget && !nothing) {
       removed([&](int tok) {
         const int i = tok - first;

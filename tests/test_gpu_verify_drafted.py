@@ -339,3 +339,22 @@ def test_greedy_rows_of_nan(mi, dev):
     tokens, rows, counts = c.run(mi)
     assert counts[0] == 1 and tokens[0].tolist() == [0, -1] and rows[0].tolist() == [0, -1]
     assert tokens[1, 0] == c.logits[4].argmax()
+
+
+@pytest.mark.parametrize("draft_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,near", [("chain", 0.1), ("tree", 0.6), ("flat", 3.0)])
+def test_draft_rows_of_nodes_without_children_are_not_read(mi, dev, shape, near, draft_dtype):
+    """What the children of a node were drawn from exists where it has some: the other rows, the ends of accepted paths among them,
+    may hold anything."""
+    ends = 0
+    for seed in range(6):
+        c = Case(dev, [5, 9, 1, 3], 20011, "draft", shape=shape, near=near, seed=seed, draft_dtype=draft_dtype)
+        leaves = [i for r in range(4) for i in range(c.cu[r], c.cu[r + 1]) if not any(p == i - c.cu[r] for p in c.parents[c.cu[r]:c.cu[r + 1]])]
+        want = c.reference()
+        for value in (math.nan, math.inf, 1e30):
+            draft = c.draft.clone()
+            draft[leaves, ::2] = value
+            got = c.run(mi, draft_probs=draft.to(dev))
+            assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want)), value
+        ends += sum(int(want[1][r, int(want[2][r]) - 1]) in leaves for r in range(4))
+    assert ends >= 6
