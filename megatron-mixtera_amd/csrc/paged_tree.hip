@@ -555,15 +555,17 @@ static __device__ __forceinline__ int tree_scan_max(int v) {
 
 // ------------------------------------------------------------------------------------------------ tiles through LDS
 // For 16-bit caches of widths 64 and 128.  Where a request has many rows per KV head the products are the work, and a CU's cache too
-// slow a feed; where it has few, tiles that wait in LDS keep more bytes on their way than registers do.  A workgroup of
-// WAVES wavefronts takes 32 * WAVES rows of one (request, KV head), and tiles of 32 tokens go straight from memory into LDS
-// (buffer loads with the LDS destination), STAGES - 1 of them ahead, a barrier for one tile or two.  The 16-byte pieces of a row lie
+// slow a feed; where it has few, calls that do not fill the memory are faster through LDS too (figures at the entry point's rule).  A
+// workgroup of WAVES wavefronts takes 32 * WAVES rows of one (request, KV head), and tiles of 32 tokens go straight from memory into
+// LDS (buffer loads with the LDS destination).  With eight stages a barrier serves two tiles, and up to six are ahead of the one at work,
+// four of them on their way behind a barrier; with four (width 128, four wavefronts) a barrier serves one, two are ahead and one is on
+// its way, 32 KB a CU where the register kernel has 64: in calls that fill the memory that one is faster.  The 16-byte pieces of a row lie
 // in another order in every row (an exclusive or with the row's number, applied where the loads pick their source), which
 // spreads the reads of 16 rows over all banks without padding; the order of a lane's own reads is an exclusive or again.
 // Rows behind the request's last token arrive as zeros (the load's descriptor ends there).  With many rows it is bound by the matrix
 // cores and LDS reads, which take about as long: 3 trees of 64 nodes and 64 heads of 128 over 40 000-60 000 tokens 358 us, 887 TFLOP/s;
 // 16 trees of 25-61 nodes, 32 heads, 111 us (a third of the 256 rows is empty); with few by memory: 64 chains of 6 nodes over 512-8 192
-// tokens 207 us, 5.4 TB/s, and 8.7 us for one of 777 tokens.  A tile's scores beside the exponentials of the tile before it, a barrier per
+// tokens 211 us, 5.3 TB/s, and 8.7 us for one of 777 tokens.  A tile's scores beside the exponentials of the tile before it, a barrier per
 // two tiles and references that move seldom are what the former gained most by.
 template <int HD> static __device__ __forceinline__ int tree_swizzle(int row) { return HD == 64 ? (row >> 1) & 7 : row & 15; }
 template <int HD, int WAVES> constexpr int tree_stages() {
