@@ -1280,9 +1280,10 @@ extern "C" int mi_paged_tree_attention(
   //   lie beside one another in a workgroup of the register kernel.  Registers and LDS, us: 64 requests of 2 000 tokens, 32 heads, 3 rows
   //   313 and 364, 12 rows 314 and 371; 128 of 1 000, 8 heads, 12 rows 97 and 106; 16 of 4 096, 16 heads, 3 rows 92 and 106; in short
   //   contexts the other way about (128 of 300, 8 heads, 12 rows 43.6 and 41.6).  With more rows to fewer heads LDS: 64 of 2 000,
-  //   8 heads, 12 rows 103.0 and 100.5, 24 rows 119 and 101; 4 heads, 3 rows 52.3 and 49.1.
+  //   8 heads, 12 rows 103.0 and 100.5, 24 rows 119 and 101; 4 heads, 3 rows 52.3 and 49.1.  Level at 3 rows and fewer from some 256
+  //   requests times heads on (16 of 1 000, 16 heads 30.7 and 31.9; 8 of them 22.7 and 23.0, 4 with 24 heads over 4 096 44.0 and 40.1).
   const int64_t mean = tree_mean_rows(T, R, G);
-  const bool flood = head_dim == 128 && Hkv % 8 == 0 && 80 * mean <= (int64_t)R * Hkv;
+  const bool flood = head_dim == 128 && Hkv % 8 == 0 && 80 * (mean > 3 ? mean : 3) <= (int64_t)R * Hkv;
   const bool many = !fp8 && chunk_tokens % 32 == 0 && ((head_dim == 128 && !flood) || (head_dim == 64 && mean >= 16));
   const TreeShape shape = tree_shape(T, R, Hq, Hkv, head_dim, many);
   const bool f16 = dtype == MI_DTYPE_FP16;
