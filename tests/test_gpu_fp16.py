@@ -282,3 +282,25 @@ def test_fp16_logits_sampling_and_log_probs(mi, dev):
     torch.cuda.synchronize()
     ref = torch.log_softmax(logits.double(), -1)[torch.arange(R), ids]
     assert (lp.cpu().double() - ref).abs().max().item() <= 2e-5
+
+
+@pytest.mark.parametrize("R,V", [(40, 5003), (3, 40000), (200, 1024), (7, 129)])
+@pytest.mark.parametrize("temperature", [0.3, 0.6, 0.48, 1.2, 0.7])
+def test_fp16_logits_are_scaled_in_two_roundings(mi, dev, R, V, temperature):
+    """Logits times the temperature's reciprocal, an fp32 number that is then rounded to fp16 (as the reference's division of an fp16
+    tensor is evaluated): the smallest kept value is exactly the k-th of those.  The draw is held between the cumulated probabilities of
+    the kept values up to 1e-5: a mass is 32-bit (2^-22 of itself from the exponential, 2^-32 of the row's largest from its
+    fixed point, which 40 000 of them bring to 9.3e-6)."""
+    gen = torch.Generator().manual_seed(R + V)
+    logits = (torch.randn(R, V, generator=gen) * 3).to(F16)
+    u = torch.rand(R, generator=gen)
+    x = osm.scaled_logits(logits, temperature)
+    for top_k, top_p in ((2, 0.0), (7, 0.0), (50, 0.0), (0, 0.0), (0, 0.7)):
+        got, _, cut = mi.ops.sample_from_logits(logits.to(dev), top_k=top_k, top_p=top_p, temperature=temperature, uniform=u.to(dev), return_cut=True)
+        got, cut = got.cpu(), cut.cpu()
+        if top_k:
+            assert torch.equal(cut, x.topk(top_k, 1)[0][:, -1])
+        p = osm.kept_probabilities(x, x >= cut[:, None])
+        hi = p.cumsum(1).gather(1, got[:, None])[:, 0]
+        assert (p.gather(1, got[:, None]) > 0).all()
+        assert (hi + 1e-5 >= u).all() and (hi - p.gather(1, got[:, None])[:, 0] - 1e-5 <= u).all()

@@ -358,3 +358,19 @@ def test_draft_rows_of_nodes_without_children_are_not_read(mi, dev, shape, near,
             assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want)), value
         ends += sum(int(want[1][r, int(want[2][r]) - 1]) in leaves for r in range(4))
     assert ends >= 6
+
+
+@pytest.mark.parametrize("temperature", [0.3, 0.6, 0.48, 1.2])
+@pytest.mark.parametrize("mode", ["draft", "target"])
+def test_fp16_logits_over_a_temperature(mi, dev, mode, temperature):
+    """Temperatures whose reciprocal brings many fp16 numbers next to the middle between two others: logits are multiplied in 32 bits,
+    then rounded, by the sampler that makes the cut as by what is held against it."""
+    for seed in range(8):
+        for top_k in (1, 2, 5):
+            Case(dev, [12, 7, 20, 1, 1, 1], 700, mode, dtype=torch.float16, temperature=temperature, top_k=top_k, seed=seed).check(mi)
+    c = Case(dev, [12, 7, 20, 1, 1, 1], 700, mode, dtype=torch.float16, temperature=temperature, seed=9)
+    for top_k in (2, 3, 9):
+        cut = mi.ops.sample_from_logits(c.logits.to(dev), top_k=top_k, temperature=temperature, uniform=c.uniform.to(dev), return_cut=True)[2]
+        c.cut = osp.scaled_logits(c.logits, temperature).topk(top_k, 1)[0][:, -1].contiguous()
+        assert torch.equal(cut.cpu(), c.cut)
+        c.check(mi)
