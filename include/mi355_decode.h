@@ -786,7 +786,7 @@ int mi_paged_tree_attention(const void* q, int64_t q_stride_tok, int64_t q_strid
  *   draft_probs NULL  accepted where uniform[i] * (mass left) < p(token); a rejected token leaves the distribution;
  *   else              row i of draft_probs is the distribution q that the children of node i were drawn from: accepted where
  *                     uniform[i] * q(token) < p(token), a rejection turns p into (p - q)+, normalised.  Rows of nodes
- *                     without children are not read.
+ *                     without children may hold anything.
  * The first accepted child is the next node.  The request's last token is drawn from what is left at the last node, by the
  * inverse CDF in vocabulary order at uniform[root] (where nothing is left: from p); greedy: the largest logit's index.
  * A path has at most max_path nodes; the children of its last one are then not tried.

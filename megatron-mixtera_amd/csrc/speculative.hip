@@ -373,9 +373,9 @@ static __device__ __forceinline__ double block_sum(double x, double* scratch) {
   return s;
 }
 
-// This thread's share of the sum of (p - c q)+ over the places [0, places) from `first` on of a row.  (Two or four lines ahead
-// of their use took more registers and as much time.)
-template <int DT>
+// This thread's share of the sum of (p - c q)+ over the places [0, places) from `first` on of a row; MINUS false: c is 0, q is not read.
+// (Two or four lines ahead of their use took more registers and as much time.)
+template <int DT, bool MINUS>
 static __device__ __forceinline__ double left_over(const VerifyParams& p, const VerifyRow<DT>& rd, const double* table, int row,
                                                    int first, int places, int threads, float top, double sum, double c) {
   const uint8_t* qr = p.draft + (int64_t)row * p.draft_stride;
@@ -386,10 +386,10 @@ static __device__ __forceinline__ double left_over(const VerifyParams& p, const 
     VerifyLine<DT> px;
     VerifyAnyLine qx;
     px.fetch(rd.row, e0, p.V);
-    qx.fetch(qr, p.draft_dtype, e0, p.V);
-    float x[8], y[8];
+    if (MINUS) qx.fetch(qr, p.draft_dtype, e0, p.V);
+    float x[8], y[8] = {};
     px.values(rd.row, e0, p.V, -INFINITY, x);
-    qx.values(qr, p.draft_dtype, e0, p.V, 0.f, y);
+    if (MINUS) qx.values(qr, p.draft_dtype, e0, p.V, 0.f, y);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float v = rd.finish(p, x[j]);
@@ -548,7 +548,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
       child = sibling[child];
       if (child >= 0) {   // (what is left matters to a sibling; the draw makes its own sum)
         const VerifyRow<DT> rd(p, begin + at);
-        left = block_sum(left_over(p, rd, table, begin + at, 0, p.V + rd.shift, kWalkThreads, top_s[at], sum_s[at], c), scratch);
+        left = block_sum(left_over<DT, true>(p, rd, table, begin + at, 0, p.V + rd.shift, kWalkThreads, top_s[at], sum_s[at], c), scratch);
       }
     }
     if (child < 0) break;
@@ -566,7 +566,8 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   }
 }
 
-// Draft probabilities: what is left of one part of the last node's distribution, sum (p - c q)+.
+// Draft probabilities: what is left of one part of the last node's distribution, sum (p - c q)+.  Where nothing was rejected that is
+// the part's own sum, which the draw's weights need with their own 64 bits: the rows' sums are good to 6e-10 here.
 template <int DT>
 __global__ __launch_bounds__(kVerifyThreads) void verify_left_kernel(VerifyParams p) {
   __shared__ double table[128];
@@ -575,9 +576,13 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_left_kernel(VerifyParam
   const VerifyState st = p.state[r];
   fill_exp_table(table);   // (the state is on its way)
   __syncthreads();
-  if (st.row < 0 || st.c == 0) return;   // (nothing was rejected: the row of a node without children may hold anything)
+  if (st.row < 0) return;
   const VerifyRow<DT> rd(p, st.row);
-  const double s = block_sum(left_over(p, rd, table, st.row, part * p.part, p.part, kVerifyThreads, st.top, st.sum, st.c), scratch);
+  const int first = part * p.part;
+  double mine;   // (the row of a node without children may hold anything)
+  if (st.c != 0) mine = left_over<DT, true>(p, rd, table, st.row, first, p.part, kVerifyThreads, st.top, st.sum, st.c);
+  else mine = left_over<DT, false>(p, rd, table, st.row, first, p.part, kVerifyThreads, st.top, st.sum, 0.0);
+  const double s = block_sum(mine, scratch);
   if (threadIdx.x == 0) p.residual[(int64_t)r * p.parts + part] = s;
 }
 
@@ -618,7 +623,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
     if (q.max > -INFINITY) whole = q.sum * chance(q.max);
   }
   double mass = whole;
-  if (MODE == kDraft && st.c != 0) mass = lane < p.parts ? p.residual[(int64_t)r * p.parts + lane] : 0.0;
+  if (MODE == kDraft) mass = lane < p.parts ? p.residual[(int64_t)r * p.parts + lane] : 0.0;
   // tokens that the rejected children took out: each once
   auto removed = [&](auto f) {
     if (MODE != kTarget || !st.tested) return;

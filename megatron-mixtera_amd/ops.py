@@ -651,7 +651,7 @@ def verify_drafted_tokens(logits: Tensor, tokens: Tensor, parents: Tensor, cu_se
     ``logits`` ``[T, V]`` (fp32, bf16 or fp16): what the target says after each node; ``tokens`` int64 ``[T]`` the nodes'
     tokens, ``parents`` int32 ``[T]`` their parents inside the request (-1: the root).  ``draft_probs`` ``[T, V]`` (fp32,
     bf16 or fp16): row i is the distribution that the children of node i were drawn from (rows of nodes without
-    children are not read); without it the drafted tokens count as chosen.  ``uniform`` fp32 ``[T]``: a root's number draws its request's last token, any other node's decides
+    children may hold anything); without it the drafted tokens count as chosen.  ``uniform`` fp32 ``[T]``: a root's number draws its request's last token, any other node's decides
     about it.  ``temperature`` and ``cut`` (``[T]``, as ``sample_from_logits(..., return_cut=True)`` returns it) make the
     target's distribution.  A path has at most ``max_path`` nodes, the root included; of a request's nodes the first 1 024
     are looked at.

@@ -374,3 +374,26 @@ def test_fp16_logits_over_a_temperature(mi, dev, mode, temperature):
         c.cut = osp.scaled_logits(c.logits, temperature).topk(top_k, 1)[0][:, -1].contiguous()
         assert torch.equal(cut.cpu(), c.cut)
         c.check(mi)
+
+
+@pytest.mark.parametrize("children", [0, 2])
+@pytest.mark.parametrize("mode", ["draft", "target"])
+def test_draws_next_to_a_border(mi, dev, mode, children):
+    """Two tokens whose border lies within 1e-10 of the uniform number, but not within 5e-12: the sums that a draw walks along are
+    64-bit wherever they come from, also where nothing was rejected, or nothing tried (paths of one node)."""
+    gen, rng, found = torch.Generator().manual_seed(15), random.Random(15), []
+    while len(found) < 200:
+        a, b = (3 * torch.rand(2, 4096, generator=gen)).float()
+        p = torch.sigmoid(a.double() - b.double())
+        grid = (p * 2 ** 24).round()
+        gap = (p - grid / 2 ** 24).abs()
+        for i in ((gap > 5e-12) & (gap < 1e-10)).nonzero()[:, 0].tolist():
+            found.append((float(a[i]), float(b[i]), float(grid[i] / 2 ** 24)))
+    found = found[:200]
+    c = Case(dev, [1 + children] * 200, 20000, mode, shape="flat", seed=15, max_path=1)
+    c.logits.fill_(-math.inf)
+    for r, (a, b, u) in enumerate(found):
+        i, j = rng.choice(((3, 9), (3, 15000), (9000, 19999)))
+        c.logits[c.cu[r]:c.cu[r + 1], i], c.logits[c.cu[r]:c.cu[r + 1], j] = a, b
+        c.uniform[c.cu[r]] = u
+    c.check(mi)
