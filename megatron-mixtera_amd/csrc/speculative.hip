@@ -23,9 +23,9 @@
 //
 // One launch for all rows (issue-bound), one workgroup per request for the walk, one launch for what a rejection leaves of the last
 // node's row, one workgroup per request for the draw: the last three are chains of dependent loads.  us, vocabulary 128 256, bf16:
-// 5 nodes, draft probabilities 4.3 + 4.7 + 3.8 + 7.7; 64 chains of 6: 34.8 + 6.8 + 12.9 + 12.7, without draft probabilities 49.1 + 5.1 +
+// 5 nodes, draft probabilities 4.3 + 4.6 + 3.8 + 8.0; 64 chains of 6: 35.0 + 6.7 + 13.5 + 13.3, without draft probabilities 49.1 + 5.1 +
 // 13.0 (the draw); 671 nodes in 16 trees under a cut, no draft probabilities 32.6 + 9.6 + 7.2; 716 nodes in 16 trees, draft
-// probabilities 59.9 + 301 + 7.5 + 12.2 (the walk sums a row for every rejected child that has a further sibling, on one CU); greedy
+// probabilities 61.1 + 299 + 7.7 + 12.6 (the walk sums a row for every rejected child that has a further sibling, on one CU); greedy
 // over 270 rows of 32 003 fp32 logits 9.2 + 4.1.
 #include <type_traits>
 
@@ -264,7 +264,7 @@ static __device__ __forceinline__ void add_exps(const double* table, const float
 // Maximum and sum of exponentials (greedy: maximum and its first place) of one part of one row, which the threads hold in
 // registers: all loads are on their way before the first value is used.  Scaling and cut keep the order of logits, so that the
 // largest of eight says whether any of them counts.  Bound by the rate at which vector instructions issue (some 27 a logit, 11 of
-// them for its exponential): 384 rows of 128 256 bf16 logits 34.8 us, 2.8 TB/s; 671 rows of which a cut leaves 50 logits each 32.6 us,
+// them for its exponential): 384 rows of 128 256 bf16 logits 35.0 us, 2.8 TB/s; 671 rows of which a cut leaves 50 logits each 32.6 us,
 // 5.3 TB/s.  With 64-bit exponentials the former took 47.5 us, and 52 with a running maximum per thread; without the looks at eights and
 // at single elements under a cut the latter took 45.6.  The 64-bit form is what a call without draft probabilities needs (64 chains of
 // 6, the whole call: 51.3 -> 62.2 us, their rows 49.1; under a cut, which leaves few exponentials, 30.7 and 30.4).
@@ -404,8 +404,8 @@ static __device__ __forceinline__ double left_over(const VerifyParams& p, const 
 
 // The walk of one request's tree, one workgroup each.  A chain of dependent steps: parents and tokens, the logits that they name
 // (beside the partial sums of all the request's rows), then LDS only, but for draft probabilities after a rejection: what is left of
-// the row, some 30 us for each over 128 256 tokens.  4.7 us for 5 nodes, 9.6 for 16 trees of 25-61 nodes without draft probabilities,
-// 301 with them.
+// the row, by the one workgroup, for each that has a further sibling.  4.6 us for 5 nodes, 9.6 for 16 trees of 25-61 nodes without
+// draft probabilities, 299 with them.
 constexpr int kWalkThreads = 1024;
 enum { kGreedy = 0, kTarget = 1, kDraft = 2 };
 template <int DT, int MODE>
@@ -587,7 +587,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_left_kernel(VerifyParam
 }
 
 // The draw of a request's last token: the part that holds it (every wavefront, a part to a lane), then the place inside the
-// part, whose weights the threads hold.  Three trips to memory one after the other and two scans; 7.7 us for one request, 12.7 for 64
+// part, whose weights the threads hold.  Three trips to memory one after the other and two scans; 8.0 us for one request, 13.3 for 64
 // (with the parts' sums in one thread and the weights in LDS 24.6 and 24.8).
 constexpr int kDrawThreads = 1024;
 static_assert(kVerifyPart == 8 * kDrawThreads, "eight places to a thread");
