@@ -397,6 +397,41 @@ int mi_paged_prefill_attention_tiles(const void* q, int64_t q_stride_tok, int64_
                                      int32_t dtype, const MiTuning* tuning, void* stream);
 
 /*
+ * The same two attentions where a token sees part of what lies before it: a row at position P sees key k <= P where
+ * k > P - window (the last `window` tokens, itself included) or k < sinks (the request's first tokens).  window >= 1,
+ * sinks >= 0, of any size.  Rows that see nothing (no keys) are zeros, and so are rows behind the last request of a
+ * varlen call.  What a row does not see does not reach it, whatever the cache holds there, NaN included.
+ *
+ * `n_chunks`: chunks of the cache; `bt_columns`: of the block table (fewer than 2^31 - 512 tokens and 2^24 columns).
+ * Chunks without a token in sight of the call's rows are not needed: their table entries may hold anything.  Entries that
+ * are used are kept inside the cache, lengths inside the table.  kv_dtype, scales and everything else as in
+ * mi_paged_decode_attention (workspace: mi_decode_workspace_bytes) and mi_paged_prefill_attention / _fp8 / _tiles
+ * (workspace: mi_window_prefill_workspace_bytes with the call's own T, max_kv_len, window and sinks; `one_row_requests`
+ * 0: no request has exactly one row, nothing is launched for such).  The tuning knob prefill_two_phase takes 3 or -1.
+ */
+int mi_paged_window_decode_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                                     const void* v_cache, int64_t kv_stride_chunk, int64_t kv_stride_tok,
+                                     int64_t kv_stride_head, int32_t n_chunks, int32_t kv_dtype, const float* k_scales,
+                                     const float* v_scales, const int32_t* block_table, int64_t bt_stride,
+                                     int32_t bt_columns, const int32_t* kv_lens, int32_t window, int32_t sinks, void* out,
+                                     int64_t o_stride_tok, int64_t o_stride_head, void* workspace,
+                                     int64_t workspace_bytes, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim,
+                                     int32_t chunk_tokens, float softmax_scale, int32_t dtype, const MiTuning* tuning,
+                                     void* stream);
+int64_t mi_window_prefill_workspace_bytes(int32_t T, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim,
+                                          int32_t max_kv_len, int32_t window, int32_t sinks, const MiTuning* tuning);
+int mi_paged_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                                      const void* v_cache, int64_t kv_stride_chunk, int64_t kv_stride_tok,
+                                      int64_t kv_stride_head, int32_t n_chunks, int32_t kv_dtype, const float* k_scales,
+                                      const float* v_scales, const int32_t* block_table, int64_t bt_stride,
+                                      int32_t bt_columns, const int32_t* cu_seqlens_q, const int32_t* kv_lens,
+                                      int32_t window, int32_t sinks, void* out, int64_t o_stride_tok,
+                                      int64_t o_stride_head, void* workspace, int64_t workspace_bytes, int32_t T,
+                                      int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t chunk_tokens,
+                                      int32_t max_kv_len, int32_t one_row_requests, float softmax_scale, int32_t dtype,
+                                      const MiTuning* tuning, void* stream);
+
+/*
  * The prompts of a step from the QKV projection's output `[T][(Hq + 2 Hkv) * head_dim]` (rows `qkv_stride_tok` elements
  * apart; per KV head: its query heads, its key head, its value head) in two calls, without a pass over the queries.
  *

@@ -85,6 +85,15 @@ SIGNATURES = {
         c_int,
         [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _P, _P, _P, _I64, _P, _P, _P, _I64, _I64, _P, _I64,
          _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F, _I32, _P, _P]),
+    "mi_paged_window_decode_attention": (
+        c_int,
+        [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P, _P, _P, _I64, _I32, _P, _I32, _I32, _P, _I64, _I64, _P, _I64,
+         _I32, _I32, _I32, _I32, _I32, _F, _I32, _P, _P]),
+    "mi_window_prefill_workspace_bytes": (_I64, [_I32] * 8 + [_P]),
+    "mi_paged_window_prefill_attention": (
+        c_int,
+        [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P, _P, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _I64, _I64, _P,
+         _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F, _I32, _P, _P]),
     "mi_qkv_key_append": (
         c_int, [_P, _I64, _P, _I64, _P, _F, _I32, _P, _I64, _I32, _F, _P, _P, _P, _P, _I64, _I64, _P, _P, _P,
                 _I32, _I32, _I32, _I32, _I32, _P]),

@@ -62,6 +62,27 @@ int mi_resolve_tuning(const MiTuning* given, MiTuning* out, const char* who) {
   return MI_OK;
 }
 
+int mi::check_window(int32_t window, int32_t sinks, int32_t n_chunks, int32_t bt_columns, int64_t bt_stride, int32_t R, int32_t chunk_tokens,
+                     const char* who, WindowArgs* out) {
+  char msg[200];
+  auto bad = [&](const char* what) {
+    snprintf(msg, sizeof msg, "%s: %s", who, what);
+    return mi_fail(MI_ERR_SHAPE, msg);
+  };
+  if (window < 1) return bad("the window must be at least 1 (a token sees itself)");
+  if (sinks < 0) return bad("sinks must not be negative");
+  if (n_chunks < 1) return bad("the cache has no chunk");
+  if (bt_columns < 1 || (R > 1 && bt_stride < bt_columns)) return bad("block_table needs a column, and rows that do not overlap");
+  if (chunk_tokens < 1) return bad("chunk size must be a positive multiple of 16");
+  // (a token's chunk is its number times 2^40 / chunk_tokens in 64 bits; positions behind the last tile have 31)
+  const int64_t tokens = (int64_t)bt_columns * chunk_tokens;
+  if (tokens > 0x7ffffe00) return bad("block tables of 2^31 tokens and more (less 512) are not served");
+  if (bt_columns >= 1 << 24) return bad("block tables of 2^24 columns and more are not served");
+  if (((int64_t)1 << 40) % chunk_tokens && tokens * chunk_tokens >= (int64_t)1 << 40) return bad("block tables of so many tokens need a chunk size that is a power of two");
+  *out = {window < kMostWindow ? window : kMostWindow, sinks < kMostWindow ? sinks : kMostWindow, n_chunks, (int32_t)tokens};
+  return MI_OK;
+}
+
 // ---- kernel timing with HIP events --------------------------------------------------
 // When enabled, the attention entry points bracket their main kernel (decode: the kernel that
 // streams the KV cache; prefill: the tile kernel, and after it the streaming kernel of the one-row

@@ -20,9 +20,11 @@
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <chrono>
 #include <cmath>
 #include <initializer_list>
+#include <optional>
 #include <string>
 #include <tuple>
 #include <type_traits>
@@ -375,8 +377,34 @@ PyObject* kv_append_fp8(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
+void same_device(const Tensor& ref, std::initializer_list<const Tensor*> others) {
+  for (const Tensor* t : others) REQUIRE(!t || t->device() == ref.device(), "all tensors must be on one device");
+}
+
+// The window of an attention call: `window` None for none (then no sinks either).
+struct Window {
+  bool on = false;
+  int window = 0, sinks = 0;
+};
+Window window_of(PyObject* window, PyObject* sinks) {
+  auto capped = [](int64_t v) { return (int)std::min<int64_t>(v, 1 << 30); };
+  Window w;
+  const int64_t n = as_int(sinks);
+  REQUIRE(n >= 0, "sinks must not be negative");
+  if (window == Py_None) {
+    REQUIRE(n == 0, "sinks go with a window (without one every token is in sight)");
+    return w;
+  }
+  const int64_t size = as_int(window);
+  REQUIRE(size >= 1, "the window must be at least 1 (a token sees itself)");
+  w.on = true;
+  w.window = capped(size);
+  w.sinks = capped(n);
+  return w;
+}
+
 // paged_decode_attention(q, k_cache, v_cache, kv_lens, block_table, softmax_scale|None, max_kv_len|None, split_tokens,
-//                        out|None, workspace|None, k_scales|None, v_scales|None, tuning|None, override|None)
+//                        out|None, workspace|None, k_scales|None, v_scales|None, tuning|None, override|None, window|None, sinks)
 PyObject* paged_decode_attention(PyObject* const* a) {
   const Tensor& q = tensor(a[0], "q");
   void* stream = stream_of(q);
@@ -404,7 +432,25 @@ PyObject* paged_decode_attention(PyObject* const* a) {
   const Rows3 o3 = rows3(out, "out");
   REQUIRE(o3.n == R && o3.h == q3.h && o3.d == q3.d && out.scalar_type() == q.scalar_type(), "out shape / dtype mismatch");
   const auto* tune = (const MiTuning*)host_struct(a[12]);
+  const Window win = window_of(a[14], a[15]);
+  if (win.on) {
+    same_device(q, {&kc, &vc, &lens, &table, ks, vs, &out});
+    REQUIRE(split == 0, "split_tokens is not served with a window");
+    REQUIRE(!ks == !fp8 && !vs == !fp8, "scales go with an fp8 cache");
+  }
+  std::optional<c10::DeviceGuard> guard;
+  if (win.on) guard.emplace(q.device());
   const Scratch ws = scratch(q, stream, mi_decode_workspace_bytes((int)R, (int)q3.h, (int)c.h, (int)q3.d, (int)c.c, (int)max_len, split, tune), a[9], a[13]);
+  if (win.on) {
+    check(mi_paged_window_decode_attention(q.data_ptr(), q3.sn, q3.sh, kc.data_ptr(), vc.data_ptr(), c.sc, c.st, c.sh, (int)c.n,
+                                           fp8 ? MI_KV_FP8_E4M3 : MI_KV_16BIT, (const float*)ptr(ks), (const float*)ptr(vs),
+                                           (const int32_t*)table.data_ptr(), table.stride(0), (int)table.size(1),
+                                           (const int32_t*)lens.data_ptr(), win.window, win.sinks, out.data_ptr(), o3.sn, o3.sh,
+                                           ws.ptr, ws.bytes, (int)R, (int)q3.h, (int)c.h, (int)q3.d, (int)c.c, scale, dtype_code(q),
+                                           tune, stream),
+          "mi_paged_window_decode_attention");
+    return a[8] == Py_None ? wrap(made) : same(a[8]);
+  }
   check(mi_paged_decode_attention(q.data_ptr(), q3.sn, q3.sh, kc.data_ptr(), vc.data_ptr(), c.sc, c.st, c.sh,
                                   (const int32_t*)table.data_ptr(), table.stride(0), (const int32_t*)lens.data_ptr(),
                                   out.data_ptr(), o3.sn, o3.sh, ws.ptr, ws.bytes, (int)R, (int)q3.h, (int)c.h, (int)q3.d,
@@ -452,7 +498,8 @@ PyObject* paged_mla_decode_attention(PyObject* const* a) {
 }
 
 // paged_prefill_attention(q, k_cache, v_cache, cu_seqlens_q, kv_lens, block_table, softmax_scale|None, max_kv_len|None,
-//                         out|None, k_scales|None, v_scales|None, tuning|None, override|None, one_row_requests)
+//                         out|None, k_scales|None, v_scales|None, tuning|None, override|None, one_row_requests, window|None,
+//                         sinks)
 PyObject* paged_prefill_attention(PyObject* const* a) {
   const Tensor& q = tensor(a[0], "q");
   void* stream = stream_of(q);
@@ -481,6 +528,23 @@ PyObject* paged_prefill_attention(PyObject* const* a) {
   const Rows3 o3 = rows3(out, "out");
   REQUIRE(o3.n == T && o3.h == q3.h && o3.d == q3.d && out.scalar_type() == q.scalar_type(), "out shape / dtype mismatch");
   const auto* tune = (const MiTuning*)host_struct(a[11]);
+  const Window win = window_of(a[14], a[15]);
+  if (win.on) {
+    same_device(q, {&kc, &vc, &cu, &lens, &table, ks, vs, &out});
+    REQUIRE(R > 0 && cu.dim() == 1, "cu_seqlens_q must be a row of at least two entries");
+    REQUIRE((ks != nullptr) == (vs != nullptr), "k_scales and v_scales go together");
+    const c10::DeviceGuard guard(q.device());
+    const Scratch ws = scratch(q, stream, mi_window_prefill_workspace_bytes((int)T, (int)R, (int)q3.h, (int)c.h, (int)q3.d, (int)max_len,
+                                                                            win.window, win.sinks, tune), Py_None, a[12]);
+    check(mi_paged_window_prefill_attention(q.data_ptr(), q3.sn, q3.sh, kc.data_ptr(), vc.data_ptr(), c.sc, c.st, c.sh, (int)c.n,
+                                            ks ? MI_KV_FP8_E4M3 : MI_KV_16BIT, (const float*)ptr(ks), (const float*)ptr(vs),
+                                            (const int32_t*)table.data_ptr(), table.stride(0), (int)table.size(1),
+                                            (const int32_t*)cu.data_ptr(), (const int32_t*)lens.data_ptr(), win.window, win.sinks,
+                                            out.data_ptr(), o3.sn, o3.sh, ws.ptr, ws.bytes, (int)T, (int)R, (int)q3.h, (int)c.h,
+                                            (int)q3.d, (int)c.c, (int)max_len, as_bool(a[13]), scale, dtype_code(q), tune, stream),
+          "mi_paged_window_prefill_attention");
+    return a[8] == Py_None ? wrap(made) : same(a[8]);
+  }
   const Scratch ws = scratch(q, stream, mi_prefill_workspace_bytes((int)T, (int)R, (int)q3.h, (int)c.h, (int)q3.d, (int)max_len, 0, tune), Py_None, a[12]);
   if (!as_bool(a[13])) {
     check(mi_paged_prefill_attention_tiles(q.data_ptr(), q3.sn, q3.sh, kc.data_ptr(), vc.data_ptr(), c.sc, c.st, c.sh,
@@ -1016,9 +1080,6 @@ PyObject* last_token_gather(PyObject* const* a) {
 }
 
 // ------------------------------------------------------------------------------------------ speculative decoding
-void same_device(const Tensor& ref, std::initializer_list<const Tensor*> others) {
-  for (const Tensor* t : others) REQUIRE(!t || t->device() == ref.device(), "all tensors must be on one device");
-}
 // Rows of nodes: `[R + 1]` int32, R > 0.
 int64_t requests_of(const Tensor& cu) {
   REQUIRE(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.is_contiguous() && cu.numel() >= 2,
@@ -1311,8 +1372,8 @@ PyMethodDef kMethods[] = {
     ABI(mi_prefill_workspace_bytes), ABI(mi_paged_decode_attention_noalloc),
     ABI(mi_update_requests), ABI(mi_update_requests_mask8), ABI(mi_update_requests_clearing),
     ABI(mi_add_request), ABI(mi_decode_attention_state), ABI(mi_step_attention_state),
-    OP(kv_append, 6), OP(kv_append_fp8, 9), OP(paged_decode_attention, 14), OP(paged_mla_decode_attention, 10),
-    OP(paged_prefill_attention, 14), OP(paged_prefill_attention_mla, 11), OP(norm_rope_append, 22), OP(qkv_norm_rope_append, 22), OP(qkv_key_append, 16),
+    OP(kv_append, 6), OP(kv_append_fp8, 9), OP(paged_decode_attention, 16), OP(paged_mla_decode_attention, 10),
+    OP(paged_prefill_attention, 16), OP(paged_prefill_attention_mla, 11), OP(norm_rope_append, 22), OP(qkv_norm_rope_append, 22), OP(qkv_key_append, 16),
     OP(qkv_prefill_attention, 18), OP(decode_step_attention, 29),
     OP(linear_decode, 5), OP(attention_layer_decode, 24), OP(sample_from_logits, 12), OP(selected_log_probs, 2), OP(last_token_gather, 3),
     OP(paged_tree_attention, 12), OP(verify_drafted_tokens, 11), OP(kv_keep_accepted, 9), OP(setup, 3),

@@ -47,6 +47,21 @@ struct FusedStepArgs {
   int64_t next_stride_row;
   int32_t next_rows, next_columns;
 };
+// What a call with a window hands the attention kernels beside the ordinary arguments (see mi_paged_window_decode_attention).
+struct WindowArgs {
+  int32_t window, sinks;   // at most 2^30 each
+  int32_t n_chunks;        // chunks of the cache
+  int32_t max_len;         // tokens that the block table has room for
+};
+constexpr int32_t kMostWindow = 1 << 30;   // (of more tokens than that, all are in sight of a request that 31 bits can count)
+// Keys that one of `rows` neighbouring rows sees at most, of at most `len`.
+inline int32_t window_keys(const WindowArgs& w, int64_t len, int rows) {
+  const int64_t most = (int64_t)w.window + w.sinks + rows;
+  return (int32_t)(len < most ? len : most);
+}
+// The checks that calls with a window have beyond the ordinary ones.  MI_OK or a negative code with a message.
+int check_window(int32_t window, int32_t sinks, int32_t n_chunks, int32_t bt_columns, int64_t bt_stride, int32_t R, int32_t chunk_tokens,
+                 const char* who, WindowArgs* out);
 // Rows of the matrix that one workgroup of mi_linear_decode reads, workgroup x of the grid rows [x n, x n + n); 0 where a
 // row is read by workgroups on several XCDs.
 int linear_rows_per_workgroup(int T, int N, int K);
@@ -63,5 +78,6 @@ int launch_paged_decode(const void* q, int64_t q_stride_tok, int64_t q_stride_he
                         int64_t o_stride_head, void* workspace, int64_t workspace_bytes, int32_t R, int32_t Hq,
                         int32_t Hkv, int32_t head_dim, int32_t chunk_tokens, int32_t split_tokens,
                         float softmax_scale, int32_t kv_dtype, const float* k_scales, const float* v_scales,
-                        int32_t dtype, const MiTuning& tune, void* stream, const FusedStepArgs* fused = nullptr);
+                        int32_t dtype, const MiTuning& tune, void* stream, const FusedStepArgs* fused = nullptr,
+                        const WindowArgs* win = nullptr);
 }

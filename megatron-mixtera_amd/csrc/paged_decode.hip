@@ -90,6 +90,9 @@ struct DecodeParams {
   int32_t next_n, next_bytes, next_rows, next_fetch, next_blocks;   // rows, bytes of one, rows per block, of them to fetch, blocks
   float eps, mscale;
   float scale_log2;
+  // Windowed kernels only: a request sees its last `window` tokens and its first `sinks` (both at most 2^30); table entries are
+  // kept below n_chunks, lengths below max_len, the tokens that the table has room for.
+  int32_t window, sinks, n_chunks, max_len;
 };
 
 // tok / chunk for 0 <= tok < 2^31 via a 40-bit reciprocal (exact while tok * chunk < 2^40).
@@ -109,6 +112,24 @@ static __host__ __device__ __forceinline__ int short_lds_per_wave(int head_dim, 
   return ((part > prologue ? part : prologue) + 15) & ~15;
 }
 
+// The tiles of TK tokens that a request with a window walks: those of the sinks, then those from its window on.  Token T of the
+// walk is token T + (T >= from ? skip : 0) of the request; `skip` is a multiple of TK.  What lies between is not touched, and
+// its table entries may hold anything.
+struct Walk {
+  int len;          // tokens of the request
+  int first;        // the window's first token
+  int from, skip;   // where the walk leaves the sinks' tiles, and how far it goes then
+};
+template <int TK>
+static __device__ __forceinline__ Walk window_walk(const DecodeParams& p, int len) {
+  Walk w;
+  w.len = min(len, p.max_len);
+  w.first = max(0, w.len - p.window);
+  w.from = (p.sinks + TK - 1) / TK * TK;
+  w.skip = max(0, w.first / TK * TK - w.from);
+  return w;
+}
+
 // One segment: tokens [start, end) of request r for KV head h (one wavefront) and the `gq` <= 16 query heads
 // hq0 .. hq0 + gq - 1 that share it.  `whole` = the segment is the entire request (write the 16-bit output, no
 // partial).
@@ -124,7 +145,13 @@ static __host__ __device__ __forceinline__ int short_lds_per_wave(int head_dim, 
 // row into their cache slot, and takes both from LDS for its last tile.  `q_lds` is then this wavefront's
 // piece of LDS for cos / sin of the request's position [2][HDK], the key row [HDK] (fp32) and the query rows.
 // SHORT: the partial stays in `q_lds` (see decode_short_kernel).
-template <int HDK, int HDV, int NT, bool FP8, bool F16, bool FUSED = false, bool SHORT = false>
+//
+// WIN: `start` and `end` count along the walk of window_walk.  Tiles that a border of the window or of the sinks crosses are
+// masked: scores to -inf, values to zero (zero times what lies there might be NaN), and their loads go to rows in sight where
+// the others lie on one side.  An fp8 chunk's scale is taken as sign, power of two and factor (see value_parts), and fp16
+// probabilities stand 2^14 above the running maximum: as they are, one of a thousandth of the row's largest times a scale of a hundredth
+// would be subnormal, in the numerator and in the row sum.
+template <int HDK, int HDV, int NT, bool FP8, bool F16, bool FUSED = false, bool SHORT = false, bool WIN = false>
 static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int r, int row, int h, int hq0, int gq,
                                                       int len, int start, int end, bool whole, bool final_seg,
                                                       int slot, int lane, uint8_t* q_lds) {
@@ -157,7 +184,17 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
   // Loads are clamped to the last token of this segment (not of the request): the software
   // pipeline requests one tile past the end, and that tile belongs to another workgroup's span --
   // clamped, the request degenerates to re-reading one row instead of streaming 2 tiles from HBM.
-  const int last = min(end, len) - 1;
+  static_assert(!WIN || (!FUSED && !SHARED_KV), "a window: ordinary caches, queries as they are");
+  constexpr int TK = 16 * NT;
+  Walk walk = {};
+  if constexpr (WIN) {
+    walk = window_walk<TK>(p, len);
+    walk.first = __builtin_amdgcn_readfirstlane(walk.first);
+    walk.skip = __builtin_amdgcn_readfirstlane(walk.skip);
+    len = walk.len = __builtin_amdgcn_readfirstlane(walk.len);
+  }
+  auto position = [&](int T) { return WIN && T >= walk.from ? T + walk.skip : T; };
+  const int last = WIN ? position(end - 1) : min(end, len) - 1;
 
   // Query fragments: B operand rows are the G heads of this KV head.
   uint4 qf[Q_IN_LDS ? 1 : KS];
@@ -471,7 +508,8 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
       qf[kk] = m16 < G ? *reinterpret_cast<const uint4*>(q_rows + m16 * kQPitch + 2 * frag_d0(kk)) : make_uint4(0, 0, 0, 0);
   };
 
-  float m_run = -INFINITY, l_run = 0.f;
+  // (WIN: a finite start, so that scores of -inf leave the maximum finite)
+  float m_run = WIN ? -3e38f : -INFINITY, l_run = 0.f;
   f32x4_t acc[DV];
 #pragma unroll
   for (int e = 0; e < DV; ++e) acc[e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -513,7 +551,14 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
     float sc;          // fp8: scale of (pc, h)
     float sc_next;     // per-lane copy of the next chunk's scale (load may be in flight)
   };
-  auto entry_load = [&](int ci) { return bt_row[min(ci, ci_last)]; };
+  auto entry_load = [&](int ci) {
+    const int pc = bt_row[min(ci, ci_last)];
+    return WIN ? min(max(pc, 0), p.n_chunks - 1) : pc;
+  };
+  // the chunk that follows ci along the walk
+  const int ci_near = WIN ? chunk_of(max(walk.from - 1, 0), p.chunk_magic) : 0;
+  const int ci_far = WIN && walk.skip > 0 && walk.from > 0 ? chunk_of(walk.from + walk.skip, p.chunk_magic) : 0;
+  auto next_chunk = [&](int ci) { return WIN && ci >= ci_near && ci < ci_far ? ci_far : ci + 1; };
   auto scale_load = [&](const float* scales, int pc) { return scales[(int64_t)pc * p.Hkv + h]; };
   auto uniform_f = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
   // the clamped tile start only ever moves forward, by at most one chunk per tile
@@ -522,7 +567,7 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
       c.ci = ci;
       c.pc = c.pc_next;
       c.pc_next = __builtin_amdgcn_readfirstlane(c.pc_after);
-      c.pc_after = entry_load(ci + 2);
+      c.pc_after = entry_load(next_chunk(next_chunk(ci)));
       if (FP8) {
         c.sc = uniform_f(c.sc_next);
         c.sc_next = scale_load(scales, c.pc_next);
@@ -534,8 +579,9 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
   Cursor kcur, vcur;
   float ksc_first = 1.f, vsc_first = 1.f;  // per-lane copies, loads in flight
   {
-    const int ci0 = chunk_of(min(start, last), p.chunk_magic);
-    const int e0 = entry_load(ci0), e1 = entry_load(ci0 + 1), e2 = entry_load(ci0 + 2);
+    const int ci0 = chunk_of(min(position(start), last), p.chunk_magic);
+    const int ci1 = next_chunk(ci0);
+    const int e0 = entry_load(ci0), e1 = entry_load(ci1), e2 = entry_load(next_chunk(ci1));
     kcur.ci = ci0;
     kcur.pc = __builtin_amdgcn_readfirstlane(e0);
     kcur.pc_next = __builtin_amdgcn_readfirstlane(e1);
@@ -557,32 +603,44 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
     tok0 = ci * p.chunk;
     return base + (int64_t)c.pc * chunk_bytes;
   };
+  // WIN: rows of a sub-tile at token t0 from which and up to which there is something in sight, where one of the two borders
+  // crosses it (the rows' loads are kept within; a tile with both is loaded whole)
+  auto first_row = [&](int t0) { return WIN && walk.skip > 0 && t0 >= walk.from ? (uint32_t)max(walk.first - t0, 0) : 0u; };
+  auto last_row = [&](int t0) {
+    const int end_row = WIN && walk.skip > 0 && t0 < walk.from ? min(last, p.sinks - 1) : last;
+    return (uint32_t)max(min(end_row - t0, 15), 0);
+  };
   auto load_k = [&](int T) {
+    T = position(T);
     int tok0;
     const uint8_t* chunk = tile_chunk(kcur, p.k_scale, kbase, T, tok0);
     if (FP8) ksc_tile = (FUSED && own_scale && kcur.ci == ci_last) ? own_ksc : kcur.sc;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       const int t0 = min(T + 16 * u, last);
-      const uint32_t lim = (uint32_t)min(last - t0, 15) * tok_bytes;
-      const uint8_t* krow = chunk + (uint32_t)(t0 - tok0) * tok_bytes + min(k_lane, lim + k_col);
+      const uint32_t lim = (WIN ? last_row(t0) : (uint32_t)min(last - t0, 15)) * tok_bytes;
+      uint32_t k_row = min(k_lane, lim + k_col);
+      if constexpr (WIN) k_row = max(k_row, first_row(t0) * tok_bytes + k_col);
+      const uint8_t* krow = chunk + (uint32_t)(t0 - tok0) * tok_bytes + k_row;
 #pragma unroll
       for (int kk = 0; kk < (FP8 ? KS / 2 : KS); ++kk)
         kf[u][kk] = SHARED_KV ? ld16(krow + 64 * kk) : ld16_stream(krow + 64 * kk);
     }
   };
   auto load_v = [&](int T) {
+    T = position(T);
     int tok0;
     const uint8_t* chunk = tile_chunk(vcur, p.v_scale, vbase, T, tok0);
     if (FP8) vsc_tile = (FUSED && own_scale && vcur.ci == ci_last) ? own_vsc : vcur.sc;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       const int t0 = min(T + 16 * u, last);
-      const uint32_t cap = (uint32_t)min(last - t0, 15) * tok_bytes + v_col;
+      const uint32_t cap = (WIN ? last_row(t0) : (uint32_t)min(last - t0, 15)) * tok_bytes + v_col;
+      const uint32_t from = WIN ? first_row(t0) * tok_bytes + v_col : 0u;
       const uint8_t* tile = chunk + (uint32_t)(t0 - tok0) * tok_bytes;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint8_t* vrow = tile + min(v_lane[j], cap);
+        const uint8_t* vrow = tile + (WIN ? max(min(v_lane[j], cap), from) : min(v_lane[j], cap));
         if constexpr (SHARED_KV) ld_dwords(vrow, vf[u][j]);
         else ld_dwords_stream(vrow, vf[u][j]);
       }
@@ -613,12 +671,38 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
     }
   }
   const uint2 ones = make_uint2(ones2<F16>(), ones2<F16>());  // four times 1.0
-  for (int T = start; T < end; T += 16 * NT) {
+  // WIN, fp8: a value scale's power of two goes into the conversion of the bytes, its factor into the probabilities (and out of
+  // their sum): from 1 to 2, or, where bytes times the power of two round in fp16 (below 2^-15), from 1/2 to 1.  Zero counts as
+  // 2^-126; NaN and infinite scales are in the factor.  Its sign, and a key scale's, go to the bytes, in a branch.
+  auto value_parts = [&](float scale, float& pow2, float& factor) {
+    const uint32_t bits = max(__float_as_uint(scale) & 0x7fffffffu, 0x00800000u);
+    const bool low = F16 && bits < (uint32_t)(127 - 15) << 23;
+    pow2 = __uint_as_float((bits & 0x7f800000u) + (low ? 0x00800000u : 0u));
+    factor = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((bits & 0x007fffffu) | (low ? 0x3f000000u : 0x3f800000u));
+  };
+  constexpr float kLift = WIN && F16 ? 14.f : 0.f;   // powers of two between the running maximum and one
+  for (int walked = start; walked < end; walked += 16 * NT) {
+    const int T = position(walked);
     // ---- S^T = K Q^T ---------------------------------------------------------
     // The tile lies in one chunk, so one K scale and one V scale hold for all of it; the score
     // multiplier is positive and wave-uniform, so the maximum is taken over the raw products.
-    const float mul = FP8 ? p.scale_log2 * ksc_tile : p.scale_log2;
-    const bool ragged = T + 16 * NT > end;  // only the last tile of a segment has masked tokens
+    float mul = FP8 ? p.scale_log2 * ksc_tile : p.scale_log2;
+    if constexpr (WIN && FP8) {   // (kept off zero, which times the -inf of a masked score would be NaN; a NaN stays one)
+      mul = fabsf(mul);
+      mul = mul < 1.17549435e-38f ? 1.17549435e-38f : mul;
+    }
+    // only the last tile of a segment has masked tokens (WIN: and those that a border crosses)
+    const bool ragged = WIN ? T + TK > len || (T + TK > p.sinks && T < walk.first) : T + 16 * NT > end;
+    auto hidden = [&](int tok) { return tok >= len || (tok >= p.sinks && tok < walk.first); };   // WIN
+    if constexpr (WIN && FP8) {
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(__float_as_int(ksc_tile)) < 0, 0)) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int kk = 0; kk < KS / 2; ++kk)
+            kf[u][kk] = make_uint4(kf[u][kk].x ^ 0x80808080u, kf[u][kk].y ^ 0x80808080u, kf[u][kk].z ^ 0x80808080u, kf[u][kk].w ^ 0x80808080u);
+      }
+    }
     // Fused step, the request's last tile: what the loads brought for the new token's row (and for the rows past it, which
     // re-read that one) is replaced.
     const bool new_token = FUSED && final_seg && T + 16 * NT >= len;
@@ -653,7 +737,7 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
         const int tok0 = T + 16 * u + 4 * g;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (tok0 + i >= end) sacc[i] = -INFINITY;
+          if (WIN ? hidden(tok0 + i) : tok0 + i >= end) sacc[i] = -INFINITY;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) sc[u][i] = sacc[i];
@@ -663,7 +747,7 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
     // The scheduling fences keep each batch of prefetch loads together at this point of the
     // loop instead of letting the compiler sink them next to their uses one by one.
     __builtin_amdgcn_sched_barrier(0);
-    load_k(T + 16 * NT);  // prefetch: the K registers are free again
+    load_k(walked + 16 * NT);  // prefetch: the K registers are free again
     __builtin_amdgcn_sched_barrier(0);
     tmax = fmaxf(tmax, xor16(tmax));
     tmax = fmaxf(tmax, xor32(tmax));
@@ -674,7 +758,9 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
     const float m_new = fmaxf(m_run, tmax * mul);
     const float alpha = fast_exp2(m_run - m_new);
     m_run = m_new;
-    const float neg = FP8 ? fast_log2(vscale) - m_new : -m_new;
+    float vpow2 = 1.f, vfactor = 1.f;
+    if constexpr (WIN && FP8) value_parts(vscale, vpow2, vfactor);
+    const float neg = WIN ? (FP8 ? fast_log2(vfactor) + kLift : kLift) - m_new : FP8 ? fast_log2(vscale) - m_new : -m_new;
     uint2 pf[NT];
     f32x4_t psum4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -687,7 +773,7 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
       psum4 = mfma_16x16x16<F16>(ones, pf[u], psum4);
     }
     // (every slot of psum4 holds the row sum of this lane's query row)
-    l_run = l_run * alpha + (FP8 ? psum4[0] * __builtin_amdgcn_rcpf(vscale) : psum4[0]);
+    l_run = l_run * alpha + (FP8 ? psum4[0] * __builtin_amdgcn_rcpf(WIN ? vfactor : vscale) : psum4[0]);
     if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {  // the running maximum rarely moves after the first tiles
 #pragma unroll
       for (int e = 0; e < DV; ++e) {
@@ -709,6 +795,27 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
       }
     }
 
+    if constexpr (WIN) {
+      if (ragged) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool none = hidden(T + 16 * u + 4 * g + j);
+#pragma unroll
+            for (int dw = 0; dw < VD; ++dw) vf[u][j][dw] = none ? 0u : vf[u][j][dw];
+          }
+      }
+      if (FP8 && __builtin_expect(__builtin_amdgcn_readfirstlane(__float_as_int(vscale)) < 0, 0)) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int dw = 0; dw < VD; ++dw) vf[u][j][dw] ^= 0x80808080u;
+      }
+    }
+
     // ---- O^T += V^T P^T --------------------------------------------------------
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
@@ -725,7 +832,7 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int hf = 0; hf < VD; ++hf) w[j][hf] = fp8x4_to_16x4<F16>(vf[u][j][hf]);
+          for (int hf = 0; hf < VD; ++hf) w[j][hf] = WIN ? fp8x4_to_16x4<F16>(vf[u][j][hf], vpow2) : fp8x4_to_16x4<F16>(vf[u][j][hf]);
 #pragma unroll
         for (int hf = 0; hf < VD; ++hf) {
           acc[4 * hf + 0] = mfma_16x16x16<F16>(
@@ -740,13 +847,13 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    load_v(T + 16 * NT);  // prefetch: the V registers are free again
+    load_v(walked + 16 * NT);  // prefetch: the V registers are free again
     __builtin_amdgcn_sched_barrier(0);
   }
 
   // ---- epilogue ---------------------------------------------------------------
   const float l_tot = l_run;  // already summed over the lanes of a row (matrix-core row sums)
-  const float inv = 1.f / l_tot;
+  const float inv = WIN && l_tot == 0.f ? 0.f : 1.f / l_tot;   // (WIN: a part whose scores are all -inf)
   if (m16 >= G) return;  // (no barrier follows inside a segment)
   // acc[e][i] holds d = DV*(4g+i) + e: DV*4 contiguous values per lane.
   if constexpr (SHORT) {
@@ -783,7 +890,8 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
           *reinterpret_cast<float2*>(o + DV * i + e) = make_float2(acc[e][i] * inv, acc[e + 1][i] * inv);
       }
     }
-    if (g == 0) p.part_lse[row] = m_run + fast_log2(l_tot);
+    // (WIN: parts have one lift in common; one without a finite score must not make the merge's maximum infinite)
+    if (g == 0) p.part_lse[row] = WIN && l_tot == 0.f ? -3e38f : m_run + fast_log2(l_tot);
   }
 }
 
@@ -807,7 +915,8 @@ static __device__ __forceinline__ bool decode_row(const DecodeParams& p, int r, 
 // With more, or without LANES (no register to spare), dynamic LDS starts with the inclusive prefix sums of tiles per request [R] and the request lengths [R].
 // A workgroup without a span calls idle(number of those that have one).
 struct NoIdle { __device__ __forceinline__ void operator()(int) const {} };
-template <int TK, bool LANES = true, typename Seg, typename Idle = NoIdle>
+// WIN: the tiles, and the segments' tokens, are those of the requests' walks (window_walk).
+template <int TK, bool LANES = true, bool WIN = false, typename Seg, typename Idle = NoIdle>
 static __device__ __forceinline__ void walk_segments(const DecodeParams& p, Seg seg, Idle idle = Idle()) {
   extern __shared__ int cum[];
   int* const len_s = cum + p.R;
@@ -821,7 +930,12 @@ static __device__ __forceinline__ void walk_segments(const DecodeParams& p, Seg 
     const int i = base + lane;
     int row_unused;
     len_l = i < p.R ? p.lens[i] : 0;
-    cum_l = wave_scan((i < p.R && decode_row(p, i, row_unused)) ? tiles_of(len_l, TK) : 0);
+    int walked = len_l;
+    if constexpr (WIN) {
+      const Walk w = window_walk<TK>(p, len_l);
+      walked = w.len - w.skip;
+    }
+    cum_l = wave_scan((i < p.R && decode_row(p, i, row_unused)) ? tiles_of(walked, TK) : 0);
   };
   int total;
   if (in_lanes) {
@@ -913,7 +1027,12 @@ static __device__ __forceinline__ void walk_segments(const DecodeParams& p, Seg 
       }
       int row;
       decode_row(p, r, row);
-      seg(r, row, len, tb * TK, min(te * TK, len), first && final, final, (int)blockIdx.x + r);
+      int walked = len;
+      if constexpr (WIN) {
+        const Walk w = window_walk<TK>(p, len);
+        walked = w.len - w.skip;
+      }
+      seg(r, row, len, tb * TK, min(te * TK, walked), first && final, final, (int)blockIdx.x + r);
     }
     t0 = max(t0, ue);
     ++r;
@@ -950,7 +1069,7 @@ static __device__ __forceinline__ void fetch_next_matrix(int busy) {
 }
 
 // The body of the register-streaming kernels: one wavefront per (virtual) KV head.
-template <int HDK, int HDV, int NT, bool FP8, bool F16, bool FUSED = false>
+template <int HDK, int HDV, int NT, bool FP8, bool F16, bool FUSED = false, bool WIN = false>
 static __device__ __forceinline__ void decode_stream_body(const DecodeParams& p) {
   extern __shared__ int cum[];
   const int lane = threadIdx.x & 63;
@@ -965,8 +1084,8 @@ static __device__ __forceinline__ void decode_stream_body(const DecodeParams& p)
   // row and its query rows (see decode_segment)
   uint8_t* const q_lds = reinterpret_cast<uint8_t*>(cum) + (((size_t)p.R * 8 + 15) & ~(size_t)15) +
                          (size_t)wave * (FUSED ? (size_t)fused_lds_per_wave(HDK, p.G) : (size_t)(16 * (HDK * 2 + 16)));
-  walk_segments<16 * NT>(p, [&](int r, int row, int len, int start, int end, bool whole, bool final_seg, int slot) {
-    decode_segment<HDK, HDV, NT, FP8, F16, FUSED>(p, r, row, h, hq0, gq, len, start, end, whole, final_seg, slot, lane,
+  walk_segments<16 * NT, true, WIN>(p, [&](int r, int row, int len, int start, int end, bool whole, bool final_seg, int slot) {
+    decode_segment<HDK, HDV, NT, FP8, F16, FUSED, false, WIN>(p, r, row, h, hq0, gq, len, start, end, whole, final_seg, slot, lane,
                                                   q_lds);
   }, [&](int busy) {
     // (not with an fp8 cache, whose kernel has no register to spare and spills three: 12 requests 36.2 -> 35.4 us, but 176
@@ -975,9 +1094,9 @@ static __device__ __forceinline__ void decode_stream_body(const DecodeParams& p)
   });
 }
 
-template <int HD, int NT, bool FP8, int MINW, bool F16>
+template <int HD, int NT, bool FP8, int MINW, bool F16, bool WIN = false>
 __global__ __launch_bounds__(512, MINW) void paged_decode_stream_kernel(DecodeParams p) {
-  decode_stream_body<HD, HD, NT, FP8, F16>(p);
+  decode_stream_body<HD, HD, NT, FP8, F16, false, WIN>(p);
 }
 
 // The same stream over the raw queries, keys and values of a decode step: head norm, rotary embedding and the
@@ -992,7 +1111,7 @@ __global__ __launch_bounds__(512, MINW) void decode_step_stream_kernel(DecodePar
 // chip into as many pieces as there are tiles or so and needs a second launch to find and merge them, half as long as the
 // first; here the pieces are few, and decode_short_merge_kernel knows where they are.
 constexpr int kShortWaves = 8;
-template <int HD, int NT, bool FP8, bool F16, bool FUSED>
+template <int HD, int NT, bool FP8, bool F16, bool FUSED, bool WIN = false>
 __global__ __launch_bounds__(64 * kShortWaves, 2) void decode_short_kernel(DecodeParams p) {
   extern __shared__ int cum[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1009,14 +1128,19 @@ __global__ __launch_bounds__(64 * kShortWaves, 2) void decode_short_kernel(Decod
   if (!decode_row(p, r, row)) return;
   constexpr int TK = 16 * NT, PITCH = short_pitch(HD);
   const int len = __builtin_amdgcn_readfirstlane(p.lens[r]);
-  const int tiles = tiles_of(len, TK);
+  int walked = len;
+  if constexpr (WIN) {
+    const Walk w = window_walk<TK>(p, len);
+    walked = w.len - w.skip;
+  }
+  const int tiles = tiles_of(walked, TK);
   uint8_t* const lds = reinterpret_cast<uint8_t*>(cum);
   const int per_wave = short_lds_per_wave(HD, p.G, FUSED);
   // (whole tiles, evenly over the workgroups, then over the wavefronts: a wavefront's tiles follow one another)
   const int wb = (int)((int64_t)tiles * split / p.splits), wn = (int)((int64_t)tiles * (split + 1) / p.splits) - wb;
   const int tb = wb + wn * wave / kShortWaves, te = wb + wn * (wave + 1) / kShortWaves;
   if (te > tb) {
-    decode_segment<HD, HD, NT, FP8, F16, FUSED, true>(p, r, row, h, hq0, gq, len, tb * TK, min(te * TK, len), false, te == tiles,
+    decode_segment<HD, HD, NT, FP8, F16, FUSED, true, WIN>(p, r, row, h, hq0, gq, len, tb * TK, min(te * TK, walked), false, te == tiles,
                                                       0, lane, lds + wave * per_wave);
   } else if (lane < gq) {
     *reinterpret_cast<float2*>(lds + wave * per_wave + 4 * (lane * PITCH + HD)) = make_float2(-INFINITY, 0.f);
@@ -1991,7 +2115,7 @@ int mi::launch_paged_decode(
     void* out, int64_t o_stride_tok, int64_t o_stride_head, void* workspace, int64_t workspace_bytes,
     int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t chunk_tokens,
     int32_t split_tokens, float softmax_scale, int32_t kv_dtype, const float* k_scales,
-    const float* v_scales, int32_t dtype, const MiTuning& tune, void* stream, const FusedStepArgs* fused) {
+    const float* v_scales, int32_t dtype, const MiTuning& tune, void* stream, const FusedStepArgs* fused, const WindowArgs* win) {
   if (R == 0) return MI_OK;
   if (dtype != MI_DTYPE_BF16 && dtype != MI_DTYPE_FP16)
     return mi_fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_attention: dtype must be MI_DTYPE_BF16 or MI_DTYPE_FP16");
@@ -2043,7 +2167,7 @@ int mi::launch_paged_decode(
           kv_stride_tok, kv_stride_head, block_table + (int64_t)r0 * bt_stride, bt_stride, kv_lens + r0,
           cu_seqlens_q ? cu_seqlens_q + r0 : nullptr, (uint16_t*)out + row0 * o_stride_tok, o_stride_tok, o_stride_head,
           workspace, workspace_bytes, n, Hq, Hkv, head_dim, chunk_tokens, split_tokens, softmax_scale, kv_dtype, k_scales,
-          v_scales, dtype, tune, stream, fused ? &fs : nullptr);
+          v_scales, dtype, tune, stream, fused ? &fs : nullptr, win);
       if (rc != MI_OK) return rc;
     }
     return MI_OK;
@@ -2055,6 +2179,7 @@ int mi::launch_paged_decode(
   // 16-token sub-tiles per loop iteration (0 = automatic).
   int nt = tune.decode_tile_subtiles;
   if (nt != 1 && nt != 2 && nt != 4) nt = kv_dtype == MI_KV_FP8_E4M3 ? 4 : 2;
+  if (win && kv_dtype != MI_KV_FP8_E4M3 && nt == 4) nt = 2;
   if (head_dim == 256) nt = 1;                 // (registers: 64 accumulators + 32 each for queries, keys, values)
   else if (head_dim == 192 && nt > 2) nt = 2;
   if (fused) nt = kv_dtype == MI_KV_FP8_E4M3 ? MI_FUSED_FP8_NT : 1;  // (the prologue's registers on top of two 16-bit sub-tiles in flight would spill)
@@ -2078,6 +2203,9 @@ int mi::launch_paged_decode(
   p.min_span_tiles = split_tokens > 0 ? (split_tokens + tk - 1) / tk : 0;
   p.grid = grid_x;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  if (win) {
+    p.window = win->window; p.sinks = win->sinks; p.n_chunks = win->n_chunks; p.max_len = win->max_len;
+  }
   if (fused) {
     p.q_gst = fused->q_stride_group;
     p.nk = (const uint16_t*)fused->k_new; p.nk_st = fused->k_stride_tok; p.nk_hst = fused->k_stride_head;
@@ -2110,7 +2238,8 @@ int mi::launch_paged_decode(
   hipEvent_t ev_a, ev_b;
   const bool timed = mi_profile_next(&ev_a, &ev_b);
   if (timed) (void)hipEventRecord(ev_a, st);
-  p.splits = short_splits(R, waves, head_dim, bt_stride * chunk_tokens, esz, chunk_tokens, grid_x, tune, split_tokens);
+  const int64_t most = win ? window_keys(*win, win->max_len, 0) : bt_stride * chunk_tokens;
+  p.splits = short_splits(R, waves, head_dim, most, esz, chunk_tokens, grid_x, tune, split_tokens);
   if (p.splits > 0) {
     const int busy = R * waves * p.splits;
     const dim3 sgrid(p.next_w && fused && busy < grid_x ? grid_x : busy), sblock(64 * kShortWaves);
@@ -2120,7 +2249,18 @@ int mi::launch_paged_decode(
       if (f16) hipLaunchKernelGGL((decode_short_kernel<HD_, NT_, FP8_, true, FUSED_>), sgrid, sblock, slds, st, p);     \
       else hipLaunchKernelGGL((decode_short_kernel<HD_, NT_, FP8_, false, FUSED_>), sgrid, sblock, slds, st, p);        \
     } while (0)
-    if (fused && kv_dtype == MI_KV_FP8_E4M3) MI_LAUNCH_SHORT(128, kShortTile, true, true);
+#define MI_LAUNCH_SHORT_WINDOW(HD_, FP8_)                                                                               \
+    do {                                                                                                                \
+      if (f16) hipLaunchKernelGGL((decode_short_kernel<HD_, kShortTile, FP8_, true, false, true>), sgrid, sblock, slds, st, p);  \
+      else hipLaunchKernelGGL((decode_short_kernel<HD_, kShortTile, FP8_, false, false, true>), sgrid, sblock, slds, st, p);     \
+    } while (0)
+    if (win) {
+      if (kv_dtype == MI_KV_FP8_E4M3 && head_dim == 128) MI_LAUNCH_SHORT_WINDOW(128, true);
+      else if (kv_dtype == MI_KV_FP8_E4M3) MI_LAUNCH_SHORT_WINDOW(64, true);
+      else if (head_dim == 128) MI_LAUNCH_SHORT_WINDOW(128, false);
+      else MI_LAUNCH_SHORT_WINDOW(64, false);
+    }
+    else if (fused && kv_dtype == MI_KV_FP8_E4M3) MI_LAUNCH_SHORT(128, kShortTile, true, true);
     else if (fused && head_dim == 128) MI_LAUNCH_SHORT(128, kShortTile, false, true);
     else if (fused) MI_LAUNCH_SHORT(64, kShortTile, false, true);
     else if (kv_dtype == MI_KV_FP8_E4M3 && head_dim == 128) MI_LAUNCH_SHORT(128, kShortTile, true, false);
@@ -2128,6 +2268,7 @@ int mi::launch_paged_decode(
     else if (head_dim == 128) MI_LAUNCH_SHORT(128, kShortTile, false, false);
     else MI_LAUNCH_SHORT(64, kShortTile, false, false);
 #undef MI_LAUNCH_SHORT
+#undef MI_LAUNCH_SHORT_WINDOW
     if (timed) (void)hipEventRecord(ev_b, st);
     if (p.splits > 1) {
       const dim3 mgrid((Hq * head_dim / 4 + 255) / 256, R);
@@ -2161,7 +2302,34 @@ int mi::launch_paged_decode(
   } while (0)
 #define MI_LAUNCH_STEP(HD_, F16_) hipLaunchKernelGGL((decode_step_stream_kernel<HD_, 1, F16_>), grid, block, lds, st, p)
 #define MI_LAUNCH_STEP_WIDE(HD_, F16_) hipLaunchKernelGGL((decode_step_stream_kernel<HD_, 1, F16_, 2>), grid, block, lds, st, p)
-  if (fused && kv_dtype == MI_KV_FP8_E4M3 && f16)
+  // with a window: the default number of wavefronts per SIMD, sub-tiles as the chunk size allows
+#define MI_LAUNCH_WINDOW(HD_, NT_, FP8_)                                                                               \
+  do {                                                                                                                 \
+    constexpr int minw_ = HD_ > 128 || NT_ == 4 ? 2 : 3;                                                               \
+    if (f16) hipLaunchKernelGGL((paged_decode_stream_kernel<HD_, NT_, FP8_, minw_, true, true>), grid, block, lds, st, p);   \
+    else hipLaunchKernelGGL((paged_decode_stream_kernel<HD_, NT_, FP8_, minw_, false, true>), grid, block, lds, st, p);      \
+  } while (0)
+#define MI_LAUNCH_WINDOW_NT(HD_)                                                                                       \
+  do {                                                                                                                 \
+    if (nt == 1) MI_LAUNCH_WINDOW(HD_, 1, false);                                                                      \
+    else MI_LAUNCH_WINDOW(HD_, 2, false);                                                                              \
+  } while (0)
+#define MI_LAUNCH_WINDOW_FP8(HD_)                                                                                      \
+  do {                                                                                                                 \
+    if (nt == 4) MI_LAUNCH_WINDOW(HD_, 4, true);                                                                       \
+    else if (nt == 2) MI_LAUNCH_WINDOW(HD_, 2, true);                                                                  \
+    else MI_LAUNCH_WINDOW(HD_, 1, true);                                                                               \
+  } while (0)
+  if (win) {
+    if (kv_dtype == MI_KV_FP8_E4M3 && head_dim == 64) MI_LAUNCH_WINDOW_FP8(64);
+    else if (kv_dtype == MI_KV_FP8_E4M3) MI_LAUNCH_WINDOW_FP8(128);
+    else if (head_dim == 64) MI_LAUNCH_WINDOW_NT(64);
+    else if (head_dim == 96) MI_LAUNCH_WINDOW_NT(96);
+    else if (head_dim == 128) MI_LAUNCH_WINDOW_NT(128);
+    else if (head_dim == 192) MI_LAUNCH_WINDOW_NT(192);
+    else MI_LAUNCH_WINDOW(256, 1, false);
+  }
+  else if (fused && kv_dtype == MI_KV_FP8_E4M3 && f16)
     hipLaunchKernelGGL((decode_step_stream_kernel<128, MI_FUSED_FP8_NT, true, 3, true>), grid, block, lds, st, p);
   else if (fused && kv_dtype == MI_KV_FP8_E4M3)
     hipLaunchKernelGGL((decode_step_stream_kernel<128, MI_FUSED_FP8_NT, false, 3, true>), grid, block, lds, st, p);
@@ -2193,6 +2361,9 @@ int mi::launch_paged_decode(
 #undef MI_LAUNCH_DECODE_WIDE
 #undef MI_LAUNCH_STEP
 #undef MI_LAUNCH_STEP_WIDE
+#undef MI_LAUNCH_WINDOW
+#undef MI_LAUNCH_WINDOW_NT
+#undef MI_LAUNCH_WINDOW_FP8
   if (timed) (void)hipEventRecord(ev_b, st);
   launch_merge(p, p.grid, R, Hq, head_dim, f16, st);
   return mi_check_launch("mi_paged_decode_attention");
@@ -2214,6 +2385,27 @@ extern "C" int mi_paged_decode_attention(
                              kv_stride_head, block_table, bt_stride, kv_lens, nullptr, out, o_stride_tok,
                              o_stride_head, workspace, workspace_bytes, R, Hq, Hkv, head_dim, chunk_tokens,
                              split_tokens, softmax_scale, kv_dtype, k_scales, v_scales, dtype, tune, stream);
+}
+
+extern "C" int mi_paged_window_decode_attention(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache, const void* v_cache,
+    int64_t kv_stride_chunk, int64_t kv_stride_tok, int64_t kv_stride_head, int32_t n_chunks, int32_t kv_dtype,
+    const float* k_scales, const float* v_scales, const int32_t* block_table, int64_t bt_stride, int32_t bt_columns,
+    const int32_t* kv_lens, int32_t window, int32_t sinks, void* out, int64_t o_stride_tok, int64_t o_stride_head,
+    void* workspace, int64_t workspace_bytes, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t chunk_tokens,
+    float softmax_scale, int32_t dtype, const MiTuning* tuning, void* stream) {
+  if (R == 0) return MI_OK;
+  MiTuning tune;
+  int rc = mi_resolve_tuning(tuning, &tune, "mi_paged_window_decode_attention");
+  if (rc != MI_OK) return rc;
+  WindowArgs w;
+  rc = check_window(window, sinks, n_chunks, bt_columns, bt_stride, R, chunk_tokens, "mi_paged_window_decode_attention", &w);
+  if (rc != MI_OK) return rc;
+  if (!(softmax_scale > 0.f)) return mi_fail(MI_ERR_SHAPE, "mi_paged_window_decode_attention: softmax_scale must be positive");
+  return launch_paged_decode(q, q_stride_tok, q_stride_head, k_cache, v_cache, kv_stride_chunk, kv_stride_tok, kv_stride_head,
+                             block_table, bt_stride, kv_lens, nullptr, out, o_stride_tok, o_stride_head, workspace,
+                             workspace_bytes, R, Hq, Hkv, head_dim, chunk_tokens, 0, softmax_scale, kv_dtype, k_scales, v_scales,
+                             dtype, tune, stream, nullptr, &w);
 }
 
 static int decode_step_entry(

@@ -18,13 +18,16 @@
 #include "mi_common.h"
 #include "mi_capi_internal.h"
 #include "paged_prefill_params.h"
+#include "paged_prefill_remake.h"
 
 namespace mi {
 
 // NQ = 16-row tiles per wave, WAVES wavefronts per workgroup (256 rows for the narrow heads, 128 at width 256).
 // HDK = width of queries and keys, HDV = width of values and of the output (they differ for the
 // decompressed caches of multi-latent attention: 192 / 128); the value cache has its own strides.
-template <int HDK, int HDV, int NT, int NQ, bool F16, int WAVES = 16 / NQ>
+// WIN: a row sees the last `window` keys up to its own and the first `sinks` (see PrefillParams).  The walk goes by tiles of
+// 16 NT keys: those of the sinks, then those from the wavefront's first row's window on.
+template <int HDK, int HDV, int NT, int NQ, bool F16, int WAVES = 16 / NQ, bool WIN = false>
 __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams p) {
   constexpr int KS = HDK / 32;
   constexpr int DV = HDV / 16;
@@ -65,7 +68,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams
   const int q0 = (sb - (q_begin / SBQ + r)) * SBQ + wave * BQ;  // first query of this wave
   if (q0 >= Lq) return;
   if (p.skip_single && Lq == 1) return;
-  const int Lk = p.lens[r];
+  const int Lk = WIN ? min(p.lens[r], p.max_len) : p.lens[r];
   const int shift = Lk - Lq;  // key position of query 0
   const int nq = min(BQ, Lq - q0);
   const int kend = min(Lk, shift + q0 + nq);  // keys [0, kend) are visible to some row
@@ -118,29 +121,42 @@ __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams
     return;
   }
 
+  // WIN: tiles of the walk, and where the walk's next token T lies
+  constexpr int TILE = 16 * NT;
+  WindowTiles wt = {};
+  if constexpr (WIN) wt = window_tiles(p.window, p.sinks, TILE, shift + q0);
+  const int walk_end = WIN ? kend - wt.skip * TILE : kend;
+  auto position = [&](int T) { return WIN && T >= wt.ns * TILE ? T + wt.skip * TILE : T; };
+
   // K / V staging registers of one tile of 16*NT keys; the loop is software pipelined on them
   // (K of the next tile is requested once all scores of this one exist, V once P.V is done).
   uint4 kf[NT][KS];
   uint32_t vf[NT][4][VD];
-  auto load_k = [&](int T) {
+  auto chunk_entry = [&](int ci) {
+    const int pc = p.bt[(int64_t)r * p.bt_stride + ci];
+    return WIN ? clamp_chunk(pc, p.n_chunks) : pc;
+  };
+  auto load_k = [&](int walked) {
+    const int T = position(walked);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       const int T0 = T + 16 * u;
       const int tu = min(T0, last);
       const int ci = (int)(((uint64_t)(uint32_t)tu * p.chunk_magic) >> 40);
-      const int pc = p.bt[(int64_t)r * p.bt_stride + ci];
+      const int pc = chunk_entry(ci);
       const uint8_t* krow = kbase + (int64_t)pc * chunk_bytes + (min(T0 + m16, last) - ci * p.chunk) * tok_bytes;
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) kf[u][kk] = ld16(krow + (32 * kk + 8 * g) * 2);
     }
   };
-  auto load_v = [&](int T) {
+  auto load_v = [&](int walked) {
+    const int T = position(walked);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       const int T0 = T + 16 * u;
       const int tu = min(T0, last);
       const int ci = (int)(((uint64_t)(uint32_t)tu * p.chunk_magic) >> 40);
-      const int pc = p.bt[(int64_t)r * p.bt_stride + ci];
+      const int pc = chunk_entry(ci);
       const uint8_t* vc = vbase + (int64_t)pc * v_chunk_bytes;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -158,7 +174,9 @@ __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams
   load_k(0);
   load_v(0);
   __builtin_amdgcn_sched_barrier(0);
-  for (int T = 0; T < kend; T += 16 * NT) {
+  const int gone_wave = full_until + nq - 1 - p.window;   // WIN: keys up to here are behind some row's window
+  for (int walked = 0; walked < walk_end; walked += TILE) {
+    const int T = position(walked);
     // ---- S^T = K Q^T for every 16-row tile of the wave (raw, unscaled) ----------------
     f32x4_t s[NQ][NT];
 #pragma unroll
@@ -173,11 +191,11 @@ __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    load_k(T + 16 * NT);
+    load_k(walked + TILE);
     __builtin_amdgcn_sched_barrier(0);
 
     // ---- online softmax per 16-row tile ----------------------------------------------
-    const bool need_mask = T + 16 * NT - 1 > full_until;  // wave-uniform
+    const bool need_mask = T + TILE - 1 > full_until || (WIN && T <= gone_wave && T + TILE > p.sinks);  // wave-uniform
     uint2 pf[NQ][NT];
 #pragma unroll
     for (int nt = 0; nt < NQ; ++nt) {
@@ -189,7 +207,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams
           const int tok0 = T + 16 * u + 4 * g;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (tok0 + i > qpos[nt]) s[nt][u][i] = -INFINITY;
+            if (tok0 + i > qpos[nt] || (WIN && tok0 + i <= qpos[nt] - p.window && tok0 + i >= p.sinks)) s[nt][u][i] = -INFINITY;
         }
         tmax = fmaxf(fmaxf(fmaxf(s[nt][u][0], s[nt][u][1]), fmaxf(s[nt][u][2], s[nt][u][3])), tmax);
       }
@@ -264,7 +282,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    load_v(T + 16 * NT);
+    load_v(walked + TILE);
     __builtin_amdgcn_sched_barrier(0);
   }
 
@@ -275,7 +293,11 @@ __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams
     const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
     const int n = 16 * nt + m16;
     const int qi = (n * g_magic) >> 16, u = n - qi * G;  // n / G, n % G
-    if (qi < nq) {
+    bool fine = true;
+    if constexpr (WIN)
+      fine = finite_or_remade<HDV, TILE, false, F16>(p, acc[nt], l_tot, nt, nq, G, g_magic, r, q_begin + q0, h, hq0, shift + q0, Lk, wt, 0,
+                                                     (walk_end + TILE - 1) / TILE, -1);
+    if (qi < nq && fine) {
       uint16_t* o = p.out + (int64_t)(q_begin + q0 + qi) * p.o_st + (int64_t)(hq0 + u) * p.o_sh + 4 * DV * g;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -325,7 +347,8 @@ template <int HD> constexpr int pp_tile() { return HD == 256 ? 32 : 64; }
 // ordinary kernel carries no tile offsets).
 // HD = width of values and output, HDK = width of queries and keys: equal, or 192 / 128 for the decompressed
 // caches of multi-latent attention, whose value cache has its own strides.
-template <bool STAGGER, bool FP8, bool SPLIT, int HD, int HDK, bool F16>
+// WIN: a row sees the last `window` keys up to its own and the first `sinks` (see PrefillParams), as in the one-stream kernel.
+template <bool STAGGER, bool FP8, bool SPLIT, int HD, int HDK, bool F16, bool WIN = false>
 __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams p) {
   static_assert((HD == 128 && HDK == 128) || (HD == 64 && HDK == 64) ||
                     ((HD == 96 || HD == 192 || HD == 256) && HDK == HD && !FP8) || (HD == 128 && HDK == 192 && !FP8),
@@ -378,11 +401,17 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
 
   QueryBlock qb;
   if (!find_query_block(p, SBQ, rank, (int)(gridDim.x / HV), &qb)) return;  // workgroup-uniform
-  const int r = qb.r, q_begin = qb.q_begin, Lq = qb.Lq, Lk = qb.Lk, q0_wg = qb.q0;
+  const int r = qb.r, q_begin = qb.q_begin, Lq = qb.Lq, Lk = WIN ? min(qb.Lk, p.max_len) : qb.Lk, q0_wg = qb.q0;
   const int shift = Lk - Lq;
   const int last = Lk - 1;
   const int kend_wg = min(Lk, shift + min(q0_wg + SBQ, Lq));
-  const int ntl_all = (kend_wg + kPPTile - 1) / kPPTile;  // staged tiles the rows of this workgroup can see
+  WindowTiles wt = {};
+  if constexpr (WIN) {
+    wt = window_tiles(p.window, p.sinks, kPPTile, shift + q0_wg);
+    wt.ns = __builtin_amdgcn_readfirstlane(wt.ns);
+    wt.skip = __builtin_amdgcn_readfirstlane(wt.skip);
+  }
+  const int ntl_all = (kend_wg + kPPTile - 1) / kPPTile - wt.skip;  // staged tiles the rows of this workgroup can see
   // this workgroup's share of them: tiles [tb, tb + ntl)
   const int n_split = SPLIT ? (int)gridDim.y : 1, split = SPLIT ? (int)blockIdx.y : 0;
   const int tb = SPLIT ? (int)((int64_t)ntl_all * split / n_split) : 0;
@@ -474,12 +503,15 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
     auto cursor_at = [&](int t) {
       Cursor c;
       c.tile = min(t, te - 1);
-      c.ci = c.tile / tiles_per_chunk;
-      c.tin = c.tile - c.ci * tiles_per_chunk;
-      c.room = (last - c.tile * kPPTile) * tok_bytes;
+      const int real = WIN ? wt.real(c.tile) : c.tile;
+      c.ci = real / tiles_per_chunk;
+      c.tin = real - c.ci * tiles_per_chunk;
+      c.room = (WIN ? min(last - real * kPPTile, kPPTile) : last - real * kPPTile) * tok_bytes;
       c.room_v = MLA ? (last - c.tile * kPPTile) * v_tok_bytes : 0;
       return c;
     };
+    // WIN: where the walk goes on behind the sinks
+    const int far_ci = WIN ? (wt.ns + wt.skip) / tiles_per_chunk : 0, far_tin = WIN ? wt.ns + wt.skip - far_ci * tiles_per_chunk : 0;
     auto cursor_next = [&](Cursor& c) {  // one tile forward, sticking to the last tile
       const bool adv = c.tile + 1 < te;
       const bool wrap = adv && (c.tin + 1 == tiles_per_chunk);
@@ -488,6 +520,13 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
       if constexpr (MLA) c.room_v -= adv ? v_tile_bytes : 0;
       c.tin = wrap ? 0 : c.tin + (adv ? 1 : 0);
       c.ci += wrap ? 1 : 0;
+      if constexpr (WIN) {
+        const bool far = adv && c.tile == wt.ns;
+        c.tin = far ? far_tin : c.tin;
+        c.ci = far ? far_ci : c.ci;
+        // (a tile's rows and no more: a walk that jumps can be longer than 2^31 bytes)
+        c.room = min(last - wt.real(c.tile) * kPPTile, kPPTile) * tok_bytes;
+      }
     };
     // fp8: the scales of a tile's chunk, requested when the tile's loads are issued
     auto tile_scales = [&](int pc) {
@@ -498,7 +537,8 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
     };
     // byte offset of the cursor's tile inside a cache, given its physical chunk
     auto tile_offset = [&](const Cursor& c, int pc_lane) -> int64_t {
-      const int pc = __builtin_amdgcn_readfirstlane(pc_lane);
+      int pc = __builtin_amdgcn_readfirstlane(pc_lane);
+      if constexpr (WIN) pc = clamp_chunk(pc, p.n_chunks);
       tile_scales(pc);
       return (int64_t)pc * chunk_bytes + (int64_t)c.tin * tile_bytes;
     };
@@ -573,6 +613,7 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
       if constexpr (NPASS == 2) *reinterpret_cast<uint4*>(dst + RPP * kVPitch) = lds_piece(vreg[1], vsc_staged);
     };
 
+    const int gone_wave = WIN ? full_until + max(nq, 1) - 1 - p.window : 0;   // keys up to here are behind some row's window
     const float scale = p.scale_log2;
     const float win = (F16 ? 8.f : 30.f) / scale;  // probabilities stay below 2^8 (fp16 operands) or 2^30
     const uint4 ones = make_uint4(ones2<F16>(), ones2<F16>(), ones2<F16>(), ones2<F16>());
@@ -789,8 +830,8 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
     };
     // ---- online softmax of tile t: s -> pf, rescale of the accumulators when the reference moved ----
     auto softmax = [&](int t) {  // t counts from this workgroup's first tile
-      const int T = (tb + t) * kPPTile;
-      const bool need_mask = T + kPPTile - 1 > full_until;
+      const int T = (WIN ? wt.real(tb + t) : tb + t) * kPPTile;
+      const bool need_mask = T + kPPTile - 1 > full_until || (WIN && T <= gone_wave && T + kPPTile > p.sinks);
 #pragma unroll
       for (int nt = 0; nt < NQ; ++nt) {
         if (need_mask) {
@@ -803,7 +844,7 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
             const int tok0 = Tm + 16 * u + 4 * g;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (tok0 + i > qpos[nt]) s[nt][u][i] = -INFINITY;
+              if (tok0 + i > qpos[nt] || (WIN && tok0 + i <= qpos[nt] - p.window && tok0 + i >= p.sinks)) s[nt][u][i] = -INFINITY;
           }
         }
         float tmax = fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), s[nt][0][2]);
@@ -907,7 +948,11 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
     const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
     const int n = 16 * nt + m16;
     const int qi = (n * g_magic) >> 16, u = n - qi * G;  // n / G, n % G
-    if (qi < nq) {
+    bool fine = true;
+    if constexpr (WIN)
+      fine = finite_or_remade<HD, kPPTile, FP8, F16>(p, acc[nt], l_tot, nt, nq, G, g_magic, r, q_begin + q0, h, hq0, shift + q0, Lk, wt, tb, te,
+                                                     SPLIT ? split : -1);
+    if (qi < nq && fine) {
       if (!SPLIT) {
         uint16_t* o = p.out + (int64_t)(q_begin + q0 + qi) * p.o_st + (int64_t)(hq0 + u) * p.o_sh + 4 * g;
 #pragma unroll
@@ -1065,6 +1110,38 @@ static int prefill_woven_waves(int head_dim, bool fp8, bool raw, int n_split, in
     else hipLaunchKernelGGL((paged_prefill_pp_kernel<false, FP8_, false, HD_, HDK_, F16_>), lgrid, dim3(512), 0, st, p);                      \
   } while (0)
 
+// Keys that a workgroup of the tile kernels walks at most, with a window: what its up to 256 rows see.
+static int window_walk(const WindowArgs& w, int max_kv_len) { return window_keys(w, max_kv_len > 0 ? max_kv_len : w.max_len, 256); }
+
+// The kernels of calls with a window other than the one-stream kernel (which see).
+static void launch_window_pp(const PrefillParams& p, dim3 grid, int head_dim, bool f16, hipStream_t st) {
+#define MI_WIN_PP(HD_, F16_)                                                                                                  \
+  do {                                                                                                                        \
+    if (grid.y > 1) hipLaunchKernelGGL((paged_prefill_pp_kernel<true, false, true, HD_, HD_, F16_, true>), grid, dim3(512), 0, st, p); \
+    else hipLaunchKernelGGL((paged_prefill_pp_kernel<true, false, false, HD_, HD_, F16_, true>), grid, dim3(512), 0, st, p);  \
+  } while (0)
+  if (head_dim == 96 && f16) MI_WIN_PP(96, true);
+  else if (head_dim == 96) MI_WIN_PP(96, false);
+  else if (head_dim == 192 && f16) MI_WIN_PP(192, true);
+  else if (head_dim == 192) MI_WIN_PP(192, false);
+  else if (f16) MI_WIN_PP(256, true);
+  else MI_WIN_PP(256, false);
+#undef MI_WIN_PP
+}
+static void launch_window_registers(const PrefillParams& p, dim3 grid, int head_dim, bool f16, hipStream_t st) {
+#define MI_WIN_REGISTERS(HD_, NT_, NQ_)                                                                                       \
+  do {                                                                                                                        \
+    if (f16) hipLaunchKernelGGL((paged_prefill_kernel<HD_, HD_, NT_, NQ_, true, 8, true>), grid, dim3(512), 0, st, p);        \
+    else hipLaunchKernelGGL((paged_prefill_kernel<HD_, HD_, NT_, NQ_, false, 8, true>), grid, dim3(512), 0, st, p);           \
+  } while (0)
+  if (head_dim == 64) MI_WIN_REGISTERS(64, 2, 2);
+  else if (head_dim == 96) MI_WIN_REGISTERS(96, 2, 2);
+  else if (head_dim == 128) MI_WIN_REGISTERS(128, 2, 2);
+  else if (head_dim == 192) MI_WIN_REGISTERS(192, 1, 2);
+  else MI_WIN_REGISTERS(256, 1, 1);
+#undef MI_WIN_REGISTERS
+}
+
 // queries of the QKV projection's output (see PrefillParams)
 struct RawQueries {
   int64_t group_stride;
@@ -1081,7 +1158,7 @@ static int launch_paged_prefill(
     void* workspace, int64_t workspace_bytes, int32_t T, int32_t R, int32_t Hq, int32_t Hkv,
     int32_t head_dim, int32_t chunk_tokens, int32_t max_kv_len, int32_t split_tokens, float softmax_scale,
     int32_t kv_dtype, const float* k_scales, const float* v_scales, int32_t dtype, const MiTuning* tuning,
-    void* stream, bool one_row_requests = true, const RawQueries* raw = nullptr) {
+    void* stream, bool one_row_requests = true, const RawQueries* raw = nullptr, const WindowArgs* win = nullptr) {
   const bool fp8 = kv_dtype == MI_KV_FP8_E4M3;
   if (T == 0 || R == 0) return MI_OK;
   MiTuning tune;
@@ -1147,6 +1224,12 @@ static int launch_paged_prefill(
   p.eps = raw ? raw->eps : 0.f;
   p.norm = raw ? raw->norm : MI_NORM_NONE;
   p.interleaved = raw ? raw->interleaved : 0;
+  p.window = win ? win->window : 0;
+  p.sinks = win ? win->sinks : 0;
+  p.n_chunks = win ? win->n_chunks : 0;
+  p.max_len = win ? win->max_len : 0;
+  // (a workgroup with a window has at most so many keys to walk)
+  if (win) max_kv_len = window_walk(*win, max_kv_len);
   if (raw && !(two_phase && tune.prefill_two_phase == 3 && (head_dim == 64 || head_dim == 128)))
     return mi_fail(MI_ERR_UNSUPPORTED, "mi_qkv_prefill_attention: head_dim 64 or 128 and a chunk size that is a multiple of 64");
 
@@ -1162,7 +1245,7 @@ static int launch_paged_prefill(
   if (two_phase) {
     // head_dim 64 and 128: the one-stream tile kernel (measured at every size tried the faster of the two there: 1-3 %
     // at 128, 8-14 % at 64); the knob asks for the two-phase one
-    const bool woven = tune.prefill_two_phase == 3 && (head_dim == 64 || head_dim == 128);
+    const bool woven = (tune.prefill_two_phase == 3 || win) && (head_dim == 64 || head_dim == 128);   // (with a window: no other)
     const bool stagger = tune.prefill_two_phase != 2;
     // key ranges per request (with a workspace only): partials behind the decode part's scratch
     int n_split = 1;
@@ -1186,6 +1269,7 @@ static int launch_paged_prefill(
     const bool timed = mi_profile_next(&ev_a, &ev_b);
     if (timed) (void)hipEventRecord(ev_a, st);
     if (woven) launch_prefill_woven(p, lgrid, head_dim, fp8, f16, waves, st);
+    else if (win) launch_window_pp(p, lgrid, head_dim, f16, st);
     else if (fp8 && head_dim == 64 && f16) MI_PP_LAUNCH(true, 64, 64, true);
     else if (fp8 && head_dim == 64) MI_PP_LAUNCH(true, 64, 64, false);
     else if (fp8 && f16) MI_PP_LAUNCH(true, 128, 128, true);
@@ -1207,7 +1291,7 @@ static int launch_paged_prefill(
   } else {
     // register-only kernel: any chunk size that is a multiple of 16; 16 or 32 keys per iteration
     // (wide heads: fewer rows per wavefront and keys per iteration, so that accumulators and fragments fit)
-    const int nq = head_dim == 256 ? 1 : head_dim == 192 ? 2 : tune.prefill_row_tiles == 4 ? 4 : 2;
+    const int nq = head_dim == 256 ? 1 : head_dim == 192 ? 2 : tune.prefill_row_tiles == 4 && !win ? 4 : 2;
     const int waves = head_dim == 256 ? 8 : 16 / nq;
     const int sbq = waves * ((16 * nq) / Gw);  // query tokens per workgroup: whole tokens in each wavefront's rows
     dim3 grid((T + sbq - 1) / sbq + R, Hkv * parts), block(64 * waves);
@@ -1222,7 +1306,8 @@ static int launch_paged_prefill(
     else if (nt == 1) hipLaunchKernelGGL((paged_prefill_kernel<HD_, HD_, 1, 2, F16_>), grid, block, 0, st, p);        \
     else hipLaunchKernelGGL((paged_prefill_kernel<HD_, HD_, 2, 2, F16_>), grid, block, 0, st, p);                     \
   } while (0)
-    if (head_dim == 128 && f16) MI_LAUNCH_PREFILL(128, true);
+    if (win) launch_window_registers(p, grid, head_dim, f16, st);
+    else if (head_dim == 128 && f16) MI_LAUNCH_PREFILL(128, true);
     else if (head_dim == 128) MI_LAUNCH_PREFILL(128, false);
     else if (head_dim == 64 && f16) MI_LAUNCH_PREFILL(64, true);
     else if (head_dim == 64) MI_LAUNCH_PREFILL(64, false);
@@ -1240,7 +1325,33 @@ static int launch_paged_prefill(
   return launch_paged_decode(q, q_stride_tok, q_stride_head, k_cache, v_cache, kv_stride_chunk, kv_stride_tok,
                              kv_stride_head, block_table, bt_stride, kv_lens, cu_seqlens_q, out, o_stride_tok,
                              o_stride_head, workspace, workspace_bytes, R, Hq, Hkv, head_dim, chunk_tokens,
-                             split_tokens, softmax_scale, kv_dtype, k_scales, v_scales, dtype, tune, stream);
+                             split_tokens, softmax_scale, kv_dtype, k_scales, v_scales, dtype, tune, stream, nullptr, win);
+}
+
+extern "C" int64_t mi_window_prefill_workspace_bytes(int32_t T, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t max_kv_len,
+                                                     int32_t window, int32_t sinks, const MiTuning* tuning) {
+  const WindowArgs w = {window < kMostWindow ? window : kMostWindow, sinks < kMostWindow ? sinks : kMostWindow, 0, 0x7fffffff};
+  return mi_prefill_workspace_bytes(T, R, Hq, Hkv, head_dim, window_walk(w, max_kv_len), 0, tuning);
+}
+
+extern "C" int mi_paged_window_prefill_attention(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache, const void* v_cache,
+    int64_t kv_stride_chunk, int64_t kv_stride_tok, int64_t kv_stride_head, int32_t n_chunks, int32_t kv_dtype,
+    const float* k_scales, const float* v_scales, const int32_t* block_table, int64_t bt_stride, int32_t bt_columns,
+    const int32_t* cu_seqlens_q, const int32_t* kv_lens, int32_t window, int32_t sinks, void* out, int64_t o_stride_tok,
+    int64_t o_stride_head, void* workspace, int64_t workspace_bytes, int32_t T, int32_t R, int32_t Hq, int32_t Hkv,
+    int32_t head_dim, int32_t chunk_tokens, int32_t max_kv_len, int32_t one_row_requests, float softmax_scale,
+    int32_t dtype, const MiTuning* tuning, void* stream) {
+  if (T == 0 || R == 0) return MI_OK;
+  WindowArgs w;
+  const int rc = check_window(window, sinks, n_chunks, bt_columns, bt_stride, R, chunk_tokens, "mi_paged_window_prefill_attention", &w);
+  if (rc != MI_OK) return rc;
+  if (tuning && tuning->prefill_two_phase > 0 && tuning->prefill_two_phase < 3)
+    return mi_fail(MI_ERR_UNSUPPORTED, "mi_paged_window_prefill_attention: prefill_two_phase 1 and 2 have no kernel with a window");
+  return launch_paged_prefill(q, q_stride_tok, q_stride_head, k_cache, v_cache, kv_stride_chunk, kv_stride_tok, kv_stride_head,
+                              block_table, bt_stride, cu_seqlens_q, kv_lens, out, o_stride_tok, o_stride_head, workspace,
+                              workspace_bytes, T, R, Hq, Hkv, head_dim, chunk_tokens, max_kv_len, 0, softmax_scale, kv_dtype,
+                              k_scales, v_scales, dtype, tuning, stream, one_row_requests != 0, nullptr, &w);
 }
 
 extern "C" int mi_paged_prefill_attention(

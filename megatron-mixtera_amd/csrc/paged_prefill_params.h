@@ -40,6 +40,10 @@ struct PrefillParams {
   const uint16_t* q_w;     // RMS norm weight or null
   float eps;
   int32_t norm, interleaved;
+  // Windowed kernels only: a row at position P sees key k <= P where k > P - window or k < sinks (both at most 2^30).
+  int32_t window, sinks;
+  int32_t n_chunks;        // of the cache: table entries are kept below it
+  int32_t max_len;         // keys that the block table has room for: lengths are kept below it
 };
 
 // The query heads one workgroup serves: with at most 16 query heads per KV head, all G of KV head `hv`; with more,
@@ -63,6 +67,21 @@ static __device__ __forceinline__ HeadSlice head_slice(const PrefillParams& p, i
   }
   return s;
 }
+
+// The key tiles that a workgroup with a window walks: those of the sinks, then those from its first row's window on.  Tile v
+// of the walk is tile real(v) of the request; what lies between is not touched, block table included.
+struct WindowTiles {
+  int ns, skip;   // tiles of the sinks, tiles passed over behind them
+  __device__ __forceinline__ int real(int v) const { return v < ns ? v : v + skip; }
+  __device__ __forceinline__ int walk(int t) const { return t < ns ? t : max(ns, t - skip); }   // the first tile of the walk from tile t on
+};
+static __device__ __forceinline__ WindowTiles window_tiles(int window, int sinks, int tile, int first_pos) {
+  WindowTiles w;
+  w.ns = (sinks + tile - 1) / tile;
+  w.skip = max(0, max(0, first_pos - window + 1) / tile - w.ns);
+  return w;
+}
+static __device__ __forceinline__ int clamp_chunk(int pc, int n_chunks) { return min(max(pc, 0), n_chunks - 1); }
 
 // The query block a workgroup of the tile kernels takes.
 struct QueryBlock {

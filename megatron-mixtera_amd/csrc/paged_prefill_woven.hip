@@ -52,6 +52,7 @@
 #include "mi_common.h"
 #include "mi_capi_internal.h"
 #include "paged_prefill_params.h"
+#include "paged_prefill_remake.h"
 
 namespace mi {
 
@@ -77,7 +78,9 @@ template <int HD> constexpr bool wv_piece_division_ok() {
 }
 static_assert(wv_piece_division_ok<128>() && wv_piece_division_ok<64>(), "piece -> (row, column)");
 
-template <int HD, bool FP8, bool SPLIT, bool F16, int WAVES, int PER_SIMD>
+// WIN: a row sees the last `window` keys up to its own and the first `sinks` (see PrefillParams).  The workgroup walks the tiles
+// that one of its rows sees (window_tiles), masks those that a border crosses and makes rows that are not finite again.
+template <int HD, bool FP8, bool SPLIT, bool F16, int WAVES, int PER_SIMD, bool WIN>
 __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kernel(PrefillParams p) {
   constexpr int KS = HD / 32, DV = HD / 16, NQ = 2, THREADS = 64 * WAVES;
   constexpr bool FACTOR = FP8 && HD == 128;   // the value scales' mantissas go into the probabilities (see above)
@@ -114,11 +117,17 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
 
   QueryBlock qb;
   if (!find_query_block(p, SBQ, rank, (int)(gridDim.x / HV), &qb)) return;  // workgroup-uniform
-  const int r = qb.r, q_begin = qb.q_begin, Lq = qb.Lq, Lk = qb.Lk, q0_wg = qb.q0;
+  const int r = qb.r, q_begin = qb.q_begin, Lq = qb.Lq, Lk = WIN ? min(qb.Lk, p.max_len) : qb.Lk, q0_wg = qb.q0;
   const int shift = Lk - Lq;
   const int last = Lk - 1;
   const int kend_wg = min(Lk, shift + min(q0_wg + SBQ, Lq));
-  const int ntl_all = (kend_wg + kWvTile - 1) / kWvTile;  // staged tiles the rows of this workgroup can see
+  WindowTiles wt = {};
+  if constexpr (WIN) {
+    wt = window_tiles(p.window, p.sinks, kWvTile, shift + q0_wg);
+    wt.ns = __builtin_amdgcn_readfirstlane(wt.ns);
+    wt.skip = __builtin_amdgcn_readfirstlane(wt.skip);
+  }
+  const int ntl_all = (kend_wg + kWvTile - 1) / kWvTile - wt.skip;  // staged tiles the rows of this workgroup can see
   const int n_split = SPLIT ? (int)gridDim.y : 1, split = SPLIT ? (int)blockIdx.y : 0;
   // (workgroup-uniform values the tile loop's bookkeeping is built from: held in scalar registers)
   const int tb = __builtin_amdgcn_readfirstlane(SPLIT ? (int)((int64_t)ntl_all * split / n_split) : 0);
@@ -146,7 +155,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
   // launch.  A row's values lie in four lanes (g), the partner of a half-split pair KS / 2 fragments away in the same
   // lane.  What that needs is requested here, together with the queries; the arithmetic (some 900 instructions, three
   // microseconds of a workgroup's tens) runs while the first tiles are on their way.
-  const bool raw = p.norm != MI_NORM_NONE || p.angles;
+  const bool raw = !WIN && (p.norm != MI_NORM_NONE || p.angles);
   uint4 cw[NQ][KS], sw[NQ][KS], qw[KS];
   if (raw) {
 #pragma unroll
@@ -367,23 +376,37 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
                    : "memory", "m0");
     };
     // the tile cursor: all members wave-uniform; it sticks to the workgroup's last tile
-    struct Cursor { int tile, ci, tin; };
+    struct Cursor { int tile, ci, tin; };   // (WIN: the tile of the walk)
     auto cursor_at = [&](int t) {
       Cursor c;
       c.tile = __builtin_amdgcn_readfirstlane(min(t, te - 1));
-      c.ci = __builtin_amdgcn_readfirstlane(c.tile / tiles_per_chunk);
-      c.tin = c.tile - c.ci * tiles_per_chunk;
+      const int real = WIN ? wt.real(c.tile) : c.tile;
+      c.ci = __builtin_amdgcn_readfirstlane(real / tiles_per_chunk);
+      c.tin = real - c.ci * tiles_per_chunk;
       return c;
     };
+    // where the walk goes on behind the sinks
+    const int far_ci = WIN ? __builtin_amdgcn_readfirstlane((wt.ns + wt.skip) / tiles_per_chunk) : 0;
+    const int far_tin = WIN ? wt.ns + wt.skip - far_ci * tiles_per_chunk : 0;
     auto cursor_next = [&](Cursor& c) {
       const bool adv = c.tile + 1 < te;
       const bool wrap = adv && (c.tin + 1 == tiles_per_chunk);
       c.tile += adv ? 1 : 0;
       c.tin = wrap ? 0 : c.tin + (adv ? 1 : 0);
       c.ci += wrap ? 1 : 0;
+      if constexpr (WIN) {
+        const bool far = adv && c.tile == wt.ns;
+        c.tin = far ? far_tin : c.tin;
+        c.ci = far ? far_ci : c.ci;
+      }
     };
-    auto tile_off = [&](const Cursor& c, int pc) { return (int64_t)pc * chunk_bytes + (int64_t)c.tin * tile_bytes; };
-    auto tile_nrec = [&](const Cursor& c) { return (uint32_t)(min(last_key - c.tile * kWvTile, kWvTile - 1) + 1) * (uint32_t)tok_bytes; };
+    auto tile_off = [&](const Cursor& c, int pc) {
+      return (int64_t)(WIN ? clamp_chunk(pc, p.n_chunks) : pc) * chunk_bytes + (int64_t)c.tin * tile_bytes;
+    };
+    auto tile_nrec = [&](const Cursor& c) {
+      const int real = WIN ? wt.real(c.tile) : c.tile;
+      return (uint32_t)(min(last_key - real * kWvTile, kWvTile - 1) + 1) * (uint32_t)tok_bytes;
+    };
     // block-table entries by scalar loads the compiler does not see (a vector load in the tile loop would make it
     // wait on the vector-memory counter, i.e. for the direct loads in flight)
     auto bt_request = [&](int ci) {
@@ -400,13 +423,27 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
     int pc_v = 0;
     float ks_v = 1.f, vs_v = 1.f;
     auto scales_request = [&](int pc) {
+      if constexpr (WIN) pc = clamp_chunk(pc, p.n_chunks);
       ks_v = p.k_scale[(int64_t)pc * p.Hkv + h + vzero];
       vs_v = p.v_scale[(int64_t)pc * p.Hkv + h + vzero];
     };
     auto uniform_float = [](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); };
 
     // 16-bit: one scale for all scores.  fp8: a tile's own (kept off zero: zero times the -inf of a masked score would be NaN).
-    auto tile_scale = [&](float ks) { return FP8 ? fmaxf(ks * p.scale_log2, 1.17549435e-38f) : p.scale_log2; };
+    // (WIN: a NaN stays one, and a negative scale's sign goes to the fetched bytes, in a branch, as the values')
+    auto tile_scale = [&](float ks) {
+      if constexpr (WIN && FP8) {
+        const float x = fabsf(ks * p.scale_log2);
+        return x < 1.17549435e-38f ? 1.17549435e-38f : x;
+      }
+      return FP8 ? fmaxf(ks * p.scale_log2, 1.17549435e-38f) : p.scale_log2;
+    };
+    auto negate_keys_fp8 = [&](int32_t sign) {
+      if (__builtin_expect(sign >= 0, 1)) return;
+#pragma unroll
+      for (int i = 0; i < NP8; ++i) kraw[i] = make_uint2(kraw[i].x ^ 0x80808080u, kraw[i].y ^ 0x80808080u);
+    };
+    int32_t ksign_first = 0;   // WIN: of the first tile's scale
     float scale_prev = p.scale_log2, scale_cur = p.scale_log2, scale_next = p.scale_log2, vscale = 1.f;
     float factor_prev = 1.f, factor_cur = 1.f;   // fp8: value_factor of the tiles whose scales are scale_prev and scale_cur
     float factor_next = 1.f;                     // (and of the tile of `vscale`, whose sign is `vsign`'s)
@@ -565,11 +602,12 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
       auto mask_step = [&](int nt) {
         if (!MASK) return;
         const int dpos = qpos[nt] - (key0 + 4 * g);
+        const int gone = WIN ? dpos - p.window : 0, sunk = WIN ? p.sinks - (key0 + 4 * g) : 0;   // hidden: from `sunk` to `gone`
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i2 = 0; i2 < 4; ++i2)
-            if (16 * u + i2 > dpos) Sn[nt][u][i2] = -INFINITY;
+            if (16 * u + i2 > dpos || (WIN && 16 * u + i2 <= gone && 16 * u + i2 >= sunk)) Sn[nt][u][i2] = -INFINITY;
       };
       // values; beside them the last probabilities, then the mask of the scores just multiplied
 #pragma unroll
@@ -613,6 +651,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
       if constexpr (FP8) {
         scales_request(pc);
         if (i == 0) {
+          if constexpr (WIN) ksign_first = __float_as_int(uniform_float(ks_v));
           scale_prev = scale_cur = tile_scale(uniform_float(ks_v));
           values_scale(uniform_float(vs_v));
           factor_prev = factor_cur = factor_next;
@@ -648,6 +687,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
       MI_SB();
       if (raw) norm_and_rotate();
       MI_SB();
+      if constexpr (WIN) negate_keys_fp8(ksign_first);
 #pragma unroll
       for (int i = 0; i < NP8; ++i) store_k_fp8(&Ks[0][0], i);
       fetch_fp8(kbase, off_first[1], nrec_first[1], kraw);  // stored by iteration 0
@@ -680,7 +720,10 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
     MI_SB();
 
     const int t_mask = max(0, (full_until + 1) >> 6);              // first tile with a masked score for this wavefront
-    const int jm = min(max(t_mask - tb, 0), ntl);                  // iterations [0, jm) need no mask
+    const int jm = min(max((WIN ? wt.walk(t_mask) : t_mask) - tb, 0), ntl);   // iterations [0, jm) need no mask
+    // WIN: ... but those up to the last tile that holds a key behind some row's window, if one is no sink
+    const int gone_wave = full_until + max(nq, 1) - 1 - p.window;
+    const int jw = WIN && gone_wave >= p.sinks ? min(max(wt.walk((gone_wave >> 6) + 1) - tb, 0), ntl) : 0;
     int j = 0;
     int even = 0;   // BUF where j is odd
 #pragma unroll
@@ -698,7 +741,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
       const uint8_t* ka = k_lane + even;
       const uint8_t* ka_next = k_lane + (BUF - even);
       const uint8_t* va = v_lane + (BUF - even);
-      const int key0 = (tb + j) * kWvTile;
+      const int key0 = (WIN ? wt.real(tb + j) : tb + j) * kWvTile;
       u32x4_t rs_k, rs_v0, rs_v1;
       const uint32_t kdst = ks_lds + (uint32_t)even, v0dst = vs_lds + (uint32_t)(BUF - even), v1dst = vs_lds + (uint32_t)even;
       // fp8: key tile j+1 and the first half of value tile j, fetched since the last barrier, go into LDS before this one
@@ -707,6 +750,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
       slot(std::integral_constant<int, 0>{}, Mc, ka, ka_next, va, key0, [](auto) {}, [](int) {},
            [&](int e) {
              if constexpr (FP8) {
+               if (WIN && e == NVF - NP8) negate_keys_fp8(__float_as_int(uniform_float(ks_v)));   // (of key tile j+1)
                if (e >= NVF - NP8) store_k_fp8(kst, e - (NVF - NP8));
              }
            });
@@ -765,8 +809,16 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
       ++j;
       even = BUF - even;
     };
-    for (; j < jm;) iteration(std::false_type{});
-    for (; j < ntl;) iteration(std::true_type{});
+    if constexpr (WIN) {   // (one copy of either loop)
+#pragma clang loop unroll(disable)
+      for (int border = 1; border >= 0; --border) {
+        for (; j < (border ? 0 : jm);) iteration(std::false_type{});
+        for (; j < (border ? jw : ntl);) iteration(std::true_type{});
+      }
+    } else {
+      for (; j < jm;) iteration(std::false_type{});
+      for (; j < ntl;) iteration(std::true_type{});
+    }
 
     // ---- drain: the last two steps' values (tile ntl - 1), the second half when it has landed; S[1] is masked already ----
     {
@@ -805,7 +857,11 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
     const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
     const int n = 16 * nt + m16;
     const int qi = (n * g_magic) >> 16, u = n - qi * G;  // n / G, n % G
-    if (qi < nq) {
+    bool fine = true;
+    if constexpr (WIN)
+      fine = finite_or_remade<HD, kWvTile, FP8, F16>(p, acc[nt], l_tot, nt, nq, G, g_magic, r, q_begin + q0, h, hq0, shift + q0, Lk, wt, tb, te,
+                                                     SPLIT ? split : -1);
+    if (qi < nq && fine) {
       if (!SPLIT) {
         uint16_t* o = p.out + (int64_t)(q_begin + q0 + qi) * p.o_st + (int64_t)(hq0 + u) * p.o_sh + 4 * g;
 #pragma unroll
@@ -826,15 +882,16 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
 }
 
 
-void launch_prefill_woven(const PrefillParams& p, dim3 grid, int head_dim, bool fp8, bool f16, int waves, hipStream_t st) {
+template <bool WIN>
+static void launch(const PrefillParams& p, dim3 grid, int head_dim, bool fp8, bool f16, int waves, hipStream_t st) {
   const bool split = grid.y > 1;
 #define MI_WV_LAUNCH(HD_, FP8_, W_, PS_)                                                                                 \
   do {                                                                                                              \
     const dim3 block(64 * W_);                                                                                      \
-    if (split && f16) hipLaunchKernelGGL((paged_prefill_woven_kernel<HD_, FP8_, true, true, W_, PS_>), grid, block, 0, st, p); \
-    else if (split) hipLaunchKernelGGL((paged_prefill_woven_kernel<HD_, FP8_, true, false, W_, PS_>), grid, block, 0, st, p); \
-    else if (f16) hipLaunchKernelGGL((paged_prefill_woven_kernel<HD_, FP8_, false, true, W_, PS_>), grid, block, 0, st, p); \
-    else hipLaunchKernelGGL((paged_prefill_woven_kernel<HD_, FP8_, false, false, W_, PS_>), grid, block, 0, st, p);      \
+    if (split && f16) hipLaunchKernelGGL((paged_prefill_woven_kernel<HD_, FP8_, true, true, W_, PS_, WIN>), grid, block, 0, st, p); \
+    else if (split) hipLaunchKernelGGL((paged_prefill_woven_kernel<HD_, FP8_, true, false, W_, PS_, WIN>), grid, block, 0, st, p); \
+    else if (f16) hipLaunchKernelGGL((paged_prefill_woven_kernel<HD_, FP8_, false, true, W_, PS_, WIN>), grid, block, 0, st, p); \
+    else hipLaunchKernelGGL((paged_prefill_woven_kernel<HD_, FP8_, false, false, W_, PS_, WIN>), grid, block, 0, st, p);      \
   } while (0)
   if (head_dim == 64 && fp8 && (int64_t)grid.x * grid.y <= 3 * device_cu_count()) MI_WV_LAUNCH(64, true, 4, 2);
   else if (head_dim == 64 && fp8) MI_WV_LAUNCH(64, true, 4, 3);
@@ -844,6 +901,11 @@ void launch_prefill_woven(const PrefillParams& p, dim3 grid, int head_dim, bool 
   else if (waves == 4) MI_WV_LAUNCH(128, false, 4, 2);
   else MI_WV_LAUNCH(128, false, 8, 2);
 #undef MI_WV_LAUNCH
+}
+
+void launch_prefill_woven(const PrefillParams& p, dim3 grid, int head_dim, bool fp8, bool f16, int waves, hipStream_t st) {
+  if (p.window > 0) launch<true>(p, grid, head_dim, fp8, f16, waves, st);
+  else launch<false>(p, grid, head_dim, fp8, f16, waves, st);
 }
 
 }  // namespace mi

@@ -274,10 +274,14 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, kv_lens:
                            *, softmax_scale: Optional[float] = None, max_kv_len: Optional[int] = None,
                            split_tokens: int = 0, out: Optional[Tensor] = None,
                            workspace: Optional[Tensor] = None, k_scales: Optional[Tensor] = None,
-                           v_scales: Optional[Tensor] = None) -> Tensor:
-    """One query token per request against the paged cache; returns a tensor shaped like ``q``."""
+                           v_scales: Optional[Tensor] = None, window: Optional[int] = None, sinks: int = 0) -> Tensor:
+    """One query token per request against the paged cache; returns a tensor shaped like ``q``.
+
+    With a ``window`` a request sees its last ``window`` tokens (the newest included) and its first ``sinks``; chunks that
+    hold none of them are not read, and their entries in ``block_table`` may hold anything."""
     return _native().paged_decode_attention(q, k_cache, v_cache, kv_lens, block_table, softmax_scale, max_kv_len,
-                                            split_tokens, out, workspace, k_scales, v_scales, _tuning_arg(), _override())
+                                            split_tokens, out, workspace, k_scales, v_scales, _tuning_arg(), _override(),
+                                            window, sinks)
 
 
 def paged_decode_attention_noalloc(q: Tensor, k_cache: Tensor, v_cache: Tensor, kv_lens: Tensor, block_table: Tensor,
@@ -345,14 +349,17 @@ def paged_prefill_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, cu_seql
                             block_table: Tensor, *, softmax_scale: Optional[float] = None,
                             max_kv_len: Optional[int] = None, out: Optional[Tensor] = None,
                             k_scales: Optional[Tensor] = None, v_scales: Optional[Tensor] = None,
-                            one_row_requests: bool = True) -> Tensor:
+                            one_row_requests: bool = True, window: Optional[int] = None, sinks: int = 0) -> Tensor:
     """Varlen causal attention of new tokens over the paged cache (bottom-right aligned mask).
     Byte caches with ``k_scales`` / ``v_scales`` ``[N, Hkv]`` select the fp8-e4m3 path.  ``one_row_requests=False``
     says that no request has exactly one query row, so the decode kernels need not be launched (a request that has
-    one all the same is served by the tile kernel)."""
+    one all the same is served by the tile kernel).
+
+    With a ``window`` a token sees the last ``window`` tokens up to itself and the request's first ``sinks``; chunks that no
+    row of the call sees are not read, and their entries in ``block_table`` may hold anything."""
     return _native().paged_prefill_attention(q, k_cache, v_cache, cu_seqlens_q, kv_lens, block_table, softmax_scale,
                                              max_kv_len, out, k_scales, v_scales, _tuning_arg(), _override(),
-                                             one_row_requests)
+                                             one_row_requests, window, sinks)
 
 
 # ---------------------------------------------------------------------------------------------
