@@ -516,6 +516,37 @@ int mi_norm_rope_append(const void* q, int64_t q_stride_tok, void* q_out, int64_
                         int32_t faithful_rounding, int32_t dtype, const MiTuning* tuning, void* stream);
 
 /*
+ * The same where a token has positions on up to four axes (time, height, width of images and video; text counts alike on
+ * all): rotary pair i belongs to axis pair_axes[i] and turns by row positions[axis][t] of rotary_angles.  Half-split pairs
+ * are (i, i + rot_dim / 2), interleaved ones (2 i, 2 i + 1); each element takes its own column of the row, as above.
+ * `positions`: `axes` rows of T int64, positions_stride apart, for queries and keys alike; positions are kept inside the
+ * table's `angles_rows` rows.  pair_axes: rot_dim / 2 bytes of HOST memory, read during the call.  Everything else as in
+ * mi_norm_rope_append and mi_qkv_norm_rope_append; rotary_angles may not be null.
+ */
+int mi_norm_rope_append_axes(const void* q, int64_t q_stride_tok, void* q_out, int64_t q_out_stride_tok, const void* k,
+                             int64_t k_stride_tok, void* k_out, int64_t k_out_stride_tok, const void* v,
+                             int64_t v_stride_tok, const void* q_weight, const void* k_weight, float eps,
+                             int32_t norm_kind, const float* rotary_angles, int64_t angles_stride, int32_t angles_rows,
+                             int32_t rot_dim, int32_t rotary_interleaved, float mscale, const int64_t* positions,
+                             int64_t positions_stride, int32_t axes, const uint8_t* pair_axes, void* k_cache,
+                             void* v_cache, int64_t kv_stride_chunk, int64_t kv_stride_tok,
+                             const int64_t* token_to_chunk_idx, const int64_t* token_to_local_pos,
+                             const int32_t* block_table, int64_t bt_stride, const int32_t* kv_lens, int32_t chunk_tokens,
+                             int32_t T, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t faithful_rounding,
+                             int32_t dtype, const MiTuning* tuning, void* stream);
+int mi_qkv_norm_rope_append_axes(const void* mixed_qkv, int64_t qkv_stride_tok, void* q_out, int64_t q_out_stride_tok,
+                                 void* k_out, int64_t k_out_stride_tok, const void* q_weight, const void* k_weight,
+                                 float eps, int32_t norm_kind, const float* rotary_angles, int64_t angles_stride,
+                                 int32_t angles_rows, int32_t rot_dim, int32_t rotary_interleaved, float mscale,
+                                 const int64_t* positions, int64_t positions_stride, int32_t axes,
+                                 const uint8_t* pair_axes, void* k_cache, void* v_cache, int64_t kv_stride_chunk,
+                                 int64_t kv_stride_tok, const int64_t* token_to_chunk_idx,
+                                 const int64_t* token_to_local_pos, const int32_t* block_table, int64_t bt_stride,
+                                 const int32_t* kv_lens, int32_t chunk_tokens, int32_t T, int32_t Hq, int32_t Hkv,
+                                 int32_t head_dim, int32_t faithful_rounding, int32_t dtype, const MiTuning* tuning,
+                                 void* stream);
+
+/*
  * The same launch reading the QKV projection's output directly: replaces the split of
  * SelfAttention.get_query_key_value_tensors (megatron/core/transformer/attention.py:985-1030:
  * view `[T, Hkv, (Hq/Hkv + 2) * d]`, split into G = Hq/Hkv query heads, one key head and one

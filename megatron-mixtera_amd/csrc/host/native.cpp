@@ -290,6 +290,30 @@ Angles angles_of(const Tensor* e) {
   a.rot = (int)e->size(dims - 1);
   return a;
 }
+// Positions with several axes: `pair_axes` (bytes, one per rotary pair) None for none, else positions [axes, >= T].
+struct Axes {
+  const uint8_t* pairs = nullptr;
+  const int64_t* positions = nullptr;
+  int64_t stride = 0;
+  int axes = 0, rows = 0;
+};
+Axes axes_of(PyObject* pair_axes, const Tensor* emb, const Tensor* positions, const Tensor* k_positions, int64_t T) {
+  Axes x;
+  if (pair_axes == Py_None) return x;
+  REQUIRE(emb && positions, "rotary_axes need rotary_emb and q_positions");
+  REQUIRE(!k_positions, "with rotary_axes queries and keys have one set of positions, q_positions");
+  REQUIRE(PyBytes_Check(pair_axes) && PyBytes_GET_SIZE(pair_axes) * 2 == emb->size(-1), "rotary_axes must be bytes, one per rotary pair");
+  REQUIRE(positions->scalar_type() == at::kLong && positions->dim() == 2 && positions->size(1) >= T && positions->size(0) >= 1 &&
+              positions->size(0) <= 4 && (positions->stride(1) == 1 || positions->size(1) == 1),
+          "with rotary_axes q_positions must be int64 [axes, >= T] of up to four contiguous rows");
+  REQUIRE(emb->size(0) >= 1 && emb->size(0) < (int64_t)1 << 31, "rotary table must have rows (fewer than 2^31)");
+  x.pairs = reinterpret_cast<const uint8_t*>(PyBytes_AS_STRING(pair_axes));
+  x.positions = static_cast<const int64_t*>(positions->data_ptr());
+  x.stride = positions->size(0) > 1 ? positions->stride(0) : T;
+  x.axes = (int)positions->size(0);
+  x.rows = (int)emb->size(0);
+  return x;
+}
 void check_norm_weight(const Tensor* w, const Tensor& ref, int64_t d) {
   REQUIRE(!w || (w->scalar_type() == ref.scalar_type() && w->numel() == d && w->is_contiguous()),
           "norm weights must be [d] of the tensors' 16-bit type");
@@ -631,7 +655,7 @@ CacheSlots slots_of(const Tensor* kc, const Tensor* vc, const Tensor* table, con
 // norm_rope_append(query|None, key|None, value|None, q_weight|None, k_weight|None, eps, norm_kind, rotary_emb|None,
 //                  q_positions|None, k_positions|None, interleaved, mscale, query_out|None, key_out|None, k_cache|None,
 //                  v_cache|None, token_to_chunk_idx|None, token_to_local_pos|None, block_table|None, kv_lens|None,
-//                  faithful_rounding, tuning|None)
+//                  faithful_rounding, tuning|None, rotary_axes|None)
 PyObject* norm_rope_append(PyObject* const* a) {
   const Tensor *query = opt_tensor(a[0], "query"), *key = opt_tensor(a[1], "key"), *value = opt_tensor(a[2], "value");
   REQUIRE(query || key, "need query and/or key");
@@ -669,7 +693,8 @@ PyObject* norm_rope_append(PyObject* const* a) {
   check_norm_weight(kw, ref, D);
   const Tensor *qp = opt_tensor(a[8], "q_positions"), *kp = opt_tensor(a[9], "k_positions");
   const Tensor *ci = opt_tensor(a[16], "token_to_chunk_idx"), *lp = opt_tensor(a[17], "token_to_local_pos");
-  for (const Tensor* t : {qp, kp, ci, lp}) check_index_row(t, T, "index rows must be int64 [>=T]");
+  const Axes axes = axes_of(a[22], opt_tensor(a[7], "rotary_emb"), qp, kp, T);
+  for (const Tensor* t : {axes.pairs ? nullptr : qp, kp, ci, lp}) check_index_row(t, T, "index rows must be int64 [>=T]");
   const Tensor *kc = opt_tensor(a[14], "k_cache"), *vc = opt_tensor(a[15], "v_cache");
   const Tensor *bt = opt_tensor(a[18], "block_table"), *lens = opt_tensor(a[19], "kv_lens");
   const CacheSlots s = slots_of(kc, vc, bt, lens, ref, D, "the caches must have the tensors' 16-bit type");
@@ -677,6 +702,21 @@ PyObject* norm_rope_append(PyObject* const* a) {
     REQUIRE(!r->t || r->t->scalar_type() == ref.scalar_type(), "query / key / value / outputs must share one 16-bit type");
   const int code = dtype_code(ref, "query / key");
   const auto* tune = (const MiTuning*)host_struct(a[21]);
+  if (axes.pairs) {
+    void* stream = stream_of(ref);
+    same_device(ref, {query, key, value, qw, kw, qp, ci, lp, kc, vc, bt, lens, qo.t, ko.t, opt_tensor(a[7], "rotary_emb")});
+    REQUIRE(!key || !kc || (kc->size(2) == k3.h && kc->size(3) == D), "cache shape mismatch");
+    REQUIRE(!bt || (bt->dim() == 2 && bt->size(0) >= T && lens->numel() >= T), "block_table / kv_lens shorter than the batch");
+    const c10::DeviceGuard guard(ref.device());
+    check(mi_norm_rope_append_axes(q3.ptr(), q3.sn, qo.ptr(), qo.sn, k3.ptr(), k3.sn, ko.ptr(), ko.sn, v3.ptr(), v3.sn, ptr(qw), ptr(kw),
+                                   (float)as_float(a[5]), (int)as_int(a[6]), ang.ptr, ang.stride, axes.rows, ang.rot, as_bool(a[10]),
+                                   (float)as_float(a[11]), axes.positions, axes.stride, axes.axes, axes.pairs, ptr(kc), ptr(vc), s.sc,
+                                   s.st, (const int64_t*)ptr(ci), (const int64_t*)ptr(lp), (const int32_t*)ptr(bt),
+                                   bt ? bt->stride(0) : 0, (const int32_t*)ptr(lens), s.chunk, (int)T, (int)q3.h, (int)k3.h, (int)D,
+                                   as_bool(a[20]), code, tune, stream),
+          "mi_norm_rope_append_axes");
+    Py_RETURN_NONE;
+  }
   check(mi_norm_rope_append(q3.ptr(), q3.sn, qo.ptr(), qo.sn, k3.ptr(), k3.sn, ko.ptr(), ko.sn, v3.ptr(), v3.sn, ptr(qw), ptr(kw),
                             (float)as_float(a[5]), (int)as_int(a[6]), ang.ptr, ang.stride, ang.rot, as_bool(a[10]),
                             (float)as_float(a[11]), (const int64_t*)ptr(qp), (const int64_t*)ptr(kp), ptr(kc), ptr(vc), s.sc, s.st,
@@ -710,7 +750,7 @@ Mixed mixed_of(PyObject* o, PyObject* hq, PyObject* hkv, const char* shape3) {
 // qkv_norm_rope_append(mixed_qkv, num_query_heads, num_kv_heads, query_out, key_out|None, q_weight|None, k_weight|None,
 //                      eps, norm_kind, rotary_emb|None, q_positions|None, k_positions|None, interleaved, mscale,
 //                      k_cache|None, v_cache|None, token_to_chunk_idx|None, token_to_local_pos|None, block_table|None,
-//                      kv_lens|None, faithful_rounding, tuning|None)
+//                      kv_lens|None, faithful_rounding, tuning|None, rotary_axes|None)
 PyObject* qkv_norm_rope_append(PyObject* const* a) {
   const Mixed m = mixed_of(a[0], a[1], a[2], "mixed_qkv must be [T, 1, W]");
   const Tensor& ref = *m.t;
@@ -731,10 +771,26 @@ PyObject* qkv_norm_rope_append(PyObject* const* a) {
   check_norm_weight(kw, ref, m.D);
   const Tensor *qp = opt_tensor(a[10], "q_positions"), *kp = opt_tensor(a[11], "k_positions");
   const Tensor *ci = opt_tensor(a[16], "token_to_chunk_idx"), *lp = opt_tensor(a[17], "token_to_local_pos");
-  for (const Tensor* t : {qp, kp, ci, lp}) check_index_row(t, m.T, "index rows must be int64 [>=T]");
+  const Axes axes = axes_of(a[22], opt_tensor(a[9], "rotary_emb"), qp, kp, m.T);
+  for (const Tensor* t : {axes.pairs ? nullptr : qp, kp, ci, lp}) check_index_row(t, m.T, "index rows must be int64 [>=T]");
   const Tensor *bt = opt_tensor(a[18], "block_table"), *lens = opt_tensor(a[19], "kv_lens");
   const CacheSlots s = slots_of(kc, vc, bt, lens, ref, m.D, "the caches must have the projection's 16-bit type");
   const auto* tune = (const MiTuning*)host_struct(a[21]);
+  if (axes.pairs) {
+    same_device(ref, {&query_out, ko.t, qw, kw, qp, ci, lp, kc, vc, bt, lens, opt_tensor(a[9], "rotary_emb")});
+    REQUIRE(!ko.t || ko.t->scalar_type() == ref.scalar_type(), "key_out must be [T, Hkv, d]");
+    REQUIRE(!kc || (kc->size(2) == m.Hkv && kc->size(3) == m.D), "cache shape mismatch");
+    REQUIRE(!bt || (bt->dim() == 2 && bt->size(0) >= m.T && lens->numel() >= m.T), "block_table / kv_lens shorter than the batch");
+    const c10::DeviceGuard guard(ref.device());
+    check(mi_qkv_norm_rope_append_axes(ref.data_ptr(), m.st, query_out.data_ptr(), qo.sn, ko.ptr(), ko.sn, ptr(qw), ptr(kw),
+                                       (float)as_float(a[7]), (int)as_int(a[8]), ang.ptr, ang.stride, axes.rows, ang.rot, as_bool(a[12]),
+                                       (float)as_float(a[13]), axes.positions, axes.stride, axes.axes, axes.pairs, ptr(kc), ptr(vc),
+                                       s.sc, s.st, (const int64_t*)ptr(ci), (const int64_t*)ptr(lp), (const int32_t*)ptr(bt),
+                                       bt ? bt->stride(0) : 0, (const int32_t*)ptr(lens), s.chunk, (int)m.T, (int)m.Hq, (int)m.Hkv,
+                                       (int)m.D, as_bool(a[20]), dtype_code(ref), tune, stream_of(ref)),
+          "mi_qkv_norm_rope_append_axes");
+    Py_RETURN_NONE;
+  }
   check(mi_qkv_norm_rope_append(ref.data_ptr(), m.st, query_out.data_ptr(), qo.sn, ko.ptr(), ko.sn, ptr(qw), ptr(kw),
                                 (float)as_float(a[7]), (int)as_int(a[8]), ang.ptr, ang.stride, ang.rot, as_bool(a[12]),
                                 (float)as_float(a[13]), (const int64_t*)ptr(qp), (const int64_t*)ptr(kp), ptr(kc), ptr(vc), s.sc,
@@ -1373,7 +1429,7 @@ PyMethodDef kMethods[] = {
     ABI(mi_update_requests), ABI(mi_update_requests_mask8), ABI(mi_update_requests_clearing),
     ABI(mi_add_request), ABI(mi_decode_attention_state), ABI(mi_step_attention_state),
     OP(kv_append, 6), OP(kv_append_fp8, 9), OP(paged_decode_attention, 16), OP(paged_mla_decode_attention, 10),
-    OP(paged_prefill_attention, 16), OP(paged_prefill_attention_mla, 11), OP(norm_rope_append, 22), OP(qkv_norm_rope_append, 22), OP(qkv_key_append, 16),
+    OP(paged_prefill_attention, 16), OP(paged_prefill_attention_mla, 11), OP(norm_rope_append, 23), OP(qkv_norm_rope_append, 23), OP(qkv_key_append, 16),
     OP(qkv_prefill_attention, 18), OP(decode_step_attention, 29),
     OP(linear_decode, 5), OP(attention_layer_decode, 24), OP(sample_from_logits, 12), OP(selected_log_probs, 2), OP(last_token_gather, 3),
     OP(paged_tree_attention, 12), OP(verify_drafted_tokens, 11), OP(kv_keep_accepted, 9), OP(setup, 3),

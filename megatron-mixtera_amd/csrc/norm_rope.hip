@@ -23,6 +23,8 @@
 // LDS so that any rotary pairing (half-split, interleaved, partial rotary width) reads its partner from there.
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "mi_common.h"
 #include "mi_capi_internal.h"
 
@@ -58,6 +60,15 @@ struct NormRopeParams {
   float eps, mscale;
 };
 
+// Positions with several axes: every rotary pair belongs to one of up to four, and turns by the angle at the token's position on
+// that axis.  Queries and keys have one set of positions, q_pos: axis a of token t at a * pos_st + t.
+struct AxesParams : NormRopeParams {
+  int64_t pos_st;
+  int32_t n_axes, emb_rows;   // positions are kept inside the table's rows
+  uint32_t axes[8];           // two bits per pair, from the lowest
+  int32_t waves_per_token;
+};
+
 // one rounding to the tensors' 16-bit type and back
 template <bool F16>
 static __device__ __forceinline__ float round16(float x) { return to_f32<F16>(f32_to_16<F16>(x)); }
@@ -79,8 +90,30 @@ static __device__ __forceinline__ const uint16_t* head_vector(const NormRopePara
   return p.k + (int64_t)t * p.k_st + (int64_t)(vec - p.Hq) * p.k_hst;
 }
 
-template <int D, bool F16>
-__global__ __launch_bounds__(256) void norm_rope_append_kernel(NormRopeParams p) {
+// The row of the angle table that element e of the token's heads turns by; pos: the token's positions, kept inside the table.
+static __device__ __forceinline__ int64_t axis_position(const AxesParams& p, const int64_t (&pos)[4], int e) {
+  const int half = p.rot >> 1, pair = p.interleaved ? e >> 1 : e < half ? e : e - half;
+  uint32_t word = p.axes[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) word = pair >> 4 == i ? p.axes[i] : word;
+  const int axis = word >> (2 * (pair & 15)) & 3;
+  int64_t at = pos[0];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) at = axis == i ? pos[i] : at;
+  return at;
+}
+static __device__ __forceinline__ void load_axes(const AxesParams& p, int t, int64_t (&pos)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t at = i < p.n_axes ? p.q_pos[i * p.pos_st + t] : 0;
+    pos[i] = at < 0 ? 0 : at < p.emb_rows ? at : p.emb_rows - 1;
+  }
+}
+
+// P: NormRopeParams, or AxesParams for positions with several axes.
+template <int D, bool F16, typename P = NormRopeParams>
+__global__ __launch_bounds__(256) void norm_rope_append_kernel(P p) {
+  constexpr bool AXES = std::is_same_v<P, AxesParams>;
   constexpr int LPV = D >= 128 ? 64 : 32;  // lanes per head vector
   constexpr int EPL = D / LPV;             // elements per lane: i, i + LPV, ...
   constexpr int VPW = 64 / LPV;     // head vectors per wave
@@ -117,8 +150,10 @@ __global__ __launch_bounds__(256) void norm_rope_append_kernel(NormRopeParams p)
   float sign[EPL] = {};
   bool rotate[EPL] = {};
   if (p.emb) {
-    const int64_t qp = p.q_pos ? p.q_pos[t] : 0;
-    const int64_t kp = p.k_pos ? p.k_pos[t] : qp;
+    const int64_t qp = !AXES && p.q_pos ? p.q_pos[t] : 0;
+    const int64_t kp = !AXES && p.k_pos ? p.k_pos[t] : qp;
+    int64_t axes_pos[4];
+    if constexpr (AXES) load_axes(p, t, axes_pos);
 #pragma unroll
     for (int w = 0; w < EPL; ++w) {
       const int e = i + w * LPV;
@@ -140,7 +175,9 @@ __global__ __launch_bounds__(256) void norm_rope_append_kernel(NormRopeParams p)
             continue;
           }
           if ((which == 0 && p.Hq == 0) || (which == 1 && p.Hkv == 0)) continue;
-          const float a = p.emb[(which ? kp : qp) * p.emb_stride + e];
+          float a;
+          if constexpr (AXES) a = p.emb[axis_position(p, axes_pos, e) * p.emb_stride + e];
+          else a = p.emb[(which ? kp : qp) * p.emb_stride + e];
           float c, sn;
           rotary_sincos(a, &sn, &c);
           c *= p.mscale;
@@ -432,6 +469,208 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6, 8))) voi
   }
 }
 
+// Positions with several axes, 16 bytes to a lane: one wavefront per token (or several, where tokens are few), which works the
+// token's angles out once, two elements to a lane, hands them round through its own LDS and keeps those of its lanes' eight
+// columns in registers for all of the token's heads: a lane has the same columns of every head.  Then a stream of head vectors,
+// four loads ahead: queries, keys, values.  No barrier anywhere.
+//
+// In one rounding (`faithful` 0) the norm weight is multiplied into cos and sin beforehand and the reciprocal norm comes last:
+// out = rstd (x (w cos) + x' (w' sin)), three multiply-adds a value; the partner's values come from its lane as packed words.
+template <int D, bool F16, bool FAITHFUL>
+__global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
+  constexpr int LPV = D / 8;                               // lanes that hold a head vector
+  constexpr int LPG = LPV <= 8 ? 8 : LPV <= 16 ? 16 : 32;  // lane group of one (a power of two)
+  constexpr int VPP = 64 / LPG;                            // head vectors per pass
+  constexpr int NE = (D + 63) / 64;                        // angles per lane
+  __shared__ __align__(16) float cs_all[4][2][D];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int job = blockIdx.x * 4 + wave;
+  const int t = job / p.waves_per_token, part = job - t * p.waves_per_token;
+  if (t >= p.T) return;
+  float (&cs)[2][D] = cs_all[wave];
+  const int li = lane % LPG, sub = lane / LPG;
+  const bool on = LPG == LPV || li < LPV;
+  const int e0 = on ? 8 * li : 0;
+
+  // passes: query heads, key heads, values; this wavefront's share
+  const bool to_cache = p.kc != nullptr;
+  const int nq = (p.Hq + VPP - 1) / VPP, nk = (p.Hkv + VPP - 1) / VPP, all = nq + nk + (to_cache ? nk : 0);
+  const int first = (int)((int64_t)all * part / p.waves_per_token), end = (int)((int64_t)all * (part + 1) / p.waves_per_token);
+  auto head_of = [&](int pass) { return (pass < nq ? pass : pass < nq + nk ? pass - nq : pass - nq - nk) * VPP + sub; };
+  auto load = [&](int pass) -> uint4 {
+    const int h = head_of(pass);
+    if (pass >= end || !on || h >= (pass < nq ? p.Hq : p.Hkv)) return make_uint4(0, 0, 0, 0);
+    if (pass < nq + nk) return ld16(head_vector(p, t, pass < nq ? h : p.Hq + h) + e0);
+    return ld16(p.v + (int64_t)t * p.v_st + (int64_t)h * p.v_hst + e0);
+  };
+  constexpr int AHEAD = 4;
+  uint4 next[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) next[i] = load(first + i);
+
+  int64_t cache_off = -1;
+  if (to_cache) {
+    if (p.tok_chunk) {
+      cache_off = p.tok_chunk[t] * p.chunk_elems + p.tok_local[t] * p.tok_elems;
+    } else {
+      const int len = p.lens[t];
+      if (len > 0) {
+        const int pos = len - 1, ci = pos / p.chunk;
+        cache_off = (int64_t)p.bt[(int64_t)t * p.bt_stride + ci] * p.chunk_elems + (int64_t)(pos - ci * p.chunk) * p.tok_elems;
+      }
+    }
+  }
+  const int half = p.rot >> 1;
+  const bool rotate = p.emb && e0 < p.rot;   // (whole lanes: see the launch)
+  const int pe = p.interleaved ? e0 : e0 < half ? e0 + half : e0 - half;   // the partners' first column
+  auto weight = [&](const uint16_t* w, int at) {
+    return p.norm == MI_NORM_RMS && w ? ld16(w + at) : make_uint4(ones2<F16>(), ones2<F16>(), ones2<F16>(), ones2<F16>());
+  };
+  const int at_p = rotate ? pe : e0;
+  const uint4 wq = weight(p.q_w, e0), wk = weight(p.k_w, e0);
+  const uint4 wq_p = FAITHFUL ? wq : weight(p.q_w, at_p), wk_p = FAITHFUL ? wk : weight(p.k_w, at_p);
+  if (p.emb) {
+    int64_t pos[4];
+    load_axes(p, t, pos);
+    float a[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int e = lane + 64 * i;
+      a[i] = e < p.rot ? p.emb[axis_position(p, pos, e) * p.emb_stride + e] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int e = lane + 64 * i;
+      float c = 1.f, sn = 0.f;
+      if (e < p.rot) {
+        rotary_sincos(a[i], &sn, &c);
+        c *= p.mscale;
+        sn *= p.mscale;
+        if (FAITHFUL) {
+          c = round16<F16>(c);
+          sn = round16<F16>(sn);
+        }
+        if (p.interleaved ? (e & 1) == 0 : e < half) sn = -sn;
+      }
+      if (e < D) {
+        cs[0][e] = c;
+        cs[1][e] = sn;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  auto unpack = [](const uint4& w, float (&y)[8]) {
+    const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { y[2 * j] = lo_to_f32<F16>(w4[j]); y[2 * j + 1] = hi_to_f32<F16>(w4[j]); }
+  };
+  float c[8], sn[8], w[8];   // of the lane's columns, times the weights where rounded once
+  auto factors = [&](const uint4& own, const uint4& partners) {
+    unpack(own, w);
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+      const float4 c4 = p.emb ? *reinterpret_cast<const float4*>(&cs[0][e0 + j]) : make_float4(1.f, 1.f, 1.f, 1.f);
+      const float4 s4 = p.emb ? *reinterpret_cast<const float4*>(&cs[1][e0 + j]) : make_float4(0.f, 0.f, 0.f, 0.f);
+      c[j] = c4.x; c[j + 1] = c4.y; c[j + 2] = c4.z; c[j + 3] = c4.w;
+      sn[j] = s4.x; sn[j + 1] = s4.y; sn[j + 2] = s4.z; sn[j + 3] = s4.w;
+    }
+    if (!FAITHFUL) {
+      float wp[8];
+      unpack(partners, wp);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        c[j] *= w[j];
+        sn[j] *= p.interleaved ? wp[j ^ 1] : wp[j];
+      }
+    }
+  };
+  // the words that hold the partners of a lane's eight values
+  const int plane = half >> 3;
+  const bool pow2 = plane > 0 && (plane & (plane - 1)) == 0 && 2 * plane <= LPG;
+  const int src_lane = lane - li + (pe >> 3);
+  auto partners = [&](const uint4& x) -> uint4 {
+    auto through = [&](auto&& move) { return make_uint4(move(x.x), move(x.y), move(x.z), move(x.w)); };
+    auto xored = [&](auto Pc) {
+      return through([](uint32_t v) { return __float_as_uint(lane_xor<decltype(Pc)::value>(__uint_as_float(v))); });
+    };
+    if (p.interleaved) return through([](uint32_t v) { return __builtin_amdgcn_alignbit(v, v, 16); });
+    if (pow2) {
+      if (plane == 8) return xored(std::integral_constant<int, 8>{});
+      if (plane == 4) return xored(std::integral_constant<int, 4>{});
+      if (plane == 16) return xored(std::integral_constant<int, 16>{});
+      if (plane == 2) return xored(std::integral_constant<int, 2>{});
+      return xored(std::integral_constant<int, 1>{});
+    }
+    return through([&](uint32_t v) { return (uint32_t)__shfl((int)v, src_lane, 64); });
+  };
+  auto turned = [&](const uint4& raw) -> uint4 {
+    float x[8], xp[8], o[8], rstd = 1.f;
+    unpack(raw, x);
+    if (p.norm != MI_NORM_NONE) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
+      rstd = rsqrtf(lane_group_sum<LPG>(ss) * (1.f / D) + p.eps);
+    }
+    if (FAITHFUL) {
+      uint4 y = raw;
+      if (p.norm != MI_NORM_NONE) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = p.norm == MI_NORM_RMS ? x[j] * rstd * w[j] : x[j] * rstd;
+        y = make_uint4(pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(x[4], x[5]), pack2<F16>(x[6], x[7]));
+        unpack(y, x);
+      }
+      if (!p.emb) return y;
+      unpack(partners(y), xp);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        float a0 = x[j] * c[j], a1 = x[j + 1] * c[j + 1], b0 = xp[j] * sn[j], b1 = xp[j + 1] * sn[j + 1];
+        round16_pair<F16>(a0, a1);
+        round16_pair<F16>(b0, b1);
+        o[j] = rotate ? a0 + b0 : x[j];
+        o[j + 1] = rotate ? a1 + b1 : x[j + 1];
+      }
+    } else {
+      if (p.emb) unpack(partners(raw), xp);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float turn = p.emb ? __builtin_fmaf(xp[j], sn[j], x[j] * c[j]) : x[j] * c[j];
+        o[j] = (rotate ? turn : x[j] * w[j]) * rstd;
+      }
+    }
+    return make_uint4(pack2<F16>(o[0], o[1]), pack2<F16>(o[2], o[3]), pack2<F16>(o[4], o[5]), pack2<F16>(o[6], o[7]));
+  };
+  factors(first < nq ? wq : wk, first < nq ? wq_p : wk_p);
+  for (int pass0 = first; pass0 < end; pass0 += AHEAD) {
+    uint4 now[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) now[i] = next[i];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) next[i] = load(pass0 + AHEAD + i);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int pass = pass0 + i, h = head_of(pass);
+      if (pass >= end) break;
+      if (pass == nq && first < nq) factors(wk, wk_p);
+      const bool mine = on && h < (pass < nq ? p.Hq : p.Hkv);
+      if (pass < nq + nk) {
+        const uint4 out = turned(now[i]);
+        if (!mine) continue;
+        if (pass < nq) {
+          st16(p.q_out + (int64_t)t * p.qo_st + (int64_t)h * D + e0, out);
+        } else {
+          if (p.k_out) st16(p.k_out + (int64_t)t * p.ko_st + (int64_t)h * D + e0, out);
+          if (cache_off >= 0) st16(p.kc + cache_off + (int64_t)h * D + e0, out);
+        }
+      } else if (mine && cache_off >= 0) {
+        st16(p.vc + cache_off + (int64_t)h * D + e0, now[i]);
+      }
+    }
+  }
+}
+
 }  // namespace mi
 
 namespace mi {
@@ -549,9 +788,34 @@ using namespace mi;
 
 namespace {
 
+// Wavefronts per token of norm_rope_axes_kernel: one where tokens fill the chip, else as many as give 4 096 in all, at most one
+// pass each.
+void launch_axes(AxesParams& p, bool f16, hipStream_t st) {
+  const int vpp = p.d == 64 ? 8 : p.d <= 128 ? 4 : 2;
+  const int nq = (p.Hq + vpp - 1) / vpp, nk = (p.Hkv + vpp - 1) / vpp, all = nq + nk * (p.kc ? 2 : 1);
+  int n = (4096 + p.T - 1) / p.T;
+  p.waves_per_token = n < 1 ? 1 : n > all ? all : n;
+  const dim3 grid((unsigned)(((int64_t)p.T * p.waves_per_token + 3) / 4));
+#define MI_AXES(D_)                                                                                                         \
+  do {                                                                                                                      \
+    if (f16 && p.faithful) hipLaunchKernelGGL((norm_rope_axes_kernel<D_, true, true>), grid, dim3(256), 0, st, p);          \
+    else if (f16) hipLaunchKernelGGL((norm_rope_axes_kernel<D_, true, false>), grid, dim3(256), 0, st, p);                  \
+    else if (p.faithful) hipLaunchKernelGGL((norm_rope_axes_kernel<D_, false, true>), grid, dim3(256), 0, st, p);           \
+    else hipLaunchKernelGGL((norm_rope_axes_kernel<D_, false, false>), grid, dim3(256), 0, st, p);                          \
+  } while (0)
+  if (p.d == 64) MI_AXES(64);
+  else if (p.d == 96) MI_AXES(96);
+  else if (p.d == 128) MI_AXES(128);
+  else if (p.d == 192) MI_AXES(192);
+  else MI_AXES(256);
+#undef MI_AXES
+}
+
 // Argument checks shared by both entry points, kernel choice and launch.  `p` carries every pointer,
 // stride and size; `name` prefixes error messages.
-int norm_rope_launch(NormRopeParams& p, int32_t dtype, const MiTuning* tuning, hipStream_t st, const char* name) {
+template <typename P>
+int norm_rope_launch(P& p, int32_t dtype, const MiTuning* tuning, hipStream_t st, const char* name) {
+  constexpr bool AXES = std::is_same_v<P, AxesParams>;
   char msg[160];
   auto fail = [&](int code, const char* what) {
     snprintf(msg, sizeof msg, "%s: %s", name, what);
@@ -573,7 +837,7 @@ int norm_rope_launch(NormRopeParams& p, int32_t dtype, const MiTuning* tuning, h
   if (p.emb) {
     if (p.rot <= 0 || p.rot > p.d || (p.rot & 1) || p.emb_stride < p.rot)
       return fail(MI_ERR_SHAPE, "rot_dim must be even and within head_dim");
-    if ((p.Hq > 0 && !p.q_pos) || (p.Hkv > 0 && !p.k_pos)) return fail(MI_ERR_NULL, "rotary positions missing");
+    if (AXES ? !p.q_pos : (p.Hq > 0 && !p.q_pos) || (p.Hkv > 0 && !p.k_pos)) return fail(MI_ERR_NULL, "rotary positions missing");
   }
   const bool to_cache = p.kc != nullptr;
   if (to_cache) {
@@ -597,7 +861,15 @@ int norm_rope_launch(NormRopeParams& p, int32_t dtype, const MiTuning* tuning, h
   // The 16-byte-per-lane kernel wins on many tokens; on a decode batch (a few hundred rows at most) the
   // element-wise kernel's shorter dependent chain does (4.8 against 5.7 us at 64 tokens).
   const int mode = tune.norm_rope_vectorised;  // -1 never, 1 whenever the shapes allow, 2 automatic
-  const bool vec = rot_ok && (ptrs & 15) == 0 && (strides & 7) == 0 && (mode == 1 || (mode == 2 && p.T >= 256));
+  const bool aligned = (ptrs & 15) == 0 && (strides & 7) == 0;
+  if constexpr (AXES) {
+    // (whole lanes turn or do not: rotated columns end at a multiple of eight)
+    if (rot_ok && aligned && mode >= 0 && (!p.emb || p.rot % 8 == 0)) {
+      launch_axes(p, f16, st);
+      return mi_check_launch(name);
+    }
+  }
+  const bool vec = !AXES && rot_ok && aligned && (mode == 1 || (mode == 2 && p.T >= 256));
   // head vectors per workgroup pass (see the kernels)
   const int vpb = vec ? (p.d == 64 ? 32 : p.d <= 128 ? 16 : 8) : (p.d >= 128 ? 4 : 8);
   const int passes = (p.Hq + p.Hkv + vpb - 1) / vpb;
@@ -617,25 +889,39 @@ int norm_rope_launch(NormRopeParams& p, int32_t dtype, const MiTuning* tuning, h
     else if (f16) hipLaunchKernelGGL((KERNEL_<256, true>), grid, dim3(256), 0, st, p);            \
     else hipLaunchKernelGGL((KERNEL_<256, false>), grid, dim3(256), 0, st, p);                    \
   } while (0)
-  if (vec) MI_NR_LAUNCH(norm_rope_append_vec_kernel);
-  else MI_NR_LAUNCH(norm_rope_append_kernel);
+  if constexpr (AXES) {
+#define MI_NR_ELEMENTS(D_)                                                                                                  \
+  do {                                                                                                                      \
+    if (f16) hipLaunchKernelGGL((norm_rope_append_kernel<D_, true, AxesParams>), grid, dim3(256), 0, st, p);                \
+    else hipLaunchKernelGGL((norm_rope_append_kernel<D_, false, AxesParams>), grid, dim3(256), 0, st, p);                   \
+  } while (0)
+    if (p.d == 64) MI_NR_ELEMENTS(64);
+    else if (p.d == 96) MI_NR_ELEMENTS(96);
+    else if (p.d == 128) MI_NR_ELEMENTS(128);
+    else if (p.d == 192) MI_NR_ELEMENTS(192);
+    else MI_NR_ELEMENTS(256);
+#undef MI_NR_ELEMENTS
+  } else if (vec) {
+    MI_NR_LAUNCH(norm_rope_append_vec_kernel);
+  } else {
+    MI_NR_LAUNCH(norm_rope_append_kernel);
+  }
 #undef MI_NR_LAUNCH
   return mi_check_launch(name);
 }
 
 }  // namespace
 
-extern "C" int mi_norm_rope_append(
-    const void* q, int64_t q_stride_tok, void* q_out, int64_t q_out_stride_tok, const void* k,
-    int64_t k_stride_tok, void* k_out,
-    int64_t k_out_stride_tok, const void* v, int64_t v_stride_tok, const void* q_weight,
-    const void* k_weight, float eps, int32_t norm_kind, const float* rotary_angles,
-    int64_t angles_stride, int32_t rot_dim, int32_t rotary_interleaved, float mscale,
-    const int64_t* q_positions, const int64_t* k_positions, void* k_cache, void* v_cache,
-    int64_t kv_stride_chunk, int64_t kv_stride_tok, const int64_t* token_to_chunk_idx,
-    const int64_t* token_to_local_pos, const int32_t* block_table, int64_t bt_stride,
-    const int32_t* kv_lens, int32_t chunk_tokens, int32_t T, int32_t Hq, int32_t Hkv,
-    int32_t head_dim, int32_t faithful_rounding, int32_t dtype, const MiTuning* tuning, void* stream) {
+namespace {
+
+NormRopeParams split_params(
+    const void* q, int64_t q_stride_tok, void* q_out, int64_t q_out_stride_tok, const void* k, int64_t k_stride_tok, void* k_out,
+    int64_t k_out_stride_tok, const void* v, int64_t v_stride_tok, const void* q_weight, const void* k_weight, float eps,
+    int32_t norm_kind, const float* rotary_angles, int64_t angles_stride, int32_t rot_dim, int32_t rotary_interleaved, float mscale,
+    const int64_t* q_positions, const int64_t* k_positions, void* k_cache, void* v_cache, int64_t kv_stride_chunk,
+    int64_t kv_stride_tok, const int64_t* token_to_chunk_idx, const int64_t* token_to_local_pos, const int32_t* block_table,
+    int64_t bt_stride, const int32_t* kv_lens, int32_t chunk_tokens, int32_t T, int32_t Hq, int32_t Hkv, int32_t head_dim,
+    int32_t faithful_rounding) {
   NormRopeParams p = {};
   p.q = (const uint16_t*)q; p.q_st = q_stride_tok; p.q_gst = 0; p.q_group = Hq > 0 ? Hq : 1;
   p.q_out = (uint16_t*)q_out; p.qo_st = q_out_stride_tok;
@@ -652,6 +938,70 @@ extern "C" int mi_norm_rope_append(
   p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.d = head_dim; p.rot = rot_dim; p.chunk = chunk_tokens;
   p.norm = norm_kind; p.interleaved = rotary_interleaved; p.faithful = faithful_rounding;
   p.eps = eps; p.mscale = mscale;
+  return p;
+}
+
+// The QKV projection's output in place of the split tensors; MI_OK or a negative code.
+int mixed_params(NormRopeParams& p, const void* mixed_qkv, int64_t qkv_stride_tok, const char* who) {
+  char msg[160];
+  auto fail = [&](int code, const char* what) {
+    snprintf(msg, sizeof msg, "%s: %s", who, what);
+    return mi_fail(code, msg);
+  };
+  if (!mixed_qkv) return fail(MI_ERR_NULL, "mixed_qkv missing");
+  if (p.Hq <= 0 || p.Hkv <= 0 || p.Hq % p.Hkv != 0) return fail(MI_ERR_SHAPE, "query heads must be a positive multiple of KV heads");
+  if (!p.kc && !p.k_out) return fail(MI_ERR_NULL, "the key needs a destination (k_out and/or the cache)");
+  const int G = p.Hq / p.Hkv;
+  const int64_t group = (int64_t)(G + 2) * p.d;  // elements of one query group: G q heads, k, v
+  if (qkv_stride_tok < group * p.Hkv) return fail(MI_ERR_SHAPE, "token stride smaller than (Hq + 2 Hkv) * head_dim");
+  const uint16_t* base = (const uint16_t*)mixed_qkv;
+  p.q = base; p.q_st = qkv_stride_tok; p.q_gst = group; p.q_group = G;
+  p.k = base + (int64_t)G * p.d; p.k_st = qkv_stride_tok; p.k_hst = group;
+  p.v = p.kc ? base + (int64_t)(G + 1) * p.d : nullptr; p.v_st = qkv_stride_tok; p.v_hst = group;
+  return MI_OK;
+}
+
+int axes_launch(const NormRopeParams& base, const int64_t* positions, int64_t positions_stride, int32_t n_axes,
+                const uint8_t* pair_axes, int32_t angles_rows, int32_t dtype, const MiTuning* tuning, void* stream, const char* who) {
+  char msg[160];
+  auto fail = [&](int code, const char* what) {
+    snprintf(msg, sizeof msg, "%s: %s", who, what);
+    return mi_fail(code, msg);
+  };
+  AxesParams p;
+  static_cast<NormRopeParams&>(p) = base;
+  if (!p.emb || !pair_axes || !positions) return fail(MI_ERR_NULL, "angles, positions or the pairs' axes missing");
+  if (n_axes < 1 || n_axes > 4) return fail(MI_ERR_UNSUPPORTED, "one to four axes");
+  if (angles_rows < 1) return fail(MI_ERR_SHAPE, "the table of angles has no row");
+  if (positions_stride < p.T && n_axes > 1) return fail(MI_ERR_SHAPE, "positions of two axes overlap");
+  if (p.rot <= 0 || p.rot > 256 || (p.rot & 1)) return fail(MI_ERR_SHAPE, "rot_dim must be even and within head_dim");
+  p.q_pos = positions; p.k_pos = nullptr; p.pos_st = positions_stride; p.n_axes = n_axes; p.emb_rows = angles_rows;
+  for (uint32_t& w : p.axes) w = 0;
+  for (int i = 0; i < p.rot / 2; ++i) {
+    if (pair_axes[i] >= n_axes) return fail(MI_ERR_SHAPE, "a pair's axis is not among the positions'");
+    p.axes[i / 16] |= (uint32_t)pair_axes[i] << (2 * (i % 16));
+  }
+  p.waves_per_token = 1;
+  return norm_rope_launch(p, dtype, tuning, (hipStream_t)stream, who);
+}
+
+}  // namespace
+
+extern "C" int mi_norm_rope_append(
+    const void* q, int64_t q_stride_tok, void* q_out, int64_t q_out_stride_tok, const void* k,
+    int64_t k_stride_tok, void* k_out,
+    int64_t k_out_stride_tok, const void* v, int64_t v_stride_tok, const void* q_weight,
+    const void* k_weight, float eps, int32_t norm_kind, const float* rotary_angles,
+    int64_t angles_stride, int32_t rot_dim, int32_t rotary_interleaved, float mscale,
+    const int64_t* q_positions, const int64_t* k_positions, void* k_cache, void* v_cache,
+    int64_t kv_stride_chunk, int64_t kv_stride_tok, const int64_t* token_to_chunk_idx,
+    const int64_t* token_to_local_pos, const int32_t* block_table, int64_t bt_stride,
+    const int32_t* kv_lens, int32_t chunk_tokens, int32_t T, int32_t Hq, int32_t Hkv,
+    int32_t head_dim, int32_t faithful_rounding, int32_t dtype, const MiTuning* tuning, void* stream) {
+  NormRopeParams p = split_params(q, q_stride_tok, q_out, q_out_stride_tok, k, k_stride_tok, k_out, k_out_stride_tok, v, v_stride_tok,
+                                  q_weight, k_weight, eps, norm_kind, rotary_angles, angles_stride, rot_dim, rotary_interleaved, mscale,
+                                  q_positions, k_positions, k_cache, v_cache, kv_stride_chunk, kv_stride_tok, token_to_chunk_idx,
+                                  token_to_local_pos, block_table, bt_stride, kv_lens, chunk_tokens, T, Hq, Hkv, head_dim, faithful_rounding);
   return norm_rope_launch(p, dtype, tuning, (hipStream_t)stream, "mi_norm_rope_append");
 }
 
@@ -665,33 +1015,47 @@ extern "C" int mi_qkv_norm_rope_append(
     const int32_t* kv_lens, int32_t chunk_tokens, int32_t T, int32_t Hq, int32_t Hkv,
     int32_t head_dim, int32_t faithful_rounding, int32_t dtype, const MiTuning* tuning, void* stream) {
   if (T == 0) return MI_OK;
-  if (!mixed_qkv) return mi_fail(MI_ERR_NULL, "mi_qkv_norm_rope_append: mixed_qkv missing");
-  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
-    return mi_fail(MI_ERR_SHAPE, "mi_qkv_norm_rope_append: query heads must be a positive multiple of KV heads");
-  if (!k_cache && !k_out)
-    return mi_fail(MI_ERR_NULL, "mi_qkv_norm_rope_append: the key needs a destination (k_out and/or the cache)");
-  const int G = Hq / Hkv;
-  const int64_t group = (int64_t)(G + 2) * head_dim;  // elements of one query group: G q heads, k, v
-  if (qkv_stride_tok < group * Hkv)
-    return mi_fail(MI_ERR_SHAPE, "mi_qkv_norm_rope_append: token stride smaller than (Hq + 2 Hkv) * head_dim");
-  const uint16_t* base = (const uint16_t*)mixed_qkv;
-  NormRopeParams p = {};
-  p.q = base; p.q_st = qkv_stride_tok; p.q_gst = group; p.q_group = G;
-  p.q_out = (uint16_t*)q_out; p.qo_st = q_out_stride_tok;
-  p.k = base + (int64_t)G * head_dim; p.k_st = qkv_stride_tok; p.k_hst = group;
-  p.k_out = (uint16_t*)k_out; p.ko_st = k_out_stride_tok;
-  p.v = k_cache ? base + (int64_t)(G + 1) * head_dim : nullptr; p.v_st = qkv_stride_tok; p.v_hst = group;
-  p.q_w = (const uint16_t*)q_weight; p.k_w = (const uint16_t*)k_weight;
-  p.emb = rotary_angles; p.emb_stride = angles_stride;
-  p.q_pos = q_positions; p.k_pos = k_positions;
-  p.kc = (uint16_t*)k_cache; p.vc = (uint16_t*)v_cache;
-  p.chunk_elems = kv_stride_chunk; p.tok_elems = kv_stride_tok;
-  p.tok_chunk = token_to_chunk_idx; p.tok_local = token_to_local_pos;
-  p.bt = block_table; p.bt_stride = bt_stride; p.lens = kv_lens;
-  p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.d = head_dim; p.rot = rot_dim; p.chunk = chunk_tokens;
-  p.norm = norm_kind; p.interleaved = rotary_interleaved; p.faithful = faithful_rounding;
-  p.eps = eps; p.mscale = mscale;
-  return norm_rope_launch(p, dtype, tuning, (hipStream_t)stream, "mi_qkv_norm_rope_append");
+  NormRopeParams p = split_params(nullptr, 0, q_out, q_out_stride_tok, nullptr, 0, k_out, k_out_stride_tok, nullptr, 0, q_weight,
+                                  k_weight, eps, norm_kind, rotary_angles, angles_stride, rot_dim, rotary_interleaved, mscale,
+                                  q_positions, k_positions, k_cache, v_cache, kv_stride_chunk, kv_stride_tok, token_to_chunk_idx,
+                                  token_to_local_pos, block_table, bt_stride, kv_lens, chunk_tokens, T, Hq, Hkv, head_dim, faithful_rounding);
+  const int rc = mixed_params(p, mixed_qkv, qkv_stride_tok, "mi_qkv_norm_rope_append");
+  return rc != MI_OK ? rc : norm_rope_launch(p, dtype, tuning, (hipStream_t)stream, "mi_qkv_norm_rope_append");
+}
+
+extern "C" int mi_norm_rope_append_axes(
+    const void* q, int64_t q_stride_tok, void* q_out, int64_t q_out_stride_tok, const void* k, int64_t k_stride_tok, void* k_out,
+    int64_t k_out_stride_tok, const void* v, int64_t v_stride_tok, const void* q_weight, const void* k_weight, float eps,
+    int32_t norm_kind, const float* rotary_angles, int64_t angles_stride, int32_t angles_rows, int32_t rot_dim,
+    int32_t rotary_interleaved, float mscale, const int64_t* positions, int64_t positions_stride, int32_t axes,
+    const uint8_t* pair_axes, void* k_cache, void* v_cache, int64_t kv_stride_chunk, int64_t kv_stride_tok,
+    const int64_t* token_to_chunk_idx, const int64_t* token_to_local_pos, const int32_t* block_table, int64_t bt_stride,
+    const int32_t* kv_lens, int32_t chunk_tokens, int32_t T, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t faithful_rounding,
+    int32_t dtype, const MiTuning* tuning, void* stream) {
+  if (T == 0) return MI_OK;
+  const NormRopeParams p = split_params(
+      q, q_stride_tok, q_out, q_out_stride_tok, k, k_stride_tok, k_out, k_out_stride_tok, v, v_stride_tok, q_weight, k_weight, eps, norm_kind,
+      rotary_angles, angles_stride, rot_dim, rotary_interleaved, mscale, nullptr, nullptr, k_cache, v_cache, kv_stride_chunk, kv_stride_tok,
+      token_to_chunk_idx, token_to_local_pos, block_table, bt_stride, kv_lens, chunk_tokens, T, Hq, Hkv, head_dim, faithful_rounding);
+  return axes_launch(p, positions, positions_stride, axes, pair_axes, angles_rows, dtype, tuning, stream, "mi_norm_rope_append_axes");
+}
+
+extern "C" int mi_qkv_norm_rope_append_axes(
+    const void* mixed_qkv, int64_t qkv_stride_tok, void* q_out, int64_t q_out_stride_tok, void* k_out, int64_t k_out_stride_tok,
+    const void* q_weight, const void* k_weight, float eps, int32_t norm_kind, const float* rotary_angles, int64_t angles_stride,
+    int32_t angles_rows, int32_t rot_dim, int32_t rotary_interleaved, float mscale, const int64_t* positions,
+    int64_t positions_stride, int32_t axes, const uint8_t* pair_axes, void* k_cache, void* v_cache, int64_t kv_stride_chunk,
+    int64_t kv_stride_tok, const int64_t* token_to_chunk_idx, const int64_t* token_to_local_pos, const int32_t* block_table,
+    int64_t bt_stride, const int32_t* kv_lens, int32_t chunk_tokens, int32_t T, int32_t Hq, int32_t Hkv, int32_t head_dim,
+    int32_t faithful_rounding, int32_t dtype, const MiTuning* tuning, void* stream) {
+  if (T == 0) return MI_OK;
+  NormRopeParams p = split_params(
+      nullptr, 0, q_out, q_out_stride_tok, nullptr, 0, k_out, k_out_stride_tok, nullptr, 0, q_weight, k_weight, eps, norm_kind, rotary_angles,
+      angles_stride, rot_dim, rotary_interleaved, mscale, nullptr, nullptr, k_cache, v_cache, kv_stride_chunk, kv_stride_tok,
+      token_to_chunk_idx, token_to_local_pos, block_table, bt_stride, kv_lens, chunk_tokens, T, Hq, Hkv, head_dim, faithful_rounding);
+  const int rc = mixed_params(p, mixed_qkv, qkv_stride_tok, "mi_qkv_norm_rope_append_axes");
+  if (rc != MI_OK) return rc;
+  return axes_launch(p, positions, positions_stride, axes, pair_axes, angles_rows, dtype, tuning, stream, "mi_qkv_norm_rope_append_axes");
 }
 
 extern "C" int mi_qkv_key_append(

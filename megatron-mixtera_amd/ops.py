@@ -374,13 +374,33 @@ def norm_rope_append(query: Optional[Tensor], key: Optional[Tensor], *, value: O
                      k_cache: Optional[Tensor] = None, v_cache: Optional[Tensor] = None,
                      token_to_chunk_idx: Optional[Tensor] = None, token_to_local_pos: Optional[Tensor] = None,
                      block_table: Optional[Tensor] = None, kv_lens: Optional[Tensor] = None,
-                     faithful_rounding: bool = True) -> None:
+                     faithful_rounding: bool = True, rotary_axes: Optional[bytes] = None) -> None:
     """Norm (none / rms / l2) then RoPE on ``query`` (in place unless ``query_out`` is given) and on
-    ``key`` (result to ``key_out`` and/or straight into the cache slot, together with ``value``)."""
+    ``key`` (result to ``key_out`` and/or straight into the cache slot, together with ``value``).
+
+    With ``rotary_axes`` (one byte per rotary pair, see :func:`rotary_axes`) positions have several axes: ``q_positions`` is
+    int64 ``[axes, T]`` (up to four), for queries and keys alike, and a pair turns by the angle at its axis's position.
+    Positions outside the table count as its first or last row."""
     _native().norm_rope_append(query, key, value, q_weight, k_weight, eps, _NORM_KINDS[norm], rotary_emb, q_positions,
                                k_positions, rotary_interleaved, mscale, query_out, key_out, k_cache, v_cache,
                                token_to_chunk_idx, token_to_local_pos, block_table, kv_lens, faithful_rounding,
-                               _tuning_arg())
+                               _tuning_arg(), rotary_axes)
+
+
+def rotary_axes(sections, alternate: bool = False) -> bytes:
+    """The axis of every rotary pair for ``rotary_axes=`` of the calls here: ``sections`` says how many pairs each axis has
+    (time, height, width).  The sections follow one another; with ``alternate`` the axes take turns instead, pair i axis
+    i modulo their number as far as that axis's section goes, and the rest belongs to the first."""
+    sections = [int(n) for n in sections]
+    _require(1 <= len(sections) <= 4 and all(n >= 0 for n in sections) and sum(sections) >= 1, "one to four axes, and a pair")
+    if not alternate:
+        return bytes(axis for axis, n in enumerate(sections) for _ in range(n))
+    pairs, step = bytearray(sum(sections)), len(sections)
+    for axis, n in enumerate(sections[1:], 1):
+        places = range(axis, min(axis + step * n, len(pairs)), step)
+        _require(len(places) == n, "the axes' turns end before a section does")
+        pairs[axis:axis + step * n:step] = bytes([axis]) * n
+    return bytes(pairs)
 
 
 def qkv_norm_rope_append(mixed_qkv: Tensor, *, num_query_heads: int, num_kv_heads: int, query_out: Tensor,
@@ -391,14 +411,15 @@ def qkv_norm_rope_append(mixed_qkv: Tensor, *, num_query_heads: int, num_kv_head
                          mscale: float = 1.0, k_cache: Optional[Tensor] = None, v_cache: Optional[Tensor] = None,
                          token_to_chunk_idx: Optional[Tensor] = None, token_to_local_pos: Optional[Tensor] = None,
                          block_table: Optional[Tensor] = None, kv_lens: Optional[Tensor] = None,
-                         faithful_rounding: bool = True) -> None:
+                         faithful_rounding: bool = True, rotary_axes: Optional[bytes] = None) -> None:
     """:func:`norm_rope_append` reading the QKV projection's output ``[T, (1,) (Hq + 2 Hkv) * d]`` (per
     query group: its query heads, then its key head, then its value head -- the layout that
-    ``get_query_key_value_tensors`` splits, attention.py:985-1030) without materialising the split."""
+    ``get_query_key_value_tensors`` splits, attention.py:985-1030) without materialising the split.
+    ``rotary_axes`` as there."""
     _native().qkv_norm_rope_append(mixed_qkv, num_query_heads, num_kv_heads, query_out, key_out, q_weight, k_weight, eps,
                                    _NORM_KINDS[norm], rotary_emb, q_positions, k_positions, rotary_interleaved, mscale,
                                    k_cache, v_cache, token_to_chunk_idx, token_to_local_pos, block_table, kv_lens,
-                                   faithful_rounding, _tuning_arg())
+                                   faithful_rounding, _tuning_arg(), rotary_axes)
 
 
 def qkv_prefill_supported(head_dim: int, chunk_tokens: int, rotary_emb: Optional[Tensor]) -> bool:
