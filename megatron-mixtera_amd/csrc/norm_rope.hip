@@ -67,6 +67,9 @@ struct AxesParams : NormRopeParams {
   int32_t n_axes, emb_rows;   // positions are kept inside the table's rows
   uint32_t axes[8];           // two bits per pair, from the lowest
   int32_t waves_per_token;
+  uint32_t wpt_magic;         // ceil(2^32 / waves_per_token), for more than one
+  int32_t q_gap;              // elements between the heads of two groups of queries, beyond their width
+  float q_group_inv;
 };
 
 // one rounding to the tensors' 16-bit type and back
@@ -90,24 +93,18 @@ static __device__ __forceinline__ const uint16_t* head_vector(const NormRopePara
   return p.k + (int64_t)t * p.k_st + (int64_t)(vec - p.Hq) * p.k_hst;
 }
 
-// The row of the angle table that element e of the token's heads turns by; pos: the token's positions, kept inside the table.
-static __device__ __forceinline__ int64_t axis_position(const AxesParams& p, const int64_t (&pos)[4], int e) {
+// The token's position on the axis of element e of its heads (e below the rotary width), as it stands in memory.
+static __device__ __forceinline__ int64_t axis_position(const AxesParams& p, int t, int e) {
   const int half = p.rot >> 1, pair = p.interleaved ? e >> 1 : e < half ? e : e - half;
-  uint32_t word = p.axes[0];
+  uint32_t word = 0;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) word = pair >> 4 == i ? p.axes[i] : word;
-  const int axis = word >> (2 * (pair & 15)) & 3;
-  int64_t at = pos[0];
-#pragma unroll
-  for (int i = 1; i < 4; ++i) at = axis == i ? pos[i] : at;
-  return at;
-}
-static __device__ __forceinline__ void load_axes(const AxesParams& p, int t, int64_t (&pos)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t at = i < p.n_axes ? p.q_pos[i * p.pos_st + t] : 0;
-    pos[i] = at < 0 ? 0 : at < p.emb_rows ? at : p.emb_rows - 1;
+  for (int i = 0; i < 8; ++i) {
+    uint32_t w = p.axes[i];
+    asm volatile("" : "+v"(w));   // (eight words and a choice: an indexed load would be a trip to memory of its own)
+    word = pair >> 4 == i ? w : word;
   }
+  const int axis = word >> (2 * (pair & 15)) & 3;
+  return p.q_pos[axis * p.pos_st + t];
 }
 
 // P: NormRopeParams, or AxesParams for positions with several axes.
@@ -152,8 +149,6 @@ __global__ __launch_bounds__(256) void norm_rope_append_kernel(P p) {
   if (p.emb) {
     const int64_t qp = !AXES && p.q_pos ? p.q_pos[t] : 0;
     const int64_t kp = !AXES && p.k_pos ? p.k_pos[t] : qp;
-    int64_t axes_pos[4];
-    if constexpr (AXES) load_axes(p, t, axes_pos);
 #pragma unroll
     for (int w = 0; w < EPL; ++w) {
       const int e = i + w * LPV;
@@ -176,8 +171,10 @@ __global__ __launch_bounds__(256) void norm_rope_append_kernel(P p) {
           }
           if ((which == 0 && p.Hq == 0) || (which == 1 && p.Hkv == 0)) continue;
           float a;
-          if constexpr (AXES) a = p.emb[axis_position(p, axes_pos, e) * p.emb_stride + e];
-          else a = p.emb[(which ? kp : qp) * p.emb_stride + e];
+          if constexpr (AXES) {
+            const int64_t pos = axis_position(p, t, e);
+            a = p.emb[(pos < 0 ? 0 : pos < p.emb_rows ? pos : p.emb_rows - 1) * p.emb_stride + e];
+          } else a = p.emb[(which ? kp : qp) * p.emb_stride + e];
           float c, sn;
           rotary_sincos(a, &sn, &c);
           c *= p.mscale;
@@ -469,90 +466,102 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6, 8))) voi
   }
 }
 
+// c ? a : b with both at hand: as branches that read one or the other, variables that lambdas share would go through memory.
+template <typename T>
+static __device__ __forceinline__ T pick(bool c, T a, T b) { return c ? a : b; }
+
 // Positions with several axes, 16 bytes to a lane: one wavefront per token (or several, where tokens are few), which works the
 // token's angles out once, two elements to a lane, hands them round through its own LDS and keeps those of its lanes' eight
 // columns in registers for all of the token's heads: a lane has the same columns of every head.  Then a stream of head vectors,
-// four loads ahead: queries, keys, values.  No barrier anywhere.
+// two at a time with the next two on their way: queries, keys, values.  No barrier anywhere.
 //
 // In one rounding (`faithful` 0) the norm weight is multiplied into cos and sin beforehand and the reciprocal norm comes last:
 // out = rstd (x (w cos) + x' (w' sin)), three multiply-adds a value; the partner's values come from its lane as packed words.
-template <int D, bool F16, bool FAITHFUL>
+//
+// PARTNER: 0 a pair's elements are neighbours, in one lane; 1 they are D / 2 apart, half a vector's lanes; 2 any whole number of
+// lanes apart.  (A kernel of its own each: the code of a short call is fetched anew, 18 us of 64 tokens were its 16 KB.)
+template <int D, bool F16, bool FAITHFUL, int PARTNER>
 __global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
   constexpr int LPV = D / 8;                               // lanes that hold a head vector
   constexpr int LPG = LPV <= 8 ? 8 : LPV <= 16 ? 16 : 32;  // lane group of one (a power of two)
-  constexpr int VPP = 64 / LPG;                            // head vectors per pass
+  constexpr int VPP = 64 / LPG;                            // head vectors a load of the wavefront brings
   constexpr int NE = (D + 63) / 64;                        // angles per lane
+  static_assert(PARTNER != 1 || LPG == LPV, "half a power of two of lanes apart");
   __shared__ __align__(16) float cs_all[4][2][D];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int job = blockIdx.x * 4 + wave;
-  const int t = job / p.waves_per_token, part = job - t * p.waves_per_token;
+  const uint32_t job = blockIdx.x * 4u + (uint32_t)wave;
+  const int wpt = p.waves_per_token;
+  const int t = wpt == 1 ? (int)job : (int)__umulhi(job, p.wpt_magic), part = (int)job - t * wpt;
   if (t >= p.T) return;
   float (&cs)[2][D] = cs_all[wave];
   const int li = lane % LPG, sub = lane / LPG;
   const bool on = LPG == LPV || li < LPV;
   const int e0 = on ? 8 * li : 0;
 
-  // passes: query heads, key heads, values; this wavefront's share
-  const bool to_cache = p.kc != nullptr;
-  const int nq = (p.Hq + VPP - 1) / VPP, nk = (p.Hkv + VPP - 1) / VPP, all = nq + nk + (to_cache ? nk : 0);
-  const int first = (int)((int64_t)all * part / p.waves_per_token), end = (int)((int64_t)all * (part + 1) / p.waves_per_token);
-  auto head_of = [&](int pass) { return (pass < nq ? pass : pass < nq + nk ? pass - nq : pass - nq - nk) * VPP + sub; };
-  auto load = [&](int pass) -> uint4 {
-    const int h = head_of(pass);
-    if (pass >= end || !on || h >= (pass < nq ? p.Hq : p.Hkv)) return make_uint4(0, 0, 0, 0);
-    if (pass < nq + nk) return ld16(head_vector(p, t, pass < nq ? h : p.Hq + h) + e0);
-    return ld16(p.v + (int64_t)t * p.v_st + (int64_t)h * p.v_hst + e0);
+  // steps of two loads: query heads, key heads, values; this wavefront's share
+  const int Hq = p.Hq, Hkv = p.Hkv, k_hst = (int)p.k_hst, v_hst = (int)p.v_hst, q_gap = p.q_gap;
+  const uint16_t *const q_w = p.q_w, *const k_w = p.k_w;
+  uint16_t *const kc = p.kc, *const vc = p.vc;
+  const bool to_cache = kc != nullptr;
+  const int nq = (Hq + 2 * VPP - 1) / (2 * VPP), nk = (Hkv + 2 * VPP - 1) / (2 * VPP), all = nq + nk + (to_cache ? nk : 0);
+  const int first = wpt == 1 ? 0 : (int)__umulhi((uint32_t)(all * part), p.wpt_magic);
+  const int end = wpt == 1 ? all : (int)__umulhi((uint32_t)(all * (part + 1)), p.wpt_magic);
+  const uint16_t* const q_row = p.q + (int64_t)t * p.q_st;
+  const uint16_t* const k_row = p.k + (int64_t)t * p.k_st;
+  const uint16_t* const v_row = p.v + (int64_t)t * p.v_st;
+  struct Two { uint4 a, b; };
+  auto load = [&](int step) -> Two {
+    Two x = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (step >= end) return x;   // (uniform)
+    const bool is_q = step < nq, is_k = step < nq + nk;
+    const uint16_t* const row = pick(is_q, q_row, pick(is_k, k_row, v_row));
+    const int heads = pick(is_q, Hq, Hkv), stride = pick(is_q, D, pick(is_k, k_hst, v_hst)), gap = pick(is_q, q_gap, 0);
+    const int h = 2 * VPP * (step - pick(is_q, 0, pick(is_k, nq, nq + nk))) + sub;
+    auto at = [&](int head) { return row + (uint32_t)(head * stride + (int)(((float)head + 0.5f) * p.q_group_inv) * gap + e0); };
+    if (on && h < heads) x.a = ld16(at(h));
+    if (on && h + VPP < heads) x.b = ld16(at(h + VPP));
+    return x;
   };
-  constexpr int AHEAD = 4;
-  uint4 next[AHEAD];
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) next[i] = load(first + i);
+  Two next = load(first);
 
-  int64_t cache_off = -1;
-  if (to_cache) {
-    if (p.tok_chunk) {
-      cache_off = p.tok_chunk[t] * p.chunk_elems + p.tok_local[t] * p.tok_elems;
-    } else {
-      const int len = p.lens[t];
-      if (len > 0) {
-        const int pos = len - 1, ci = pos / p.chunk;
-        cache_off = (int64_t)p.bt[(int64_t)t * p.bt_stride + ci] * p.chunk_elems + (int64_t)(pos - ci * p.chunk) * p.tok_elems;
-      }
-    }
+  // the token's slot, its positions, the norm weights: all on their way before anything waits
+  int64_t slot_chunk = 0, slot_local = 0;
+  if (to_cache && p.tok_chunk) {
+    slot_chunk = p.tok_chunk[t];
+    slot_local = p.tok_local[t];
   }
   const int half = p.rot >> 1;
+  int64_t row[NE] = {};
+  if (p.emb) {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) row[i] = axis_position(p, t, min(lane + 64 * i, p.rot - 1));
+  }
   const bool rotate = p.emb && e0 < p.rot;   // (whole lanes: see the launch)
-  const int pe = p.interleaved ? e0 : e0 < half ? e0 + half : e0 - half;   // the partners' first column
+  const int pe = PARTNER == 0 || !rotate ? e0 : e0 < half ? e0 + half : e0 - half;   // the partners' first column
   auto weight = [&](const uint16_t* w, int at) {
     return p.norm == MI_NORM_RMS && w ? ld16(w + at) : make_uint4(ones2<F16>(), ones2<F16>(), ones2<F16>(), ones2<F16>());
   };
-  const int at_p = rotate ? pe : e0;
-  const uint4 wq = weight(p.q_w, e0), wk = weight(p.k_w, e0);
-  const uint4 wq_p = FAITHFUL ? wq : weight(p.q_w, at_p), wk_p = FAITHFUL ? wk : weight(p.k_w, at_p);
+  uint4 w_own = weight(pick(first < nq, q_w, k_w), e0), w_partner = FAITHFUL ? w_own : weight(pick(first < nq, q_w, k_w), pe);
   if (p.emb) {
-    int64_t pos[4];
-    load_axes(p, t, pos);
     float a[NE];
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const int e = lane + 64 * i;
-      a[i] = e < p.rot ? p.emb[axis_position(p, pos, e) * p.emb_stride + e] : 0.f;
+      const int64_t at = row[i] < 0 ? 0 : row[i] < p.emb_rows ? row[i] : p.emb_rows - 1;
+      a[i] = p.emb[at * p.emb_stride + min(lane + 64 * i, p.rot - 1)];
     }
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
       const int e = lane + 64 * i;
-      float c = 1.f, sn = 0.f;
-      if (e < p.rot) {
-        rotary_sincos(a[i], &sn, &c);
-        c *= p.mscale;
-        sn *= p.mscale;
-        if (FAITHFUL) {
-          c = round16<F16>(c);
-          sn = round16<F16>(sn);
-        }
-        if (p.interleaved ? (e & 1) == 0 : e < half) sn = -sn;
+      float c, sn;
+      rotary_sincos(a[i], &sn, &c);
+      c *= p.mscale;
+      sn *= p.mscale;
+      if (FAITHFUL) {
+        c = round16<F16>(c);
+        sn = round16<F16>(sn);
       }
-      if (e < D) {
+      if (PARTNER == 0 ? (e & 1) == 0 : e < half) sn = -sn;
+      if (e < D) {   // (columns beyond the rotary width: never used)
         cs[0][e] = c;
         cs[1][e] = sn;
       }
@@ -561,49 +570,55 @@ __global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
+  int64_t cache_off = -1;
+  if (to_cache) {
+    if (p.tok_chunk) {
+      cache_off = slot_chunk * p.chunk_elems + slot_local * p.tok_elems;
+    } else {
+      const int len = p.lens[t];
+      if (len > 0) {
+        const int pos = len - 1, ci = pos / p.chunk;
+        cache_off = (int64_t)p.bt[(int64_t)t * p.bt_stride + ci] * p.chunk_elems + (int64_t)(pos - ci * p.chunk) * p.tok_elems;
+      }
+    }
+  }
   auto unpack = [](const uint4& w, float (&y)[8]) {
     const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) { y[2 * j] = lo_to_f32<F16>(w4[j]); y[2 * j + 1] = hi_to_f32<F16>(w4[j]); }
   };
-  float c[8], sn[8], w[8];   // of the lane's columns, times the weights where rounded once
-  auto factors = [&](const uint4& own, const uint4& partners) {
-    unpack(own, w);
+  float c[8], sn[8], w[8];   // of the lane's columns, times the weights where rounded once; w: the weights, or (once) 1 where c has them
+  auto factors = [&] {
+    unpack(w_own, w);
 #pragma unroll
     for (int j = 0; j < 8; j += 4) {
-      const float4 c4 = p.emb ? *reinterpret_cast<const float4*>(&cs[0][e0 + j]) : make_float4(1.f, 1.f, 1.f, 1.f);
-      const float4 s4 = p.emb ? *reinterpret_cast<const float4*>(&cs[1][e0 + j]) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 c4 = *reinterpret_cast<const float4*>(&cs[0][e0 + j]);
+      const float4 s4 = *reinterpret_cast<const float4*>(&cs[1][e0 + j]);
       c[j] = c4.x; c[j + 1] = c4.y; c[j + 2] = c4.z; c[j + 3] = c4.w;
       sn[j] = s4.x; sn[j + 1] = s4.y; sn[j + 2] = s4.z; sn[j + 3] = s4.w;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      c[j] = rotate ? c[j] : 1.f;
+      sn[j] = rotate ? sn[j] : 0.f;
+    }
     if (!FAITHFUL) {
       float wp[8];
-      unpack(partners, wp);
+      unpack(w_partner, wp);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         c[j] *= w[j];
-        sn[j] *= p.interleaved ? wp[j ^ 1] : wp[j];
+        sn[j] *= PARTNER == 0 ? wp[j ^ 1] : wp[j];
       }
     }
   };
   // the words that hold the partners of a lane's eight values
-  const int plane = half >> 3;
-  const bool pow2 = plane > 0 && (plane & (plane - 1)) == 0 && 2 * plane <= LPG;
   const int src_lane = lane - li + (pe >> 3);
   auto partners = [&](const uint4& x) -> uint4 {
     auto through = [&](auto&& move) { return make_uint4(move(x.x), move(x.y), move(x.z), move(x.w)); };
-    auto xored = [&](auto Pc) {
-      return through([](uint32_t v) { return __float_as_uint(lane_xor<decltype(Pc)::value>(__uint_as_float(v))); });
-    };
-    if (p.interleaved) return through([](uint32_t v) { return __builtin_amdgcn_alignbit(v, v, 16); });
-    if (pow2) {
-      if (plane == 8) return xored(std::integral_constant<int, 8>{});
-      if (plane == 4) return xored(std::integral_constant<int, 4>{});
-      if (plane == 16) return xored(std::integral_constant<int, 16>{});
-      if (plane == 2) return xored(std::integral_constant<int, 2>{});
-      return xored(std::integral_constant<int, 1>{});
-    }
-    return through([&](uint32_t v) { return (uint32_t)__shfl((int)v, src_lane, 64); });
+    if constexpr (PARTNER == 0) return through([](uint32_t v) { return __builtin_amdgcn_alignbit(v, v, 16); });
+    else if constexpr (PARTNER == 1) return through([](uint32_t v) { return __float_as_uint(lane_xor<LPV / 2>(__uint_as_float(v))); });
+    else return through([&](uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_bpermute(4 * src_lane, (int)v); });
   };
   auto turned = [&](const uint4& raw) -> uint4 {
     float x[8], xp[8], o[8], rstd = 1.f;
@@ -618,11 +633,10 @@ __global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
       uint4 y = raw;
       if (p.norm != MI_NORM_NONE) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = p.norm == MI_NORM_RMS ? x[j] * rstd * w[j] : x[j] * rstd;
+        for (int j = 0; j < 8; ++j) x[j] = x[j] * rstd * w[j];   // (without weights they are ones)
         y = make_uint4(pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(x[4], x[5]), pack2<F16>(x[6], x[7]));
         unpack(y, x);
       }
-      if (!p.emb) return y;
       unpack(partners(y), xp);
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
@@ -633,41 +647,39 @@ __global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
         o[j + 1] = rotate ? a1 + b1 : x[j + 1];
       }
     } else {
-      if (p.emb) unpack(partners(raw), xp);
+      unpack(partners(raw), xp);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float turn = p.emb ? __builtin_fmaf(xp[j], sn[j], x[j] * c[j]) : x[j] * c[j];
-        o[j] = (rotate ? turn : x[j] * w[j]) * rstd;
+        const float own = x[j] * c[j];   // (columns that pass through: times the weight, and no zero times a partner)
+        o[j] = (rotate ? __builtin_fmaf(xp[j], sn[j], own) : own) * rstd;
       }
     }
     return make_uint4(pack2<F16>(o[0], o[1]), pack2<F16>(o[2], o[3]), pack2<F16>(o[4], o[5]), pack2<F16>(o[6], o[7]));
   };
-  factors(first < nq ? wq : wk, first < nq ? wq_p : wk_p);
-  for (int pass0 = first; pass0 < end; pass0 += AHEAD) {
-    uint4 now[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) now[i] = next[i];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) next[i] = load(pass0 + AHEAD + i);
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int pass = pass0 + i, h = head_of(pass);
-      if (pass >= end) break;
-      if (pass == nq && first < nq) factors(wk, wk_p);
-      const bool mine = on && h < (pass < nq ? p.Hq : p.Hkv);
-      if (pass < nq + nk) {
-        const uint4 out = turned(now[i]);
-        if (!mine) continue;
-        if (pass < nq) {
-          st16(p.q_out + (int64_t)t * p.qo_st + (int64_t)h * D + e0, out);
-        } else {
-          if (p.k_out) st16(p.k_out + (int64_t)t * p.ko_st + (int64_t)h * D + e0, out);
-          if (cache_off >= 0) st16(p.kc + cache_off + (int64_t)h * D + e0, out);
-        }
-      } else if (mine && cache_off >= 0) {
-        st16(p.vc + cache_off + (int64_t)h * D + e0, now[i]);
+  factors();
+#pragma clang loop unroll(disable)
+  for (int step = first; step < end; ++step) {
+    Two now = next;
+    next = load(step + 1);
+    const bool is_q = step < nq, is_k = step < nq + nk;
+    if (is_k) {
+      if (step == nq && first < nq) {   // from the queries' weights to the keys'
+        w_own = weight(k_w, e0);
+        if (!FAITHFUL) w_partner = weight(k_w, pe);
+        factors();
       }
+      now.a = turned(now.a);
+      now.b = turned(now.b);
     }
+    const int heads = pick(is_q, Hq, Hkv), h = 2 * VPP * (step - pick(is_q, 0, pick(is_k, nq, nq + nk))) + sub;
+    const bool mine_a = on && h < heads, mine_b = on && h + VPP < heads;
+    auto store = [&](uint16_t* dst) {
+      if (mine_a) st16(dst + (uint32_t)(h * D + e0), now.a);
+      if (mine_b) st16(dst + (uint32_t)((h + VPP) * D + e0), now.b);
+    };
+    if (is_q) store(p.q_out + (int64_t)t * p.qo_st);
+    else if (is_k && p.k_out) store(p.k_out + (int64_t)t * p.ko_st);
+    if (!is_q && cache_off >= 0) store(pick(is_k, kc, vc) + cache_off);
   }
 }
 
@@ -789,26 +801,40 @@ using namespace mi;
 namespace {
 
 // Wavefronts per token of norm_rope_axes_kernel: one where tokens fill the chip, else as many as give 4 096 in all, at most one
-// pass each.
+// step each.
 void launch_axes(AxesParams& p, bool f16, hipStream_t st) {
-  const int vpp = p.d == 64 ? 8 : p.d <= 128 ? 4 : 2;
-  const int nq = (p.Hq + vpp - 1) / vpp, nk = (p.Hkv + vpp - 1) / vpp, all = nq + nk * (p.kc ? 2 : 1);
+  const int per_step = p.d == 64 ? 16 : p.d <= 128 ? 8 : 4;
+  const int nq = (p.Hq + per_step - 1) / per_step, nk = (p.Hkv + per_step - 1) / per_step, all = nq + nk * (p.kc ? 2 : 1);
   int n = (4096 + p.T - 1) / p.T;
-  p.waves_per_token = n < 1 ? 1 : n > all ? all : n;
-  const dim3 grid((unsigned)(((int64_t)p.T * p.waves_per_token + 3) / 4));
-#define MI_AXES(D_)                                                                                                         \
+  n = n < 1 ? 1 : n > all ? all : n;
+  p.waves_per_token = n;
+  p.wpt_magic = n > 1 ? (uint32_t)((((uint64_t)1 << 32) + n - 1) / n) : 0u;   // (exact below 2^32 / n: at most 4 096 + n jobs)
+  p.q_gap = p.q_gst ? (int32_t)(p.q_gst - (int64_t)p.q_group * p.d) : 0;
+  p.q_group_inv = 1.f / (float)p.q_group;
+  const dim3 grid((unsigned)(((int64_t)p.T * n + 3) / 4));
+#define MI_AXES(D_, PARTNER_)                                                                                               \
   do {                                                                                                                      \
-    if (f16 && p.faithful) hipLaunchKernelGGL((norm_rope_axes_kernel<D_, true, true>), grid, dim3(256), 0, st, p);          \
-    else if (f16) hipLaunchKernelGGL((norm_rope_axes_kernel<D_, true, false>), grid, dim3(256), 0, st, p);                  \
-    else if (p.faithful) hipLaunchKernelGGL((norm_rope_axes_kernel<D_, false, true>), grid, dim3(256), 0, st, p);           \
-    else hipLaunchKernelGGL((norm_rope_axes_kernel<D_, false, false>), grid, dim3(256), 0, st, p);                          \
+    if (f16 && p.faithful) hipLaunchKernelGGL((norm_rope_axes_kernel<D_, true, true, PARTNER_>), grid, dim3(256), 0, st, p);\
+    else if (f16) hipLaunchKernelGGL((norm_rope_axes_kernel<D_, true, false, PARTNER_>), grid, dim3(256), 0, st, p);        \
+    else if (p.faithful) hipLaunchKernelGGL((norm_rope_axes_kernel<D_, false, true, PARTNER_>), grid, dim3(256), 0, st, p); \
+    else hipLaunchKernelGGL((norm_rope_axes_kernel<D_, false, false, PARTNER_>), grid, dim3(256), 0, st, p);                \
   } while (0)
-  if (p.d == 64) MI_AXES(64);
-  else if (p.d == 96) MI_AXES(96);
-  else if (p.d == 128) MI_AXES(128);
-  else if (p.d == 192) MI_AXES(192);
-  else MI_AXES(256);
+#define MI_AXES_ANY(D_)                                                                                                     \
+  do {                                                                                                                      \
+    if (p.interleaved) MI_AXES(D_, 0);                                                                                      \
+    else MI_AXES(D_, 2);                                                                                                    \
+  } while (0)
+  const bool across = !p.interleaved && p.rot == p.d;
+  if (p.d == 64 && across) MI_AXES(64, 1);
+  else if (p.d == 64) MI_AXES_ANY(64);
+  else if (p.d == 96) MI_AXES_ANY(96);
+  else if (p.d == 128 && across) MI_AXES(128, 1);
+  else if (p.d == 128) MI_AXES_ANY(128);
+  else if (p.d == 192) MI_AXES_ANY(192);
+  else if (across) MI_AXES(256, 1);
+  else MI_AXES_ANY(256);
 #undef MI_AXES
+#undef MI_AXES_ANY
 }
 
 // Argument checks shared by both entry points, kernel choice and launch.  `p` carries every pointer,
