@@ -295,7 +295,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams
     const int qi = (n * g_magic) >> 16, u = n - qi * G;  // n / G, n % G
     bool fine = true;
     if constexpr (WIN)
-      fine = finite_or_remade<HDV, TILE, false, F16>(p, acc[nt], l_tot, nt, nq, G, g_magic, r, q_begin + q0, h, hq0, shift + q0, Lk, wt, 0,
+      fine = finite_or_remade<HDV, TILE, false, F16>(p, acc[nt], l_tot, nt, nq, G, g_magic, r, q_begin + q0, h, hq0, shift + q0, Lk, wt, false, 0,
                                                      (walk_end + TILE - 1) / TILE, -1);
     if (qi < nq && fine) {
       uint16_t* o = p.out + (int64_t)(q_begin + q0 + qi) * p.o_st + (int64_t)(hq0 + u) * p.o_sh + 4 * DV * g;
@@ -950,7 +950,7 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
     const int qi = (n * g_magic) >> 16, u = n - qi * G;  // n / G, n % G
     bool fine = true;
     if constexpr (WIN)
-      fine = finite_or_remade<HD, kPPTile, FP8, F16>(p, acc[nt], l_tot, nt, nq, G, g_magic, r, q_begin + q0, h, hq0, shift + q0, Lk, wt, tb, te,
+      fine = finite_or_remade<HD, kPPTile, FP8, F16>(p, acc[nt], l_tot, nt, nq, G, g_magic, r, q_begin + q0, h, hq0, shift + q0, Lk, wt, false, tb, te,
                                                      SPLIT ? split : -1);
     if (qi < nq && fine) {
       if (!SPLIT) {

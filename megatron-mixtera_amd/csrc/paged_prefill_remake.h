@@ -12,11 +12,11 @@
 
 namespace mi {
 
-// One row: query head hq (KV head h) of row `row` at position `pos` of request r, over tiles [v0, v1) of the walk `wt`.  Every
-// argument is the same in all lanes.  `split` >= 0: the row's partial of that range instead of its result.
+// One row: query head hq (KV head h) of row `row` at position `pos` of request r, over tiles [v0, v1) of the walk `wt` (and tile
+// 0 where `sinks_too`).  Every argument is the same in all lanes.  `split` >= 0: the row's partial of that range instead of its result.
 template <int HD, int TILE, bool FP8, bool F16>
 static __device__ __forceinline__ void remake_row(const PrefillParams& p, int r, int row, int h, int hq, int pos, int Lk, const WindowTiles& wt,
-                                                  int v0, int v1, int split) {
+                                                  bool sinks_too, int v0, int v1, int split) {
   static_assert(TILE <= 64, "a lane per key");
   constexpr int ESZ = FP8 ? 1 : 2, NC = (HD + 63) / 64;
   const int lane = threadIdx.x & 63;
@@ -35,16 +35,17 @@ static __device__ __forceinline__ void remake_row(const PrefillParams& p, int r,
     return s * (FP8 ? p.k_scale[(int64_t)pc * p.Hkv + h] : 1.f) * p.scale_log2;
   };
   float m = -INFINITY;
-  for (int v = v0; v < v1; ++v) {
-    const int key = wt.real(v) * TILE + lane;
+  const int before = sinks_too ? v0 - 1 : v0;
+  for (int v = before; v < v1; ++v) {
+    const int key = (v < v0 ? 0 : wt.real(v)) * TILE + lane;
     if (seen(key)) m = fmaxf(m, score(key));
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f, acc[NC] = {};
-  for (int v = v0; v < v1; ++v) {
-    const int key0 = wt.real(v) * TILE, key = key0 + lane;
+  for (int v = before; v < v1; ++v) {
+    const int key0 = (v < v0 ? 0 : wt.real(v)) * TILE, key = key0 + lane;
     const bool mine = seen(key);
     const float e = mine ? fast_exp2(score(key) - ref) : 0.f;
     l += e;
@@ -84,8 +85,8 @@ static __device__ __forceinline__ void remake_row(const PrefillParams& p, int r,
 // heads of each from hq0 on.
 template <int HD, int TILE, bool FP8, bool F16, int N>
 static __device__ __forceinline__ bool finite_or_remade(const PrefillParams& p, const f32x4_t (&acc)[N], float l_tot, int nt, int nq, int G, int g_magic,
-                                                        int r, int row0, int h, int hq0, int pos0, int Lk, const WindowTiles& wt, int v0, int v1,
-                                                        int split) {
+                                                        int r, int row0, int h, int hq0, int pos0, int Lk, const WindowTiles& wt, bool sinks_too,
+                                                        int v0, int v1, int split) {
   float mark = l_tot * 0.f;
 #pragma unroll
   for (int e = 0; e < N; ++e)
@@ -97,7 +98,7 @@ static __device__ __forceinline__ bool finite_or_remade(const PrefillParams& p, 
   bad = (bad | bad >> 16) & 0xffffu;
   for (uint32_t left = (uint32_t)bad; left; left &= left - 1) {
     const int n = 16 * nt + __builtin_ctz(left), i = (n * g_magic) >> 16;   // n / G
-    if (i < nq) remake_row<HD, TILE, FP8, F16>(p, r, row0 + i, h, hq0 + n - i * G, pos0 + i, Lk, wt, v0, v1, split);
+    if (i < nq) remake_row<HD, TILE, FP8, F16>(p, r, row0 + i, h, hq0 + n - i * G, pos0 + i, Lk, wt, sinks_too, v0, v1, split);
   }
   return !(bad >> (threadIdx.x & 15) & 1);
 }

@@ -68,6 +68,9 @@ template <int HD> constexpr int wv_pitch() { return 2 * HD + 32; }
 // operands, whose exponents reach far below, 2^-30 under the 2 that the check looks for (one bit of a word); with fp16 1
 // under 2^8.
 template <bool F16> constexpr float kWvHeadroom = F16 ? 0.f : 30.f;
+// WIN: sinks that are taken ahead of the walk, as the value tile before the first.  A tile of their own is one of eleven for a
+// window of 500 (width 64: 11 ragged prompts 148 -> 130 us), one of nineteen for 1 024 (width 128: 292 -> 275).
+constexpr int kWvSinks = 32;
 constexpr float kNoReference = 3e38f;   // any score leaves the window; a masked one (-inf) stays a probability of zero
 // piece u of a tile's line -> its row, by multiplication
 template <int HD> constexpr unsigned wv_magic() { return 65536u / (wv_pitch<HD>() / 16) + 1; }
@@ -122,8 +125,14 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
   const int last = Lk - 1;
   const int kend_wg = min(Lk, shift + min(q0_wg + SBQ, Lq));
   WindowTiles wt = {};
+  bool sinks_first = false;   // WIN: this workgroup takes the sinks ahead of its walk
   if constexpr (WIN) {
     wt = window_tiles(p.window, p.sinks, kWvTile, shift + q0_wg);
+    if (p.sinks > 0 && p.sinks <= kWvSinks && wt.skip > 0) {   // (all of the workgroup's rows see them)
+      sinks_first = !SPLIT || blockIdx.y + 1 == gridDim.y;     // (the range that always has a tile)
+      wt.skip += wt.ns;
+      wt.ns = 0;
+    }
     wt.ns = __builtin_amdgcn_readfirstlane(wt.ns);
     wt.skip = __builtin_amdgcn_readfirstlane(wt.skip);
   }
@@ -461,6 +470,11 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
     const uint8_t* const k_lane = &Ks[0][0] + m16 * PITCH + 16 * g;
     const uint8_t* const v_lane = &Vs[0][0] + (4 * g + (m16 >> 2)) * PITCH + 8 * (m16 & 3);
 
+    // WIN, a tile that a border crosses: only the rows' ends, only the windows' starts, or both, or the sinks' end
+    enum { kBorderAny, kBorderEnd, kBorderWindow };
+    int border = kBorderAny;
+    const int gone_wave = full_until + max(nq, 1) - 1 - p.window;   // keys up to here are behind some row's window
+
     // S[x]: scores of the even (x = 0) / odd (x = 1) 32-key steps, P[x]: their probabilities as the B operand
     f32x4_t S[2][NQ][2];
     uint4 P[2][NQ];
@@ -602,12 +616,22 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
       auto mask_step = [&](int nt) {
         if (!MASK) return;
         const int dpos = qpos[nt] - (key0 + 4 * g);
-        const int gone = WIN ? dpos - p.window : 0, sunk = WIN ? p.sinks - (key0 + 4 * g) : 0;   // hidden: from `sunk` to `gone`
+        auto hide = [&](auto&& hidden) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i2 = 0; i2 < 4; ++i2)
-            if (16 * u + i2 > dpos || (WIN && 16 * u + i2 <= gone && 16 * u + i2 >= sunk)) Sn[nt][u][i2] = -INFINITY;
+            for (int i2 = 0; i2 < 4; ++i2)
+              if (hidden(16 * u + i2)) Sn[nt][u][i2] = -INFINITY;
+        };
+        if constexpr (!WIN) {
+          hide([&](int k) { return k > dpos; });
+        } else {
+          // (one border crosses most of the tiles that one crosses at all: one comparison for a score, not three)
+          const int gone = dpos - p.window, sunk = p.sinks - (key0 + 4 * g);   // hidden: from `sunk` to `gone`
+          if (border == kBorderEnd) hide([&](int k) { return k > dpos; });
+          else if (border == kBorderWindow) hide([&](int k) { return k <= gone; });
+          else hide([&](int k) { return k > dpos || (k <= gone && k >= sunk); });
+        }
       };
       // values; beside them the last probabilities, then the mask of the scores just multiplied
 #pragma unroll
@@ -638,7 +662,63 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
 
     // ---- prologue: clear the buffer of the value tile "before the first" (its probabilities are zeros, and zero times
     // a stale value must not be NaN; every other buffer is filled whole before it is read), start the first tiles ----
-    for (int i = tid * 16; i < BUF; i += THREADS * 16) *reinterpret_cast<uint4*>(&Vs[1][0] + i) = make_uint4(0u, 0u, 0u, 0u);
+    int sinks_chunk = 0;
+    if constexpr (WIN) {
+      // ... or the sinks' values, in its first rows
+      if (sinks_first) sinks_chunk = clamp_chunk(__builtin_amdgcn_readfirstlane(bt_row[0]), p.n_chunks);
+    }
+    float sinks_kscale = 1.f, sinks_vscale = 1.f;
+    if constexpr (WIN && FP8) {
+      if (sinks_first) {
+        sinks_kscale = uniform_float(p.k_scale[(int64_t)sinks_chunk * p.Hkv + h]);
+        sinks_vscale = uniform_float(p.v_scale[(int64_t)sinks_chunk * p.Hkv + h]);
+      }
+    }
+    uint4 sinks_k[2][KS] = {};   // operand fragments: keys 16 u + m16
+    if constexpr (WIN) {
+      if (sinks_first) {
+        const uint8_t* const base = reinterpret_cast<const uint8_t*>(kbase + (uint64_t)((int64_t)sinks_chunk * chunk_bytes));
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint8_t* const krow = base + (int64_t)min(16 * u + m16, p.sinks - 1) * tok_bytes;
+#pragma unroll
+          for (int kk = 0; kk < KS; ++kk) {
+            if constexpr (FP8) {
+              const uint2 raw8 = ld8(krow + 32 * kk + 8 * g);
+              sinks_k[u][kk] = make_uint4(raw8.x, raw8.y, 0u, 0u);
+            } else {
+              sinks_k[u][kk] = ld16(krow + 64 * kk + 16 * g);
+            }
+          }
+        }
+      }
+    }
+    for (int i = tid * 16; i < BUF; i += THREADS * 16) {
+      uint4 piece = make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (WIN) {
+        const uint32_t n = (uint32_t)i >> 4, prow = (n * wv_magic<HD>()) >> 16, pcol = n - (uint32_t)PIECES * prow;
+        if (sinks_first && (int)prow < p.sinks && pcol < (uint32_t)(HD / 8)) {
+          const uint8_t* const from = reinterpret_cast<const uint8_t*>(vbase + (uint64_t)((int64_t)sinks_chunk * chunk_bytes)) +
+                                      (int64_t)prow * tok_bytes + (8 * ESZ) * pcol;
+          if constexpr (FP8) {
+            const uint2 raw8 = ld8(from);
+            if constexpr (FACTOR) {
+              const uint32_t sign = sinks_vscale < 0.f ? 0x80808080u : 0u;
+              const float pow2 = value_pow2(sinks_vscale);
+              const uint2 lo = fp8x4_to_16x4<F16>(raw8.x ^ sign, pow2), hi = fp8x4_to_16x4<F16>(raw8.y ^ sign, pow2);
+              piece = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            } else {
+              const f32x2_t a = fp8x2_lo_to_f32(raw8.x), b = fp8x2_hi_to_f32(raw8.x), c = fp8x2_lo_to_f32(raw8.y), d = fp8x2_hi_to_f32(raw8.y);
+              piece = make_uint4(pack2<F16>(a.x * sinks_vscale, a.y * sinks_vscale), pack2<F16>(b.x * sinks_vscale, b.y * sinks_vscale),
+                                 pack2<F16>(c.x * sinks_vscale, c.y * sinks_vscale), pack2<F16>(d.x * sinks_vscale, d.y * sinks_vscale));
+            }
+          } else {
+            piece = ld16(from);
+          }
+        }
+      }
+      *reinterpret_cast<uint4*>(&Vs[1][0] + i) = piece;
+    }
     Cursor cur = cursor_at(tb + 2);
     int64_t off_first[2];   // tiles tb and tb + 1, started here
     uint32_t nrec_first[2];
@@ -668,6 +748,13 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk)
         asm volatile("" ::"v"(qf[nt][kk].x), "v"(qf[nt][kk].y), "v"(qf[nt][kk].z), "v"(qf[nt][kk].w));
+    if constexpr (WIN) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+          asm volatile("" ::"v"(sinks_k[u][kk].x), "v"(sinks_k[u][kk].y), "v"(sinks_k[u][kk].z), "v"(sinks_k[u][kk].w));
+    }
     if (raw) {
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
@@ -712,6 +799,46 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
       if (raw) norm_and_rotate();
       MI_SB();
     }
+    // The sinks' probabilities, against a reference of their own, wait for the first value product as those of a tile before the first.
+    if constexpr (WIN) {
+      if (sinks_first) {
+        const float scale = FP8 ? tile_scale(sinks_kscale) : p.scale_log2;
+        const uint32_t sign = FP8 && sinks_kscale < 0.f ? 0x80808080u : 0u;
+        if constexpr (FACTOR) factor_prev = value_factor(sinks_vscale);
+#pragma unroll
+        for (int nt = 0; nt < NQ; ++nt) {
+          f32x4_t s2[2];
+          float most = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            s2[u] = zero4;
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+              uint4 k4 = sinks_k[u][kk];
+              if constexpr (FP8) {
+                const uint2 lo = fp8x4_to_16x4<F16>(k4.x ^ sign), hi = fp8x4_to_16x4<F16>(k4.y ^ sign);
+                k4 = make_uint4(lo.x, lo.y, hi.x, hi.y);
+              }
+              s2[u] = mfma_16x16x32<F16>(k4, qf[nt][kk], s2[u]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (16 * u + 4 * g + i >= p.sinks) s2[u][i] = -INFINITY;
+              most = fmaxf(most, s2[u][i]);
+            }
+          }
+          neg_run[nt] = fminf(kNoReference, __builtin_fmaf(-rowgroup_max(most), scale, -kWvHeadroom<F16>));
+          const float neg = FACTOR ? neg_run[nt] + fast_log2(factor_prev) : neg_run[nt];
+          uint32_t w4[4];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              w4[2 * u + j] = pack2<F16>(fast_exp2(__builtin_fmaf(s2[u][2 * j], scale, neg)), fast_exp2(__builtin_fmaf(s2[u][2 * j + 1], scale, neg)));
+          P[0][nt] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+        }
+      }
+    }
     // key tile 0 has landed (this wavefront's share): only the loads issued after it may still be on their way
     if constexpr (!FP8) {
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
@@ -722,7 +849,6 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
     const int t_mask = max(0, (full_until + 1) >> 6);              // first tile with a masked score for this wavefront
     const int jm = min(max((WIN ? wt.walk(t_mask) : t_mask) - tb, 0), ntl);   // iterations [0, jm) need no mask
     // WIN: ... but those up to the last tile that holds a key behind some row's window, if one is no sink
-    const int gone_wave = full_until + max(nq, 1) - 1 - p.window;
     const int jw = WIN && gone_wave >= p.sinks ? min(max(wt.walk((gone_wave >> 6) + 1) - tb, 0), ntl) : 0;
     int j = 0;
     int even = 0;   // BUF where j is odd
@@ -738,6 +864,10 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
     // has left key tile j, the first half of value tile j-1 and the second half of value tile j-2: key tile j+2 and value
     // tiles j+1 (first half) and j (second half) take their places, under the products that follow, for the next barrier.
     auto iteration = [&](auto Mc) {
+      if constexpr (WIN && decltype(Mc)::value) {
+        const int t0 = wt.real(tb + j) * kWvTile;
+        border = t0 > gone_wave ? kBorderEnd : t0 + kWvTile - 1 <= full_until && t0 >= p.sinks ? kBorderWindow : kBorderAny;
+      }
       const uint8_t* ka = k_lane + even;
       const uint8_t* ka_next = k_lane + (BUF - even);
       const uint8_t* va = v_lane + (BUF - even);
@@ -859,7 +989,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
     const int qi = (n * g_magic) >> 16, u = n - qi * G;  // n / G, n % G
     bool fine = true;
     if constexpr (WIN)
-      fine = finite_or_remade<HD, kWvTile, FP8, F16>(p, acc[nt], l_tot, nt, nq, G, g_magic, r, q_begin + q0, h, hq0, shift + q0, Lk, wt, tb, te,
+      fine = finite_or_remade<HD, kWvTile, FP8, F16>(p, acc[nt], l_tot, nt, nq, G, g_magic, r, q_begin + q0, h, hq0, shift + q0, Lk, wt, sinks_first, tb, te,
                                                      SPLIT ? split : -1);
     if (qi < nq && fine) {
       if (!SPLIT) {
