@@ -396,6 +396,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
     };
     // where the walk goes on behind the sinks
     const int far_ci = WIN ? __builtin_amdgcn_readfirstlane((wt.ns + wt.skip) / tiles_per_chunk) : 0;
+    const int sinks_entry = WIN && sinks_first ? bt_row[0] : 0;
     const int far_tin = WIN ? wt.ns + wt.skip - far_ci * tiles_per_chunk : 0;
     auto cursor_next = [&](Cursor& c) {
       const bool adv = c.tile + 1 < te;
@@ -673,63 +674,108 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
 
     // ---- prologue: clear the buffer of the value tile "before the first" (its probabilities are zeros, and zero times
     // a stale value must not be NaN; every other buffer is filled whole before it is read), start the first tiles ----
-    int sinks_chunk = 0;
-    if constexpr (WIN) {
-      // ... or the sinks' values, in its first rows
-      if (sinks_first) sinks_chunk = clamp_chunk(__builtin_amdgcn_readfirstlane(bt_row[0]), p.n_chunks);
-    }
+    for (int i = tid * 16; i < BUF; i += THREADS * 16) *reinterpret_cast<uint4*>(&Vs[1][0] + i) = make_uint4(0u, 0u, 0u, 0u);
+    // WIN: the sinks, all on their way at once: operand fragments of the keys (16 u + m16), and the pieces of the values that go
+    // over the cleared buffer's first rows
+    constexpr int NSV = (kWvSinks * PIECES + THREADS - 1) / THREADS;
+    uint4 sinks_k[2][KS] = {}, sinks_v[NSV] = {};
     float sinks_kscale = 1.f, sinks_vscale = 1.f;
-    if constexpr (WIN && FP8) {
-      if (sinks_first) {
-        sinks_kscale = uniform_float(p.k_scale[(int64_t)sinks_chunk * p.Hkv + h]);
-        sinks_vscale = uniform_float(p.v_scale[(int64_t)sinks_chunk * p.Hkv + h]);
+    auto sinks_value_at = [&](int i, uint32_t& prow, uint32_t& pcol) {   // piece i of this thread: row and column in the buffer
+      const uint32_t n = (uint32_t)(tid + THREADS * i);
+      prow = (n * wv_magic<HD>()) >> 16;
+      pcol = n - (uint32_t)PIECES * prow;
+      return (int)prow < p.sinks && pcol < (uint32_t)(HD / 8);
+    };
+    auto sinks_request = [&] {
+      const int64_t chunk = clamp_chunk(__builtin_amdgcn_readfirstlane(sinks_entry), p.n_chunks);
+      if constexpr (FP8) {
+        sinks_kscale = p.k_scale[chunk * p.Hkv + h];
+        sinks_vscale = p.v_scale[chunk * p.Hkv + h];
       }
-    }
-    uint4 sinks_k[2][KS] = {};   // operand fragments: keys 16 u + m16
-    if constexpr (WIN) {
-      if (sinks_first) {
-        const uint8_t* const base = reinterpret_cast<const uint8_t*>(kbase + (uint64_t)((int64_t)sinks_chunk * chunk_bytes));
+      const uint8_t* const krows = reinterpret_cast<const uint8_t*>(kbase + (uint64_t)(chunk * chunk_bytes));
+      const uint8_t* const vrows = reinterpret_cast<const uint8_t*>(vbase + (uint64_t)(chunk * chunk_bytes));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t* const krow = krows + (int64_t)min(16 * u + m16, p.sinks - 1) * tok_bytes;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+          if constexpr (FP8) {
+            const uint2 raw8 = ld8(krow + 32 * kk + 8 * g);
+            sinks_k[u][kk] = make_uint4(raw8.x, raw8.y, 0u, 0u);
+          } else {
+            sinks_k[u][kk] = ld16(krow + 64 * kk + 16 * g);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NSV; ++i) {
+        uint32_t prow, pcol;
+        if (!sinks_value_at(i, prow, pcol)) continue;
+        const uint8_t* const from = vrows + (int64_t)prow * tok_bytes + (8 * ESZ) * pcol;
+        if constexpr (FP8) {
+          const uint2 raw8 = ld8(from);
+          sinks_v[i] = make_uint4(raw8.x, raw8.y, 0u, 0u);
+        } else {
+          sinks_v[i] = ld16(from);
+        }
+      }
+    };
+    // The sinks' probabilities, against a reference of their own, wait for the first value product as those of a tile before the first.
+    auto sinks_work = [&] {
+#pragma unroll
+      for (int i = 0; i < NSV; ++i) {
+        uint32_t prow, pcol;
+        if (!sinks_value_at(i, prow, pcol)) continue;
+        uint4 piece = sinks_v[i];
+        if constexpr (FACTOR) {
+          const uint32_t sign = sinks_vscale < 0.f ? 0x80808080u : 0u;
+          const float pow2 = value_pow2(sinks_vscale);
+          const uint2 lo = fp8x4_to_16x4<F16>(piece.x ^ sign, pow2), hi = fp8x4_to_16x4<F16>(piece.y ^ sign, pow2);
+          piece = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else if constexpr (FP8) {
+          const f32x2_t a = fp8x2_lo_to_f32(piece.x), b = fp8x2_hi_to_f32(piece.x), c = fp8x2_lo_to_f32(piece.y), d = fp8x2_hi_to_f32(piece.y);
+          piece = make_uint4(pack2<F16>(a.x * sinks_vscale, a.y * sinks_vscale), pack2<F16>(b.x * sinks_vscale, b.y * sinks_vscale),
+                             pack2<F16>(c.x * sinks_vscale, c.y * sinks_vscale), pack2<F16>(d.x * sinks_vscale, d.y * sinks_vscale));
+        }
+        *reinterpret_cast<uint4*>(&Vs[1][0] + prow * PITCH + 16 * pcol) = piece;
+      }
+      const float scale = FP8 ? tile_scale(sinks_kscale) : p.scale_log2;
+      const uint32_t sign = FP8 && sinks_kscale < 0.f ? 0x80808080u : 0u;
+      if constexpr (FACTOR) factor_prev = value_factor(sinks_vscale);
+#pragma unroll
+      for (int nt = 0; nt < NQ; ++nt) {
+        f32x4_t s2[2];
+        float most = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint8_t* const krow = base + (int64_t)min(16 * u + m16, p.sinks - 1) * tok_bytes;
+          s2[u] = zero4;
 #pragma unroll
           for (int kk = 0; kk < KS; ++kk) {
+            uint4 k4 = sinks_k[u][kk];
             if constexpr (FP8) {
-              const uint2 raw8 = ld8(krow + 32 * kk + 8 * g);
-              sinks_k[u][kk] = make_uint4(raw8.x, raw8.y, 0u, 0u);
-            } else {
-              sinks_k[u][kk] = ld16(krow + 64 * kk + 16 * g);
+              const uint2 lo = fp8x4_to_16x4<F16>(k4.x ^ sign), hi = fp8x4_to_16x4<F16>(k4.y ^ sign);
+              k4 = make_uint4(lo.x, lo.y, hi.x, hi.y);
             }
+            s2[u] = mfma_16x16x32<F16>(k4, qf[nt][kk], s2[u]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (16 * u + 4 * g + i >= p.sinks) s2[u][i] = -INFINITY;
+            most = fmaxf(most, s2[u][i]);
           }
         }
+        neg_run[nt] = fminf(kNoReference, __builtin_fmaf(-rowgroup_max(most), scale, -kWvHeadroom<F16>));
+        const float neg = FACTOR ? neg_run[nt] + fast_log2(factor_prev) : neg_run[nt];
+        uint32_t w4[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            w4[2 * u + j] = pack2<F16>(fast_exp2(__builtin_fmaf(s2[u][2 * j], scale, neg)), fast_exp2(__builtin_fmaf(s2[u][2 * j + 1], scale, neg)));
+        P[0][nt] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
       }
-    }
-    for (int i = tid * 16; i < BUF; i += THREADS * 16) {
-      uint4 piece = make_uint4(0u, 0u, 0u, 0u);
-      if constexpr (WIN) {
-        const uint32_t n = (uint32_t)i >> 4, prow = (n * wv_magic<HD>()) >> 16, pcol = n - (uint32_t)PIECES * prow;
-        if (sinks_first && (int)prow < p.sinks && pcol < (uint32_t)(HD / 8)) {
-          const uint8_t* const from = reinterpret_cast<const uint8_t*>(vbase + (uint64_t)((int64_t)sinks_chunk * chunk_bytes)) +
-                                      (int64_t)prow * tok_bytes + (8 * ESZ) * pcol;
-          if constexpr (FP8) {
-            const uint2 raw8 = ld8(from);
-            if constexpr (FACTOR) {
-              const uint32_t sign = sinks_vscale < 0.f ? 0x80808080u : 0u;
-              const float pow2 = value_pow2(sinks_vscale);
-              const uint2 lo = fp8x4_to_16x4<F16>(raw8.x ^ sign, pow2), hi = fp8x4_to_16x4<F16>(raw8.y ^ sign, pow2);
-              piece = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            } else {
-              const f32x2_t a = fp8x2_lo_to_f32(raw8.x), b = fp8x2_hi_to_f32(raw8.x), c = fp8x2_lo_to_f32(raw8.y), d = fp8x2_hi_to_f32(raw8.y);
-              piece = make_uint4(pack2<F16>(a.x * sinks_vscale, a.y * sinks_vscale), pack2<F16>(b.x * sinks_vscale, b.y * sinks_vscale),
-                                 pack2<F16>(c.x * sinks_vscale, c.y * sinks_vscale), pack2<F16>(d.x * sinks_vscale, d.y * sinks_vscale));
-            }
-          } else {
-            piece = ld16(from);
-          }
-        }
-      }
-      *reinterpret_cast<uint4*>(&Vs[1][0] + i) = piece;
-    }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
     Cursor cur = cursor_at(tb + 2);
     int64_t off_first[2];   // tiles tb and tb + 1, started here
     uint32_t nrec_first[2];
@@ -754,18 +800,14 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
     else pc_next = __builtin_amdgcn_readfirstlane(bt_row[cur.ci]);
     // (the query fragments count as used here: the compiler then waits for their loads now and not in the tile
     // loop, where a wait on the vector-memory counter would wait for the direct loads in flight as well)
+    auto queries_here = [&] {
 #pragma unroll
-    for (int nt = 0; nt < NQ; ++nt)
-#pragma unroll
-      for (int kk = 0; kk < KS; ++kk)
-        asm volatile("" ::"v"(qf[nt][kk].x), "v"(qf[nt][kk].y), "v"(qf[nt][kk].z), "v"(qf[nt][kk].w));
-    if constexpr (WIN) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int nt = 0; nt < NQ; ++nt)
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk)
-          asm volatile("" ::"v"(sinks_k[u][kk].x), "v"(sinks_k[u][kk].y), "v"(sinks_k[u][kk].z), "v"(sinks_k[u][kk].w));
-    }
+          asm volatile("" ::"v"(qf[nt][kk].x), "v"(qf[nt][kk].y), "v"(qf[nt][kk].z), "v"(qf[nt][kk].w));
+    };
+    if constexpr (!WIN) queries_here();
     if (raw) {
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
@@ -777,10 +819,19 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
         }
       }
     }
-    __syncthreads();
+    if constexpr (WIN) {
+      // (walks are short here: the queries are waited for behind the first tiles' loads, not ahead of them)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+    } else {
+      __syncthreads();
+    }
     int64_t off_prev, off_prev2 = off_first[0];   // of tiles j+1 and j
     uint32_t nrec_prev, nrec_prev2 = nrec_first[0];
     if constexpr (FP8) {
+      if constexpr (WIN) {
+        if (sinks_first) sinks_request();
+      }
       fetch_fp8(kbase, off_first[0], nrec_first[0], kraw);
       MI_SB();
       if (raw) norm_and_rotate();
@@ -810,45 +861,12 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
       if (raw) norm_and_rotate();
       MI_SB();
     }
-    // The sinks' probabilities, against a reference of their own, wait for the first value product as those of a tile before the first.
     if constexpr (WIN) {
       if (sinks_first) {
-        const float scale = FP8 ? tile_scale(sinks_kscale) : p.scale_log2;
-        const uint32_t sign = FP8 && sinks_kscale < 0.f ? 0x80808080u : 0u;
-        if constexpr (FACTOR) factor_prev = value_factor(sinks_vscale);
-#pragma unroll
-        for (int nt = 0; nt < NQ; ++nt) {
-          f32x4_t s2[2];
-          float most = -INFINITY;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            s2[u] = zero4;
-#pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-              uint4 k4 = sinks_k[u][kk];
-              if constexpr (FP8) {
-                const uint2 lo = fp8x4_to_16x4<F16>(k4.x ^ sign), hi = fp8x4_to_16x4<F16>(k4.y ^ sign);
-                k4 = make_uint4(lo.x, lo.y, hi.x, hi.y);
-              }
-              s2[u] = mfma_16x16x32<F16>(k4, qf[nt][kk], s2[u]);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (16 * u + 4 * g + i >= p.sinks) s2[u][i] = -INFINITY;
-              most = fmaxf(most, s2[u][i]);
-            }
-          }
-          neg_run[nt] = fminf(kNoReference, __builtin_fmaf(-rowgroup_max(most), scale, -kWvHeadroom<F16>));
-          const float neg = FACTOR ? neg_run[nt] + fast_log2(factor_prev) : neg_run[nt];
-          uint32_t w4[4];
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              w4[2 * u + j] = pack2<F16>(fast_exp2(__builtin_fmaf(s2[u][2 * j], scale, neg)), fast_exp2(__builtin_fmaf(s2[u][2 * j + 1], scale, neg)));
-          P[0][nt] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-        }
+        if constexpr (!FP8) sinks_request();
+        sinks_work();
       }
+      queries_here();
     }
     // key tile 0 has landed (this wavefront's share): only the loads issued after it may still be on their way
     if constexpr (!FP8) {
