@@ -23,9 +23,9 @@ def _split(mi, **change):
 
 
 def _mixed(mi, **change):
-    a = dict(m=P, mst=24 * 128, qo=P, qost=1024, ko=None, kost=0, qw=None, kw=None, eps=1e-5, norm=0, emb=P, est=128, rows=100,
+    a = dict(m=P, mst=12 * 128, qo=P, qost=1024, ko=None, kost=0, qw=None, kw=None, eps=1e-5, norm=0, emb=P, est=128, rows=100,
              rot=128, inter=0, ms=1.0, pos=P, pst=5, axes=3, pairs=PAIRS, kc=P, vc=P, sc=65536, st=1024, ci=P, lp=P, bt=None, bts=0,
-             lens=None, chunk=64, T=5, Hq=8, Hkv=8, d=128, faith=1, dtype=0, tune=None, stream=None)
+             lens=None, chunk=64, T=5, Hq=8, Hkv=2, d=128, faith=1, dtype=0, tune=None, stream=None)
     assert not set(change) - set(a)
     a.update(change)
     return mi._lib.load().mi_qkv_norm_rope_append_axes(*a.values())
@@ -44,7 +44,7 @@ def test_split(mi, change, word):
     _error(mi, _split(mi, **change), word)
 
 
-@pytest.mark.parametrize("change,word", BOTH + [(dict(m=None), "missing"), (dict(Hq=12), "multiple"), (dict(mst=1024), "stride"),
+@pytest.mark.parametrize("change,word", BOTH + [(dict(m=None), "missing"), (dict(Hq=9), "multiple"), (dict(mst=1024), "stride"),
                                                 (dict(kc=None), "destination")])
 def test_mixed(mi, change, word):
     _error(mi, _mixed(mi, **change), word)
