@@ -540,14 +540,21 @@ class DynamicInferenceContext:
     def fused_qk_norm_rope_append(self, layer_number: int, query: Tensor, key: Tensor, value: Tensor, *,
                                   rotary_pos_emb: Optional[Tensor], config=None, q_weight: Optional[Tensor] = None,
                                   k_weight: Optional[Tensor] = None, norm: Optional[str] = None, eps: float = 1e-5,
-                                  mscale: float = 1.0, faithful_rounding: bool = True) -> Tensor:
+                                  mscale: float = 1.0, faithful_rounding: bool = True,
+                                  rotary_axes: Optional[bytes] = None, axis_positions: Optional[Tensor] = None) -> Tensor:
         """One launch for q/k norm -> RoPE(q, k) -> append(k, v) of a layer.
 
         Equivalent to q_layernorm/k_layernorm + ``apply_rotary_emb_key`` +
         ``append_key_value_cache`` + ``apply_rotary_emb_query`` of the reference
         (attention.py:1026-1030, 394-404, 766).  ``query`` is updated in place and returned.
+
+        With ``rotary_axes`` (``ops.rotary_axes``) query and key rotate by ``axis_positions``, int64 ``[axes, >= n]`` for
+        the ``n`` tokens of the padded step: where a token stands among several axes, which the cache's own order of
+        tokens (slots, lengths, what attention sees) does not tell.  Any value is a position; the table's first or last row
+        is taken for those beyond it.
         """
         n = self.padded_active_token_count
+        positions = self._rotary_positions(rotary_axes, axis_positions)
         if self.cache_mla_latent:
             raise NotImplementedError("the fused q/k norm + RoPE + append launch serves per-head KV caches, not MLA latents")
         if self.kv_cache_fp8:
@@ -555,23 +562,31 @@ class DynamicInferenceContext:
             key_out = torch.empty_like(key[:n])
             ops.norm_rope_append(
                 query[:n], key[:n], key_out=key_out, q_weight=q_weight, k_weight=k_weight, eps=eps, norm=norm,
-                rotary_emb=rotary_pos_emb, q_positions=self.token_to_pos_ids,
-                k_positions=self.token_to_position_in_request,
+                rotary_emb=rotary_pos_emb,
                 rotary_interleaved=self._rope_flags(config) if config is not None else False, mscale=mscale,
-                faithful_rounding=faithful_rounding)
+                faithful_rounding=faithful_rounding, **positions)
             self.append_key_value_cache(layer_number, key_out, value[:n])
             return query
         k_cache, v_cache = self._layer_cache(layer_number)
         ops.norm_rope_append(
             _first(query, n), _first(key, n), value=_first(value, n), q_weight=q_weight, k_weight=k_weight, eps=eps, norm=norm,
-            rotary_emb=rotary_pos_emb, q_positions=self.token_to_pos_ids,
-            k_positions=self.token_to_position_in_request,
+            rotary_emb=rotary_pos_emb,
             rotary_interleaved=self._rope_flags(config) if config is not None else False, mscale=mscale,
             k_cache=k_cache, v_cache=v_cache,
             token_to_chunk_idx=self.token_to_chunk_idx,
             token_to_local_pos=self.token_to_local_position_within_kv_chunk,
-            faithful_rounding=faithful_rounding)
+            faithful_rounding=faithful_rounding, **positions)
         return query
+
+    def _rotary_positions(self, rotary_axes: Optional[bytes], axis_positions: Optional[Tensor]) -> dict:
+        """The position arguments of the norm / RoPE / append calls: the context's own rows, or the caller's axes."""
+        if rotary_axes is None:
+            if axis_positions is not None:
+                raise ValueError("axis_positions go with rotary_axes")
+            return dict(q_positions=self.token_to_pos_ids, k_positions=self.token_to_position_in_request)
+        if axis_positions is None:
+            raise ValueError("rotary_axes need axis_positions, int64 [axes, tokens]")
+        return dict(q_positions=axis_positions, rotary_axes=rotary_axes)
 
     def decode_step_fusable(self, head_dim: int, rotary_pos_emb: Optional[Tensor], config=None) -> bool:
         """Whether this step can run :meth:`fused_decode_step_attention`: a decode-only step over per-head caches
@@ -645,15 +660,18 @@ class DynamicInferenceContext:
                                    rotary_pos_emb: Optional[Tensor], config=None,
                                    q_weight: Optional[Tensor] = None, k_weight: Optional[Tensor] = None,
                                    norm: Optional[str] = None, eps: float = 1e-5, mscale: float = 1.0,
-                                   faithful_rounding: bool = True, query_out: Optional[Tensor] = None) -> Tensor:
+                                   faithful_rounding: bool = True, query_out: Optional[Tensor] = None,
+                                   rotary_axes: Optional[bytes] = None, axis_positions: Optional[Tensor] = None) -> Tensor:
         """:meth:`fused_qk_norm_rope_append` starting from the QKV projection's output.
 
         ``mixed_qkv`` is ``[T, 1, (Hq + 2 Hkv) * d]`` in the per-query-group order that
         ``SelfAttention.get_query_key_value_tensors`` splits (attention.py:985-1030); the split, the
         query reshape (a copy in the reference), both norms, both RoPE calls and the append run as one
         launch.  Returns the query ``[T, 1, Hq, d]`` (``query_out`` if given, else a new tensor).
+        ``rotary_axes`` and ``axis_positions`` as there.
         """
         n = self.padded_active_token_count
+        positions = self._rotary_positions(rotary_axes, axis_positions)
         if self.cache_mla_latent:
             raise NotImplementedError("the fused QKV launch serves per-head KV caches, not MLA latents")
         hkv = self.num_kv_heads_per_partition
@@ -666,9 +684,8 @@ class DynamicInferenceContext:
             ops.qkv_norm_rope_append(
                 mixed_qkv[:n], num_query_heads=num_query_heads, num_kv_heads=hkv, query_out=query_out[:n],
                 key_out=key_out, q_weight=q_weight, k_weight=k_weight, eps=eps, norm=norm, rotary_emb=rotary_pos_emb,
-                q_positions=self.token_to_pos_ids, k_positions=self.token_to_position_in_request,
                 rotary_interleaved=self._rope_flags(config) if config is not None else False, mscale=mscale,
-                faithful_rounding=faithful_rounding)
+                faithful_rounding=faithful_rounding, **positions)
             group = num_query_heads // hkv
             value = mixed_qkv[:n].reshape(n, hkv, (group + 2) * d)[:, :, (group + 1) * d:]
             self.append_key_value_cache(layer_number, key_out, value.unsqueeze(1))
@@ -677,12 +694,11 @@ class DynamicInferenceContext:
         ops.qkv_norm_rope_append(
             _first(mixed_qkv, n), num_query_heads=num_query_heads, num_kv_heads=hkv, query_out=_first(query_out, n),
             q_weight=q_weight, k_weight=k_weight, eps=eps, norm=norm, rotary_emb=rotary_pos_emb,
-            q_positions=self.token_to_pos_ids, k_positions=self.token_to_position_in_request,
             rotary_interleaved=self._rope_flags(config) if config is not None else False, mscale=mscale,
             k_cache=k_cache, v_cache=v_cache,
             token_to_chunk_idx=self.token_to_chunk_idx,
             token_to_local_pos=self.token_to_local_position_within_kv_chunk,
-            faithful_rounding=faithful_rounding)
+            faithful_rounding=faithful_rounding, **positions)
         return query_out
 
     def prefill_fusable(self, mixed_qkv: Tensor, head_dim: int, rotary_pos_emb: Optional[Tensor],

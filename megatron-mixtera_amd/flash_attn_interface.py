@@ -4,8 +4,9 @@
 resolves the module-level names ``flash_attn_with_kvcache`` and ``flash_attn_varlen_func``;
 these functions accept the keyword surface used there and run the paged kernels of
 ``libmi355_decode.so``.  Arguments the reference never passes on this path (dropout,
-windows, alibi, rotary fusion, new-token append inside the call) are rejected rather than
-silently ignored.
+alibi, rotary fusion, new-token append inside the call) are rejected rather than
+silently ignored.  ``window_size`` is flash-attn's ``(left, right)``: a token sees the ``left`` tokens
+before it and itself, and ``sink_tokens`` (an addition) keeps a request's first tokens in sight.
 """
 from __future__ import annotations
 
@@ -53,6 +54,22 @@ def _reject(**unsupported) -> None:
         raise NotImplementedError(f"unsupported flash-attn arguments on the paged MI355X path: {bad}")
 
 
+def window_argument(window_size, sink_tokens: int) -> dict:
+    """``window_size`` and ``sink_tokens`` as the ``window`` / ``sinks`` of the paged calls: of the tokens before it a token
+    sees the last ``left``, and every one where ``left`` is -1.  There are no keys to the right of a causal row, so ``right`` is
+    -1 or 0."""
+    left, right = (-1, -1) if window_size is None else window_size
+    if left < -1 or right not in (-1, 0):
+        raise NotImplementedError(f"window_size on the paged MI355X path is (left, 0), (left, -1) or (-1, -1), not {window_size}")
+    if sink_tokens < 0:
+        raise ValueError("sink_tokens must not be negative")
+    if left == -1:
+        if sink_tokens:
+            raise ValueError("sink_tokens go with a window (without one every token is in sight)")
+        return {}
+    return dict(window=left + 1, sinks=sink_tokens)
+
+
 def flash_attn_with_kvcache(q: Tensor, k_cache: Tensor, v_cache: Tensor, k: Optional[Tensor] = None,
                             v: Optional[Tensor] = None, rotary_cos=None, rotary_sin=None,
                             cache_seqlens: Optional[Tensor] = None, cache_batch_idx=None,
@@ -61,7 +78,8 @@ def flash_attn_with_kvcache(q: Tensor, k_cache: Tensor, v_cache: Tensor, k: Opti
                             window_size=(-1, -1), softcap: float = 0.0, rotary_interleaved: bool = True,
                             alibi_slopes=None, num_splits: int = 0, return_softmax_lse: bool = False,
                             *, page_table: Optional[Tensor] = None, k_scales: Optional[Tensor] = None,
-                            v_scales: Optional[Tensor] = None, max_seqlen_k: Optional[int] = None) -> Tensor:
+                            v_scales: Optional[Tensor] = None, max_seqlen_k: Optional[int] = None,
+                            sink_tokens: int = 0) -> Tensor:
     """Paged decode attention: ``q`` is ``[batch, 1, Hq, d]``, one query token per request.
 
     ``cache_seqlens`` (int32 ``[batch]``) already counts the token appended this step;
@@ -69,15 +87,15 @@ def flash_attn_with_kvcache(q: Tensor, k_cache: Tensor, v_cache: Tensor, k: Opti
     token the causal mask is a no-op, so ``causal`` is accepted either way.
     """
     _reject(k=k, v=v, rotary_cos=rotary_cos, rotary_sin=rotary_sin, cache_batch_idx=cache_batch_idx,
-            cache_leftpad=cache_leftpad, window_size=window_size, softcap=softcap, alibi_slopes=alibi_slopes,
-            return_softmax_lse=return_softmax_lse)
+            cache_leftpad=cache_leftpad, softcap=softcap, alibi_slopes=alibi_slopes, return_softmax_lse=return_softmax_lse)
     table = block_table if block_table is not None else page_table
     if table is None or cache_seqlens is None:
         raise ValueError("the paged path needs block_table (or page_table) and cache_seqlens")
     if q.dim() != 4 or q.size(1) != 1:
         raise NotImplementedError("flash_attn_with_kvcache on this path takes one query token per request: q [B,1,Hq,d]")
     return ops.paged_decode_attention(q, k_cache, v_cache, cache_seqlens, table, softmax_scale=softmax_scale,
-                                      max_kv_len=max_seqlen_k, k_scales=k_scales, v_scales=v_scales)
+                                      max_kv_len=max_seqlen_k, k_scales=k_scales, v_scales=v_scales,
+                                      **window_argument(window_size, sink_tokens))
 
 
 def flash_attn_varlen_func(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor, cu_seqlens_k: Optional[Tensor],
@@ -86,7 +104,8 @@ def flash_attn_varlen_func(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor
                            softcap: float = 0.0, alibi_slopes=None, deterministic: bool = False,
                            return_attn_probs: bool = False, block_table: Optional[Tensor] = None,
                            *, seqused_k: Optional[Tensor] = None, k_scales: Optional[Tensor] = None,
-                           v_scales: Optional[Tensor] = None, one_row_requests: Optional[bool] = None) -> Tensor:
+                           v_scales: Optional[Tensor] = None, one_row_requests: Optional[bool] = None,
+                           sink_tokens: int = 0) -> Tensor:
     """Paged varlen causal attention: ``q`` is ``[T, Hq, d]``, ``k``/``v`` are the paged caches.
 
     Per-request key counts come from ``seqused_k`` if given, else from the differences of
@@ -94,8 +113,8 @@ def flash_attn_varlen_func(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor
     that no request has exactly one query row; without a word from the caller that is known when the rows are more
     than requests of at most ``max_seqlen_q`` rows could have with one of them at one row.
     """
-    _reject(dropout_p=dropout_p, window_size=window_size, softcap=softcap, alibi_slopes=alibi_slopes,
-            return_attn_probs=return_attn_probs)
+    _reject(dropout_p=dropout_p, softcap=softcap, alibi_slopes=alibi_slopes, return_attn_probs=return_attn_probs)
+    window = window_argument(window_size, sink_tokens)
     if block_table is None:
         raise NotImplementedError("only the paged form (block_table given) exists on this path")
     if not causal:
@@ -110,6 +129,8 @@ def flash_attn_varlen_func(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor
         # decompressed multi-latent caches: keys carry the shared rotary slice, values do not
         if k_scales is not None or v_scales is not None:
             raise NotImplementedError("no fp8 variant for caches with different key / value widths")
+        if window:
+            raise NotImplementedError("no window over caches with different key / value widths")
         return ops.paged_prefill_attention_mla(
             q, k, v, cu_seqlens_q, kv_lens.to(torch.int32), block_table, max_kv_len=max_seqlen_k,
             softmax_scale=softmax_scale if softmax_scale is not None else q.shape[-1] ** -0.5)
@@ -117,7 +138,7 @@ def flash_attn_varlen_func(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor
         one_row_requests = q.size(0) <= (cu_seqlens_q.numel() - 2) * max_seqlen_q + 1
     return ops.paged_prefill_attention(q, k, v, cu_seqlens_q, kv_lens.to(torch.int32), block_table,
                                        softmax_scale=softmax_scale, max_kv_len=max_seqlen_k,
-                                       k_scales=k_scales, v_scales=v_scales, one_row_requests=one_row_requests)
+                                       k_scales=k_scales, v_scales=v_scales, one_row_requests=one_row_requests, **window)
 
 
 def _flash_attn_forward(q: Tensor, k: Tensor, v: Tensor, k_new=None, v_new=None, qv=None, out: Optional[Tensor] = None,
@@ -134,7 +155,8 @@ def _flash_attn_forward(q: Tensor, k: Tensor, v: Tensor, k_new=None, v_new=None,
     ``seqused_k`` (or the running sums ``cu_seqlens_k``), the block table as ``page_table``.  Returns
     ``(out, None)``: the reference keeps the first element and discards the rest, and the log-sum-exp is not
     produced.  Scheduling hints (``scheduler_metadata``, ``num_splits``, ``pack_gqa``, ``sm_margin``) have no
-    meaning here and are ignored; arguments that would change the result are rejected."""
+    meaning here and are ignored; arguments that would change the result are rejected, windows among them (the
+    flash-attention-2 forms above take them)."""
     _reject(k_new=k_new, v_new=v_new, qv=qv, cu_seqlens_k_new=cu_seqlens_k_new, seqused_q=seqused_q,
             kv_batch_idx=kv_batch_idx, leftpad_k=leftpad_k, rotary_cos=rotary_cos, rotary_sin=rotary_sin,
             seqlens_rotary=seqlens_rotary, q_descale=q_descale, k_descale=k_descale, v_descale=v_descale,

@@ -35,16 +35,21 @@ class DecodeLayerGraphs:
     ``replay(layer_index, query, key, value)`` copies the step's tensors into the static inputs
     of the graph for ``context.padded_active_token_count`` and the step's kind, and returns the
     static output ``[padded, 1, Hq*d]`` (valid until the next replay of the same graph).
+    Layers with ``rotary_sections`` need ``axis_positions``, one int64 ``[axes, tokens]`` tensor that the graphs read.
     """
 
     def __init__(self, context, layers: Sequence[torch.nn.Module], *, num_query_heads: int,
-                 rotary_pos_emb: Optional[Tuple[Tensor, Tensor]] = None):
+                 rotary_pos_emb: Optional[Tuple[Tensor, Tensor]] = None, axis_positions: Optional[Tensor] = None):
         if context.cuda_graph_token_counts is None:
             raise ValueError("the context was built without cuda-graph sizes (num_cuda_graphs=None)")
         self.context = context
         self.layers = list(layers)
         self.num_query_heads = num_query_heads
         self.rotary_pos_emb = rotary_pos_emb
+        # (read by every replay: the caller writes a step's positions into it, as the context does with its rows)
+        if axis_positions is not None and axis_positions.size(-1) < max(context.cuda_graph_token_counts):
+            raise ValueError("axis_positions are shorter than the largest graph's tokens")
+        self.axis_positions = axis_positions
         # (layer index, padded tokens, decode-only?) -> (graph, q, k, v, out)
         self._graphs: Dict[Tuple[int, int, bool], Tuple[torch.cuda.CUDAGraph, Tensor, Tensor, Tensor, Tensor]] = {}
         self._pool = None
@@ -99,7 +104,9 @@ class DecodeLayerGraphs:
 
     def _run(self, layer, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
         with ops.use_workspace(self.workspace):
-            return layer(q, k, v, self.context, self.rotary_pos_emb)
+            if self.axis_positions is None:
+                return layer(q, k, v, self.context, self.rotary_pos_emb)
+            return layer(q, k, v, self.context, self.rotary_pos_emb, self.axis_positions)
 
     def replay(self, layer_index: int, query: Tensor, key: Tensor, value: Tensor) -> Tensor:
         ctx = self.context

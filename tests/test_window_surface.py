@@ -1,0 +1,56 @@
+"""Windows, sinks and positions with several axes: what the layers and the flash-attention forms refuse, before any GPU is asked."""
+import pytest
+import torch
+
+
+@pytest.mark.parametrize("more,error", [
+    (dict(window_size=(-2, 0)), NotImplementedError), (dict(window_size=(5, 1)), NotImplementedError),
+    (dict(window_size=(-1, 3)), NotImplementedError), (dict(window_size=(5, -2)), NotImplementedError),
+    (dict(window_size=(5, 0), sink_tokens=-1), ValueError), (dict(sink_tokens=4), ValueError),
+    (dict(window_size=(-1, -1), sink_tokens=4), ValueError),
+])
+def test_windows_that_there_are_not(mi, more, error):
+    q, cache = torch.zeros(4, 2, 64), torch.zeros(1, 16, 2, 64)
+    i32 = dict(dtype=torch.int32)
+    with pytest.raises(error):
+        mi.flash_attn_varlen_func(q, cache, cache, torch.tensor([0, 4], **i32), None, 4, 4, causal=True,
+                                  block_table=torch.zeros(1, 1, **i32), seqused_k=torch.tensor([4], **i32), **more)
+    with pytest.raises(error):
+        mi.flash_attn_with_kvcache(q[:1, None], cache, cache, cache_seqlens=torch.tensor([4], **i32),
+                                   block_table=torch.zeros(1, 1, **i32), **more)
+    with pytest.raises(error):
+        mi.PagedSelfAttentionCore(1, 64, **more)
+    with pytest.raises(error):
+        mi.PagedSelfAttentionLayer(1, 64, 2, 2, 64, **more)
+
+
+def test_no_window_over_latent_caches(mi):
+    from importlib import import_module
+    attention = import_module(mi.__name__ + ".attention")
+    i32 = dict(dtype=torch.int32)
+    lens, table = torch.tensor([4], **i32), torch.zeros(1, 1, **i32)
+    with pytest.raises(NotImplementedError, match="window"):   # keys wider than values
+        mi.flash_attn_varlen_func(torch.zeros(4, 2, 192), torch.zeros(1, 16, 2, 192), torch.zeros(1, 16, 2, 128),
+                                  torch.tensor([0, 4], **i32), None, 4, 4, causal=True, block_table=table, seqused_k=lens,
+                                  window_size=(3, 0))
+    with pytest.raises(NotImplementedError, match="window"):
+        attention.flash_decode_and_prefill(torch.zeros(1, 1, 2, 576), torch.zeros(1, 16, 576), None, 1, 4, None, None, lens, table,
+                                           mla_head_dim_v=512, window_size=(3, 0))
+
+
+def test_positions_go_with_axes(mi):
+    positions, emb = torch.zeros(3, 4, dtype=torch.int64), torch.zeros(8, 64)
+    plain, several = mi.PagedSelfAttentionCore(1, 64), mi.PagedSelfAttentionCore(1, 64, rotary_sections=(8, 12, 12))
+    q, kv, mixed = torch.zeros(4, 1, 2, 64), torch.zeros(4, 1, 1, 64), torch.zeros(4, 1, 4 * 64)
+    for call in (lambda c, *a: c(q, kv, kv, None, emb, *a), lambda c, *a: c.forward_mixed_qkv(mixed, 2, None, emb, *a)):
+        with pytest.raises(ValueError, match="rotary_sections"):
+            call(plain, positions)
+        with pytest.raises(ValueError, match="axis_positions"):
+            call(several)
+    with pytest.raises(NotImplementedError, match="fused"):
+        mi.PagedSelfAttentionCore(1, 64, rotary_sections=(8, 12, 12), fused=False)
+    with pytest.raises(ValueError):
+        mi.PagedSelfAttentionCore(1, 64, rotary_sections=())
+    layer = mi.PagedSelfAttentionLayer(1, 64, 2, 1, 64)
+    with pytest.raises(ValueError, match="rotary_sections"):
+        layer.core.forward_mixed_qkv(mixed, 2, None, emb, positions)
