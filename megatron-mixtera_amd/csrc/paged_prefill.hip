@@ -400,7 +400,7 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
   }
 
   QueryBlock qb;
-  if (!find_query_block(p, SBQ, rank, (int)(gridDim.x / HV), &qb)) return;  // workgroup-uniform
+  if (!find_query_block<WIN>(p, SBQ, rank, (int)(gridDim.x / HV), &qb)) return;  // workgroup-uniform
   const int r = qb.r, q_begin = qb.q_begin, Lq = qb.Lq, Lk = WIN ? min(qb.Lk, p.max_len) : qb.Lk, q0_wg = qb.q0;
   const int shift = Lk - Lq;
   const int last = Lk - 1;
@@ -1229,7 +1229,10 @@ static int launch_paged_prefill(
   p.n_chunks = win ? win->n_chunks : 0;
   p.max_len = win ? win->max_len : 0;
   // (a workgroup with a window has at most so many keys to walk)
+  const int longest = max_kv_len > 0 || !win ? max_kv_len : win->max_len;
   if (win) max_kv_len = window_walk(*win, max_kv_len);
+  // (requests that another kernel serves would leave empty blocks, which the order by keys leaves out)
+  p.ordered = R > 1 && R <= kOrderedRequests && (p.skip_single || max_kv_len > longest / 4);
   if (raw && !(two_phase && tune.prefill_two_phase == 3 && (head_dim == 64 || head_dim == 128)))
     return mi_fail(MI_ERR_UNSUPPORTED, "mi_qkv_prefill_attention: head_dim 64 or 128 and a chunk size that is a multiple of 64");
 
@@ -1264,7 +1267,7 @@ static int launch_paged_prefill(
     const int waves = woven ? prefill_woven_waves(head_dim, fp8, raw != nullptr, n_split, T, R, Gw, one_row_requests, max_kv_len) : 8;
     // wavefronts x whole tokens in a wavefront's 32 (wide heads: 16) rows
     const int sbq_lds = waves * ((head_dim >= 192 ? 16 : 32) / Gw);
-    const dim3 lgrid(prefill_query_blocks(T, R, sbq_lds) * Hkv * parts, n_split);
+    const dim3 lgrid(prefill_query_blocks(T, R, sbq_lds, !win || p.ordered || R == 1) * Hkv * parts, n_split);
     hipEvent_t ev_a, ev_b;
     const bool timed = mi_profile_next(&ev_a, &ev_b);
     if (timed) (void)hipEventRecord(ev_a, st);

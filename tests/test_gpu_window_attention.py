@@ -169,6 +169,13 @@ def test_prompt_shapes_of_other_widths(mi, dev, new, lens, window, sinks, d, dty
     Case(dev, new, lens, window, sinks, d=d, dtype=dtype, seed=sum(lens) + d, spare=2).check(mi, one_row_requests=False)
 
 
+@pytest.mark.parametrize("new,lens", [([130, 3, 0, 257, 7], [1600, 90, 40, 2500, 2500]), ([300, 299], [3000, 299]), ([5] * 130, [1500] * 130)])
+@pytest.mark.parametrize("d,fp8", [(64, False), (128, False), (96, False), (128, True)])
+def test_windows_short_beside_the_requests(mi, dev, new, lens, d, fp8):
+    """Query blocks in the batch's order: a walk of at most a quarter of the longest request, no requests of one row."""
+    Case(dev, new, lens, 20, 3, d=d, fp8=fp8, seed=d + len(lens), spare=3).check(mi, one_row_requests=False, max_kv_len=max(lens))
+
+
 @pytest.mark.parametrize("chunk", [16, 48, 80])
 @pytest.mark.parametrize("d", [64, 96, 128, 192, 256])
 def test_prompts_over_chunks_of_other_sizes(mi, dev, chunk, d):
