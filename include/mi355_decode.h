@@ -406,7 +406,7 @@ int mi_paged_prefill_attention_tiles(const void* q, int64_t q_stride_tok, int64_
  * Chunks without a token in sight of the call's rows are not needed: their table entries may hold anything.  Entries that
  * are used are kept inside the cache, lengths inside the table.  kv_dtype, scales and everything else as in
  * mi_paged_decode_attention (workspace: mi_decode_workspace_bytes) and mi_paged_prefill_attention / _fp8 / _tiles
- * (workspace: mi_window_prefill_workspace_bytes with the call's own T, max_kv_len, window and sinks; `one_row_requests`
+ * (workspace: mi_window_prefill_workspace_bytes with the call's own T, max_kv_len, window and sinks, -1 for ones that are refused; `one_row_requests`
  * 0: no request has exactly one row, nothing is launched for such).  The tuning knob prefill_two_phase takes 3 or -1.
  */
 int mi_paged_window_decode_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,

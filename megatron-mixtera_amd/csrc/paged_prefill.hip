@@ -1333,6 +1333,7 @@ static int launch_paged_prefill(
 
 extern "C" int64_t mi_window_prefill_workspace_bytes(int32_t T, int32_t R, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t max_kv_len,
                                                      int32_t window, int32_t sinks, const MiTuning* tuning) {
+  if (window < 1 || sinks < 0) return -1;
   const WindowArgs w = {window < kMostWindow ? window : kMostWindow, sinks < kMostWindow ? sinks : kMostWindow, 0, 0x7fffffff};
   return mi_prefill_workspace_bytes(T, R, Hq, Hkv, head_dim, window_walk(w, max_kv_len), 0, tuning);
 }

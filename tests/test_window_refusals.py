@@ -70,6 +70,8 @@ def test_the_workspace_goes_by_what_is_in_sight(mi):
     assert 0 < windowed < full
     assert lib.mi_window_prefill_workspace_bytes(300, 1, 8, 8, 128, 100000, 2000000000, 2000000000, None) == full
     assert lib.mi_window_prefill_workspace_bytes(300, 1, 8, 8, 128, 0, 1000, 4, None) == windowed
+    for window, sinks in ((0, 4), (-5, 4), (1000, -1)):
+        assert lib.mi_window_prefill_workspace_bytes(300, 1, 8, 8, 128, 100000, window, sinks, None) == -1
 
 
 def _tensors():
