@@ -630,22 +630,28 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
         if constexpr (!WIN) {
           hide([&](int k) { return k > dpos; });
         } else {
-          // (one border crosses most of the tiles that one crosses at all: one comparison for a score, not three)
-          const int gone = dpos - p.window, sunk = p.sinks - (key0 + 4 * g);   // hidden: from `sunk` to `gone`
-          // (scheduling barriers: without them the three come out as one with all comparisons, up to 1 % of a launch)
+          // Hidden: behind `end`, and from `sunk` to `gone`.  One border crosses most of the tiles that one crosses at all: one
+          // comparison for a score, not three.  Every comparison has a number of its own as far as the compiler can tell: where one
+          // told it something of the next, it made branches of them, eight deep.
+          int end = dpos, gone = dpos - p.window, sunk = p.sinks - (key0 + 4 * g);
+          f32x4_t hid[2] = {Sn[nt][0], Sn[nt][1]};
+#define MI_HIDE(CONDITION_)                                          \
+  _Pragma("unroll") for (int k8 = 0; k8 < 8; ++k8) {                 \
+    const int k = 16 * (k8 >> 2) + (k8 & 3);                         \
+    asm("" : "+v"(end), "+v"(gone), "+v"(sunk));                     \
+    const bool hidden = CONDITION_;                                  \
+    hid[k8 >> 2][k8 & 3] = hidden ? -INFINITY : hid[k8 >> 2][k8 & 3]; \
+  }
           if (border == kBorderEnd) {
-            MI_SB();
-            hide([&](int k) { return k > dpos; });
-            MI_SB();
+            MI_HIDE(k > end);
           } else if (border == kBorderWindow) {
-            MI_SB();
-            hide([&](int k) { return k <= gone; });
-            MI_SB();
+            MI_HIDE(k <= gone);
           } else {
-            MI_SB();
-            hide([&](int k) { return k > dpos || (k <= gone && k >= sunk); });
-            MI_SB();
+            MI_HIDE((k > end) | ((k <= gone) & (k >= sunk)));
           }
+#undef MI_HIDE
+          Sn[nt][0] = hid[0];
+          Sn[nt][1] = hid[1];
         }
       };
       // values; beside them the last probabilities, then the mask of the scores just multiplied
