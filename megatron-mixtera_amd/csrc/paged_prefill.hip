@@ -205,9 +205,13 @@ __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams
       for (int u = 0; u < NT; ++u) {
         if (need_mask) {
           const int tok0 = T + 16 * u + 4 * g;
+          if constexpr (WIN) {
+            s[nt][u] = hide_keys(s[nt][u], tok0, qpos[nt], p.window, p.sinks);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (tok0 + i > qpos[nt] || (WIN && tok0 + i <= qpos[nt] - p.window && tok0 + i >= p.sinks)) s[nt][u][i] = -INFINITY;
+            for (int i = 0; i < 4; ++i)
+              if (tok0 + i > qpos[nt]) s[nt][u][i] = -INFINITY;
+          }
         }
         tmax = fmaxf(fmaxf(fmaxf(s[nt][u][0], s[nt][u][1]), fmaxf(s[nt][u][2], s[nt][u][3])), tmax);
       }
@@ -842,9 +846,13 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
 #pragma unroll
           for (int u = 0; u < NT; ++u) {
             const int tok0 = Tm + 16 * u + 4 * g;
+            if constexpr (WIN) {
+              s[nt][u] = hide_keys(s[nt][u], tok0, qpos[nt], p.window, p.sinks);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (tok0 + i > qpos[nt] || (WIN && tok0 + i <= qpos[nt] - p.window && tok0 + i >= p.sinks)) s[nt][u][i] = -INFINITY;
+              for (int i = 0; i < 4; ++i)
+                if (tok0 + i > qpos[nt]) s[nt][u][i] = -INFINITY;
+            }
           }
         }
         float tmax = fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), s[nt][0][2]);

@@ -83,6 +83,18 @@ static __device__ __forceinline__ WindowTiles window_tiles(int window, int sinks
   return w;
 }
 static __device__ __forceinline__ int clamp_chunk(int pc, int n_chunks) { return min(max(pc, 0), n_chunks - 1); }
+// The scores of four keys from `key` on, of a row at position `pos`: those that it does not see become -inf.  Every comparison
+// has numbers of its own as far as the compiler can tell: where one told it something of the next, it made branches of them.
+static __device__ __forceinline__ f32x4_t hide_keys(f32x4_t s, int key, int pos, int window, int sinks) {
+  int end = pos - key, gone = end - window, sunk = sinks - key;   // hidden: behind `end`, and from `sunk` to `gone`
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    asm("" : "+v"(end), "+v"(gone), "+v"(sunk));
+    const bool hidden = (i > end) | ((i <= gone) & (i >= sunk));
+    s[i] = hidden ? -INFINITY : s[i];
+  }
+  return s;
+}
 
 // The query block a workgroup of the tile kernels takes.
 struct QueryBlock {
