@@ -169,6 +169,22 @@ def test_prompt_shapes_of_other_widths(mi, dev, new, lens, window, sinks, d, dty
     Case(dev, new, lens, window, sinks, d=d, dtype=dtype, seed=sum(lens) + d, spare=2).check(mi, one_row_requests=False)
 
 
+@pytest.mark.parametrize("where", ["keys", "values", "queries"])
+@pytest.mark.parametrize("d,fp8", [(64, False), (128, True), (96, False)])
+@pytest.mark.parametrize("new,lens,parts", [([257, 3], [300, 3], 0), ([40], [5000], 5)])
+def test_nothing_but_nan(mi, dev, new, lens, parts, d, fp8, where):
+    """Every row is made again and ends at its first tile."""
+    c = Case(dev, new, lens, 200, 3, d=d, fp8=fp8, seed=d)
+    if where == "queries":
+        c.q.fill_(math.nan)
+    elif fp8:
+        c.scales[where == "values"].fill_(math.nan)
+    else:
+        (c.v if where == "values" else c.k).fill_(math.nan)
+    with mi.ops.tuning(prefill_kv_split=parts):
+        assert c.run(mi, one_row_requests=False).isnan().all()
+
+
 @pytest.mark.parametrize("new,lens", [([130, 3, 0, 257, 7], [1600, 90, 40, 2500, 2500]), ([300, 299], [3000, 299]), ([5] * 130, [1500] * 130)])
 @pytest.mark.parametrize("d,fp8", [(64, False), (128, False), (96, False), (128, True)])
 def test_windows_short_beside_the_requests(mi, dev, new, lens, d, fp8):
