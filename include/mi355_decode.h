@@ -404,7 +404,7 @@ int mi_paged_prefill_attention_tiles(const void* q, int64_t q_stride_tok, int64_
  *
  * `n_chunks`: chunks of the cache; `bt_columns`: of the block table (fewer than 2^31 - 512 tokens and 2^24 columns).
  * Chunks without a token in sight of the call's rows are not needed: their table entries may hold anything.  Entries that
- * are used are kept inside the cache, lengths inside the table.  kv_dtype, scales and everything else as in
+ * are used are kept inside the cache, lengths from 0 to what the table has room for.  kv_dtype, scales and everything else as in
  * mi_paged_decode_attention (workspace: mi_decode_workspace_bytes) and mi_paged_prefill_attention / _fp8 / _tiles
  * (workspace: mi_window_prefill_workspace_bytes with the call's own T, max_kv_len, window and sinks, -1 for ones that are refused; `one_row_requests`
  * 0: no request has exactly one row, nothing is launched for such).  The tuning knob prefill_two_phase takes 3 or -1.

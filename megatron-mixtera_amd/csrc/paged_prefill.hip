@@ -68,7 +68,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_prefill_kernel(PrefillParams
   const int q0 = (sb - (q_begin / SBQ + r)) * SBQ + wave * BQ;  // first query of this wave
   if (q0 >= Lq) return;
   if (p.skip_single && Lq == 1) return;
-  const int Lk = WIN ? min(p.lens[r], p.max_len) : p.lens[r];
+  const int Lk = WIN ? max(0, min(p.lens[r], p.max_len)) : p.lens[r];
   const int shift = Lk - Lq;  // key position of query 0
   const int nq = min(BQ, Lq - q0);
   const int kend = min(Lk, shift + q0 + nq);  // keys [0, kend) are visible to some row
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(512, 2) void paged_prefill_pp_kernel(PrefillParams 
 
   QueryBlock qb;
   if (!find_query_block<WIN>(p, SBQ, rank, (int)(gridDim.x / HV), &qb)) return;  // workgroup-uniform
-  const int r = qb.r, q_begin = qb.q_begin, Lq = qb.Lq, Lk = WIN ? min(qb.Lk, p.max_len) : qb.Lk, q0_wg = qb.q0;
+  const int r = qb.r, q_begin = qb.q_begin, Lq = qb.Lq, Lk = qb.Lk, q0_wg = qb.q0;
   const int shift = Lk - Lq;
   const int last = Lk - 1;
   const int kend_wg = min(Lk, shift + min(q0_wg + SBQ, Lq));

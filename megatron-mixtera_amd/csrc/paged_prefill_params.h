@@ -43,7 +43,7 @@ struct PrefillParams {
   // Windowed kernels only: a row at position P sees key k <= P where k > P - window or k < sinks (both at most 2^30).
   int32_t window, sinks;
   int32_t n_chunks;        // of the cache: table entries are kept below it
-  int32_t max_len;         // keys that the block table has room for: lengths are kept below it
+  int32_t max_len;         // keys that the block table has room for: lengths are kept from 0 to it
   int32_t ordered;         // query blocks by their requests' keys (find_query_block); without a window the requests decide
 };
 
@@ -137,6 +137,7 @@ template <bool WIN = false>
 static __device__ __forceinline__ bool find_query_block(const PrefillParams& p, int SBQ, int rank, int blocks,
                                                         QueryBlock* o) {
   const int lane = threadIdx.x & 63;
+  auto length = [&](int i) { return WIN ? min(max(p.lens[i], 0), p.max_len) : p.lens[i]; };
   if (WIN ? p.ordered != 0 : p.R > 1 && p.R <= kOrderedRequests) {
     const float inv = 1.f / (float)SBQ;
     auto div = [&](int n) {  // n / SBQ for n >= 0: the estimate is at most one off
@@ -152,7 +153,7 @@ static __device__ __forceinline__ bool find_query_block(const PrefillParams& p, 
       if (i < p.R) {
         cq[c] = p.cu_q[i];
         lq[c] = p.cu_q[i + 1] - cq[c];
-        lk[c] = p.lens[i];
+        lk[c] = length(i);
         nb[c] = p.skip_single && lq[c] == 1 ? 0 : div(max(lq[c], 0) + SBQ - 1);
       }
     }
@@ -200,7 +201,7 @@ static __device__ __forceinline__ bool find_query_block(const PrefillParams& p, 
     const int stride = (n + 63) >> 6;
     const int idx = r + lane * stride;
     const bool in = lane * stride < n;
-    const int cq = in ? p.cu_q[idx] : 0, cq1 = in ? p.cu_q[idx + 1] : 0, len = in ? p.lens[idx] : 0;
+    const int cq = in ? p.cu_q[idx] : 0, cq1 = in ? p.cu_q[idx + 1] : 0, len = in ? length(idx) : 0;
     const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && cq / SBQ + idx <= sb)) - 1;  // >= 0: the first candidate always qualifies
     r += c * stride;
     n = min(stride, n - c * stride);

@@ -123,7 +123,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
 
   QueryBlock qb;
   if (!find_query_block<WIN>(p, SBQ, rank, (int)(gridDim.x / HV), &qb)) return;  // workgroup-uniform
-  const int r = qb.r, q_begin = qb.q_begin, Lq = qb.Lq, Lk = WIN ? min(qb.Lk, p.max_len) : qb.Lk, q0_wg = qb.q0;
+  const int r = qb.r, q_begin = qb.q_begin, Lq = qb.Lq, Lk = qb.Lk, q0_wg = qb.q0;
   const int shift = Lk - Lq;
   const int last = Lk - 1;
   const int kend_wg = min(Lk, shift + min(q0_wg + SBQ, Lq));

@@ -192,6 +192,19 @@ def test_windows_short_beside_the_requests(mi, dev, new, lens, d, fp8):
     Case(dev, new, lens, 20, 3, d=d, fp8=fp8, seed=d + len(lens), spare=3).check(mi, one_row_requests=False, max_kv_len=max(lens))
 
 
+@pytest.mark.parametrize("d,chunk", [(64, 64), (96, 64), (128, 64), (128, 16)])
+@pytest.mark.parametrize("lens", [[-5, 90, -2000000000, 70], [90, 2147483647, -1, 90], [-1] * 4])
+@pytest.mark.parametrize("form", ["decode", "prompts", "many prompts"])
+def test_lengths_are_kept_in_the_table(mi, dev, form, lens, d, chunk):
+    """Below zero as zero, above the table's tokens as those."""
+    more = 33 if form == "many prompts" else 1   # (more requests than the blocks are ordered for)
+    new = None if form == "decode" else [40, 3, 7, 33] * more
+    c = Case(dev, new, [min(n, 90) for n in lens] * more, 20, 3, d=d, chunk=chunk, seed=d)
+    c.lens = lens * more
+    c.table = c.table[:, :-(-90 // chunk)].contiguous()
+    c.check(mi, one_row_requests=False) if new else c.check(mi)
+
+
 @pytest.mark.parametrize("chunk", [16, 48, 80])
 @pytest.mark.parametrize("d", [64, 96, 128, 192, 256])
 def test_prompts_over_chunks_of_other_sizes(mi, dev, chunk, d):
