@@ -562,10 +562,10 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
     const int pc = __builtin_amdgcn_readfirstlane(loaded);
     return WIN ? min(max(pc, 0), p.n_chunks - 1) : pc;
   };
-  // the chunk that follows ci along the walk
+  // the chunk that is `steps` (1 or 2) behind chunk ci along the walk: behind the sinks' last one are those that it passes over
   const int ci_near = WIN ? chunk_of(max(walk.from - 1, 0), p.chunk_magic) : 0;
-  const int ci_far = WIN && walk.skip > 0 && walk.from > 0 ? chunk_of(walk.from + walk.skip, p.chunk_magic) : 0;
-  auto next_chunk = [&](int ci) { return WIN && ci >= ci_near && ci < ci_far ? ci_far : ci + 1; };
+  const int passed = WIN && walk.skip > 0 && walk.from > 0 ? max(0, chunk_of(walk.from + walk.skip, p.chunk_magic) - ci_near - 1) : 0;
+  auto chunk_behind = [&](int ci, int steps) { return ci + steps + (WIN && (uint32_t)(ci_near - ci) < (uint32_t)steps ? passed : 0); };
   auto scale_load = [&](const float* scales, int pc) { return scales[(int64_t)pc * p.Hkv + h]; };
   auto uniform_f = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
   // the clamped tile start only ever moves forward, by at most one chunk per tile
@@ -574,7 +574,7 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
       c.ci = ci;
       c.pc = c.pc_next;
       c.pc_next = entry(c.pc_after);
-      c.pc_after = entry_load(next_chunk(next_chunk(ci)));
+      c.pc_after = entry_load(chunk_behind(ci, 2));
       if (FP8) {
         c.sc = uniform_f(c.sc_next);
         c.sc_next = scale_load(scales, c.pc_next);
@@ -587,8 +587,7 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
   float ksc_first = 1.f, vsc_first = 1.f;  // per-lane copies, loads in flight
   {
     const int ci0 = chunk_of(min(position(start), last), p.chunk_magic);
-    const int ci1 = next_chunk(ci0);
-    const int e0 = entry_load(ci0), e1 = entry_load(ci1), e2 = entry_load(next_chunk(ci1));
+    const int e0 = entry_load(ci0), e1 = entry_load(chunk_behind(ci0, 1)), e2 = entry_load(chunk_behind(ci0, 2));
     kcur.ci = ci0;
     kcur.pc = entry(e0);
     kcur.pc_next = entry(e1);
