@@ -1001,12 +1001,13 @@ static __device__ __forceinline__ void walk_segments(const DecodeParams& p, Seg 
     const int per = total_units / p.grid, rem = total_units - per * p.grid;
     t0 = (int)blockIdx.x * per + min((int)blockIdx.x, rem);
     t1 = t0 + per + ((int)blockIdx.x < rem ? 1 : 0);
-    // Windows make requests alike: where the grid has one or two workgroups for each, and hardly any are left over, no span starts in
-    // one request and ends in the next (32 / 8 heads of 128: 256 requests of 4 560-5 060 tokens, window 512, 105.7 -> 95.4 us, 1 024
-    // over fp8 110.4 -> 104.3; 128 requests, window 1 024, 98.6 -> 94.4.  Three and more for each: 3 % faster to 6 % slower).
+    // Windows make requests alike: where the grid has one or two workgroups for each, or each workgroup the same number of them, and hardly
+    // any workgroup is left over, no span starts in one request and ends in the next (32 / 8 heads of 128: 256 requests of 4 560-5 060
+    // tokens, window 512, 105.7 -> 95.4 us, 1 024 over fp8 110.4 -> 104.3; 128 requests, window 1 024, 98.6 -> 94.4.  Three and
+    // more workgroups for each: 3 % faster to 6 % slower).
     if constexpr (WIN) {
-      const int each = p.grid / p.R;
-      if (lead && (each == 1 || each == 2) && 32 * each * p.R >= 31 * p.grid) {
+      const int each = p.grid / p.R, held = (p.R + p.grid - 1) / p.grid;   // workgroups of a request, or requests of a workgroup
+      if (lead && each <= 2 && 32 * (each ? each * p.R : p.R) >= 31 * (each ? 1 : held) * p.grid) {
         int most = 0;
         for (int base = 0; base < p.R; base += 64) {
           const int i = base + lane;
@@ -1018,12 +1019,20 @@ static __device__ __forceinline__ void walk_segments(const DecodeParams& p, Seg 
         for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
         most = __builtin_amdgcn_readfirstlane(most);
         if ((int64_t)most * p.R * 32 <= (int64_t)total * 33 + 32 * p.R) {
-          const int i = (int)blockIdx.x / each, j = (int)blockIdx.x - i * each;
           t0 = t1 = 0;
-          if (i < p.R) {
-            const int rb = i ? units(i - 1) : 0, tiles = units(i) - rb - 1, share = tiles / each, more = tiles - share * each;
-            t0 = rb + (j ? 1 + share * j + min(j, more) : 0);
-            t1 = rb + 1 + share * (j + 1) + min(j + 1, more);
+          if (each) {
+            const int i = (int)blockIdx.x / each, j = (int)blockIdx.x - i * each;
+            if (i < p.R) {
+              const int rb = i ? units(i - 1) : 0, tiles = units(i) - rb - 1, share = tiles / each, more = tiles - share * each;
+              t0 = rb + (j ? 1 + share * j + min(j, more) : 0);
+              t1 = rb + 1 + share * (j + 1) + min(j + 1, more);
+            }
+          } else {
+            const int i = (int)blockIdx.x * held;
+            if (i < p.R) {
+              t0 = i ? units(i - 1) : 0;
+              t1 = units(min(i + held, p.R) - 1);
+            }
           }
         }
       }
