@@ -139,6 +139,19 @@ def test_decode_fp8_caches(mi, dev, d, chunk, dtype):
         c.check(mi)
 
 
+@pytest.mark.parametrize("R", [4, 8, 16, 24, 31, 70, 127])
+@pytest.mark.parametrize("d,fp8,alike", [(128, False, True), (64, True, True), (64, False, False)])
+def test_workgroups_dealt_out_by_requests(mi, dev, R, d, fp8, alike):
+    """Half a request, one, two and more for each of the grid's eight workgroups, and (requests not alike, or not going into the grid)
+    spans by tiles: every part of every request once."""
+    lens = [1000 + 17 * (7 * i % 5) for i in range(R)]
+    if not alike:
+        lens[R // 2] = 100
+    c = Case(dev, None, lens, 700, 3, d=d, fp8=fp8, seed=R)
+    with mi.ops.tuning(decode_grid=8):
+        c.check(mi)
+
+
 def test_many_requests_in_the_lanes_and_in_shared_memory(mi, dev):
     rng = random.Random(3)
     for n in (64, 65, 200):
