@@ -56,7 +56,8 @@ def flash_decode_and_prefill(q: Tensor, k: Tensor, v: Tensor, max_seqlen_q, max_
     ``flash_attn_varlen_func``.  ``window_size`` is flash-attn's ``(left, right)``, ``sink_tokens`` the first tokens of a
     request that stay in sight of every token.
     """
-    seen = dict(window_size=window_size, sink_tokens=sink_tokens)
+    # (named only where there is one: functions put in the places of the two below need not know them)
+    seen = {} if window_size is None and not sink_tokens else dict(window_size=window_size, sink_tokens=sink_tokens)
     if max_seqlen_q > 1:
         out = flash_attn_varlen_func(q.squeeze(1), k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
                                      softmax_scale=softmax_scale if softmax_scale is not None else q.shape[-1] ** -0.5,
@@ -97,6 +98,8 @@ class PagedSelfAttentionCore(torch.nn.Module):
     ``[axes, tokens]`` on the device, then goes with every call: where each token of the step stands, which is not where
     the cache holds it.  A layer with either runs norm, rotation and append as one launch and attention as another.
     """
+
+    window_size, sink_tokens, rotary_axes = None, 0, None   # (of layers made before these were)
 
     def __init__(self, layer_number: int, head_dim: int, *, qk_norm: Optional[str] = None, eps: float = 1e-5,
                  softmax_scale: Optional[float] = None, rotary_interleaved: bool = False, fused: bool = True,
@@ -228,9 +231,10 @@ class PagedSelfAttentionCore(torch.nn.Module):
             cu_q, max_q = ctx.cu_query_lengths()
             cu_k, kv_lens, max_k = ctx.cu_kv_lengths()
         k_scales, v_scales = ctx.key_value_scales(self.layer_number) if hasattr(ctx, "key_value_scales") else (None, None)
+        seen = {} if self.window_size is None else dict(window_size=self.window_size, sink_tokens=self.sink_tokens)
         out = flash_decode_and_prefill(query, k_cache, v_cache, max_q, max_k, cu_q, cu_k, kv_lens, block_table,
                                        softmax_scale=self.softmax_scale, k_scales=k_scales, v_scales=v_scales,
-                                       one_row_requests=one_row, window_size=self.window_size, sink_tokens=self.sink_tokens)
+                                       one_row_requests=one_row, **seen)
         return out.reshape(out.size(0), out.size(1), -1)
 
 
@@ -299,8 +303,8 @@ class PagedSelfAttentionLayer(torch.nn.Module):
             proj = self.linear_proj
             return output, (_parameter(proj, "bias") if proj.skip_bias_add else None)
         mixed_qkv, _ = self.linear_qkv(hidden_states)
-        core_attn_out = self.core.forward_mixed_qkv(mixed_qkv, self.num_query_heads, inference_context, rotary_pos_emb,
-                                                    axis_positions)
+        axes = () if axis_positions is None else (axis_positions,)   # (a core that was put here need not know them)
+        core_attn_out = self.core.forward_mixed_qkv(mixed_qkv, self.num_query_heads, inference_context, rotary_pos_emb, *axes)
         return self.linear_proj(core_attn_out)
 
     def _decode_in_one_call(self, hidden_states: Tensor, ctx, rotary_pos_emb) -> Optional[Tensor]:

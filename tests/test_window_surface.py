@@ -54,3 +54,30 @@ def test_positions_go_with_axes(mi):
     layer = mi.PagedSelfAttentionLayer(1, 64, 2, 1, 64)
     with pytest.raises(ValueError, match="rotary_sections"):
         layer.core.forward_mixed_qkv(mixed, 2, None, emb, positions)
+
+
+def test_calls_without_a_window_are_what_they_were(mi, monkeypatch):
+    """Functions in the places of the two attention calls, contexts and stored layers that know no windows."""
+    from importlib import import_module
+    attention = import_module(mi.__name__ + ".attention")
+    calls = []
+    for name in ("flash_attn_varlen_func", "flash_attn_with_kvcache"):
+        monkeypatch.setattr(attention, name, lambda *a, name=name, **k: calls.append((name, set(k))) or torch.zeros(4, 2, 64))
+    q = torch.zeros(4, 1, 2, 64)
+    attention.flash_decode_and_prefill(q, None, None, 4, 4, None, None, None, None)
+    attention.flash_decode_and_prefill(q, None, None, 1, 4, None, None, None, None)
+    assert [c[0] for c in calls] == ["flash_attn_varlen_func", "flash_attn_with_kvcache"]
+    assert all(not c[1] & {"window_size", "sink_tokens"} for c in calls)
+    attention.flash_decode_and_prefill(q, None, None, 1, 4, None, None, None, None, window_size=(3, 0), sink_tokens=2)
+    assert {"window_size", "sink_tokens"} <= calls[-1][1]
+    core = mi.PagedSelfAttentionCore(1, 64, window_size=(5, 0))
+    for name in ("window_size", "sink_tokens", "rotary_axes"):
+        delattr(core, name)
+    assert (core.window_size, core.sink_tokens, core.rotary_axes) == (None, 0, None)
+    layer = mi.PagedSelfAttentionLayer(1, 64, 2, 1, 64)
+    seen = []
+    layer.linear_qkv.forward = lambda x: (x, None)
+    layer.linear_proj.forward = lambda x: (x, None)
+    layer.core.forward_mixed_qkv = lambda mixed, heads, context, emb=None: seen.append(emb) or mixed
+    layer(torch.zeros(4, 1, 64), None, None)
+    assert seen == [None]
