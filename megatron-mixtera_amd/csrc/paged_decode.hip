@@ -2224,8 +2224,19 @@ int mi::launch_paged_decode(
 
   // 16-token sub-tiles per loop iteration (0 = automatic).
   int nt = tune.decode_tile_subtiles;
-  if (nt != 1 && nt != 2 && nt != 4) nt = kv_dtype == MI_KV_FP8_E4M3 ? 4 : 2;
-  if (win && kv_dtype != MI_KV_FP8_E4M3 && nt == 4) nt = 2;
+  const bool fp8_cache = kv_dtype == MI_KV_FP8_E4M3;
+  if (nt == 1 || nt == 2 || nt == 4) {
+    if (win && !fp8_cache && nt == 4) nt = 2;
+  } else if (!win) {
+    nt = fp8_cache ? 4 : 2;
+  } else {
+    // With a window less of a smaller tile is out of sight, and over an fp8 cache a third wavefront fits the SIMD: 32 tokens there (256
+    // requests, 32 / 8 heads, windows of 512 / 2 048 / 20 000, 64 tokens a tile and 32: width 128 55.9 / 184 / 1 615 us -> 53.8 / 179 /
+    // 1 544, width 64 39.3 / 132 / 1 318 -> 36.9 / 106 / 1 037).  Over a 16-bit cache 16, but for long walks of width 128 (256 requests,
+    // windows of 128 / 512 / 2 048: 38.1 / 94.4 / 327 -> 30.4 / 93.5 / 327, 4 096: 639 -> 644; 16 requests, 2 048: 34.0 -> 32.6; width 64,
+    // 256 requests, 512 / 4 096: 52.1 / 326 -> 51.1 / 321; width 192, 48 requests, 512: 45.7 -> 40.9).
+    nt = fp8_cache ? 2 : head_dim != 128 || window_keys(*win, win->max_len, 0) <= 2560 ? 1 : 2;
+  }
   if (head_dim == 256) nt = 1;                 // (registers: 64 accumulators + 32 each for queries, keys, values)
   else if (head_dim == 192 && nt > 2) nt = 2;
   if (fused) nt = kv_dtype == MI_KV_FP8_E4M3 ? MI_FUSED_FP8_NT : 1;  // (the prologue's registers on top of two 16-bit sub-tiles in flight would spill)
