@@ -151,7 +151,7 @@ static __device__ __forceinline__ Walk window_walk(const DecodeParams& p, int le
 // the others lie on one side.  An fp8 chunk's scale is taken as sign, power of two and factor (see value_parts), and fp16
 // probabilities stand 2^14 above the running maximum: as they are, one of a thousandth of the row's largest times a scale of a hundredth
 // would be subnormal, in the numerator and in the row sum.  Bound by HBM as the kernel without a window: 64 requests of 512-8 192 tokens,
-// window 2 048, 86 us (6.1 TB/s); 16 of 131 072, window 32 768, 331 us (6.5); fp8, 256 of 1 024-32 768, window 4 096, 325 us (6.3).
+// window 2 048, 83.5 us (6.3 TB/s); 16 of 131 072, window 32 768, 330 us (6.5); fp8, 256 of 1 024-32 768, window 4 096, 320 us (6.4).
 template <int HDK, int HDV, int NT, bool FP8, bool F16, bool FUSED = false, bool SHORT = false, bool WIN = false>
 static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int r, int row, int h, int hq0, int gq,
                                                       int len, int start, int end, bool whole, bool final_seg,
