@@ -139,6 +139,22 @@ def test_decode_fp8_caches(mi, dev, d, chunk, dtype):
         c.check(mi)
 
 
+@pytest.mark.parametrize("tiles", [1, 2, 4])
+@pytest.mark.parametrize("d,fp8,dtype", [(128, False, BF16), (64, False, FP16), (192, False, BF16), (128, True, BF16), (64, True, FP16)])
+@pytest.mark.parametrize("lens,window,sinks", SHAPES[3::2] + [([0, 200, 5, 0], 33, 2)])
+def test_decode_tiles_of_every_size(mi, dev, lens, window, sinks, d, fp8, dtype, tiles):
+    c = Case(dev, None, lens, window, sinks, d=d, fp8=fp8, dtype=dtype, seed=sum(lens) + d)
+    for grid in (3, 17):
+        with mi.ops.tuning(decode_tile_subtiles=tiles, decode_grid=grid):
+            c.check(mi)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_decode_of_long_walks(mi, dev, d):
+    """Walks past the line between small tiles and large ones."""
+    Case(dev, None, [2900, 4100, 60], 2600, 4, Hq=4, Hkv=2, d=d, seed=d).check(mi)
+
+
 @pytest.mark.parametrize("R", [4, 8, 16, 24, 31, 70, 127])
 @pytest.mark.parametrize("d,fp8,alike", [(128, False, True), (64, True, True), (64, False, False)])
 def test_workgroups_dealt_out_by_requests(mi, dev, R, d, fp8, alike):
