@@ -123,7 +123,7 @@ struct Walk {
 template <int TK>
 static __device__ __forceinline__ Walk window_walk(const DecodeParams& p, int len) {
   Walk w;
-  w.len = min(len, p.max_len);
+  w.len = min(max(len, 0), p.max_len);   // (from below as well: a length far below zero less a window would wrap to a long walk)
   w.first = max(0, w.len - p.window);
   w.from = (p.sinks + TK - 1) / TK * TK;
   w.skip = max(0, w.first / TK * TK - w.from);

@@ -234,6 +234,22 @@ def test_lengths_are_kept_in_the_table(mi, dev, form, lens, d, chunk):
     c.check(mi, one_row_requests=False) if new else c.check(mi)
 
 
+@pytest.mark.parametrize("d,fp8", [(64, False), (96, False), (128, False), (128, True)])
+@pytest.mark.parametrize("window,sinks", [(20, 3), (1, 0), (1 << 62, 3), (1 << 29, 0)])
+@pytest.mark.parametrize("form", ["decode", "one row", "stream", "stream of many"])
+def test_lengths_far_below_zero_are_zero(mi, dev, form, window, sinks, d, fp8):
+    """Such a length less the window does not wrap: nothing is walked, the row is zeros, in decode calls and for one-row requests of prompts."""
+    more = 40 if form == "stream of many" else 1
+    lens = [-(1 << 31), 90, -2000000000, -1, 70, -(1 << 31) + 1] * more
+    c = Case(dev, [1, 1, 1, 1, 7, 1] * more if form == "one row" else None, [max(n, 0) for n in lens], window, sinks, d=d, fp8=fp8, seed=d)
+    c.lens = lens
+    if form.startswith("stream"):
+        with mi.ops.tuning(decode_grid=7):
+            c.check(mi)
+    else:
+        c.check(mi)
+
+
 @pytest.mark.parametrize("chunk", [16, 48, 80])
 @pytest.mark.parametrize("d", [64, 96, 128, 192, 256])
 def test_prompts_over_chunks_of_other_sizes(mi, dev, chunk, d):
