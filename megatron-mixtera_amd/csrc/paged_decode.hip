@@ -900,8 +900,11 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
           *reinterpret_cast<float2*>(o + DV * i + e) = make_float2(acc[e][i] * inv, acc[e + 1][i] * inv);
       }
     }
-    // (WIN: parts have one lift in common; one without a finite score must not make the merge's maximum infinite)
-    if (g == 0) p.part_lse[row] = WIN && l_tot == 0.f ? -3e38f : m_run + fast_log2(l_tot);
+    // (WIN: parts have one lift in common; one without a finite score must not make the merge's maximum infinite, nor one whose sum is
+    // no number be taken there for no part at all: its values carry that on)
+    float lse = m_run + fast_log2(l_tot);
+    if constexpr (WIN) lse = l_tot == 0.f ? -3e38f : __builtin_isnan(l_tot) ? m_run : lse;
+    if (g == 0) p.part_lse[row] = lse;
   }
 }
 

@@ -353,6 +353,18 @@ def test_infinite_scores(mi, dev, form):
     c.check(mi)
 
 
+@pytest.mark.parametrize("d,fp8", [(128, False), (64, True), (256, False)])
+@pytest.mark.parametrize("grid", [7, 9, 17, 25, 40])
+def test_a_part_of_nothing_but_nan_reaches_the_result(mi, dev, grid, d, fp8):
+    """A key that is no number, in the first, a middle or the last of the parts that a request is cut into: its part's sum is NaN, and so
+    is the row, also where the merge has that part in a group of its own."""
+    for pos in (0, 7, 700, 1151, 1300, 1499):
+        c = Case(dev, None, [1500], 1480, 20, Hq=4, Hkv=2, d=d, fp8=fp8, seed=pos)
+        _spoil(c, 0, pos, math.nan, None)
+        with mi.ops.tuning(decode_grid=grid):
+            assert c.check(mi).isnan().all()
+
+
 def test_chunks_out_of_sight_need_not_exist(mi, dev):
     """Table entries of chunks that no row sees: anything, ids outside the cache among it."""
     for form in ("decode", "prompts"):
