@@ -21,7 +21,9 @@ import torch
 from torch import Tensor
 
 from . import ops
+from .attention import PagedSelfAttentionCore
 from .contexts.dynamic_context import WarmupEngineMode
+from .flash_attn_interface import window_argument
 
 
 class DecodeLayerGraphs:
@@ -61,9 +63,12 @@ class DecodeLayerGraphs:
                                           ctx.max_sequence_length, 0)
         if ctx.non_decode_cuda_graphs:  # prefill / mixed steps may split the keys of a request: more scratch
             table_tokens = ctx.request_to_kv_chunk_ids.size(1) * ctx.chunk_size_tokens
+            windows = [window_argument(layer.window_size, layer.sink_tokens) for layer in self.layers
+                       if isinstance(layer, PagedSelfAttentionCore)]
             for n in ctx.cuda_graph_token_counts:
                 for max_kv in (ctx.max_sequence_length, table_tokens):
-                    need = max(need, ops.prefill_workspace_bytes(n, ctx.max_requests, num_query_heads, hkv, d, max_kv, 0))
+                    for window in [{}] + [w for w in windows if w]:
+                        need = max(need, ops.prefill_workspace_bytes(n, ctx.max_requests, num_query_heads, hkv, d, max_kv, 0, **window))
         self.workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=ctx.device)
 
     @property

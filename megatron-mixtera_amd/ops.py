@@ -264,9 +264,14 @@ def decode_workspace_bytes(R: int, Hq: int, Hkv: int, head_dim: int, chunk: int,
 
 
 def prefill_workspace_bytes(T: int, R: int, Hq: int, Hkv: int, head_dim: int, max_kv_len: int,
-                            split_tokens: int = 0) -> int:
+                            split_tokens: int = 0, window: Optional[int] = None, sinks: int = 0) -> int:
     """Scratch of one varlen attention call over ``T`` query rows of ``R`` requests: the decode part's
-    partials and, when the tile kernel splits the keys, its partials behind them."""
+    partials and, when the tile kernel splits the keys, its partials behind them.  A call with a ``window`` has a
+    number of its own: its shorter walks may be split into fewer parts than the whole keys or into more."""
+    if window is not None:
+        _require(window >= 1 and sinks >= 0 and split_tokens == 0, "a window of at least 1, sinks of at least 0, no split_tokens")
+        return _native().abi_mi_window_prefill_workspace_bytes(T, R, Hq, Hkv, head_dim, max_kv_len, min(window, 1 << 30),
+                                                               min(sinks, 1 << 30), _tuning_arg())
     return _native().abi_mi_prefill_workspace_bytes(T, R, Hq, Hkv, head_dim, max_kv_len, split_tokens, _tuning_arg())
 
 

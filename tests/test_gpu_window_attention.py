@@ -508,3 +508,15 @@ def test_drawn_cases(mi, dev, seed):
     knobs = dict(decode_grid=rng.choice((1, 2, 9, 50)), prefill_kv_split=rng.choice((-1, 2, 4)))
     with mi.ops.tuning(**knobs):
         c.check(mi)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_buffer_sized_for_the_window(mi, dev, d):
+    """``prefill_workspace_bytes`` with the call's window is what the call takes, where that is more than without one as well."""
+    c = Case(dev, [9, 7], [560, 570], 189, 4, Hq=32, Hkv=8, d=d, seed=d)
+    need = mi.ops.prefill_workspace_bytes(16, 2, 32, 8, d, 576, window=189, sinks=4)
+    assert need > mi.ops.prefill_workspace_bytes(16, 2, 32, 8, d, 576)
+    with mi.ops.use_workspace(torch.empty(need, dtype=torch.uint8, device=dev)):
+        c.check(mi, max_kv_len=576)
+    with mi.ops.use_workspace(torch.empty(need - 1, dtype=torch.uint8, device=dev)), pytest.raises(ValueError, match="too small"):
+        c.run(mi, max_kv_len=576)

@@ -81,3 +81,27 @@ def test_calls_without_a_window_are_what_they_were(mi, monkeypatch):
     layer.core.forward_mixed_qkv = lambda mixed, heads, context, emb=None: seen.append(emb) or mixed
     layer(torch.zeros(4, 1, 64), None, None)
     assert seen == [None]
+
+
+def test_the_workspace_of_captured_windows(mi):
+    """A walk of 449 keys of 576 is cut into more parts than the whole 576 are: the graphs' buffer has room for either."""
+    cls = mi.DynamicInferenceContext
+    saved = (cls.TOKEN_ROUNDER, cls.REQUEST_ROUNDER)
+    cls.TOKEN_ROUNDER = cls.REQUEST_ROUNDER = 4
+    try:
+        ctx = cls(params_dtype=torch.bfloat16, num_layers=1, kv_channels=128, num_attention_heads=8, max_sequence_length=576,
+                  buffer_size_gb=0.05, buffer_guaranteed_fraction=0.1, chunk_size_tokens=64, max_requests_override=16,
+                  max_tokens_override=1024, num_cuda_graphs=2, device="cpu")
+    finally:
+        cls.TOKEN_ROUNDER, cls.REQUEST_ROUNDER = saved
+    core = mi.PagedSelfAttentionCore(1, 128, window_size=(188, 0), sink_tokens=4)
+    need, plain = mi.ops.prefill_workspace_bytes(16, 16, 32, 8, 128, 576, window=189, sinks=4), mi.ops.prefill_workspace_bytes(16, 16, 32, 8, 128, 576)
+    assert need == mi._lib.load().mi_window_prefill_workspace_bytes(16, 16, 32, 8, 128, 576, 189, 4, None) > plain
+    assert mi.DecodeLayerGraphs(ctx, [torch.nn.Identity(), core], num_query_heads=32).workspace.numel() >= need
+    foreign = torch.nn.Identity()
+    foreign.window_size = 7   # (another module's own: not read)
+    assert mi.DecodeLayerGraphs(ctx, [foreign], num_query_heads=32).workspace.numel() < need
+    assert mi.ops.prefill_workspace_bytes(16, 16, 32, 8, 128, 576, window=1 << 62, sinks=1 << 62) == plain
+    for bad in (dict(window=0), dict(window=5, sinks=-1), dict(window=5, split_tokens=16)):
+        with pytest.raises(ValueError):
+            mi.ops.prefill_workspace_bytes(16, 16, 32, 8, 128, 576, **bad)
