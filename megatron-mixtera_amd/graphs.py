@@ -37,7 +37,8 @@ class DecodeLayerGraphs:
     ``replay(layer_index, query, key, value)`` copies the step's tensors into the static inputs
     of the graph for ``context.padded_active_token_count`` and the step's kind, and returns the
     static output ``[padded, 1, Hq*d]`` (valid until the next replay of the same graph).
-    Layers with ``rotary_sections`` need ``axis_positions``, one int64 ``[axes, tokens]`` tensor that the graphs read.
+    Layers with ``rotary_sections`` need ``axis_positions``, one int64 ``[axes, tokens]`` tensor that the graphs read; layers
+    without may be in the same list.
     """
 
     def __init__(self, context, layers: Sequence[torch.nn.Module], *, num_query_heads: int,
@@ -109,7 +110,8 @@ class DecodeLayerGraphs:
 
     def _run(self, layer, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
         with ops.use_workspace(self.workspace):
-            if self.axis_positions is None:
+            # (a core without axes has no use for positions, and refuses them)
+            if self.axis_positions is None or (isinstance(layer, PagedSelfAttentionCore) and layer.rotary_axes is None):
                 return layer(q, k, v, self.context, self.rotary_pos_emb)
             return layer(q, k, v, self.context, self.rotary_pos_emb, self.axis_positions)
 

@@ -239,6 +239,44 @@ def test_graphs(mi, dev):
         cls.TOKEN_ROUNDER, cls.REQUEST_ROUNDER = saved
 
 
+@pytest.mark.parametrize("order", [(True, False), (False, True)])
+def test_graphs_of_layers_with_and_without_axes(mi, dev, order):
+    """One set of graphs over a layer of each kind: the positions go to those that have axes."""
+    cls = mi.DynamicInferenceContext
+    saved = (cls.TOKEN_ROUNDER, cls.REQUEST_ROUNDER)
+    cls.TOKEN_ROUNDER = cls.REQUEST_ROUNDER = 4
+    try:
+        gen = torch.Generator().manual_seed(11)
+        table = orn.rotary_table(MOST, 128).to(dev)
+        cores = [mi.PagedSelfAttentionCore(i + 1, 128, rotary_sections=(16, 24, 24) if several else None, device=dev).requires_grad_(False)
+                 for i, several in enumerate(order)]
+        captured, eager = _context(mi, dev, 128, BF16, num_cuda_graphs=1), _context(mi, dev, 128, BF16)
+        held = torch.zeros(3, max(captured.cuda_graph_token_counts), dtype=torch.int64, device=dev)
+        graphs = mi.DecodeLayerGraphs(captured, cores, num_query_heads=HQ, rotary_pos_emb=(table, table), axis_positions=held)
+        graphs.capture()
+        for i, n in enumerate((2, 1, 3)):
+            for ctx in (captured, eager):
+                ctx.add_request(i, torch.arange(n, device=dev), num_tokens_to_generate=60)
+        for step in range(6):
+            for ctx in (captured, eager):
+                ctx.initialize_attention_state()
+            act, m = eager.active_token_count, eager.padded_active_token_count
+            n = max(m, captured.padded_active_token_count)
+            positions = torch.randint(0, MOST, (3, n), generator=gen).to(dev)
+            held[:, :n] = positions
+            for i, (core, several) in enumerate(zip(cores, order)):
+                q, k, v = (torch.randn(n, 1, h, 128, generator=gen).bfloat16().to(dev) for h in (HQ, HKV, HKV))
+                got = graphs.replay(i, q, k, v).clone()
+                want = core(q[:m].clone(), k[:m], v[:m], eager, (table, table), *((positions,) if several else ()))
+                # (a decode step of the layer without axes is one launch here and there: the same kernels on both sides)
+                assert torch.equal(got[:act], want[:act]), f"step {step}, layer {i}"
+            live = eager.total_request_count
+            for ctx in (captured, eager):
+                ctx.update_requests(torch.ones(live, dtype=torch.int32, device=dev), torch.arange(live, device=dev))
+    finally:
+        cls.TOKEN_ROUNDER, cls.REQUEST_ROUNDER = saved
+
+
 def test_flash_attention_forms(mi, dev):
     """``window_size`` and ``sink_tokens`` of the adapters are the window and the sinks of the calls below them."""
     gen = torch.Generator(device=dev).manual_seed(1)

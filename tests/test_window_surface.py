@@ -105,3 +105,23 @@ def test_the_workspace_of_captured_windows(mi):
     for bad in (dict(window=0), dict(window=5, sinks=-1), dict(window=5, split_tokens=16)):
         with pytest.raises(ValueError):
             mi.ops.prefill_workspace_bytes(16, 16, 32, 8, 128, 576, **bad)
+
+
+def test_positions_go_to_the_layers_that_have_axes(mi):
+    """One list of captured layers may hold both kinds, and modules that are no core: those get the positions, as they always did."""
+    class Graphs(mi.DecodeLayerGraphs):
+        def __init__(self, positions):   # (no context: only what a layer is called with is looked at)
+            self.context, self.rotary_pos_emb, self.workspace, self.axis_positions = None, None, torch.empty(1), positions
+
+    class Plain(mi.PagedSelfAttentionCore):
+        def forward(self, *args):
+            return args
+
+    class Other(torch.nn.Module):
+        def forward(self, *args):
+            return args
+    positions = torch.zeros(3, 4, dtype=torch.int64)
+    plain, several = Plain(1, 64), Plain(1, 64, rotary_sections=(8, 12, 12))
+    for layer, given in ((plain, 5), (several, 6), (Other(), 6)):
+        assert len(Graphs(positions)._run(layer, None, None, None)) == given
+        assert len(Graphs(None)._run(layer, None, None, None)) == 5
