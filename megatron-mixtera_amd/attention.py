@@ -65,7 +65,7 @@ def flash_decode_and_prefill(q: Tensor, k: Tensor, v: Tensor, max_seqlen_q, max_
                                      k_scales=k_scales, v_scales=v_scales, one_row_requests=one_row_requests, **seen)
         return out.unsqueeze(1)
     if mla_head_dim_v is not None:
-        if window_size not in (None, (-1, -1)):
+        if window_argument(window_size, sink_tokens):
             raise NotImplementedError("no window over a latent cache")
         metadata, num_splits = get_mla_metadata(seqlens_k, q.size(2), 1)
         out, _ = flash_mla_with_kvcache(q, k.unsqueeze(-2), block_table, seqlens_k, mla_head_dim_v, metadata,

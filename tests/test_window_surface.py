@@ -125,3 +125,23 @@ def test_positions_go_to_the_layers_that_have_axes(mi):
     for layer, given in ((plain, 5), (several, 6), (Other(), 6)):
         assert len(Graphs(positions)._run(layer, None, None, None)) == given
         assert len(Graphs(None)._run(layer, None, None, None)) == 5
+
+
+def test_the_latent_decode_branch_reads_windows_as_the_others_do(mi, monkeypatch):
+    from importlib import import_module
+    attention = import_module(mi.__name__ + ".attention")
+    i32 = dict(dtype=torch.int32)
+    lens, table = torch.tensor([4], **i32), torch.zeros(1, 1, **i32)
+
+    def run(**more):
+        return attention.flash_decode_and_prefill(torch.zeros(1, 1, 2, 576), torch.zeros(1, 16, 576), None, 1, 4, None, None, lens, table,
+                                                  mla_head_dim_v=512, **more)
+    for more in (dict(sink_tokens=4), dict(window_size=(-1, -1), sink_tokens=4), dict(window_size=(3, 0), sink_tokens=-1)):
+        with pytest.raises(ValueError, match="sink_tokens"):
+            run(**more)
+    with pytest.raises(NotImplementedError, match="window"):
+        run(window_size=(3, 0), sink_tokens=2)
+    monkeypatch.setattr(attention, "get_mla_metadata", lambda *a: (None, None))
+    monkeypatch.setattr(attention, "flash_mla_with_kvcache", lambda *a, **k: ("ran", None))
+    for none in (None, (-1, -1), (-1, 0), [-1, -1]):
+        assert run(window_size=none) == "ran"
