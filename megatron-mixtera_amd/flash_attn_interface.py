@@ -10,6 +10,7 @@ before it and itself, and ``sink_tokens`` (an addition) keeps a request's first 
 """
 from __future__ import annotations
 
+import operator
 import weakref
 from typing import Optional
 
@@ -57,8 +58,13 @@ def _reject(**unsupported) -> None:
 def window_argument(window_size, sink_tokens: int) -> dict:
     """``window_size`` and ``sink_tokens`` as the ``window`` / ``sinks`` of the paged calls: of the tokens before it a token
     sees the last ``left``, and every one where ``left`` is -1.  There are no keys to the right of a causal row, so ``right`` is
-    -1 or 0."""
-    left, right = (-1, -1) if window_size is None else window_size
+    -1 or 0.  None, 0 and False are no window."""
+    if window_size is None or (isinstance(window_size, (bool, int, float)) and not window_size):
+        window_size = (-1, -1)
+    try:
+        left, right = map(operator.index, window_size if isinstance(window_size, (tuple, list)) else ())
+    except (TypeError, ValueError):   # (no pair, or not of whole numbers)
+        left = right = -2
     if left < -1 or right not in (-1, 0):
         raise NotImplementedError(f"window_size on the paged MI355X path is (left, 0), (left, -1) or (-1, -1), not {window_size}")
     if sink_tokens < 0:

@@ -145,3 +145,23 @@ def test_the_latent_decode_branch_reads_windows_as_the_others_do(mi, monkeypatch
     monkeypatch.setattr(attention, "flash_mla_with_kvcache", lambda *a, **k: ("ran", None))
     for none in (None, (-1, -1), (-1, 0), [-1, -1]):
         assert run(window_size=none) == "ran"
+
+
+def test_window_sizes_that_are_no_pairs(mi):
+    """0 and False are no window, as they were before there were any; whatever else is no pair of whole numbers is refused by name."""
+    from importlib import import_module
+    window = import_module(mi.__name__ + ".flash_attn_interface").window_argument
+    for none in (None, 0, False, 0.0, (-1, -1), [-1, 0]):
+        assert window(none, 0) == {}
+        assert mi.PagedSelfAttentionCore(1, 64, window_size=none).window_size is None
+        with pytest.raises(ValueError, match="sink_tokens"):
+            window(none, 4)
+    assert window([5, 0], 2) == window((5, -1), 2) == dict(window=6, sinks=2)
+    q, cache = torch.zeros(4, 2, 64), torch.zeros(1, 16, 2, 64)
+    i32 = dict(dtype=torch.int32)
+    for other in (5, True, 1.5, "5", (5,), (5, 0, 0), (None, 0), (5.0, 0), torch.tensor([-1, -1]), object()):
+        with pytest.raises(NotImplementedError, match="window_size"):
+            window(other, 0)
+        with pytest.raises(NotImplementedError, match="window_size"):
+            mi.flash_attn_with_kvcache(q[:1, None], cache, cache, cache_seqlens=torch.tensor([4], **i32),
+                                       block_table=torch.zeros(1, 1, **i32), window_size=other)
