@@ -519,8 +519,8 @@ int mi_norm_rope_append(const void* q, int64_t q_stride_tok, void* q_out, int64_
  * The same where a token has positions on up to four axes (time, height, width of images and video; text counts alike on
  * all): rotary pair i belongs to axis pair_axes[i] and turns by row positions[axis][t] of rotary_angles.  Half-split pairs
  * are (i, i + rot_dim / 2), interleaved ones (2 i, 2 i + 1); each element takes its own column of the row, as above.
- * `positions`: `axes` rows of T int64, positions_stride apart, for queries and keys alike; positions are kept inside the
- * table's `angles_rows` rows.  pair_axes: rot_dim / 2 bytes of HOST memory, read during the call.  Everything else as in
+ * `positions`: `axes` rows of T int64, positions_stride apart (0: one row for all axes), for queries and keys alike; positions
+ * are kept inside the table's `angles_rows` rows.  pair_axes: rot_dim / 2 bytes of HOST memory, read during the call.  Everything else as in
  * mi_norm_rope_append and mi_qkv_norm_rope_append; rotary_angles may not be null.
  */
 int mi_norm_rope_append_axes(const void* q, int64_t q_stride_tok, void* q_out, int64_t q_out_stride_tok, const void* k,

@@ -1003,7 +1003,8 @@ int axes_launch(const NormRopeParams& base, const int64_t* positions, int64_t po
   if (!p.emb || !pair_axes || !positions) return fail(MI_ERR_NULL, "angles, positions or the pairs' axes missing");
   if (n_axes < 1 || n_axes > 4) return fail(MI_ERR_UNSUPPORTED, "one to four axes");
   if (angles_rows < 1) return fail(MI_ERR_SHAPE, "the table of angles has no row");
-  if (positions_stride < p.T && n_axes > 1) return fail(MI_ERR_SHAPE, "positions of two axes overlap");
+  // (0: one row for every axis, as text has it; rows that overlap otherwise are a caller's slip)
+  if (positions_stride != 0 && positions_stride < p.T && n_axes > 1) return fail(MI_ERR_SHAPE, "positions of two axes overlap");
   if (p.rot <= 0 || p.rot > 256 || (p.rot & 1)) return fail(MI_ERR_SHAPE, "rot_dim must be even and within head_dim");
   p.q_pos = positions; p.k_pos = nullptr; p.pos_st = positions_stride; p.n_axes = n_axes; p.emb_rows = angles_rows;
   for (uint32_t& w : p.axes) w = 0;

@@ -384,8 +384,8 @@ def norm_rope_append(query: Optional[Tensor], key: Optional[Tensor], *, value: O
     ``key`` (result to ``key_out`` and/or straight into the cache slot, together with ``value``).
 
     With ``rotary_axes`` (one byte per rotary pair, see :func:`rotary_axes`) positions have several axes: ``q_positions`` is
-    int64 ``[axes, T]`` (up to four), for queries and keys alike, and a pair turns by the angle at its axis's position.
-    Positions outside the table count as its first or last row."""
+    int64 ``[axes, T]`` (up to four; one row expanded over the axes is fine), for queries and keys alike, and a pair turns by the angle
+    at its axis's position.  Positions outside the table count as its first or last row."""
     _native().norm_rope_append(query, key, value, q_weight, k_weight, eps, _NORM_KINDS[norm], rotary_emb, q_positions,
                                k_positions, rotary_interleaved, mscale, query_out, key_out, k_cache, v_cache,
                                token_to_chunk_idx, token_to_local_pos, block_table, kv_lens, faithful_rounding,

@@ -248,6 +248,23 @@ def test_text_counts_alike_on_all_axes(mi, dev):
     assert (axes != plain).float().mean() < 0.01
 
 
+@pytest.mark.parametrize("T", [1, 64, 1000])
+@pytest.mark.parametrize("axes", [2, 3, 4])
+def test_one_row_of_positions_for_every_axis(mi, dev, T, axes):
+    """Steps of text come as one row expanded over the axes (stride 0): the same as rows of their own, in every kernel and call."""
+    class Text(Case):
+        def common(self, mi, **over):
+            more = super().common(mi, **over)
+            more["q_positions"] = more["q_positions"][0].expand(axes, T)
+            assert more["q_positions"].stride(0) == 0
+            return more
+    c = Text(dev, T, sections=_sections(64, axes), seed=T)
+    c.positions[:] = c.positions[:1].clone()
+    for tuned in (0, -1):
+        c.check(mi, tuned=tuned)
+        c.check(mi, mixed=True, faithful=True, tuned=tuned)
+
+
 def test_many_tokens(mi, dev):
     Case(dev, 5001, Hq=4, Hkv=1, d=64, seed=10).check(mi, mixed=True)
     Case(dev, 4500, Hq=2, Hkv=2, d=128, seed=10).check(mi, faithful=True)
