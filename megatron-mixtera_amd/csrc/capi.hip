@@ -72,7 +72,8 @@ int mi::check_window(int32_t window, int32_t sinks, int32_t n_chunks, int32_t bt
   if (window < 1) return bad("the window must be at least 1 (a token sees itself)");
   if (sinks < 0) return bad("sinks must not be negative");
   if (n_chunks < 1) return bad("the cache has no chunk");
-  if (bt_columns < 1 || (R > 1 && bt_stride < bt_columns)) return bad("block_table needs a column, and rows that do not overlap");
+  // (a stride of 0: one row for all requests)
+  if (bt_columns < 1 || (R > 1 && bt_stride != 0 && bt_stride < bt_columns)) return bad("block_table needs a column, and rows that do not overlap");
   if (chunk_tokens < 1) return bad("chunk size must be a positive multiple of 16");
   // (a token's chunk is its number times 2^40 / chunk_tokens in 64 bits; positions behind the last tile have 31)
   const int64_t tokens = (int64_t)bt_columns * chunk_tokens;

@@ -394,6 +394,24 @@ def test_strides_and_outputs_given(mi, dev):
         assert got.data_ptr() == out.data_ptr() and torch.equal(got.squeeze(1), plain) and (out[..., 128:] == 7).all()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("form", ["decode", "prompts"])
+def test_one_row_of_the_table_for_every_request(mi, dev, form, fp8):
+    """Requests over the same tokens: a table expanded over them (stride 0), with a window as without one."""
+    c = Case(dev, None if form == "decode" else [40, 1, 70], [500, 300, 411], 130, 5, fp8=fp8, seed=13)
+    c.table = c.table[:1].expand(3, -1)
+    args, more = c.inputs()
+    args[-1] = args[-1][0].expand(3, -1)
+    assert args[-1].stride(0) == 0
+    run = mi.ops.paged_decode_attention if form == "decode" else mi.ops.paged_prefill_attention
+    c.check(mi, got=run(*args, **more))
+    with mi.ops.tuning(decode_grid=5):
+        c.check(mi, got=run(*args, **more))
+    more.update(window=None, sinks=0)
+    c.window, c.sinks = 1000, 0
+    c.check(mi, got=run(*args, **more))
+
+
 def test_a_cache_of_more_than_four_gibibytes(mi, dev):
     """Chunks on both sides of 2^32 bytes."""
     chunk, Hkv, d = 256, 8, 128
