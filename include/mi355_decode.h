@@ -403,7 +403,7 @@ int mi_paged_prefill_attention_tiles(const void* q, int64_t q_stride_tok, int64_
  * varlen call.  What a row does not see does not reach it, whatever the cache holds there, NaN included.
  *
  * `n_chunks`: chunks of the cache; `bt_columns`: of the block table (fewer than 2^31 - 512 tokens and 2^24 columns; a bt_stride
- * of 0: one row for all requests).
+ * of 0: one row for all requests).  min(R, 7 680) requests must not see 2^31 tiles of 16 tokens, by the window and the table.
  * Chunks without a token in sight of the call's rows are not needed: their table entries may hold anything.  Entries that
  * are used are kept inside the cache, lengths from 0 to what the table has room for.  kv_dtype, scales and everything else as in
  * mi_paged_decode_attention (workspace: mi_decode_workspace_bytes) and mi_paged_prefill_attention / _fp8 / _tiles

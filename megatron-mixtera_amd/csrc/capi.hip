@@ -80,6 +80,10 @@ int mi::check_window(int32_t window, int32_t sinks, int32_t n_chunks, int32_t bt
   if (tokens > 0x7ffffe00) return bad("block tables of 2^31 tokens and more (less 512) are not served");
   if (bt_columns >= 1 << 24) return bad("block tables of 2^24 columns and more are not served");
   if (((int64_t)1 << 40) % chunk_tokens && tokens * chunk_tokens >= (int64_t)1 << 40) return bad("block tables of so many tokens need a chunk size that is a power of two");
+  // (the decode stream counts the tiles of a launch's requests in 32 bits, each one longer for its start)
+  const int64_t seen = (int64_t)window + sinks < tokens ? (int64_t)window + sinks : tokens;
+  if ((seen / 16 + 8) * (R < kMaxRequestsPerLaunch ? R : kMaxRequestsPerLaunch) > INT32_MAX)
+    return bad("batches that see 2^31 tiles of 16 tokens and more are not served");
   *out = {window < kMostWindow ? window : kMostWindow, sinks < kMostWindow ? sinks : kMostWindow, n_chunks, (int32_t)tokens};
   return MI_OK;
 }

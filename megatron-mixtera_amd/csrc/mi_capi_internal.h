@@ -53,6 +53,8 @@ struct WindowArgs {
   int32_t n_chunks;        // chunks of the cache
   int32_t max_len;         // tokens that the block table has room for
 };
+// Requests one launch of the streaming decode kernels takes: their tile prefix sums and lengths sit in LDS.
+constexpr int kMaxRequestsPerLaunch = 7680;
 constexpr int32_t kMostWindow = 1 << 30;   // (of more tokens than that, all are in sight of a request that 31 bits can count)
 // Keys that one of `rows` neighbouring rows sees at most, of at most `len`.
 inline int32_t window_keys(const WindowArgs& w, int64_t len, int rows) {

@@ -2043,9 +2043,6 @@ static void launch_merge(const DecodeParams& p, int grid_x, int R, int Hq, int h
 // 4096, its 33.5 MB all read: 35.8 -> 34.4 us; with 20 or 26 MiB read of it, 35.5: the rest sets the projection's time.)
 constexpr int64_t kFetchBytes = (int64_t)32 << 20;
 
-// Requests one launch of the streaming kernels takes: their tile prefix sums and lengths sit in LDS.
-constexpr int kMaxRequestsPerLaunch = 7680;
-
 // Wavefronts along the heads: one per KV head and 16 query heads that share it.
 static int head_waves(int Hq, int Hkv) { return Hkv * ((Hq / Hkv + 15) / 16); }
 

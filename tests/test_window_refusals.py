@@ -52,6 +52,17 @@ def test_prompts(mi, change, word):
     _error(mi, _prompts(mi, **change), word)
 
 
+@pytest.mark.parametrize("call", [_decode, _prompts])
+def test_more_tiles_than_32_bits_count(mi, call):
+    """What all requests see, in tiles of 16 tokens, is counted in 32 bits: 2 048 requests of 2^24 tokens each are too many."""
+    room = dict(cols=1 << 16, bts=1 << 16, chunk=256, sc=256 * 1024)
+    _error(mi, call(mi, R=2048, window=1 << 30, **room), "2^31")
+    _error(mi, call(mi, R=2048, window=1 << 23, sinks=1 << 23, **room), "2^31")
+    _error(mi, call(mi, R=1 << 20, window=1 << 23, **room), "2^31")   # (slices of 7 680 requests, 2^19 tiles each)
+    for fine in (dict(R=2048, window=1 << 23), dict(R=1024, window=1 << 30), dict(R=1 << 20, window=1 << 21)):
+        _error(mi, call(mi, lens=None, **fine, **room), "null")   # (refused for what comes after)
+
+
 def test_kernels_that_have_no_window(mi):
     import ctypes
     for knob in (1, 2):
