@@ -61,10 +61,10 @@ struct NormRopeParams {
 };
 
 // Positions with several axes: every rotary pair belongs to one of up to four, and turns by the angle at the token's position on
-// that axis.  Queries and keys have one set of positions, q_pos: axis a of token t at a * pos_st + t.
+// that axis.  Queries and keys have one set of positions, q_pos: axis a of token t at a * pos_st + t.  There is a table (emb), always.
 struct AxesParams : NormRopeParams {
   int64_t pos_st;
-  int32_t n_axes, emb_rows;   // positions are kept inside the table's rows
+  int32_t emb_rows;           // positions are kept inside the table's rows
   uint32_t axes[8];           // two bits per pair, from the lowest
   int32_t waves_per_token;
   uint32_t wpt_magic;         // ceil(2^32 / waves_per_token), for more than one
@@ -535,45 +535,41 @@ __global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
     slot_local = p.tok_local[t];
   }
   const int half = p.rot >> 1;
-  int64_t row[NE] = {};
-  if (p.emb) {
+  int64_t row[NE];
 #pragma unroll
-    for (int i = 0; i < NE; ++i) row[i] = axis_position(p, t, min(lane + 64 * i, p.rot - 1));
-  }
-  const bool rotate = p.emb && e0 < p.rot;   // (whole lanes: see the launch)
+  for (int i = 0; i < NE; ++i) row[i] = axis_position(p, t, min(lane + 64 * i, p.rot - 1));
+  const bool rotate = e0 < p.rot;   // (whole lanes: see the launch)
   const int pe = PARTNER == 0 || !rotate ? e0 : e0 < half ? e0 + half : e0 - half;   // the partners' first column
   auto weight = [&](const uint16_t* w, int at) {
     return p.norm == MI_NORM_RMS && w ? ld16(w + at) : make_uint4(ones2<F16>(), ones2<F16>(), ones2<F16>(), ones2<F16>());
   };
   uint4 w_own = weight(pick(first < nq, q_w, k_w), e0), w_partner = FAITHFUL ? w_own : weight(pick(first < nq, q_w, k_w), pe);
-  if (p.emb) {
-    float a[NE];
+  float a[NE];
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int64_t at = row[i] < 0 ? 0 : row[i] < p.emb_rows ? row[i] : p.emb_rows - 1;
-      a[i] = p.emb[at * p.emb_stride + min(lane + 64 * i, p.rot - 1)];
-    }
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int e = lane + 64 * i;
-      float c, sn;
-      rotary_sincos(a[i], &sn, &c);
-      c *= p.mscale;
-      sn *= p.mscale;
-      if (FAITHFUL) {
-        c = round16<F16>(c);
-        sn = round16<F16>(sn);
-      }
-      if (PARTNER == 0 ? (e & 1) == 0 : e < half) sn = -sn;
-      if (e < D) {   // (columns beyond the rotary width: never used)
-        cs[0][e] = c;
-        cs[1][e] = sn;
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  for (int i = 0; i < NE; ++i) {
+    const int64_t at = row[i] < 0 ? 0 : row[i] < p.emb_rows ? row[i] : p.emb_rows - 1;
+    a[i] = p.emb[at * p.emb_stride + min(lane + 64 * i, p.rot - 1)];
   }
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int e = lane + 64 * i;
+    float c, sn;
+    rotary_sincos(a[i], &sn, &c);
+    c *= p.mscale;
+    sn *= p.mscale;
+    if (FAITHFUL) {
+      c = round16<F16>(c);
+      sn = round16<F16>(sn);
+    }
+    if (PARTNER == 0 ? (e & 1) == 0 : e < half) sn = -sn;
+    if (e < D) {   // (columns beyond the rotary width: never used)
+      cs[0][e] = c;
+      cs[1][e] = sn;
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   int64_t cache_off = -1;
   if (to_cache) {
     if (p.tok_chunk) {
@@ -812,7 +808,7 @@ void launch_axes(AxesParams& p, bool f16, hipStream_t st) {
   int n = (4096 + p.T - 1) / p.T;
   n = n < 1 ? 1 : n > all ? all : n;
   p.waves_per_token = n;
-  p.wpt_magic = n > 1 ? (uint32_t)((((uint64_t)1 << 32) + n - 1) / n) : 0u;   // (exact below 2^32 / n: at most 4 096 + n jobs)
+  p.wpt_magic = n > 1 ? (uint32_t)((((uint64_t)1 << 32) + n - 1) / n) : 0u;   // (exact for less than 2^32 / n jobs: fewer than 4 096 + T of them, and T below 4 096 where n is not 1)
   p.q_gap = p.q_gst ? (int32_t)(p.q_gst - (int64_t)p.q_group * p.d) : 0;
   p.q_group_inv = 1.f / (float)p.q_group;
   const dim3 grid((unsigned)(((int64_t)p.T * n + 3) / 4));
@@ -894,7 +890,7 @@ int norm_rope_launch(P& p, int32_t dtype, const MiTuning* tuning, hipStream_t st
   const bool aligned = (ptrs & 15) == 0 && (strides & 7) == 0;
   if constexpr (AXES) {
     // (whole lanes turn or do not: rotated columns end at a multiple of eight)
-    if (rot_ok && aligned && mode >= 0 && (!p.emb || p.rot % 8 == 0)) {
+    if (rot_ok && aligned && mode >= 0 && p.rot % 8 == 0) {
       launch_axes(p, f16, st);
       return mi_check_launch(name);
     }
@@ -1006,7 +1002,7 @@ int axes_launch(const NormRopeParams& base, const int64_t* positions, int64_t po
   // (0: one row for every axis, as text has it; rows that overlap otherwise are a caller's slip)
   if (positions_stride != 0 && positions_stride < p.T && n_axes > 1) return fail(MI_ERR_SHAPE, "positions of two axes overlap");
   if (p.rot <= 0 || p.rot > 256 || (p.rot & 1)) return fail(MI_ERR_SHAPE, "rot_dim must be even and within head_dim");
-  p.q_pos = positions; p.k_pos = nullptr; p.pos_st = positions_stride; p.n_axes = n_axes; p.emb_rows = angles_rows;
+  p.q_pos = positions; p.k_pos = nullptr; p.pos_st = positions_stride; p.emb_rows = angles_rows;
   for (uint32_t& w : p.axes) w = 0;
   for (int i = 0; i < p.rot / 2; ++i) {
     if (pair_axes[i] >= n_axes) return fail(MI_ERR_SHAPE, "a pair's axis is not among the positions'");

@@ -979,9 +979,9 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void paged_prefill_woven_kern
     };
     if constexpr (WIN) {   // (one copy of either loop)
 #pragma clang loop unroll(disable)
-      for (int border = 1; border >= 0; --border) {
-        for (; j < (border ? 0 : jm);) iteration(std::false_type{});
-        for (; j < (border ? jw : ntl);) iteration(std::true_type{});
+      for (int starts = 1; starts >= 0; --starts) {   // the tiles of the windows' starts, then those to the rows' ends
+        for (; j < (starts ? 0 : jm);) iteration(std::false_type{});
+        for (; j < (starts ? jw : ntl);) iteration(std::true_type{});
       }
     } else {
       for (; j < jm;) iteration(std::false_type{});
