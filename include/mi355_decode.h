@@ -408,7 +408,8 @@ int mi_paged_prefill_attention_tiles(const void* q, int64_t q_stride_tok, int64_
  * are used are kept inside the cache, lengths from 0 to what the table has room for.  kv_dtype, scales and everything else as in
  * mi_paged_decode_attention (workspace: mi_decode_workspace_bytes) and mi_paged_prefill_attention / _fp8 / _tiles
  * (workspace: mi_window_prefill_workspace_bytes with the call's own T, max_kv_len, window and sinks, -1 for ones that are refused; `one_row_requests`
- * 0: no request has exactly one row, nothing is launched for such).  The tuning knob prefill_two_phase takes 3 or -1.
+ * 0: no request has exactly one row, nothing is launched for such).  The tuning knob prefill_two_phase takes 3 or -1, decode_tile_subtiles 4
+ * counts as 2 over a 16-bit cache; decode_min_waves, prefill_row_tiles and prefill_tile_subtiles change nothing.
  */
 int mi_paged_window_decode_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
                                      const void* v_cache, int64_t kv_stride_chunk, int64_t kv_stride_tok,

@@ -475,9 +475,12 @@ static __device__ __forceinline__ T pick(bool c, T a, T b) { return c ? a : b; }
 // columns in registers for all of the token's heads: a lane has the same columns of every head.  Then a stream of head vectors,
 // two at a time with the next two on their way: queries, keys, values.  No barrier anywhere.
 //
-// 13 190 tokens, 32 / 8 heads of 128, three axes: 57 us, 5.7 TB/s of reads and writes (a large copy: 4.8); what is left is memory.
-// 64 tokens: 4.5 us, a launch and one trip after the other: positions, angles, result.  Without the hand-round (every lane with the
-// angles of its own columns, head by head) 79 and 17.7 us.
+// 13 199 tokens, 32 / 8 heads of 128, three axes: 68-70 us in a stream of calls, 4.7-4.8 TB/s of reads and writes, a large copy's rate
+// (over the same inputs again and again, partly from the last-level cache, 57); what is left is memory, in the 16-bit chain of the layers
+// as well (`faithful`: 69-70 us with a third more vector instructions).  64 tokens, either form: 4.2-4.7 us, a launch and one trip after the
+// other: positions, angles, result.  Without the hand-round (every lane with the angles of its own columns, head by head) 79 (same inputs)
+// and 17.7 us.  What this kernel cannot take (rotary widths that are no whole lanes, rows off 16 bytes) goes to the element-wise kernel:
+// 13 357 tokens 183 us, bound by its instructions (four times as many), 64 tokens 4.2.
 //
 // In one rounding (`faithful` 0) the norm weight is multiplied into cos and sin beforehand and the reciprocal norm comes last:
 // out = rstd (x (w cos) + x' (w' sin)), three multiply-adds a value; the partner's values come from its lane as packed words.

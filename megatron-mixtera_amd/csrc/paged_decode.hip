@@ -151,7 +151,7 @@ static __device__ __forceinline__ Walk window_walk(const DecodeParams& p, int le
 // the others lie on one side.  An fp8 chunk's scale is taken as sign, power of two and factor (see value_parts), and fp16
 // probabilities stand 2^14 above the running maximum: as they are, one of a thousandth of the row's largest times a scale of a hundredth
 // would be subnormal, in the numerator and in the row sum.  Bound by HBM as the kernel without a window: 64 requests of 512-8 192 tokens,
-// window 2 048, 83.5 us (6.3 TB/s); 16 of 131 072, window 32 768, 330 us (6.5); fp8, 256 of 1 024-32 768, window 4 096, 320 us (6.4).
+// window 2 048, 83.5 us (6.3 TB/s); 16 of 131 072, window 32 768, 330 us (6.5); fp8, 256 of 1 024-32 768, window 4 096, 322 us (6.4).
 template <int HDK, int HDV, int NT, bool FP8, bool F16, bool FUSED = false, bool SHORT = false, bool WIN = false>
 static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int r, int row, int h, int hq0, int gq,
                                                       int len, int start, int end, bool whole, bool final_seg,
@@ -2230,9 +2230,10 @@ int mi::launch_paged_decode(
   } else if (!win) {
     nt = fp8_cache ? 4 : 2;
   } else {
-    // With a window less of a smaller tile is out of sight, and over an fp8 cache a third wavefront fits the SIMD: 32 tokens there (256
-    // requests, 32 / 8 heads, windows of 512 / 2 048 / 20 000, 64 tokens a tile and 32: width 128 55.9 / 184 / 1 615 us -> 53.8 / 179 /
-    // 1 544, width 64 39.3 / 132 / 1 318 -> 36.9 / 106 / 1 037).  Over a 16-bit cache 16, but for long walks of width 128 (256 requests,
+    // With a window less of a smaller tile is out of sight, and loads are asked for more often: 32 tokens over an fp8 cache (256
+    // requests, 32 / 8 heads, windows of 512 / 2 048 / 20 000, 64 tokens a tile and 32: width 128 56.5 / 184 / 1 538 us -> 54.8 / 182 /
+    // 1 538, width 64 37.4 / 126 / 1 307 -> 35.8 / 106 / 1 022: by counter its wavefronts, two to a SIMD either way, wait for memory 54 %
+    // of their time with 64 tokens, 18 % with 32; width 128 61 and 50 %).  Over a 16-bit cache 16, but for long walks of width 128 (256 requests,
     // windows of 128 / 512 / 2 048: 38.1 / 94.4 / 327 -> 30.4 / 93.5 / 327, 4 096: 639 -> 644; 16 requests, 2 048: 34.0 -> 32.6; width 64,
     // 256 requests, 512 / 4 096: 52.1 / 326 -> 51.1 / 321; width 192, 48 requests, 512: 45.7 -> 40.9).
     nt = fp8_cache ? 2 : head_dim != 128 || window_keys(*win, win->max_len, 0) <= 2560 ? 1 : 2;

@@ -83,7 +83,7 @@ static_assert(wv_piece_division_ok<128>() && wv_piece_division_ok<64>(), "piece 
 
 // WIN: a row sees the last `window` keys up to its own and the first `sinks` (see PrefillParams).  The workgroup walks the tiles
 // that one of its rows sees (window_tiles), masks those that a border crosses and makes rows that are not finite again.  Four
-// prompts of 3 500-4 100 tokens, window 1 024, 32 / 8 heads of 128: 271 us, 840 TFLOP/s of what the rows see (without a window, 471
+// prompts of 3 500-4 100 tokens, window 1 024, 32 / 8 heads of 128: 269-287 us, 790-845 TFLOP/s of what the rows see (without a window, 471
 // us).  A workgroup walks 14.8 tiles, where its rows see 13.9, in 22 of its 30 us; the rest is its start, queries, first tiles and
 // results, which the CU's other workgroup covers in part.
 template <int HD, bool FP8, bool SPLIT, bool F16, int WAVES, int PER_SIMD, bool WIN>
