@@ -679,12 +679,16 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
   const uint2 ones = make_uint2(ones2<F16>(), ones2<F16>());  // four times 1.0
   // WIN, fp8: a value scale's power of two goes into the conversion of the bytes, its factor into the probabilities (and out of
   // their sum): from 1 to 2, or, where bytes times the power of two round in fp16 (below 2^-15), from 1/2 to 1.  Zero counts as
-  // 2^-126; NaN and infinite scales are in the factor.  Its sign, and a key scale's, go to the bytes, in a branch.
-  auto value_parts = [&](float scale, float& pow2, float& factor) {
+  // 2^-126; NaN and infinite scales are in the factor.  Its sign, and a key scale's, go to the bytes, in a branch.  In fp16 bytes (up to
+  // 448) hold no power of two above 2^7: the rest is in the factor, and the row's reference stands that far above its maximum (`above`
+  // powers of two), so that the probabilities times it stay below 2^15.
+  auto value_parts = [&](float scale, float& pow2, float& factor, float& above) {
     const uint32_t bits = max(__float_as_uint(scale) & 0x7fffffffu, 0x00800000u);
-    const bool low = F16 && bits < (uint32_t)(127 - 15) << 23;
-    pow2 = __uint_as_float((bits & 0x7f800000u) + (low ? 0x00800000u : 0u));
-    factor = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((bits & 0x007fffffu) | (low ? 0x3f000000u : 0x3f800000u));
+    const bool none = bits >= 0x7f800000u, low = F16 && bits < (uint32_t)(127 - 15) << 23;
+    const uint32_t over = F16 && !none && bits >= (uint32_t)(127 + 8) << 23 ? (bits >> 23) - (127 + 7) : 0u;
+    above = (float)over;
+    pow2 = __uint_as_float((bits & 0x7f800000u) + (low ? 0x00800000u : 0u) - (over << 23));
+    factor = none ? __uint_as_float(0x7fc00000u) : __uint_as_float((bits & 0x007fffffu) | ((low ? 0x3f000000u : 0x3f800000u) + (over << 23)));
   };
   constexpr float kLift = WIN && F16 ? 14.f : 0.f;   // powers of two between the running maximum and one
   for (int walked = start; walked < end; walked += 16 * NT) {
@@ -763,11 +767,11 @@ static __device__ __forceinline__ void decode_segment(const DecodeParams& p, int
     // ---- online softmax (row = m16, all lane-local after the max) -----------
     // p = 2^(s * mul - m) [* V scale, folded into the exponent]; the row sums come from the
     // matrix cores (an all-ones A operand), complete over the 16 tokens of a sub-tile.
-    const float m_new = fmaxf(m_run, tmax * mul);
+    float vpow2 = 1.f, vfactor = 1.f, above = 0.f;
+    if constexpr (WIN && FP8) value_parts(vscale, vpow2, vfactor, above);
+    const float m_new = fmaxf(m_run, WIN && FP8 && F16 ? __builtin_fmaf(tmax, mul, above) : tmax * mul);
     const float alpha = fast_exp2(m_run - m_new);
     m_run = m_new;
-    float vpow2 = 1.f, vfactor = 1.f;
-    if constexpr (WIN && FP8) value_parts(vscale, vpow2, vfactor);
     const float neg = WIN ? (FP8 ? fast_log2(vfactor) + kLift : kLift) - m_new : FP8 ? fast_log2(vscale) - m_new : -m_new;
     uint2 pf[NT];
     f32x4_t psum4 = {0.f, 0.f, 0.f, 0.f};

@@ -304,6 +304,27 @@ def test_scales_of_every_size_and_sign(mi, dev, fp8):
                 c.check(mi)
 
 
+@pytest.mark.parametrize("scale", [255.0, 256.0, 300.0, 511.9, 512.0, 1000.0, 30000.0])
+@pytest.mark.parametrize("d,dtype", [(64, FP16), (128, FP16), (128, BF16)])
+@pytest.mark.parametrize("form", ["decode", "prompts"])
+def test_large_value_scales(mi, dev, form, d, dtype, scale):
+    """Values beyond what fp16 holds, whose weighted sums it holds: e4m3 numbers times a scale of 256 and more, beside chunks of small scales."""
+    new, lens = (None, [500, 130]) if form == "decode" else ([66, 9], [500, 130])
+    for every in (1, 3):
+        c = Case(dev, new, lens, 400, 70, d=d, dtype=dtype, fp8=True, seed=15)
+        if scale > 5000:   # (sums within fp16's range as well)
+            c.v = (c.v.float() / 50).to(c.v.dtype)
+        c.scales[1][::every] = scale
+        for grid in (0, 5):
+            with mi.ops.tuning(decode_grid=grid):
+                got = c.run(mi)
+            if dtype == FP16:   # (65 520 and more round to infinity there, and 64 bits hold them: infinities of the right sign are right)
+                wide, far = got.cpu().double().view(c.q.shape), c.reference()[0]
+                beyond = (far.abs() >= 65504) & torch.isinf(wide) & (wide.sign() == far.sign())
+                got = torch.where(beyond, far, wide)
+            c.check(mi, got=got)
+
+
 def _spoil(c, r, pos, key, value):
     """Put something that is no number into a token's key or value, all heads."""
     chunk, at = int(c.table[r, pos // c.chunk]), pos % c.chunk
