@@ -59,6 +59,8 @@ def window_argument(window_size, sink_tokens: int) -> dict:
     """``window_size`` and ``sink_tokens`` as the ``window`` / ``sinks`` of the paged calls: of the tokens before it a token
     sees the last ``left``, and every one where ``left`` is -1.  There are no keys to the right of a causal row, so ``right`` is
     -1 or 0.  None, 0 and False are no window."""
+    if type(window_size) is tuple and window_size == (-1, -1) and sink_tokens == 0:   # (the default: 0.2 us of every call, not 0.5)
+        return {}
     if window_size is None or (isinstance(window_size, (bool, int, float)) and not window_size):
         window_size = (-1, -1)
     try:
